@@ -18,7 +18,8 @@ import numpy as np
 
 __all__ = ["lib", "lib_path", "MoELayer", "HY3XError", "D_MODEL", "D_FF", "N_EXPERT",
            "K_MAX", "Q4K_MATRIX_BYTES", "ROUTE_SCALE", "SHARED", "synth_key",
-           "synth_normal", "synth_uniform_sym", "synth_zipf_bias"]
+           "synth_normal", "synth_uniform_sym", "synth_zipf_bias", "RouteSpec", "route_experts",
+           "Adapters"]
 
 D_MODEL = 4096
 D_FF = 1536
@@ -75,6 +76,11 @@ _SIGS = {
     "hy3x_layer_set_trace": (I32, [P, I32, P]),
     "hy3x_layer_stats": (I32, [P, ctypes.POINTER(U64), ctypes.POINTER(U64), I32]),
     "hy3x_layer_stage_times": (I32, [P, P, I32, ctypes.POINTER(I32)]),
+    "hy3x_route_experts": (I32, [P, P, I32, I64, P, I32, P, P, P]),
+    "hy3x_adapters_create": (I32, [ctypes.POINTER(P), I32, I32, I32, I32, I32]),
+    "hy3x_adapters_destroy": (I32, [P]),
+    "hy3x_adapters_set": (I32, [P, I32, P, P, F32, I32]),
+    "hy3x_adapters_apply": (I32, [P, P, P, I32, I64, P, I64, P, I32, I64, I32, P]),
     "hy3x_synth_layer_experts": (I32, [P, U64, U32]),
     "hy3x_synth_quantize_q4k": (I32, [P, P, I64, P]),
     "hy3x_synth_key": (U64, [U64, U32, U32, U32]),
@@ -180,6 +186,78 @@ def read_rate_us(pool_ptr, pool_bytes, nbytes, reps=200, stream=None):
     us = ctypes.c_float()
     _check(lib().hy3x_diag_read_rate(pool_ptr, pool_bytes, nbytes, reps, stream, ctypes.byref(us)))
     return us.value
+
+
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2}  # HY3X_F32, HY3X_F16, HY3X_BF16
+
+
+class RouteSpec(ctypes.Structure):
+    """A routing rule (hy3x_route_spec): the k best of n_expert experts by sigmoid or
+    softmax scores, from the best topk_group of n_group groups ("max": a group counts as
+    its best expert, "top2": as the sum of its best two)."""
+
+    _fields_ = [(n, I32) for n in ("n_expert", "k", "score", "n_group", "topk_group",
+                                   "group_score", "renorm")] + [("scale", F32)]
+    SCORES = {"sigmoid": 0, "softmax": 1}
+    GROUP_SCORES = {"max": 0, "top2": 1}
+
+    def __init__(self, n_expert=N_EXPERT, k=K_MAX, score="sigmoid", n_group=1, topk_group=1,
+                 group_score="max", renorm=True, scale=ROUTE_SCALE):
+        super().__init__(n_expert, k, self.SCORES[score], n_group, topk_group,
+                         self.GROUP_SCORES[group_score], 1 if renorm else 0, scale)
+
+
+def route_experts(spec, logits, T, ids, w, dtype="f32", row_stride=None, bias=None, stream=None):
+    """ids [T x k] (int32) and w [T x k] (fp32) of T rows of logits in device memory
+    (hy3x_route_experts)."""
+    _check(lib().hy3x_route_experts(ctypes.byref(spec), _ptr(logits), DTYPES[dtype],
+                                    spec.n_expert if row_stride is None else row_stride,
+                                    _ptr(bias), T, _ptr(ids), _ptr(w), stream))
+
+
+class Adapters:
+    """The low-rank adapters of one projection [d_out x d_in], resident on the current
+    HIP device: adapter a adds scale_a B_a (A_a x) (hy3x_adapters_*)."""
+
+    def __init__(self, count, rank, d_in, d_out, dtype="bf16"):
+        h = P()
+        _check(lib().hy3x_adapters_create(ctypes.byref(h), count, rank, d_in, d_out,
+                                          DTYPES[dtype]))
+        self._h = h
+        self.count, self.rank, self.d_in, self.d_out = count, rank, d_in, d_out
+        self.dtype = dtype
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().hy3x_adapters_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def set(self, index, a, b, scale=1.0, on_device=False):
+        """Adapter `index`: a [rank x d_in], b [d_out x rank], two-byte elements of the
+        handle's type (arrays of them, or device memory with on_device)."""
+        if not on_device:
+            a, b = np.ascontiguousarray(a), np.ascontiguousarray(b)
+            assert a.nbytes == 2 * self.rank * self.d_in and b.nbytes == 2 * self.rank * self.d_out
+        _check(lib().hy3x_adapters_set(self._h, index, _ptr(a), _ptr(b), scale,
+                                       1 if on_device else 0))
+
+    def apply(self, ids, x, y, T, base=None, x_dtype=None, y_dtype=None, x_stride=None,
+              base_stride=None, y_stride=None, stream=None):
+        """y[t] = base[t] + the product of adapter ids[t] with x[t], on device memory
+        (hy3x_adapters_apply). Types default to the adapters', strides to dense rows; no
+        base: 0."""
+        _check(lib().hy3x_adapters_apply(
+            self._h, _ptr(ids), _ptr(x), DTYPES[x_dtype or self.dtype],
+            self.d_in if x_stride is None else x_stride, _ptr(base),
+            self.d_out if base_stride is None else base_stride, _ptr(y),
+            DTYPES[y_dtype or self.dtype], self.d_out if y_stride is None else y_stride, T,
+            stream))
 
 
 class MoELayer:

@@ -262,6 +262,96 @@ int hy3x_layer_last_path(const hy3x_layer *layer, int *path);
  * benchmarks: the kernel whose roofline a benchmark reports). */
 int hy3x_layer_last_kernel(const hy3x_layer *layer, int stage, const char **name);
 
+/* ---- routing to experts, as an operator of its own --------------------------
+ * What the layer's forward does in its one fixed way (sigmoid + bias, the best
+ * K of 192, hy3.c:1272-1291), for logits that the caller has and for the other
+ * rules that such models are routed by. */
+#define HY3X_F32 0 /* element types */
+#define HY3X_F16 1
+#define HY3X_BF16 2
+
+#define HY3X_SCORE_SIGMOID 0 /* s_e = 1 / (1 + exp(-l_e))                       */
+#define HY3X_SCORE_SOFTMAX 1 /* s_e = exp(l_e - max l) / sum_e exp(l_e - max l) */
+#define HY3X_GROUP_MAX 0     /* a group counts as its best expert               */
+#define HY3X_GROUP_TOP2 1    /* ... as the sum of its best two                  */
+#define HY3X_ROUTE_MAX_EXPERT 1024
+#define HY3X_ROUTE_MAX_K 16
+#define HY3X_ROUTE_MAX_GROUP 64
+#define HY3X_ROUTE_MAX_TOKENS (1 << 24)
+
+typedef struct hy3x_route_spec {
+  int n_expert;    /* E, 1 .. HY3X_ROUTE_MAX_EXPERT */
+  int k;           /* experts per token, 1 .. HY3X_ROUTE_MAX_K, at most those of the kept groups */
+  int score;       /* HY3X_SCORE_* */
+  int n_group;     /* groups of E / n_group consecutive experts; 1: none */
+  int topk_group;  /* groups whose experts may be chosen, 1 .. n_group */
+  int group_score; /* HY3X_GROUP_* */
+  int renorm;      /* nonzero: weights are divided by (their sum + 1e-20) */
+  float scale;     /* factor of the weights */
+} hy3x_route_spec;
+
+/* For each of T tokens the k experts with the largest s_e + bias_e among the
+ * experts of its best topk_group groups, in falling order: ids[T x k], and
+ * w[T x k] = s_e (/ (sum of the k s_e + 1e-20) with renorm) * scale. The bias
+ * steers the choice and is not part of the weights.
+ *  - Without a bias experts are ordered by their logits; with one by
+ *    s_e + bias_e as 64-bit arithmetic gives it. Equal keys: the lower index
+ *    first, for groups too.
+ *  - Masked experts: a logit that is NaN, -inf or the lowest finite value of
+ *    its type, or a bias that is NaN or -inf. They have s_e = 0, come after
+ *    every other expert of the kept groups (in index order) and count in no
+ *    group score; a group of masked experts comes after every other group. A
+ *    row with nothing left gets the first k experts with weights 0.
+ *  - A logit of +inf counts as the largest finite value of its type.
+ * logits: device [T rows of E elements], `type` HY3X_F32 / F16 / BF16, rows
+ * row_stride elements apart (>= E); bias: device fp32 [E] or NULL; ids, w:
+ * device, dense, overlapping nothing else. T = 0 does nothing. No allocation,
+ * no scratch: calls on any streams may overlap, and a call may be captured
+ * into a graph. stream: a hipStream_t of the current device (NULL = default
+ * stream). Asynchronous. */
+int hy3x_route_experts(const hy3x_route_spec *spec, const void *logits, int type,
+                       int64_t row_stride, const float *bias, int T, int32_t *ids, float *w,
+                       void *stream);
+
+/* ---- low-rank adapters beside a shared projection ----------------------------
+ * count adapters of one projection [d_out x d_in], for batches whose requests
+ * use different ones: adapter a adds scale_a B_a (A_a x) to the projection's
+ * output, A_a [rank x d_in], B_a [d_out x rank]. */
+typedef struct hy3x_adapters hy3x_adapters;
+#define HY3X_ADAPTERS_MAX_COUNT 65536
+#define HY3X_ADAPTERS_MAX_RANK 128
+#define HY3X_ADAPTERS_MAX_DIM 65536
+#define HY3X_ADAPTERS_MAX_TOKENS (1 << 24)
+
+/* `count` adapters on the current device, all of them zero until set; type
+ * HY3X_F16 or HY3X_BF16: the elements of A and B. Device memory: count times
+ * about 2 (d_in + d_out) bytes for each of the rank rounded up to 16, 32, 64
+ * or 128. */
+int hy3x_adapters_create(hy3x_adapters **out, int count, int rank, int d_in, int d_out, int type);
+int hy3x_adapters_destroy(hy3x_adapters *adapters);
+/* Adapter `index`: a [rank x d_in] and b [d_out x rank], dense, row-major, in
+ * the handle's type (host pointers, or device pointers with src_on_device != 0;
+ * copied and laid out for the kernels). An adapter of a smaller rank is padded
+ * with zeros by the caller. Waits for the device before and after the copy. */
+int hy3x_adapters_set(hy3x_adapters *adapters, int index, const void *a, const void *b,
+                      float scale, int src_on_device);
+/* y[t] = base[t] + scale_a B_a (A_a x[t]) for T tokens, a = ids[t] (device
+ * int32[T]); a token whose id is outside [0, count) (-1, by convention) has no
+ * adapter: y[t] = base[t]. base NULL: 0 in its place. base may be y itself
+ * (same pointer and stride: added in place); otherwise y may overlap neither x
+ * nor base (rows of one wider buffer may lie between each other).
+ * x: device [T x d_in], x_type HY3X_F32 or the handle's type; base, y: device
+ * [T x d_out], y_type HY3X_F32 or the handle's type; strides in elements, at
+ * least the row length. Sums are fp32; y is rounded once; tokens do not affect
+ * each other's results, whatever their adapters hold. T = 0 does nothing. The
+ * handle's device must be current. No allocation, no scratch: calls on one
+ * handle may overlap, and a call may be captured into a graph.
+ * stream: a hipStream_t of the handle's device (NULL = default stream).
+ * Asynchronous. */
+int hy3x_adapters_apply(const hy3x_adapters *adapters, const int32_t *ids, const void *x,
+                        int x_type, int64_t x_stride, const void *base, int64_t base_stride,
+                        void *y, int y_type, int64_t y_stride, int T, void *stream);
+
 /* ---- synthetic inputs (test / benchmark data, not part of the MoE path) ----
  * Device-side generator + Q4_K quantiser for the seeded synthetic layers the
  * benchmark configurations describe. The quantiser reproduces hy3_convert.c's
