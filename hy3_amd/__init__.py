@@ -133,6 +133,8 @@ def _check(rc):
 def _ptr(a):
     if a is None:
         return None
+    if type(a) is int:
+        return a
     if isinstance(a, np.ndarray):
         assert a.flags["C_CONTIGUOUS"]
         return a.ctypes.data
@@ -207,12 +209,23 @@ class RouteSpec(ctypes.Structure):
                          self.GROUP_SCORES[group_score], 1 if renorm else 0, scale)
 
 
+def _dev(a):
+    """_ptr of device memory, a tensor first: a small call's host time counts."""
+    try:
+        return a.data_ptr()
+    except AttributeError:
+        return _ptr(a)
+
+
 def route_experts(spec, logits, T, ids, w, dtype="f32", row_stride=None, bias=None, stream=None):
     """ids [T x k] (int32) and w [T x k] (fp32) of T rows of logits in device memory
     (hy3x_route_experts)."""
-    _check(lib().hy3x_route_experts(ctypes.byref(spec), _ptr(logits), DTYPES[dtype],
-                                    spec.n_expert if row_stride is None else row_stride,
-                                    _ptr(bias), T, _ptr(ids), _ptr(w), stream))
+    rc = (_lib or lib()).hy3x_route_experts(
+        ctypes.byref(spec), _dev(logits), DTYPES[dtype],
+        spec.n_expert if row_stride is None else row_stride,
+        None if bias is None else _dev(bias), T, _dev(ids), _dev(w), stream)
+    if rc:
+        _check(rc)
 
 
 class Adapters:
@@ -224,6 +237,7 @@ class Adapters:
         _check(lib().hy3x_adapters_create(ctypes.byref(h), count, rank, d_in, d_out,
                                           DTYPES[dtype]))
         self._h = h
+        self._apply = lib().hy3x_adapters_apply
         self.count, self.rank, self.d_in, self.d_out = count, rank, d_in, d_out
         self.dtype = dtype
 
@@ -252,12 +266,14 @@ class Adapters:
         """y[t] = base[t] + the product of adapter ids[t] with x[t], on device memory
         (hy3x_adapters_apply). Types default to the adapters', strides to dense rows; no
         base: 0."""
-        _check(lib().hy3x_adapters_apply(
-            self._h, _ptr(ids), _ptr(x), DTYPES[x_dtype or self.dtype],
-            self.d_in if x_stride is None else x_stride, _ptr(base),
-            self.d_out if base_stride is None else base_stride, _ptr(y),
+        rc = self._apply(
+            self._h, _dev(ids), _dev(x), DTYPES[x_dtype or self.dtype],
+            self.d_in if x_stride is None else x_stride, None if base is None else _dev(base),
+            self.d_out if base_stride is None else base_stride, _dev(y),
             DTYPES[y_dtype or self.dtype], self.d_out if y_stride is None else y_stride, T,
-            stream))
+            stream)
+        if rc:
+            _check(rc)
 
 
 class MoELayer:

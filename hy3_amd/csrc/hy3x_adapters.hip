@@ -50,67 +50,102 @@ namespace {
 typedef float f4v __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef _Float16 h4v __attribute__((ext_vector_type(4)));
+typedef short s4v __attribute__((ext_vector_type(4)));
 
-constexpr int WAVES = 8;
-constexpr int SINGLE_MAX_T = 256;   // up to this many tokens a block takes one token
-constexpr int TARGET_BLOCKS = 512;  // blocks that the slices are made for
+// Waves of a block, and blocks that the slices are made for.
+#ifndef NW1
+#define NW1 16
+#endif
+#ifndef NW16
+#define NW16 8
+#endif
+#ifndef TB
+#define TB 256
+#endif
+#ifndef SMT
+#define SMT 256
+#endif
+constexpr int waves_for(int TOK, int RT) { return TOK == 1 && RT <= 2 ? NW1 : NW16; }
+constexpr int SINGLE_MAX_T = SMT;   // up to this many tokens a block takes one token
+constexpr int TARGET_BLOCKS = TB;
 
 __device__ __forceinline__ float elem(float v) { return v; }
 __device__ __forceinline__ float elem(__half v) { return __half2float(v); }
 __device__ __forceinline__ float elem(__hip_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void put(float *p, float v) { *p = v; }
-__device__ __forceinline__ void put(__half *p, float v) { *p = __float2half(v); }
-__device__ __forceinline__ void put(__hip_bfloat16 *p, float v) { *p = __float2bfloat16(v); }
-
-// Eight elements as loaded, and element j of them in fp32.
 template <class T>
-struct Eight {
-  uint4 v;
-  __device__ float at(int j) const {
-    const uint32_t w = j < 4 ? (j < 2 ? v.x : v.y) : (j < 6 ? v.z : v.w);
-    const uint16_t h = (uint16_t)(w >> (16 * (j & 1)));
-    return elem(__builtin_bit_cast(T, h));
-  }
-};
+__device__ __forceinline__ T rounded(float v);
 template <>
-struct Eight<float> {
-  float4 lo, hi;
-  __device__ float at(int j) const {
-    const float4 f = j < 4 ? lo : hi;
-    return (j & 3) == 0 ? f.x : (j & 3) == 1 ? f.y : (j & 3) == 2 ? f.z : f.w;
+__device__ __forceinline__ float rounded<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __half rounded<__half>(float v) {
+  return __float2half(v);
+}
+template <>
+__device__ __forceinline__ __hip_bfloat16 rounded<__hip_bfloat16>(float v) {
+  return __float2bfloat16(v);
+}
+
+// N elements as loaded, and element j of them in fp32. Loads are 16 bytes at
+// the elements' own alignment.
+template <class T, int N>
+struct Run {
+  uint32_t w[N * sizeof(T) / 4];
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w[j]);
+    else return elem(__builtin_bit_cast(T, (uint16_t)(w[j / 2] >> (16 * (j & 1)))));
+  }
+  // in the order of j: an even element clears the odd one behind it
+  __device__ __forceinline__ void set(int j, float v) {
+    if constexpr (sizeof(T) == 4) w[j] = __builtin_bit_cast(uint32_t, v);
+    else {
+      const uint32_t h = __builtin_bit_cast(uint16_t, rounded<T>(v));
+      w[j / 2] = j & 1 ? w[j / 2] | h << 16 : h;
+    }
+  }
+  __device__ __forceinline__ void load(const T *p) { __builtin_memcpy(w, p, sizeof(w)); }
+  __device__ __forceinline__ void store(T *p) const { __builtin_memcpy(p, w, sizeof(w)); }
+  // elements c .. of a row of n (n >= 1), zeros beyond it: every load in bounds
+  // and none waiting for another
+  __device__ __forceinline__ void load_part(const T *row, int c, int n) {
+    T e[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) e[j] = row[min(c + j, n - 1)];
+#pragma unroll
+    for (int j = 0; j < N; j++) set(j, c + j < n ? elem(e[j]) : 0.0f);
+  }
+  __device__ __forceinline__ void store_part(T *p, int n) const {
+#pragma unroll
+    for (int j = 0; j < N; j++)
+      if (j < n) {
+        if constexpr (sizeof(T) == 4) p[j] = __builtin_bit_cast(T, w[j]);
+        else p[j] = __builtin_bit_cast(T, (uint16_t)(w[j / 2] >> (16 * (j & 1))));
+      }
   }
 };
 
-// Elements k .. k + 7 of a row of n, zeros beyond its end. vec: n % 8 == 0 and
-// the row is 16-byte aligned.
-template <class T>
-__device__ __forceinline__ Eight<T> load8(const T *row, int k, int n, bool vec) {
-  Eight<T> r;
-  T e[8];
-  if (vec && k < n) {
-    __builtin_memcpy(&r, __builtin_assume_aligned(row + k, 16), sizeof(r));
-    return r;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; j++) {
-    e[j] = T(0.0f);
-    if (!vec && k + j < n) e[j] = row[k + j];
-  }
-  __builtin_memcpy(&r, e, sizeof(r));
-  return r;
+__device__ __forceinline__ f4v mma(const Run<__half, 8> &a, const Run<__half, 8> &b, f4v c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a),
+                                                __builtin_bit_cast(h8v, b), c, 0, 0, 0);
 }
-
-__device__ __forceinline__ f4v mma(const Eight<__half> &a, const Eight<__half> &b, f4v c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a.v),
-                                                __builtin_bit_cast(h8v, b.v), c, 0, 0, 0);
+__device__ __forceinline__ f4v mma(const Run<__hip_bfloat16, 8> &a,
+                                   const Run<__hip_bfloat16, 8> &b, f4v c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, a),
+                                                 __builtin_bit_cast(bf8v, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ f4v mma(const Eight<__hip_bfloat16> &a, const Eight<__hip_bfloat16> &b,
-                                   f4v c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, a.v),
-                                                 __builtin_bit_cast(bf8v, b.v), c, 0, 0, 0);
+__device__ __forceinline__ f4v mma(const Run<__half, 4> &a, const Run<__half, 4> &b, f4v c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(h4v, a),
+                                               __builtin_bit_cast(h4v, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f4v mma(const Run<__hip_bfloat16, 4> &a,
+                                   const Run<__hip_bfloat16, 4> &b, f4v c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4v, a),
+                                                   __builtin_bit_cast(s4v, b), c, 0, 0, 0);
 }
 template <class W>
-__device__ __forceinline__ f4v mma(const Eight<W> &a, const Eight<float> &b, f4v c) {
+__device__ __forceinline__ f4v mma(const Run<W, 8> &a, const Run<float, 8> &b, f4v c) {
 #pragma unroll
   for (int j = 0; j < 8; j++)
     c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.at(j), b.at(j), c, 0, 0, 0);
@@ -127,131 +162,279 @@ struct Call {
   const Y *base;
   Y *y;
   int64_t x_stride, base_stride, y_stride;
-  int T, per;   // per: 64-output blocks of a slice
-  bool vx, vy;  // rows of x / of base and y in whole aligned 16-byte pieces
+  int T, per;  // per: 64-output blocks of a slice
 };
 
+// v in PARTS parts of W's precision, largest first: v = 2^e (p0 + p1 + ..).
+// fp16 parts are of v 2^-e with e chosen so that the row's largest |v| lies in
+// [2^14, 2^15): the parts keep 11 bits each, down to 2^-24 2^-14 of the
+// largest. bf16 has fp32's range, and e = 0. An infinity or NaN is its first
+// part, the others 0.
+__device__ __forceinline__ float part_of(float v, __half *) {
+  return (float)__builtin_amdgcn_cvt_pkrtz(v, 0.0f)[0];
+}
+__device__ __forceinline__ float part_of(float v, __hip_bfloat16 *) {
+  return __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+}
+
+// Three parts hold all 24 bits of an fp32 u. Two fp16 parts hold 20 bits of
+// each value, an error that an fp16 y's rounding (11 bits) covers also where
+// the base cancels most of the product; two bf16 parts would hold 14.
+template <class W, class Y>
+constexpr int parts_for() {
+  return __is_same(W, __half) && sizeof(Y) == 2 ? 2 : 3;
+}
+
+constexpr int steps_for(int TOK, int RT, int x_size) {
+  return RT == 8 ? 1 : x_size == 2 ? (RT == 1 ? 4 : RT == 2 && TOK == 1 ? 2 : RT == 2 ? 4 : 2) : 2;
+}
+
 template <class W, class X, class Y, int RT, int TOK>
-__global__ __launch_bounds__(64 * WAVES) void k_adapters(const Call<X, Y> c) {
+__global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call<X, Y> c) {
+  constexpr int WAVES = waves_for(TOK, RT);
   constexpr int RP = 16 * RT, PITCH = RP + 4;  // floats per token in LDS
+  constexpr int PARTS = parts_for<W, Y>();
+  // 32-element steps of d_in per group; two groups are in flight
+  constexpr int U = steps_for(TOK, RT, sizeof(X));
   __shared__ __align__(16) float part[WAVES][TOK][PITCH];
   __shared__ __align__(16) float u[TOK][PITCH];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
   const int64_t tok = (int64_t)blockIdx.x * TOK + (TOK == 1 ? 0 : col);
   const bool in = tok < c.T;
-  int id = in ? c.ids[tok] : -1;
-  if (id >= c.count) id = -1;
-  const X *xr = c.x + (in ? tok : 0) * c.x_stride;
+  const int64_t row = in ? tok : 0;  // columns past the last token read row 0, for nothing
+  int id = c.ids[row];
 
-  // u of every token with an adapter, one adapter after another
-  for (uint64_t todo = __ballot(id >= 0 && g == 0); todo;) {
+  // step n of this wave: pairs of 32 (128 bytes of a two-byte row) in turn over the waves
+  const int full = c.d_in / 32;
+  auto step = [&](int n) { return 2 * WAVES * (n >> 1) + 2 * wave + (n & 1); };
+  const X *xr = c.x + row * c.x_stride;
+  Run<X, 8> xv[U], xn[U];
+  auto load_x = [&](Run<X, 8>(&v)[U], int n0) {
+#pragma unroll
+    for (int i = 0; i < U; i++) v[i].load(xr + 32 * min(step(n0 + i), full - 1) + 8 * g);
+  };
+  // what does not need the token's adapter is asked for first: x, and the base
+  // of the first 64 outputs
+  if (full) load_x(xv, 0);
+  const int last = min(c.nb, (int)(blockIdx.y + 1) * c.per), cb0 = blockIdx.y * c.per + wave;
+  const Y *br = c.base ? c.base + row * c.base_stride : nullptr;
+  auto load_base = [&](Run<Y, 16> &v, int cb) {
+    if (br && 64 * cb + 64 <= c.d_out) v.load(br + 64 * cb + 16 * g);
+    else if (br) v.load_part(br, 64 * cb + 16 * g, c.d_out);
+    else
+#pragma unroll
+      for (int i = 0; i < 16; i++) v.set(i, 0.0f);
+  };
+  Run<Y, 16> bv, bn;
+  if (cb0 < last) load_base(bv, cb0);
+
+  if (!in || id >= c.count) id = -1;
+  const uint64_t mine = __ballot(id >= 0 && g == 0);  // tokens with an adapter
+  auto pick = [&](uint64_t &todo) {  // the next adapter of those tokens
     const int a = __builtin_amdgcn_readlane(id, __ffsll((long long)todo) - 1);
     todo &= ~__ballot(id == a);
-    f4v acc[RT];
+    return a;
+  };
+  uint64_t rest = mine;
+  const int a0 = mine ? pick(rest) : 0;
+  const float sc0 = c.scale[a0];
+  Run<W, 8> wv[2 * RT], wn[2 * RT];
+  auto load_b = [&](Run<W, 8>(&v)[2 * RT], int a, int cb) {
+    const W *bw = (const W *)c.b + (((int64_t)a * c.nb + cb) * 2 * RT * 64 + lane) * 8;
 #pragma unroll
-    for (int r = 0; r < RT; r++) acc[r] = f4v{0.f, 0.f, 0.f, 0.f};
-    const uint16_t *aw = c.a + ((int64_t)a * c.kt * RT * 64 + lane) * 8;
-    auto load_a = [&](int kt, int r) {
-      Eight<W> v;
-      v.v = *reinterpret_cast<const uint4 *>(aw + ((int64_t)kt * RT + r) * 512);
+    for (int j = 0; j < 2 * RT; j++) v[j].load(bw + j * 512);
+  };
+
+  // u, rank 16 r + 4 g + i of token col in acc[r][i]: groups of U steps, and in
+  // each the adapters of these tokens one after another
+  // (DOT: this lane's eight elements of rank 16 r + col, in acc[r][0])
+  constexpr bool DOT = TOK == 1 && sizeof(X) == 4;
+  f4v acc[RT];
+#pragma unroll
+  for (int r = 0; r < RT; r++) acc[r] = f4v{0.f, 0.f, 0.f, 0.f};
+  auto product = [](const Run<W, 8> &a, const Run<X, 8> &b, f4v v) {
+    if constexpr (DOT) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[0] = __builtin_fmaf(a.at(j), b.at(j), v[0]);
       return v;
+    } else {
+      return mma(a, b, v);
+    }
+  };
+  auto load_a = [&](Run<W, 8>(&v)[RT], int a, int kt) {
+    const W *aw = (const W *)c.a + (((int64_t)a * c.kt + kt) * RT * 64 + lane) * 8;
+#pragma unroll
+    for (int r = 0; r < RT; r++) v[r].load(aw + 512 * r);
+  };
+  if (mine && step(0) < full) {
+    Run<W, 8> av[U][RT], an[U][RT];
+    auto load_group = [&](Run<W, 8>(&v)[U][RT], int a, int n0) {
+#pragma unroll
+      for (int i = 0; i < U; i++) load_a(v[i], a, min(step(n0 + i), full - 1));
     };
-    // pairs of 32: 128 bytes of a two-byte x row at a time, U of them in flight
-    constexpr int U = RT >= 4 ? 2 : 4;
-    int k0 = 2 * wave;
-    for (; k0 + 2 * WAVES * (U / 2 - 1) + 1 < c.kt; k0 += WAVES * U) {
-      Eight<X> xv[U];
-      Eight<W> av[U][RT];
-#pragma unroll
-      for (int i = 0; i < U; i++) {
-        const int kt = k0 + 2 * WAVES * (i / 2) + (i & 1);
-        xv[i] = load8(xr, 32 * kt + 8 * g, c.d_in, c.vx);
-#pragma unroll
-        for (int r = 0; r < RT; r++) av[i][r] = load_a(kt, r);
+    int n0 = 0, a = a0;
+    uint64_t todo = rest;
+    load_group(av, a, 0);
+    for (;;) {
+      // the next adapter of this group, or the first of the next group: in
+      // flight through this one's products
+      const int n1 = todo ? n0 : n0 + U;
+      const bool more = step(n1) < full;
+      int a1 = a0;
+      if (todo) a1 = pick(todo);
+      else todo = rest;
+      if (more) {
+        load_group(an, a1, n1);
+        if (n1 != n0) load_x(xn, n1);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      f4v sum[RT];
+#pragma unroll
+      for (int r = 0; r < RT; r++) sum[r] = acc[r];
 #pragma unroll
       for (int i = 0; i < U; i++)
+        if (step(n0 + i) < full) {
 #pragma unroll
-        for (int r = 0; r < RT; r++) acc[r] = mma(av[i][r], xv[i], acc[r]);
-    }
-    for (; k0 < c.kt; k0 += 2 * WAVES)
-      for (int kt = k0; kt < min(k0 + 2, c.kt); kt++) {
-        const Eight<X> xv = load8(xr, 32 * kt + 8 * g, c.d_in, c.vx);
+          for (int r = 0; r < RT; r++) sum[r] = product(av[i][r], xv[i], sum[r]);
+        }
 #pragma unroll
-        for (int r = 0; r < RT; r++) acc[r] = mma(load_a(kt, r), xv, acc[r]);
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[r][i] = id == a ? sum[r][i] : acc[r][i];
+      if (!more) break;
+#pragma unroll
+      for (int i = 0; i < U; i++) {
+#pragma unroll
+        for (int r = 0; r < RT; r++) av[i][r] = an[i][r];
+        if (n1 != n0) xv[i] = xn[i];
       }
-    if (TOK == 16 || col == 0)
+      n0 = n1;
+      a = a1;
+    }
+  }
+  if (full < c.kt && wave == WAVES - 1) {  // the last, part step of an odd d_in
+    Run<X, 8> xt;
+    xt.load_part(xr, 32 * full + 8 * g, c.d_in);
+    for (uint64_t todo = mine; todo;) {
+      const int a = pick(todo);
+      Run<W, 8> av[RT];
+      load_a(av, a, full);
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
+        const f4v sum = product(av[r], xt, acc[r]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[r][i] = id == a ? sum[i] : acc[r][i];
+      }
+    }
+  }
+  if (mine && cb0 < last) load_b(wv, a0, cb0);
+  if (mine) {  // of the block: every wave has the same tokens
+    if constexpr (DOT) {
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
+        float v = acc[r][0] + __shfl_xor(acc[r][0], 16, 64);
+        v += __shfl_xor(v, 32, 64);
+        if (g == 0) part[wave][0][16 * r + col] = v;
+      }
+    } else if (TOK == 16 || col == 0)
 #pragma unroll
       for (int r = 0; r < RT; r++)
         *reinterpret_cast<f4v *>(&part[wave][TOK == 1 ? 0 : col][16 * r + 4 * g]) = acc[r];
     __syncthreads();
     for (int i = tid; i < TOK * RP; i += 64 * WAVES) {
       const int t = i / RP, r = i % RP;
-      if (TOK == 1 || __shfl(id, t, 64) == a) {
-        float sum = 0.0f;
+      float sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) sum += part[w][t][r];
-        u[t][r] = sum;
-      }
+      for (int w = 0; w < WAVES; w++) sum += part[w][t][r];
+      u[t][r] = sum;
     }
     __syncthreads();
   }
 
-  float ur[4 * RT];  // u of this lane's token, ranks 4 RT g ..
-  if (id >= 0)
+  // this lane's token: ranks 4 RT g .. of its u, in parts
+  constexpr int NS = RT == 1 ? 4 : 8, NV = 4 * RT / NS;  // elements and count of MFMA operands
+  Run<W, NS> ur[PARTS][NV];
+  float back = 1.0f;  // 2^e
+  {
+    __align__(16) float v[4 * RT];
+    float top = 0.0f;
+    if (mine)
 #pragma unroll
-    for (int r = 0; r < RT; r++)
-      *reinterpret_cast<f4v *>(&ur[4 * r]) =
-          *reinterpret_cast<const f4v *>(&u[TOK == 1 ? 0 : col][4 * RT * g + 4 * r]);
-  else
+      for (int r = 0; r < RT; r++)
+        *reinterpret_cast<f4v *>(&v[4 * r]) =
+            *reinterpret_cast<const f4v *>(&u[TOK == 1 ? 0 : col][4 * RT * g + 4 * r]);
+    else
 #pragma unroll
-    for (int r = 0; r < 4 * RT; r++) ur[r] = 0.0f;
+      for (int r = 0; r < 4 * RT; r++) v[r] = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 4 * RT; r++) top = fmaxf(top, fabsf(v[r]));
+    if (__is_same(W, __half)) {
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const int e = top < INFINITY ? max((int)(__float_as_uint(top) >> 23) - 127 - 14, -126) : 0;
+      back = __uint_as_float((uint32_t)(e + 127) << 23);
+#pragma unroll
+      for (int r = 0; r < 4 * RT; r++) v[r] = __builtin_amdgcn_ldexpf(v[r], -e);
+    }
+#pragma unroll
+    for (int r = 0; r < 4 * RT; r++) {
+      const bool finite = fabsf(v[r]) < INFINITY;
+#pragma unroll
+      for (int p = 0; p < PARTS; p++) {
+        const float h = finite ? part_of(v[r], (W *)nullptr) : p ? 0.0f : v[r];
+        ur[p][r / NS].set(r % NS, h);
+        v[r] -= finite ? h : 0.0f;
+      }
+    }
+  }
 
-  const int last = min(c.nb, (int)(blockIdx.y + 1) * c.per);
-  for (int cb = blockIdx.y * c.per + wave; cb < last; cb += WAVES) {
+  for (int cb = cb0; cb < last; cb += WAVES) {
     float out[16];
 #pragma unroll
     for (int i = 0; i < 16; i++) out[i] = 0.0f;
-    for (uint64_t todo = __ballot(id >= 0 && g == 0); todo;) {
-      const int a = __builtin_amdgcn_readlane(id, __ffsll((long long)todo) - 1);
-      todo &= ~__ballot(id == a);
-      const uint16_t *bw = c.b + (((int64_t)a * c.nb + cb) * 2 * RT * 64 + lane) * 8;
-      Eight<W> bv[2 * RT];
-#pragma unroll
-      for (int j = 0; j < 2 * RT; j++) bv[j].v = *reinterpret_cast<const uint4 *>(bw + j * 512);
-      const float sc = c.scale[a];
+    auto add = [&](const Run<W, 8>(&v)[2 * RT], int a, float sc) {
 #pragma unroll
       for (int q = 0; q < 4; q++) {
         f4v acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < 4 * RT; s++) {
-          const int f = q * 4 * RT + s;
-          acc = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[f / 8].at(f % 8), ur[s], acc, 0, 0, 0);
-        }
+        for (int p = PARTS - 1; p >= 0; p--)
 #pragma unroll
-        for (int i = 0; i < 4; i++) out[4 * q + i] = id == a ? sc * acc[i] : out[4 * q + i];
+          for (int n = 0; n < NV; n++) {
+            Run<W, NS> o;  // elements q 4 RT + NS n .. of the lane's 16 RT
+#pragma unroll
+            for (int d = 0; d < NS / 2; d++) {
+              const int f = (q * 4 * RT + NS * n) / 2 + d;
+              o.w[d] = v[f / 4].w[f % 4];
+            }
+            acc = mma(o, ur[p][n], acc);
+          }
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[4 * q + i] = id == a ? sc * (back * acc[i]) : out[4 * q + i];
       }
+    };
+    const int next = cb + WAVES;
+    if (next < last) {  // the next outputs' operands, in flight through this step
+      if (mine) load_b(wn, a0, next);
+      load_base(bn, next);
     }
-    if (!in || (TOK == 1 && col)) continue;
-    const int c0 = 64 * cb + 16 * g;
-    const Y *br = c.base ? c.base + tok * c.base_stride : nullptr;
-    Y *yr = c.y + tok * c.y_stride;
-    constexpr int P = 16 / sizeof(Y);  // elements per 16-byte piece
-    if (c.vy) {
-#pragma unroll
-      for (int p = 0; p < 16; p += P)
-        if (c0 + p < c.d_out) {
-          __align__(16) Y v[P];
-          if (br) __builtin_memcpy(v, __builtin_assume_aligned(br + c0 + p, 16), 16);
-#pragma unroll
-          for (int i = 0; i < P; i++) put(&v[i], (br ? elem(v[i]) : 0.0f) + out[p + i]);
-          __builtin_memcpy(__builtin_assume_aligned(yr + c0 + p, 16), v, 16);
-        }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; i++)
-        if (c0 + i < c.d_out) put(yr + c0 + i, (br ? elem(br[c0 + i]) : 0.0f) + out[i]);
+    if (mine) add(wv, a0, sc0);
+    for (uint64_t todo = rest; todo;) {
+      const int a = pick(todo);
+      load_b(wv, a, cb);
+      add(wv, a, c.scale[a]);
     }
+    if (in && (TOK == 16 || col == 0)) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) out[i] += bv.at(i);
+#pragma unroll
+      for (int i = 0; i < 16; i++) bv.set(i, out[i]);
+      Y *yr = c.y + row * c.y_stride + 64 * cb + 16 * g;
+      if (64 * cb + 64 <= c.d_out) bv.store(yr);
+      else bv.store_part(yr, c.d_out - 64 * cb - 16 * g);
+    }
+#pragma unroll
+    for (int j = 0; j < 2 * RT; j++) wv[j] = wn[j];
+    bv = bn;
   }
 }
 
@@ -306,17 +489,11 @@ void launch(const hy3x_adapters *h, const int32_t *ids, const void *x, int64_t x
   c.base_stride = base_stride;
   c.y_stride = y_stride;
   c.T = T;
-  c.vx = (uintptr_t)x % 16 == 0 && h->d_in % 8 == 0 &&
-         (T == 1 || x_stride * (int64_t)sizeof(X) % 16 == 0);
-  c.vy = (uintptr_t)y % 16 == 0 && (uintptr_t)base % 16 == 0 &&
-         h->d_out % (16 / (int)sizeof(Y)) == 0 &&
-         (T == 1 || (y_stride * (int64_t)sizeof(Y) % 16 == 0 &&
-                     (!base || base_stride * (int64_t)sizeof(Y) % 16 == 0)));
   const bool single = T <= SINGLE_MAX_T;
   const int tiles = single ? T : (T + 15) / 16;
   const int slices = std::max(1, std::min(c.nb, TARGET_BLOCKS / tiles));
   c.per = (c.nb + slices - 1) / slices;
-  const dim3 grid(tiles, (c.nb + c.per - 1) / c.per), block(64 * WAVES);
+  const dim3 grid(tiles, (c.nb + c.per - 1) / c.per), block(64 * waves_for(single ? 1 : 16, h->rp / 16));
 #define HY3X_ADAPTERS(RT)                                    \
   if (h->rp == 16 * RT) {                                    \
     if (single)                                              \
