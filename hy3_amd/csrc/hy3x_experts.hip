@@ -7,13 +7,22 @@
 //   ids = the k best keys of the best topk_group groups, ties to the lower index
 //   w_j = s_ids[j] / (sum_j s_ids[j] + 1e-20) * scale
 //
-// The keys are 64-bit because a choice has no tolerance: two fp32 sums
-// s + bias closer than their rounding errors would come out in an order that
-// depends on how exp was evaluated.
+// One wave per row. With G > 1 groups a group has its own LG = 2^n lanes, so
+// that its score is a reduction inside them; each lane holds V consecutive
+// experts, and lanes ascend with the experts: the first lane's first slot that
+// holds a maximum is the lowest index of a tie.
 //
-// One wave per row; expert lane + 64 m is the lane's value m. A row's keys are
-// compared as 64-bit integers that order as the doubles do, with 1 for a
-// masked expert and 0 for one of a group that was dropped.
+// A choice has no tolerance: two keys s + bias closer than the rounding errors
+// of an fp32 evaluation come out in an order that depends on how exp was
+// evaluated. So keys are fp32 first (as integers that order as the floats do,
+// k + 1 rounds of a wave-wide maximum), and the row is decided there if each
+// chosen key lies further from the next one than both can be wrong (margin()).
+// Otherwise the candidates, every key within the margin of the k-th, get
+// 64-bit keys, a lane each, and are ranked by counting (experts of the same
+// logit and bias need none: they are equal). A row with more candidates than
+// lanes is decided by 64-bit keys throughout (choose64). Groups whose scores are
+// that close at the border are scored in 64 bits (groups64). Without a bias the keys are the logits, which
+// are exact: no margin, and ties are ties.
 #include <hip/hip_bf16.h>
 #include <math.h>
 
@@ -25,17 +34,6 @@ namespace hy3x {
 namespace {
 
 constexpr int ROUTE_WAVES = 4;
-
-// Orders as the double does: larger value, larger integer; above 1 for every
-// number, as the integers 0 and 1 are those of two NaNs.
-__device__ __forceinline__ uint64_t ordered(double v) {
-  const int64_t b = __builtin_bit_cast(int64_t, v + 0.0);  // -0 counts as 0
-  return (uint64_t)(b ^ ((b >> 63) | INT64_MIN));
-}
-__device__ __forceinline__ double from_ordered(uint64_t k) {
-  const int64_t b = (int64_t)k;
-  return __builtin_bit_cast(double, b < 0 ? (b & INT64_MAX) : ~b);
-}
 
 template <class T>
 struct Limits;
@@ -56,144 +54,388 @@ __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__hip_bfloat16 v) { return __bfloat162float(v); }
 
+// Keys as integers that order as the numbers do (-0 as 0). MASKED, for a
+// masked expert, lies below every number, GONE (taken, or of a dropped group)
+// below that.
+template <class U>
+constexpr U GONE = 0;
+template <class U>
+constexpr U MASKED = 1;
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const int32_t b = __builtin_bit_cast(int32_t, v + 0.0f);
+  return (uint32_t)(b ^ ((b >> 31) | INT32_MIN));
+}
+__device__ __forceinline__ uint64_t ordered(double v) {
+  const int64_t b = __builtin_bit_cast(int64_t, v + 0.0);
+  return (uint64_t)(b ^ ((b >> 63) | INT64_MIN));
+}
+__device__ __forceinline__ float number(uint32_t k) {
+  const int32_t b = (int32_t)k;
+  return __builtin_bit_cast(float, b < 0 ? (b & INT32_MAX) : ~b);
+}
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = max(v, (uint32_t)dppi<DPP_XOR1>((int)v));
+  v = max(v, (uint32_t)dppi<DPP_XOR2>((int)v));
+  v = max(v, (uint32_t)dppi<DPP_HALF_MIRROR>((int)v));
+  v = max(v, (uint32_t)dppi<DPP_MIRROR>((int)v));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, DPP_BCAST15, 0xA, 0xF, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, DPP_BCAST31, 0xC, 0xF, false));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// One row as its wave reads it.
+template <class T>
+struct Row {
+  const T *logits;
+  const float *bias;
+  int softmax;
+  float top;  // softmax: the largest logit that is not masked
+
+  __device__ __forceinline__ float logit(int e) const {
+    return fminf(to_f32(logits[e]), Limits<T>::max);  // a NaN: see masked()
+  }
+  __device__ __forceinline__ bool masked(int e) const {
+    return !(to_f32(logits[e]) > -Limits<T>::max) || (bias && !(bias[e] > -INFINITY));
+  }
+  // the score, in 64 bits; sum: the softmax's
+  __device__ __forceinline__ double score64(int e, double sum) const {
+    return softmax ? exp((double)logit(e) - (double)top) / sum
+                   : 1.0 / (1.0 + exp(-(double)logit(e)));
+  }
+  __device__ __forceinline__ uint64_t key64(int e, double sum) const {
+    if (masked(e)) return MASKED<uint64_t>;
+    return ordered(bias ? score64(e, sum) + (double)bias[e] : (double)logit(e));
+  }
+};
+
+// The lanes of groups: LG = 2^shift lanes each, `size` experts, V per lane.
+struct Lanes {
+  int size, shift, lane, group, first, n;  // this lane: experts first .. first + n - 1
+  __device__ __forceinline__ Lanes(const hy3x_route_spec &s, int v) {
+    lane = threadIdx.x & 63;
+    size = s.n_expert / s.n_group;
+    shift = 31 - __builtin_clz(64 / s.n_group);
+    group = lane >> shift;
+    const int at = (lane & ((1 << shift) - 1)) * v;
+    first = group * size + at;
+    n = group < s.n_group ? min(max(size - at, 0), v) : 0;
+  }
+};
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+template <class T>
+__device__ __forceinline__ double sum64(const Row<T> &row, const Lanes &L) {
+  double sum = 0.0;
+  if (row.softmax)
+    for (int j = 0; j < L.n; j++)
+      if (!row.masked(L.first + j)) sum += exp((double)row.logit(L.first + j) - (double)row.top);
+  return wave_sum64(sum);
+}
+
+// How many groups come ahead of this lane's, by 64-bit scores.
+template <class T>
+__device__ __forceinline__ int groups64(const hy3x_route_spec &spec, const Row<T> &row, int v) {
+  const Lanes L(spec, v);
+  const bool top2 = spec.group_score == HY3X_GROUP_TOP2;
+  const double sum = sum64(row, L);
+  double b0 = -INFINITY, b1 = -INFINITY;
+  int live = 0;
+  for (int j = 0; j < L.n; j++) {
+    const int e = L.first + j;
+    if (row.masked(e)) continue;
+    const double s = !top2 && !row.bias
+                         ? (double)row.logit(e)
+                         : row.score64(e, sum) + (row.bias ? (double)row.bias[e] : 0.0);
+    b1 = fmax(b1, fmin(b0, s));
+    b0 = fmax(b0, s);
+    live++;
+  }
+  for (int o = 1; o < 1 << L.shift; o <<= 1) {
+    const double o0 = __shfl_xor(b0, o, 64), o1 = __shfl_xor(b1, o, 64);
+    b1 = fmax(fmax(b1, o1), fmin(b0, o0));
+    b0 = fmax(b0, o0);
+    live += __shfl_xor(live, o, 64);
+  }
+  const uint64_t best = !live ? GONE<uint64_t> : ordered(top2 && live > 1 ? b0 + b1 : b0);
+  int before = 0;
+  for (int g = 0; g < spec.n_group; g++) {
+    const uint64_t o = __shfl(best, g << L.shift, 64);
+    before += o > best || (o == best && g < L.group);
+  }
+  return before;
+}
+
+// The choice by 64-bit keys alone, lane k < K returning the k-th expert: for
+// rows with more candidates than lanes. It forms every key again in each round
+// and keeps none.
+template <class T>
+__device__ __forceinline__ int choose64(const hy3x_route_spec spec, const Row<T> row,
+                                                  int v) {
+  const Lanes L(spec, v);
+  const double sum = sum64(row, L);
+  const bool stays = spec.n_group == 1 || groups64(spec, row, v) < spec.topk_group;
+  uint32_t taken = 0;
+  int mine = 0;
+  for (int k = 0; k < spec.k; k++) {
+    uint64_t bk = GONE<uint64_t>;
+    int be = INT32_MAX;
+    for (int j = 0; stays && j < L.n; j++) {
+      const uint64_t key = taken >> j & 1 ? GONE<uint64_t> : row.key64(L.first + j, sum);
+      if (key > bk) {
+        bk = key;
+        be = L.first + j;
+      }
+    }
+    for (int o = 32; o >= 1; o >>= 1) {
+      const uint64_t ok = __shfl_xor(bk, o, 64);
+      const int oe = __shfl_xor(be, o, 64);
+      if (ok > bk || (ok == bk && oe < be)) {
+        bk = ok;
+        be = oe;
+      }
+    }
+    if (be >= L.first && be < L.first + L.n) taken |= 1u << (be - L.first);
+    if (L.lane == k) mine = be;
+  }
+  return mine;
+}
+
+// How far two fp32 keys s + bias near `key` can be from their 64-bit order: the
+// sum's rounding (2^-24 of it each) and the scores' errors, with `most` the
+// largest score. Sigmoid: expf 2 ulp, the sum 1 + e, rcp 1 ulp, below 2^-21
+// each; softmax: besides, l - top and up to 32 + 6 roundings of the sum, below
+// 2^-18 each. Doubled once more. The last term: scores that underflow.
+__device__ __forceinline__ float margin(bool softmax, float most, float key) {
+  return (softmax ? 0x1p-16f : 0x1p-19f) * most + 0x1p-22f * fabsf(key) + 0x1p-120f;
+}
+
+// Weights of the chosen experts (lane k: the k-th) and the row's outputs.
+// sum: the softmax's. fp32, except where a score lies near or below its normal
+// numbers.
+template <class T>
+__device__ __forceinline__ void finish(const hy3x_route_spec &spec, const Row<T> &row,
+                                       const Lanes &L, float sum, int mine, int64_t t,
+                                       int32_t *ids, float *w) {
+  static_assert(HY3X_ROUTE_MAX_K <= 16, "a row of 16 lanes holds the chosen");
+  const int lane = L.lane, K = spec.k;
+  const bool live = lane < K && !row.masked(mine);
+  const float x = live ? row.logit(mine) - (row.softmax ? row.top : 0.0f) : 0.0f;
+  float v = 0.0f;
+  if (__ballot(x < -80.0f)) {
+    const double s64 = sum64(row, L);
+    double s = live ? row.score64(mine, s64) : 0.0;
+    if (spec.renorm) s /= wave_sum64(s) + 1e-20;
+    v = (float)(s * (double)spec.scale);
+  } else {
+    // softmax: e / sum, or e / (sum of the chosen e + 1e-20 sum)
+    const float s = !live ? 0.0f : row.softmax ? expf(x) : 1.0f / (1.0f + expf(-x));
+    const float all = row.softmax ? sum : 1.0f;
+    const float by = spec.renorm ? row16_sum(s) + 1e-20f * all : all;
+    if (live) v = s / by * spec.scale;
+  }
+  if (lane < K) {
+    ids[t * K + lane] = mine;
+    w[t * K + lane] = v;
+  }
+}
+
 template <class T, int V>
 __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_route_experts(
     const hy3x_route_spec spec, const T *__restrict__ logits, int64_t stride,
     const float *__restrict__ bias, int n_row, int32_t *__restrict__ ids, float *__restrict__ w) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int t = blockIdx.x * ROUTE_WAVES + wave;
-  const int E = spec.n_expert, K = spec.k, G = spec.n_group;
-  extern __shared__ double keys_l[];
-  double *kl = keys_l + (size_t)wave * E;
-  const bool live = t < n_row;
-  const T *row = logits + (live ? t : 0) * stride;
-  float l[V];
-  bool on[V];
+  const int lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * ROUTE_WAVES + (threadIdx.x >> 6);
+  if (t >= n_row) return;  // whole waves; no barriers below
+  const int K = spec.k, G = spec.n_group;
+  const bool softmax = spec.score == HY3X_SCORE_SOFTMAX, top2 = spec.group_score == HY3X_GROUP_TOP2;
+  Row<T> row{logits + t * stride, bias, softmax, 0.0f};
+  const Lanes L(spec, V);
+  float l[V], b[V];
+  if (L.size % V == 0) {  // whole lanes: V elements at once
+    const int e = min(L.first, spec.n_expert - V);
+    T lv[V];
+    __builtin_memcpy(lv, row.logits + e, sizeof(lv));
+    if (bias) __builtin_memcpy(b, bias + e, sizeof(b));
 #pragma unroll
-  for (int m = 0; m < V; m++) {
-    const int e = lane + 64 * m;
-    const float b = bias && e < E ? bias[e] : 0.0f;
-    l[m] = e < E ? fminf(to_f32(row[e]), Limits<T>::max) : -INFINITY;
-    on[m] = e < E && l[m] > -Limits<T>::max && b > -INFINITY && to_f32(row[e]) == to_f32(row[e]);
-  }
-  double s[V];
-  if (spec.score == HY3X_SCORE_SIGMOID) {
-#pragma unroll
-    for (int m = 0; m < V; m++) s[m] = on[m] ? 1.0 / (1.0 + exp(-(double)l[m])) : 0.0;
+    for (int j = 0; j < V; j++) {
+      l[j] = to_f32(lv[j]);
+      if (!bias) b[j] = 0.0f;
+    }
   } else {
-    float top = -INFINITY;
 #pragma unroll
-    for (int m = 0; m < V; m++) top = on[m] ? fmaxf(top, l[m]) : top;
-    for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    double sum = 0.0;
-#pragma unroll
-    for (int m = 0; m < V; m++) {
-      s[m] = on[m] ? exp((double)l[m] - (double)top) : 0.0;
-      sum += s[m];
-    }
-    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-#pragma unroll
-    for (int m = 0; m < V; m++) s[m] = on[m] ? s[m] / sum : 0.0;
-  }
-  uint64_t key[V];
-#pragma unroll
-  for (int m = 0; m < V; m++) {
-    const int e = lane + 64 * m;
-    const double b = bias && e < E ? (double)bias[e] : 0.0;
-    key[m] = e >= E ? 0 : on[m] ? ordered(bias ? s[m] + b : (double)l[m]) : 1;
-    if (G > 1 && e < E)
-      kl[e] = !on[m] ? __builtin_nan("") : spec.group_score == HY3X_GROUP_TOP2 ? s[m] + b
-                                         : from_ordered(key[m]);
-  }
-  if (G > 1) {
-    __syncthreads();
-    const int size = E / G;
-    uint64_t score = 0;
-    if (lane < G) {
-      double best = 0.0, second = 0.0;
-      int n = 0;
-      for (int j = 0; j < size; j++) {
-        const double v = kl[lane * size + j];
-        if (v != v) continue;
-        if (n == 0 || v > best) {
-          second = best;
-          best = v;
-        } else if (n == 1 || v > second) {
-          second = v;
-        }
-        n++;
-      }
-      if (n) score = ordered(spec.group_score == HY3X_GROUP_TOP2 && n > 1 ? best + second : best);
-    }
-    int before = 0;  // groups ahead of this lane's
-    for (int g = 0; g < G; g++) {
-      const uint64_t o = __shfl(score, g, 64);
-      before += o > score || (o == score && g < lane);
-    }
-    const uint64_t keep = __ballot(lane < G && before < spec.topk_group);
-#pragma unroll
-    for (int m = 0; m < V; m++) {
-      const int e = lane + 64 * m;
-      if (e < E && !(keep >> (e / size) & 1)) key[m] = 0;
+    for (int j = 0; j < V; j++) {
+      const int e = min(L.first + j, spec.n_expert - 1);
+      l[j] = to_f32(row.logits[e]);
+      b[j] = bias ? bias[e] : 0.0f;
     }
   }
-  if (!live) return;
-  double mine = 0.0, sum = 0.0;
-  int my_e = 0;
-  for (int k = 0; k < K; k++) {
-    uint64_t bk = 0;
-    int be = E;
-    double bs = 0.0;
+  uint32_t key[V];
+  float sum = 1.0f, most = 1.0f;  // the softmax's sum; no score is larger than `most`
+  {
+    float s[V];
+    bool on[V];
 #pragma unroll
-    for (int m = 0; m < V; m++)
-      if (key[m] > bk) {
-        bk = key[m];
-        be = lane + 64 * m;
-        bs = s[m];
+    for (int j = 0; j < V; j++) {
+      on[j] = j < L.n && l[j] > -Limits<T>::max && b[j] > -INFINITY;
+      l[j] = fminf(l[j], Limits<T>::max);
+    }
+    if (softmax) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < V; j++) top = on[j] ? max(top, ordered(l[j])) : top;
+      row.top = number(wave_max(top));
+      sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        s[j] = on[j] ? expf(l[j] - row.top) : 0.0f;
+        sum += s[j];
       }
-    for (int o = 32; o >= 1; o >>= 1) {
-      const uint64_t ok = __shfl_xor(bk, o, 64);
-      const int oe = __shfl_xor(be, o, 64);
-      const double os = __shfl_xor(bs, o, 64);
-      if (ok > bk || (ok == bk && oe < be)) {
-        bk = ok;
-        be = oe;
-        bs = os;
-      }
+      sum = wave_total(sum);
+      most = __builtin_amdgcn_rcpf(sum);
+#pragma unroll
+      for (int j = 0; j < V; j++) s[j] *= most;
+    } else if (bias || (G > 1 && top2)) {
+#pragma unroll
+      for (int j = 0; j < V; j++) s[j] = __builtin_amdgcn_rcpf(1.0f + expf(-l[j]));
     }
 #pragma unroll
-    for (int m = 0; m < V; m++)
-      if (be == lane + 64 * m) key[m] = 0;
-    sum += bs;
+    for (int j = 0; j < V; j++)
+      key[j] = j >= L.n ? GONE<uint32_t>
+               : !on[j] ? MASKED<uint32_t>
+                        : ordered(bias ? s[j] + b[j] : l[j]);
+    if (G > 1) {
+      // the group's best key, or its best two s + bias, in each of its lanes
+      uint32_t a0 = GONE<uint32_t>, a1 = GONE<uint32_t>;
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const uint32_t k = !on[j] ? GONE<uint32_t> : top2 ? ordered(s[j] + b[j]) : key[j];
+        a1 = max(a1, min(a0, k));
+        a0 = max(a0, k);
+      }
+      for (int o = 1; o < 1 << L.shift; o <<= 1) {
+        const uint32_t o0 = __shfl_xor(a0, o, 64), o1 = __shfl_xor(a1, o, 64);
+        a1 = max(max(a1, o1), min(a0, o0));
+        a0 = max(a0, o0);
+      }
+      if (top2 && a1 > MASKED<uint32_t>) a0 = ordered(number(a0) + number(a1));
+      int before = 0;  // groups ahead of this lane's
+      for (int g = 0; g < G; g++) {
+        const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)a0, g << L.shift);
+        before += o > a0 || (o == a0 && g < L.group);
+      }
+      if (spec.topk_group < G && (bias || top2)) {
+        auto at = [&](int place) {  // the score of the group at that place
+          return (uint32_t)__builtin_amdgcn_readlane(
+              (int)a0, __builtin_ctzll(__ballot(L.group < G && before == place)));
+        };
+        const uint32_t in = at(spec.topk_group - 1), out = at(spec.topk_group);
+        if (out > MASKED<uint32_t> &&
+            !(number(in) - number(out) > 2.0f * margin(softmax, most, number(in))))
+          before = groups64(spec, row, V);
+      }
+      const bool stays = L.group < G && before < spec.topk_group;
+#pragma unroll
+      for (int j = 0; j < V; j++) key[j] = stays ? key[j] : GONE<uint32_t>;
+    }
+  }
+
+  // rounds of the largest key left: lane k receives the k-th and its expert
+  uint32_t my_key = GONE<uint32_t>;
+  int mine = 0;
+  auto round = [&](int k) {
+    uint32_t v = key[0];
+#pragma unroll
+    for (int j = 1; j < V; j++) v = max(v, key[j]);
+    const uint32_t M = wave_max(v);
+    const int wl = __builtin_ctzll(__ballot(v == M));
+    int slot = 0;
+#pragma unroll
+    for (int j = V - 1; j > 0; j--) slot = key[j] == M ? j : slot;
+    slot = key[0] == M ? 0 : slot;
+#pragma unroll
+    for (int j = 0; j < V; j++) key[j] = lane == wl && slot == j ? GONE<uint32_t> : key[j];
+    const int e = __builtin_amdgcn_readlane(L.first + slot, wl);
     if (lane == k) {
-      mine = bs;
-      my_e = be;
+      my_key = M;
+      mine = e;
+    }
+    return M;
+  };
+  uint32_t kth = 0;
+  for (int k = 0; k < K; k++) kth = round(k);
+  if (bias) {
+    // close to the next chosen, or left over and close to the last
+    const float edge = margin(softmax, most, number(kth));
+    const uint32_t next = __shfl(my_key, lane + 1, 64);
+    bool close = lane < K - 1 && next > MASKED<uint32_t> &&
+                 number(my_key) - number(next) <= margin(softmax, most, number(my_key));
+    bool left[V];
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      left[j] = key[j] > MASKED<uint32_t> && !(number(kth) - number(key[j]) > edge);
+    bool any = close;
+#pragma unroll
+    for (int j = 0; j < V; j++) any |= left[j];
+    if (__ballot(any)) {
+      // experts of the same logit and bias are equal in any arithmetic
+      const float lm = row.logit(mine), bm = bias[mine];
+      const float ln = __shfl(lm, lane + 1, 64), bn = __shfl(bm, lane + 1, 64);
+      const float lk = __shfl(lm, K - 1, 64), bk = __shfl(bm, K - 1, 64);
+      any = close && (lm != ln || bm != bn);
+#pragma unroll
+      for (int j = 0; j < V; j++) any |= left[j] && (l[j] != lk || b[j] != bk);
+      if (__ballot(any)) {
+        // candidates: the k chosen and all that lies close to the last of them
+        int n = K;
+        for (uint32_t M; n < 64 && (M = round(n)) > MASKED<uint32_t> &&
+                         !(number(kth) - number(M) > edge);)
+          n++;
+        if (n == 64) {
+          mine = choose64(spec, row, V);
+        } else {
+          const double s64 = sum64(row, L);
+          const uint64_t k64 = lane < n ? row.key64(mine, s64) : GONE<uint64_t>;
+          int rank = lane < n ? 0 : lane;
+          for (int i = 0; i < n; i++) {
+            const uint64_t o = __shfl(k64, i, 64);
+            const int oe = __shfl(mine, i, 64);
+            if (lane < n) rank += o > k64 || (o == k64 && oe < mine);
+          }
+          mine = __builtin_amdgcn_ds_permute(4 * rank, mine);
+        }
+      }
     }
   }
-  if (lane < K) {
-    const double v = spec.renorm ? mine / (sum + 1e-20) : mine;
-    ids[(int64_t)t * K + lane] = my_e;
-    w[(int64_t)t * K + lane] = (float)(v * (double)spec.scale);
-  }
+  finish(spec, row, L, sum, mine, t, ids, w);
 }
 
 template <class T>
 void launch(const hy3x_route_spec &spec, const void *logits, int64_t stride, const float *bias,
             int n_row, int32_t *ids, float *w, hipStream_t st) {
   const dim3 grid((n_row + ROUTE_WAVES - 1) / ROUTE_WAVES), block(64 * ROUTE_WAVES);
-  const size_t lds = spec.n_group > 1 ? (size_t)ROUTE_WAVES * spec.n_expert * sizeof(double) : 0;
-  const T *lg = (const T *)logits;
+  int lanes = 1;  // of a group
+  while (2 * lanes * spec.n_group <= 64) lanes *= 2;
+  const int v = (spec.n_expert / spec.n_group + lanes - 1) / lanes;  // at most 32
 #define HY3X_ROUTE(V)                                                                   \
-  if (spec.n_expert <= 64 * V) {                                                        \
-    k_route_experts<T, V><<<grid, block, lds, st>>>(spec, lg, stride, bias, n_row, ids, w); \
+  if (v <= V) {                                                                         \
+    k_route_experts<T, V><<<grid, block, 0, st>>>(spec, (const T *)logits, stride, bias, \
+                                                  n_row, ids, w);                       \
     return;                                                                             \
   }
   HY3X_ROUTE(1)
   HY3X_ROUTE(2)
   HY3X_ROUTE(3)
   HY3X_ROUTE(4)
+  HY3X_ROUTE(6)
   HY3X_ROUTE(8)
   HY3X_ROUTE(16)
+  HY3X_ROUTE(32)
 #undef HY3X_ROUTE
 }
 
