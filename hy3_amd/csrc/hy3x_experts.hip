@@ -208,9 +208,11 @@ __device__ __forceinline__ int choose64(const hy3x_route_spec spec, const Row<T>
 
 // How far two fp32 keys s + bias near `key` can be from their 64-bit order: the
 // sum's rounding (2^-24 of it each) and the scores' errors, with `most` the
-// largest score. Sigmoid: expf 2 ulp, the sum 1 + e, rcp 1 ulp, below 2^-21
-// each; softmax: besides, l - top and up to 32 + 6 roundings of the sum, below
-// 2^-18 each. Doubled once more. The last term: scores that underflow.
+// largest score. exp(x) by v_exp_f32 is off by (1.5 |x| + 4) 2^-24 of itself (the
+// product x log2(e) and 2 ulp), which |x| exp(-|x|) <= 0.37 bounds: sigmoid, with
+// 1 + e and rcp (1 ulp), is off by less than 2^-21; softmax, with l - top and the
+// up to 32 + 6 roundings of its sum, by less than 2^-18 of `most`. Two keys, and
+// doubled once more. The last term: scores that underflow.
 __device__ __forceinline__ float margin(bool softmax, float most, float key) {
   return (softmax ? 0x1p-16f : 0x1p-19f) * most + 0x1p-22f * fabsf(key) + 0x1p-120f;
 }
@@ -263,18 +265,20 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_route_experts(
     __builtin_memcpy(lv, row.logits + e, sizeof(lv));
     if (bias) __builtin_memcpy(b, bias + e, sizeof(b));
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-      l[j] = to_f32(lv[j]);
-      if (!bias) b[j] = 0.0f;
-    }
+    for (int j = 0; j < V; j++) l[j] = to_f32(lv[j]);
   } else {
+    int e[V];
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-      const int e = min(L.first + j, spec.n_expert - 1);
-      l[j] = to_f32(row.logits[e]);
-      b[j] = bias ? bias[e] : 0.0f;
-    }
+    for (int j = 0; j < V; j++) e[j] = min(L.first + j, spec.n_expert - 1);
+#pragma unroll
+    for (int j = 0; j < V; j++) l[j] = to_f32(row.logits[e[j]]);
+    if (bias)
+#pragma unroll
+      for (int j = 0; j < V; j++) b[j] = bias[e[j]];
   }
+  if (!bias)
+#pragma unroll
+    for (int j = 0; j < V; j++) b[j] = 0.0f;
   uint32_t key[V];
   float sum = 1.0f, most = 1.0f;  // the softmax's sum; no score is larger than `most`
   {
@@ -293,7 +297,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_route_experts(
       sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        s[j] = on[j] ? expf(l[j] - row.top) : 0.0f;
+        s[j] = on[j] ? __expf(l[j] - row.top) : 0.0f;
         sum += s[j];
       }
       sum = wave_total(sum);
@@ -302,7 +306,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_route_experts(
       for (int j = 0; j < V; j++) s[j] *= most;
     } else if (bias || (G > 1 && top2)) {
 #pragma unroll
-      for (int j = 0; j < V; j++) s[j] = __builtin_amdgcn_rcpf(1.0f + expf(-l[j]));
+      for (int j = 0; j < V; j++) s[j] = __builtin_amdgcn_rcpf(1.0f + __expf(-l[j]));
     }
 #pragma unroll
     for (int j = 0; j < V; j++)
@@ -367,29 +371,75 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_route_experts(
     }
     return M;
   };
-  uint32_t kth = 0;
-  for (int k = 0; k < K; k++) kth = round(k);
+  uint32_t kth = GONE<uint32_t>, head = GONE<uint32_t>;  // the last chosen; this lane's largest left
+  if constexpr (V <= 8) {
+    // each lane's keys sorted once: a round is the maximum of the heads, and
+    // its lane's keys move up; the expert is found from the unsorted keys
+    uint32_t q[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) q[j] = key[j];
+#pragma unroll
+    for (int i = 0; i < V; i++)  // odd-even transposition, descending
+#pragma unroll
+      for (int j = i & 1; j + 1 < V; j += 2) {
+        const uint32_t x = q[j], y = q[j + 1];
+        q[j] = max(x, y);
+        q[j + 1] = min(x, y);
+      }
+    int from = 0, nth = 0;  // the lane, and how many equal keys it gave before
+    int last = -1, again = 0;
+    for (int k = 0; k < K; k++) {
+      const uint32_t M = wave_max(q[0]);
+      const int wl = __builtin_ctzll(__ballot(q[0] == M));
+#pragma unroll
+      for (int j = 0; j < V; j++)
+        q[j] = lane == wl ? (j + 1 < V ? q[j + 1] : GONE<uint32_t>) : q[j];
+      again = M == kth && wl == last ? again + 1 : 0;
+      kth = M;
+      last = wl;
+      if (lane == k) {
+        my_key = M;
+        from = wl;
+        nth = again;
+      }
+    }
+    head = q[0];
+    int seen = 0, slot = 0;
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      const bool hit = (uint32_t)__shfl((int)key[j], from, 64) == my_key;
+      slot = hit && seen == nth ? j : slot;
+      seen += hit;
+    }
+    mine = __shfl(L.first, from, 64) + slot;
+  } else {
+    for (int k = 0; k < K; k++) kth = round(k);
+#pragma unroll
+    for (int j = 0; j < V; j++) head = max(head, key[j]);
+  }
   if (bias) {
     // close to the next chosen, or left over and close to the last
     const float edge = margin(softmax, most, number(kth));
     const uint32_t next = __shfl(my_key, lane + 1, 64);
     bool close = lane < K - 1 && next > MASKED<uint32_t> &&
                  number(my_key) - number(next) <= margin(softmax, most, number(my_key));
-    bool left[V];
+    auto left = [&](uint32_t k) {
+      return k > MASKED<uint32_t> && !(number(kth) - number(k) > edge);
+    };
+    if (__ballot(close || left(head))) {
+      if constexpr (V <= 8)
+        for (int k = 0; k < K; k++) {
+          const int e = __builtin_amdgcn_readlane(mine, k);
 #pragma unroll
-    for (int j = 0; j < V; j++)
-      left[j] = key[j] > MASKED<uint32_t> && !(number(kth) - number(key[j]) > edge);
-    bool any = close;
-#pragma unroll
-    for (int j = 0; j < V; j++) any |= left[j];
-    if (__ballot(any)) {
+          for (int j = 0; j < V; j++) key[j] = e == L.first + j && j < L.n ? GONE<uint32_t> : key[j];
+        }
       // experts of the same logit and bias are equal in any arithmetic
       const float lm = row.logit(mine), bm = bias[mine];
       const float ln = __shfl(lm, lane + 1, 64), bn = __shfl(bm, lane + 1, 64);
       const float lk = __shfl(lm, K - 1, 64), bk = __shfl(bm, K - 1, 64);
-      any = close && (lm != ln || bm != bn);
+      bool any = close && (lm != ln || bm != bn);
 #pragma unroll
-      for (int j = 0; j < V; j++) any |= left[j] && (l[j] != lk || b[j] != bk);
+      for (int j = 0; j < V; j++) any |= left(key[j]) && (l[j] != lk || b[j] != bk);
       if (__ballot(any)) {
         // candidates: the k chosen and all that lies close to the last of them
         int n = K;
