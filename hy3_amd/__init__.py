@@ -76,6 +76,9 @@ _SIGS = {
     "hy3x_layer_set_trace": (I32, [P, I32, P]),
     "hy3x_layer_stats": (I32, [P, ctypes.POINTER(U64), ctypes.POINTER(U64), I32]),
     "hy3x_layer_stage_times": (I32, [P, P, I32, ctypes.POINTER(I32)]),
+    "hy3x_layer_set_routing": (I32, [P, P]),
+    "hy3x_layer_set_adapters": (I32, [P, I32, P]),
+    "hy3x_layer_forward_adapters": (I32, [P, P, P, P, I32, I32, F32, P]),
     "hy3x_route_experts": (I32, [P, P, I32, I64, P, I32, P, P, P]),
     "hy3x_adapters_create": (I32, [ctypes.POINTER(P), I32, I32, I32, I32, I32]),
     "hy3x_adapters_destroy": (I32, [P]),
@@ -408,6 +411,27 @@ class MoELayer:
         """x += attn_out, then the MoE block, in one forward (hy3x_layer_forward_residual)."""
         _check(lib().hy3x_layer_forward_residual(self._h, x_dev_ptr, attn_dev_ptr, T, K, scale,
                                                  stream))
+
+    PROJECTIONS = ("router", "gate", "up", "down")
+
+    def set_routing(self, spec=None):
+        """Route by `spec` (a RouteSpec; its k and scale are each forward's), or by the
+        built-in rule again (hy3x_layer_set_routing)."""
+        _check(lib().hy3x_layer_set_routing(self._h, None if spec is None else ctypes.byref(spec)))
+
+    def set_adapters(self, projection, adapters=None):
+        """Adapters beside "router", "gate", "up" or "down" for forward_adapters, or none
+        (hy3x_layer_set_adapters)."""
+        _check(lib().hy3x_layer_set_adapters(self._h, self.PROJECTIONS.index(projection),
+                                             None if adapters is None else adapters._h))
+        self._adapters = dict(getattr(self, "_adapters", {}), **{projection: adapters})
+
+    def forward_adapters(self, x_dev_ptr, adapter_ids, T, attn_dev_ptr=None, K=K_MAX,
+                         scale=ROUTE_SCALE, stream=None):
+        """The block for tokens with adapters of their own, adapter_ids [T] int32 in device
+        memory (hy3x_layer_forward_adapters)."""
+        _check(lib().hy3x_layer_forward_adapters(self._h, x_dev_ptr, attn_dev_ptr,
+                                                 _ptr(adapter_ids), T, K, scale, stream))
 
     def last_shape(self):
         """(T, K) of the last forward."""

@@ -51,6 +51,8 @@ ILP = ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"]
 FILE_FLAGS = {
     "hy3x_mfma.hip": ILP,
     "hy3x_mfma_wide.hip": ILP,
+    "hy3x_mfma_raw.hip": ILP,
+    "hy3x_mfma_raw_wide.hip": ILP,
     "hy3x_route_decode.hip": ILP,
     "hy3x_gemv.hip": ["-mllvm", "-amdgpu-use-amdgpu-trackers"],
 }

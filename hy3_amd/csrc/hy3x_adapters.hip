@@ -36,6 +36,7 @@
 #include "../../include/hy3x_moe.h"
 #include "hy3x_common.h"
 #include "hy3x_error.h"
+#include "hy3x_ops.h"
 
 struct hy3x_adapters {
   int device = 0, count = 0, rank = 0, d_in = 0, d_out = 0, type = 0;
@@ -539,6 +540,18 @@ bool overlap(const void *a, int64_t a_step, int64_t a_row, const void *b, int64_
 
 }  // namespace
 
+AdaptersShape adapters_shape(const hy3x_adapters *h) { return {h->d_in, h->d_out, h->device}; }
+
+void launch_adapters(const hy3x_adapters *h, const int32_t *ids, const void *x, int x_type,
+                     int64_t x_stride, const void *base, int64_t base_stride, void *y, int y_type,
+                     int64_t y_stride, int T, hipStream_t st) {
+  if (h->type == HY3X_F16)
+    launch_types<__half>(h, ids, x, x_type == HY3X_F32, x_stride, base, base_stride, y,
+                         y_type == HY3X_F32, y_stride, T, st);
+  else
+    launch_types<__hip_bfloat16>(h, ids, x, x_type == HY3X_F32, x_stride, base, base_stride, y,
+                                 y_type == HY3X_F32, y_stride, T, st);
+}
 
 }  // namespace hy3x
 
@@ -672,13 +685,8 @@ int hy3x_adapters_apply(const hy3x_adapters *h, const int32_t *ids, const void *
     return op_fail(HY3X_E_ARG, "y overlaps base without being base");
   const int rc = check_device(h);
   if (rc) return rc;
-  hipStream_t st = (hipStream_t)stream;
-  if (h->type == HY3X_F16)
-    launch_types<__half>(h, ids, x, x_type == HY3X_F32, x_stride, base, base_stride, y,
-                         y_type == HY3X_F32, y_stride, T, st);
-  else
-    launch_types<__hip_bfloat16>(h, ids, x, x_type == HY3X_F32, x_stride, base, base_stride, y,
-                                 y_type == HY3X_F32, y_stride, T, st);
+  launch_adapters(h, ids, x, x_type, x_stride, base, base_stride, y, y_type, y_stride, T,
+                  (hipStream_t)stream);
   OP_HIP_TRY(hipGetLastError());
   return HY3X_OK;
 }

@@ -29,6 +29,7 @@
 #include "../../include/hy3x_moe.h"
 #include "hy3x_common.h"
 #include "hy3x_error.h"
+#include "hy3x_ops.h"
 
 namespace hy3x {
 namespace {
@@ -511,6 +512,16 @@ int check_route_spec(const hy3x_route_spec *s) {
   return HY3X_OK;
 }
 
+void launch_route(const hy3x_route_spec &spec, const void *logits, int type, int64_t row_stride,
+                  const float *bias, int T, int32_t *ids, float *w, hipStream_t st) {
+  if (type == HY3X_F32)
+    launch<float>(spec, logits, row_stride, bias, T, ids, w, st);
+  else if (type == HY3X_F16)
+    launch<__half>(spec, logits, row_stride, bias, T, ids, w, st);
+  else
+    launch<__hip_bfloat16>(spec, logits, row_stride, bias, T, ids, w, st);
+}
+
 }  // namespace hy3x
 
 using namespace hy3x;
@@ -532,13 +543,7 @@ extern "C" int hy3x_route_experts(const hy3x_route_spec *spec, const void *logit
   const size_t size = type == HY3X_F32 ? 4 : 2;
   if ((uintptr_t)logits % size || (uintptr_t)bias % 4 || (uintptr_t)ids % 4 || (uintptr_t)w % 4)
     return op_fail(HY3X_E_ARG, "a pointer is not aligned to its elements");
-  hipStream_t st = (hipStream_t)stream;
-  if (type == HY3X_F32)
-    launch<float>(*spec, logits, row_stride, bias, T, ids, w, st);
-  else if (type == HY3X_F16)
-    launch<__half>(*spec, logits, row_stride, bias, T, ids, w, st);
-  else
-    launch<__hip_bfloat16>(*spec, logits, row_stride, bias, T, ids, w, st);
+  launch_route(*spec, logits, type, row_stride, bias, T, ids, w, (hipStream_t)stream);
   OP_HIP_TRY(hipGetLastError());
   return HY3X_OK;
 }

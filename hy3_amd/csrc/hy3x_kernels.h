@@ -138,6 +138,8 @@ constexpr int XCD_TILE_RR_MARGIN = 7;
 HY3X_DECLARE_MFMA(mfma_tiny, 8, 4, 1)
 HY3X_DECLARE_MFMA(mfma_narrow, 32, 4, 1)
 HY3X_DECLARE_MFMA(mfma_wide, 64, 8, 1)
+HY3X_DECLARE_MFMA(mfma_raw, 32, 4, 1)  // gate/up only, the shared expert's products stored too
+HY3X_DECLARE_MFMA(mfma_raw_wide, 64, 8, 1)
 #undef HY3X_DECLARE_MFMA
 // 128-token tiles for experts holding many tokens (hy3x_mfma_big.hip): the
 // MFMA tiles' arithmetic, each wave's dequantised
@@ -166,6 +168,10 @@ __global__ void k_down_few(const uint8_t *wq, const uint8_t *wsh, const __half *
                            const __half *act_sum, const int32_t *list, const int4 *tiles,
                            const int32_t *n_tiles, int T, float *out);
 __global__ void k_hsums(const __half *h16m, __half *hsum);
+// A forward with adapters or a routing rule of its own (hy3x_adapted.hip).
+__global__ void k_mark_routes(const int32_t *ids, const float *wpre, float scale, int T, int K,
+                              float *wout, uint32_t *bits, int wt, uint8_t *ranks);
+__global__ void k_shared_swiglu(float *raw, int T, __half *h16m);
 
 __global__ void k_synth_q4k(uint8_t *dst, int64_t nblocks, uint64_t seed, uint32_t layer,
                             const float *src);

@@ -19,6 +19,7 @@
 #include "../../include/hy3x_moe.h"
 #include "hy3x_kernels.h"
 #include "hy3x_decode.h"
+#include "hy3x_ops.h"
 #include "hy3x_q8.h"
 
 using namespace hy3x;
@@ -52,6 +53,7 @@ struct ScratchMem {
   uint8_t *mem = nullptr;
   int max_tokens = 0;
   int refs = 1;
+  float *raw = nullptr;  // shared expert's gate | up per token, for adapters (made when set)
   const hy3x_layer *owner = nullptr;  // the layer whose forward ran on it last
 };
 static std::mutex g_scratch_mu;
@@ -70,6 +72,9 @@ struct hy3x_layer {
   unsigned long long *stats = nullptr;
   float *rms_r = nullptr;      // diagnostics: RMSNorm scales substituted per token
   int rms_n = 0;               // tokens rms_r covers (0: compute r)
+  bool own_rule = false;       // route by `rule` (hy3x_layer_set_routing)
+  hy3x_route_spec rule = {};   // its k and scale are the forward's
+  const hy3x_adapters *adapters[HY3X_N_PROJ] = {};  // per projection, or null
   int last_T = 0, last_K = 0;
   struct Forward {  // launch parameters of the current / last forward
     float *x = nullptr;
@@ -82,6 +87,13 @@ struct hy3x_layer {
     bool tiny = false;  // MFMA mode: gate/up in 8-token tiles (mfma_tiny)
     bool few = false;   // MFMA mode: down by k_down_few
     const float *r_in = nullptr;  // substituted RMSNorm scales, or null
+    bool stepwise = false;        // a rule of its own or adapters: s32 and the dispatch bitmaps
+                                  // whatever T
+    bool own_rule = false;        // route by `rule`
+    hy3x_route_spec rule = {};
+    const int32_t *adapter_ids = nullptr;             // hy3x_layer_forward_adapters, or null
+    const hy3x_adapters *adapters[HY3X_N_PROJ] = {};  // those of this forward
+    float *raw = nullptr;  // shared expert's gate | up, when one of its projections is adapted
     Scratch sc;         // the scratch this forward runs on
     const hy3x_layer **owner = nullptr;  // that scratch's last-forward owner slot
   } cur;
@@ -330,6 +342,7 @@ static void release_scratch(ScratchMem *m) {
   }
   if (left == 0) {
     if (m->mem) (void)hipFree(m->mem);
+    if (m->raw) (void)hipFree(m->raw);
     delete m;
   }
 }
@@ -489,6 +502,53 @@ int hy3x_layer_set_rms_scale(hy3x_layer *L, const float *r, int n) {
   return HY3X_OK;
 }
 
+int hy3x_layer_set_routing(hy3x_layer *L, const hy3x_route_spec *rule) {
+  if (!L) return fail(HY3X_E_ARG, "NULL layer");
+  if (!rule) {
+    L->own_rule = false;
+    return HY3X_OK;
+  }
+  hy3x_route_spec r = *rule;
+  r.k = 1;
+  const int rc = check_route_spec(&r);
+  if (rc) return rc;
+  if (r.n_expert != E) return fail(HY3X_E_ARG, "n_expert %d, the layer has %d", r.n_expert, E);
+  L->rule = r;
+  L->own_rule = true;
+  return HY3X_OK;
+}
+
+int hy3x_layer_set_adapters(hy3x_layer *L, int projection, const hy3x_adapters *adapters) {
+  static const int in[HY3X_N_PROJ] = {D, D, D, F}, out[HY3X_N_PROJ] = {E, F, F, D};
+  if (!L) return fail(HY3X_E_ARG, "NULL layer");
+  if (projection < 0 || projection >= HY3X_N_PROJ)
+    return fail(HY3X_E_ARG, "projection %d outside [0,%d)", projection, HY3X_N_PROJ);
+  if (adapters) {
+    const AdaptersShape s = adapters_shape(adapters);
+    if (s.d_in != in[projection] || s.d_out != out[projection])
+      return fail(HY3X_E_ARG, "projection %d is [%d x %d], the adapters' [%d x %d]", projection,
+                  out[projection], in[projection], s.d_out, s.d_in);
+    if (s.device != L->device)
+      return fail(HY3X_E_ARG, "the adapters live on device %d, the layer on %d", s.device,
+                  L->device);
+    if (projection != HY3X_PROJ_ROUTER) {
+      std::lock_guard<std::mutex> lock(g_scratch_mu);
+      if (!L->scratch_mem->raw) {
+        int dev = -1;
+        HIP_TRY(hipGetDevice(&dev));
+        if (dev != L->device)
+          return fail(HY3X_E_ARG, "the layer lives on device %d, the current device is %d",
+                      L->device, dev);
+        const int rc = dalloc(&L->scratch_mem->raw,
+                              (size_t)L->scratch_mem->max_tokens * 2 * F * sizeof(float));
+        if (rc) return rc;
+      }
+    }
+  }
+  L->adapters[projection] = adapters;
+  return HY3X_OK;
+}
+
 int hy3x_layer_set_path(hy3x_layer *L, int path) {
   if (!L || path < 0 || path > 5) return fail(HY3X_E_ARG, "bad path");
   L->path = path;
@@ -514,6 +574,8 @@ int hy3x_layer_last_kernel(const hy3x_layer *L, int stage, const char **name) {
     *name = gu ? "k_gateup_decode" : "k_down_decode";
   else if (c.mode == Mode::GEMV)
     *name = gu ? "k_gateup_gemv<4>" : "k_down_gemv<4>";
+  else if (gu && c.raw)
+    *name = c.wide ? "mfma_raw_wide::k_moe_mfma<true>" : "mfma_raw::k_moe_mfma<true>";
   else if (gu && c.tiny)
     *name = "mfma_tiny::k_moe_mfma<true>";
   else if (!gu && c.few)
@@ -546,7 +608,7 @@ static void launch_stage(hy3x_layer *L, int stage, hipStream_t st, unsigned long
       // the routing kernels also clear (first kernel) and fill (top-K) the
       // dispatch bitmaps, or make the lists themselves (k_route_small); the
       // first kernel stages the MFMA operand
-      if (T <= ROUTE_SMALL_T) {
+      if (T <= ROUTE_SMALL_T && !c.stepwise) {
         const bool mf = c.mode == Mode::MFMA;
         k_router_logits<<<dim3(E, T), 256, 0, st>>>(x, c.xadd, L->norm_w, L->router, L->bias,
                                                     L->has_bias, S.logits, S.sig, S.score,
@@ -569,6 +631,16 @@ static void launch_stage(hy3x_layer *L, int stage, hipStream_t st, unsigned long
   else
         HY3X_ROUTER_SHAPES(HY3X_LAUNCH_ROUTER) {}
 #undef HY3X_LAUNCH_ROUTER
+        if (c.adapters[HY3X_PROJ_ROUTER])
+          launch_adapters(c.adapters[HY3X_PROJ_ROUTER], c.adapter_ids, S.s32, HY3X_F32, D,
+                          S.logits, E, S.logits, HY3X_F32, E, T, st);
+        if (c.own_rule) {
+          launch_route(c.rule, S.logits, HY3X_F32, E, L->has_bias ? L->bias : nullptr, T, S.ids,
+                       S.wpre, st);
+          k_mark_routes<<<(T * K + 255) / 256, 256, 0, st>>>(S.ids, S.wpre, c.scale, T, K, S.w,
+                                                             S.bits, S.wt, S.ranks);
+          break;
+        }
         // one wave per token; up to 256 tokens one wave per block, so that
         // few tokens still spread over many CUs
         const int wpb = T <= 256 ? 1 : 4;
@@ -578,7 +650,8 @@ static void launch_stage(hy3x_layer *L, int stage, hipStream_t st, unsigned long
       }
       break;
     case HY3X_STAGE_DISPATCH:
-      if (c.mode != Mode::DECODE && T > ROUTE_SMALL_T) {
+      if (c.mode != Mode::DECODE &&
+          (T > ROUTE_SMALL_T || c.stepwise)) {
         k_dispatch_list<<<E + 1, 256, 0, st>>>(S.ranks, T, K, c.nt, S.bits, S.wt,
                                                S.list, S.tiles, S.n_tiles, mt,
                                                c.few ? FEW_TOKENS : 0, S.tiles2, S.n_tiles2,
@@ -590,7 +663,25 @@ static void launch_stage(hy3x_layer *L, int stage, hipStream_t st, unsigned long
         k_gateup_decode<<<K * DEC_GU_BLOCKS, 64 * DEC_GU_WAVES, 0, st>>>(L->wq, S.s16, S.sig, S.score, K,
                                                           c.scale, S.ids, S.wpre, S.w,
                                                           stats, S.h16, L->trace[1]);
-      else if (c.mode == Mode::MFMA && c.tiny)
+      else if (c.raw) {
+        const uint8_t *wsh = L->shared_q8 ? L->wsh : nullptr;
+        if (c.wide)
+          mfma_raw_wide::k_moe_mfma<true>
+              <<<mt * (F / mfma_raw_wide::ROWS_GU), 64 * mfma_raw_wide::WAVES, 0, st>>>(
+                  L->wq, wsh, S.s16m, S.ssum, S.list, S.tiles, S.n_tiles, T, K, S.h16m, c.raw);
+        else
+          mfma_raw::k_moe_mfma<true>
+              <<<mt * (F / mfma_raw::ROWS_GU), 64 * mfma_raw::WAVES, 0, st>>>(
+                  L->wq, wsh, S.s16m, S.ssum, S.list, S.tiles, S.n_tiles, T, K, S.h16m, c.raw);
+        for (int p : {HY3X_PROJ_GATE, HY3X_PROJ_UP}) {
+          float *y = c.raw + (p == HY3X_PROJ_UP ? F : 0);
+          if (c.adapters[p])
+            launch_adapters(c.adapters[p], c.adapter_ids, S.s32, HY3X_F32, D, y, 2 * F, y,
+                            HY3X_F32, 2 * F, T, st);
+        }
+        k_shared_swiglu<<<(unsigned)(((int64_t)T * F + 255) / 256), 256, 0, st>>>(
+            c.raw, T, S.h16m + (size_t)T * K * F);
+      } else if (c.mode == Mode::MFMA && c.tiny)
         mfma_tiny::k_moe_mfma<true>
             <<<mt * (F / mfma_tiny::ROWS_GU), 64 * mfma_tiny::WAVES, 0, st>>>(
                 L->wq, nullptr, S.s16m, S.ssum, S.list, S.tiles, S.n_tiles, T, K, S.h16m, nullptr);
@@ -642,12 +733,16 @@ static void launch_stage(hy3x_layer *L, int stage, hipStream_t st, unsigned long
       break;
     case HY3X_STAGE_COMBINE:
       if (c.mode != Mode::DECODE) k_combine<<<dim3(D / 1024, T), 256, 0, st>>>(x, c.xadd, S.out, S.w, T, K);
+      if (c.adapters[HY3X_PROJ_DOWN])
+        launch_adapters(c.adapters[HY3X_PROJ_DOWN], c.adapter_ids, c.raw, HY3X_F32, 2 * F, x, D, x,
+                        HY3X_F32, D, T, st);
       break;
   }
 }
 
 static int forward_impl(hy3x_layer *L, const Scratch *sc, const hy3x_layer **owner, float *x,
-                        const float *xadd, int T, int K, float scale, void *stream);
+                        const float *xadd, int T, int K, float scale, void *stream,
+                        const int32_t *adapter_ids = nullptr);
 
 int hy3x_layer_forward(hy3x_layer *L, float *x, int T, int K, float scale, void *stream) {
   return forward_impl(L, L ? &L->own : nullptr, L ? &L->scratch_mem->owner : nullptr, x,
@@ -671,31 +766,70 @@ int hy3x_layer_forward_static(hy3x_layer *L, float *x, int T, int K, float scale
   return forward_impl(L, &sc, &g_static_owner[dev], x, nullptr, T, K, scale, stream);
 }
 
+// The kernels read x and attn_out through restrict pointers: no overlap at all.
+static bool overlaps(const float *x, const float *attn_out, int T) {
+  const uintptr_t a0 = (uintptr_t)x, b0 = (uintptr_t)attn_out;
+  const uintptr_t n = (uintptr_t)T * D * sizeof(float);
+  return a0 < b0 + n && b0 < a0 + n;
+}
+
 int hy3x_layer_forward_residual(hy3x_layer *L, float *x, const float *attn_out, int T, int K,
                                 float scale, void *stream) {
   if (!attn_out) return fail(HY3X_E_ARG, "NULL attn_out");
-  if (x && T > 0) {
-    // the kernels read x and attn_out through restrict pointers: no overlap at all
-    const uintptr_t a0 = (uintptr_t)x, b0 = (uintptr_t)attn_out;
-    const uintptr_t n = (uintptr_t)T * D * sizeof(float);
-    if (a0 < b0 + n && b0 < a0 + n) return fail(HY3X_E_ARG, "attn_out overlaps x");
-  }
+  if (x && T > 0 && overlaps(x, attn_out, T)) return fail(HY3X_E_ARG, "attn_out overlaps x");
   return forward_impl(L, L ? &L->own : nullptr, L ? &L->scratch_mem->owner : nullptr, x,
                       attn_out, T, K, scale, stream);
 }
 
+int hy3x_layer_forward_adapters(hy3x_layer *L, float *x, const float *attn_out,
+                                const int32_t *adapter_ids, int T, int K, float scale,
+                                void *stream) {
+  if (!L || !adapter_ids) return fail(HY3X_E_ARG, "NULL layer or adapter_ids");
+  if ((uintptr_t)adapter_ids % 4) return fail(HY3X_E_ARG, "adapter_ids is not aligned");
+  if (x && attn_out && T > 0 && overlaps(x, attn_out, T))
+    return fail(HY3X_E_ARG, "attn_out overlaps x");
+  return forward_impl(L, &L->own, &L->scratch_mem->owner, x, attn_out, T, K, scale, stream,
+                      adapter_ids);
+}
+
 static int forward_impl(hy3x_layer *L, const Scratch *sc, const hy3x_layer **owner, float *x,
-                        const float *xadd, int T, int K, float scale, void *stream) {
+                        const float *xadd, int T, int K, float scale, void *stream,
+                        const int32_t *adapter_ids) {
   if (!L || !x || !sc || !owner) return fail(HY3X_E_ARG, "NULL argument");
   if (T < 1 || T > sc->max_tokens)
     return fail(HY3X_E_ARG, "T=%d outside [1,%d]", T, sc->max_tokens);
   if (K < 1 || K > KMAX) return fail(HY3X_E_ARG, "K=%d outside [1,8]", K);
   if (!L->router_set) return fail(HY3X_E_STATE, "router not set");
-  const Mode mode = T == 1 && L->path == 0                              ? Mode::DECODE
+  hy3x_route_spec rule = L->rule;
+  if (L->own_rule) {
+    rule.k = K;
+    rule.scale = 1.0f;  // the weights before the scale; k_mark_routes applies it
+    const int rc = check_route_spec(&rule);
+    if (rc) return rc;
+  }
+  bool adapted = false, shared_adapted = false;
+  if (adapter_ids) {
+    int dev = -1;
+    HIP_TRY(hipGetDevice(&dev));
+    for (int p = 0; p < HY3X_N_PROJ; p++) {
+      if (!L->adapters[p]) continue;
+      adapted = true;
+      shared_adapted |= p != HY3X_PROJ_ROUTER;
+    }
+    if (adapted && dev != L->device)
+      return fail(HY3X_E_ARG, "the layer lives on device %d, the current device is %d", L->device,
+                  dev);
+  }
+  // these act between steps that the kernels of one and of a few tokens fuse
+  const bool stepwise = L->own_rule || adapted;
+  const Mode mode = T == 1 && L->path == 0 && stepwise                  ? Mode::MFMA
+                    : T == 1 && L->path == 0                            ? Mode::DECODE
                     : L->path >= 2 || (L->path == 0 && T >= kMfmaMinT) ? Mode::MFMA
                                                                         : Mode::GEMV;
   if (L->shared_q8 && mode == Mode::GEMV)
     return fail(HY3X_E_STATE, "the GEMV tile path needs a Q4_K shared expert");
+  if (shared_adapted && mode == Mode::GEMV)
+    return fail(HY3X_E_STATE, "the GEMV tile path runs no adapters of the shared expert");
   hipStream_t st = (hipStream_t)stream;
   auto &c = L->cur;  // of the last forward until here: a refused call leaves it
   c.mode = mode;
@@ -705,15 +839,21 @@ static int forward_impl(hy3x_layer *L, const Scratch *sc, const hy3x_layer **own
   c.K = K;
   c.scale = scale;
   c.sc = *sc;
+  c.stepwise = stepwise;
+  c.own_rule = L->own_rule;
+  c.rule = rule;
+  c.adapter_ids = adapter_ids;
+  for (int p = 0; p < HY3X_N_PROJ; p++) c.adapters[p] = adapter_ids ? L->adapters[p] : nullptr;
+  c.raw = shared_adapted ? L->scratch_mem->raw : nullptr;
   c.r_in = L->rms_n >= T ? L->rms_r : nullptr;
   L->rms_n = 0;  // a substituted scale serves one forward only
   c.big = c.mode == Mode::MFMA &&
-          (L->path == 5 || ((L->path == 0 || L->path == 2) && T >= kMfmaBigMinT));
+          (L->path == 5 || ((L->path == 0 || L->path == 2) && T >= kMfmaBigMinT)) && !c.raw;
   c.wide = c.mode == Mode::MFMA && !c.big &&
-           (L->path == 4 || (L->path != 3 && T >= kMfmaWideMinT));
+           (L->path == 4 || (L->path == 5 && c.raw) || (L->path != 3 && T >= kMfmaWideMinT));
   const bool by_t = c.mode == Mode::MFMA && (L->path == 0 || L->path == 2);
   const int row_tiles = (T * K + 1) * (F / mfma_tiny::ROWS_GU);
-  c.tiny = by_t && !L->shared_q8 && T <= mfma_tiny::TOKENS && row_tiles > kTinyMinRowTiles &&
+  c.tiny = by_t && !c.raw && !L->shared_q8 && T <= mfma_tiny::TOKENS && row_tiles > kTinyMinRowTiles &&
            row_tiles <= kTinyMaxRowTiles;
   c.few = by_t && T <= kDownFewMaxT;
   // tokens per work tile

@@ -42,10 +42,16 @@
 
 namespace hy3x {
 
-// This file is compiled three times: as the narrow shape (namespace
+// This file is compiled once per shape: as the narrow shape (namespace
 // mfma_narrow), with HY3X_MFMA_WIDE defined (hy3x_mfma_wide.hip) as the wide
-// one, and with HY3X_MFMA_TINY (hy3x_mfma_tiny.hip) as the 8-token one.
-#if defined(HY3X_MFMA_WIDE)
+// one, and with HY3X_MFMA_TINY (hy3x_mfma_tiny.hip) as the 8-token one. With
+// HY3X_MFMA_RAW (hy3x_mfma_raw.hip, hy3x_mfma_raw_wide.hip) the narrow or wide
+// gate/up GEMM also stores the shared expert's gate and up products.
+#if defined(HY3X_MFMA_RAW) && defined(HY3X_MFMA_WIDE)
+namespace mfma_raw_wide {
+#elif defined(HY3X_MFMA_RAW)
+namespace mfma_raw {
+#elif defined(HY3X_MFMA_WIDE)
 namespace mfma_wide {
 #elif defined(HY3X_MFMA_TINY)
 namespace mfma_tiny {
@@ -344,6 +350,13 @@ __device__ __forceinline__ void store_tile(
           if constexpr (GATEUP) {
             h16m[(size_t)slot * F + perm8(r)] =
                 swiglu_h(acc[rg][0][t][i], acc[rg][1][t][i]);
+#ifdef HY3X_MFMA_RAW
+            if (out) {  // a tile of the shared expert: its rows are tokens
+              float *raw = out + (size_t)t_arow[tok] * (2 * F) + r;
+              raw[0] = acc[rg][0][t][i];
+              raw[F] = acc[rg][1][t][i];
+            }
+#endif
           } else {
             out[(size_t)slot * D + r] = acc[rg][0][t][i];
           }
@@ -594,6 +607,9 @@ __global__ __launch_bounds__(MT_THREADS) void k_moe_mfma(
     t_arow[tid] = s < 0 ? -1 : (GATEUP ? (s < T * K ? s / K : s - T * K) : s);
   }
   __syncthreads();
+#ifdef HY3X_MFMA_RAW
+  if (e != E) out = nullptr;
+#endif
   if constexpr (MT_TOK > 16) {  // the 8-token shape runs with a Q4_K shared expert only
     if (wsh && e == E) {
       if constexpr (MT_TOK > 32) {
@@ -632,15 +648,15 @@ __global__ __launch_bounds__(MT_THREADS) void k_moe_mfma(
 template __global__ void k_moe_mfma<true>(const uint8_t *, const uint8_t *, const __half *,
                                           const __half *, const int32_t *, const int4 *,
                                           const int32_t *, int, int, __half *, float *);
-#ifndef HY3X_MFMA_TINY  // the 8-token shape runs gate/up only
+#if !defined(HY3X_MFMA_TINY) && !defined(HY3X_MFMA_RAW)  // these run gate/up only
 template __global__ void k_moe_mfma<false>(const uint8_t *, const uint8_t *, const __half *,
                                            const __half *, const int32_t *, const int4 *,
                                            const int32_t *, int, int, __half *, float *);
 #endif
 
-}  // namespace mfma_narrow / mfma_wide / mfma_tiny
+}  // namespace mfma_narrow / mfma_wide / mfma_tiny / mfma_raw / mfma_raw_wide
 
-#if !defined(HY3X_MFMA_WIDE) && !defined(HY3X_MFMA_TINY)
+#if !defined(HY3X_MFMA_WIDE) && !defined(HY3X_MFMA_TINY) && !defined(HY3X_MFMA_RAW)
 
 // The 48 sub-block sums of every h row (down-GEMM mins operand); one wave per slot.
 __global__ __launch_bounds__(64) void k_hsums(const __half *__restrict__ h16m,

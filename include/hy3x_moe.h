@@ -199,7 +199,8 @@ int hy3x_layer_stage_times(hy3x_layer *layer, float *ms, int n_stages, int *n_fo
 /* Diagnostics: relaunches the kernels of one stage (HY3X_STAGE_*) of the last
  * forward `reps` times back to back on `stream`, bracketed by two HIP events,
  * and returns the mean microseconds per launch in *us (synchronises). Inputs
- * are those of the last forward, so the x buffer it named must still be live;
+ * are those of the last forward, so the x buffer it named (and its adapters and
+ * their ids) must still be live;
  * the stage that writes x (down for a single token, else combine) adds into it
  * again. hy3x_layer_stats does not count replays. No reference counterpart
  * (measurement only). */
@@ -351,6 +352,41 @@ int hy3x_adapters_set(hy3x_adapters *adapters, int index, const void *a, const v
 int hy3x_adapters_apply(const hy3x_adapters *adapters, const int32_t *ids, const void *x,
                         int x_type, int64_t x_stride, const void *base, int64_t base_stride,
                         void *y, int y_type, int64_t y_stride, int T, void *stream);
+
+/* ---- the layer with a routing rule of its own, and with adapters -------------- */
+/* From the next forward on, every forward of this layer routes by this rule
+ * instead of the built-in one (NULL: the built-in one again): n_expert 192,
+ * copied; k and scale are the K and scale of each forward, which refuses
+ * (HY3X_E_ARG) a K above the experts of the kept groups. The layer's router
+ * gives the logits, its expert_bias the bias. The rule's results are those of
+ * hy3x_route_experts on these logits; the built-in rule, whose fp32 order of
+ * operations is hy3.c's, stays its own. A single token then runs on the MFMA
+ * tiles. */
+int hy3x_layer_set_routing(hy3x_layer *layer, const hy3x_route_spec *rule);
+
+/* The projections of the block that adapters can stand beside: the router's
+ * logits [192 x 4096], the shared expert's gate, up [1536 x 4096] and down
+ * [4096 x 1536]. */
+#define HY3X_PROJ_ROUTER 0
+#define HY3X_PROJ_GATE 1
+#define HY3X_PROJ_UP 2
+#define HY3X_PROJ_DOWN 3
+#define HY3X_N_PROJ 4
+/* Adapters of one projection for hy3x_layer_forward_adapters (NULL: none). The
+ * handle stays the caller's, who keeps it while it is set; one handle may serve
+ * several layers. The first of the shared expert's allocates 12 KB per token of
+ * max_tokens, shared as the layer's scratch is. */
+int hy3x_layer_set_adapters(hy3x_layer *layer, int projection, const hy3x_adapters *adapters);
+
+/* hy3x_layer_forward_residual (attn_out NULL: hy3x_layer_forward) for a batch
+ * whose tokens use different adapters: token t of every adapted projection uses
+ * adapter adapter_ids[t] (device int32[T]; outside the table: none, the block as
+ * it is). Router adapters act before the routing, gate's and up's before SwiGLU,
+ * down's on the fp32 SwiGLU product. A single token runs on the MFMA tiles.
+ * Otherwise as hy3x_layer_forward; the other forwards use no adapters. */
+int hy3x_layer_forward_adapters(hy3x_layer *layer, float *x, const float *attn_out,
+                                const int32_t *adapter_ids, int T, int K, float scale,
+                                void *stream);
 
 /* ---- synthetic inputs (test / benchmark data, not part of the MoE path) ----
  * Device-side generator + Q4_K quantiser for the seeded synthetic layers the
