@@ -64,6 +64,9 @@ typedef short s4v __attribute__((ext_vector_type(4)));
 #ifndef TB
 #define TB 256
 #endif
+#ifndef R4
+#define R4 2
+#endif
 #ifndef SMT
 #define SMT 256
 #endif
@@ -163,7 +166,7 @@ struct Call {
   const Y *base;
   Y *y;
   int64_t x_stride, base_stride, y_stride;
-  int T, per;  // per: 64-output blocks of a slice
+  int T, slices, per;  // per: 64-output blocks of a slice
 };
 
 // v in PARTS parts of W's precision, largest first: v = 2^e (p0 + p1 + ..).
@@ -187,7 +190,7 @@ constexpr int parts_for() {
 }
 
 constexpr int steps_for(int TOK, int RT, int x_size) {
-  return RT == 8 ? 1 : x_size == 2 ? (RT == 1 ? 4 : RT == 2 && TOK == 1 ? 2 : RT == 2 ? 4 : 2) : 2;
+  return RT == 8 ? 1 : x_size == 2 ? (RT == 1 ? 4 : RT == 2 && TOK == 1 ? 2 : RT == 2 ? 4 : R4) : 2;
 }
 
 template <class W, class X, class Y, int RT, int TOK>
@@ -200,7 +203,12 @@ __global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call
   __shared__ __align__(16) float part[WAVES][TOK][PITCH];
   __shared__ __align__(16) float u[TOK][PITCH];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
-  const int64_t tok = (int64_t)blockIdx.x * TOK + (TOK == 1 ? 0 : col);
+  // each XCD on a contiguous run of (tokens, slice) items: the slices of one
+  // tile share x and A in its L2, neighbouring tiles their adapters
+  const uint32_t n = gridDim.x, xcd = blockIdx.x % 8;
+  const uint32_t item = xcd * (n / 8) + min(xcd, n % 8) + blockIdx.x / 8;
+  const uint32_t tile = item / c.slices, slice = item % c.slices;
+  const int64_t tok = (int64_t)tile * TOK + (TOK == 1 ? 0 : col);
   const bool in = tok < c.T;
   const int64_t row = in ? tok : 0;  // columns past the last token read row 0, for nothing
   int id = c.ids[row];
@@ -217,7 +225,7 @@ __global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call
   // what does not need the token's adapter is asked for first: x, and the base
   // of the first 64 outputs
   if (full) load_x(xv, 0);
-  const int last = min(c.nb, (int)(blockIdx.y + 1) * c.per), cb0 = blockIdx.y * c.per + wave;
+  const int last = min(c.nb, (int)(slice + 1) * c.per), cb0 = slice * c.per + wave;
   const Y *br = c.base ? c.base + row * c.base_stride : nullptr;
   auto load_base = [&](Run<Y, 16> &v, int cb) {
     if (br && 64 * cb + 64 <= c.d_out) v.load(br + 64 * cb + 16 * g);
@@ -238,7 +246,6 @@ __global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call
   };
   uint64_t rest = mine;
   const int a0 = mine ? pick(rest) : 0;
-  const float sc0 = c.scale[a0];
   Run<W, 8> wv[2 * RT], wn[2 * RT];
   auto load_b = [&](Run<W, 8>(&v)[2 * RT], int a, int cb) {
     const W *bw = (const W *)c.b + (((int64_t)a * c.nb + cb) * 2 * RT * 64 + lane) * 8;
@@ -389,11 +396,29 @@ __global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call
     }
   }
 
-  for (int cb = cb0; cb < last; cb += WAVES) {
-    float out[16];
+  // 64 outputs of each token after another, and for each the adapters of these
+  // tokens; the next step's operands in flight through this one's products
+  if (cb0 >= last) return;
+  float out[16];
 #pragma unroll
-    for (int i = 0; i < 16; i++) out[i] = 0.0f;
-    auto add = [&](const Run<W, 8>(&v)[2 * RT], int a, float sc) {
+  for (int i = 0; i < 16; i++) out[i] = 0.0f;
+  int cb = cb0, a = a0;
+  uint64_t todo = rest;
+  float sc = c.scale[a0];
+  for (;;) {
+    const int cb1 = todo ? cb : cb + WAVES;
+    const bool more = cb1 < last, done = !todo;
+    int a1 = a0;
+    if (todo) a1 = pick(todo);
+    else todo = rest;
+    float sc1 = sc;
+    if (more) {
+      if (mine) load_b(wn, a1, cb1);
+      if (rest) sc1 = c.scale[a1];
+      if (done) load_base(bn, cb1);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (mine)
 #pragma unroll
       for (int q = 0; q < 4; q++) {
         f4v acc = {0.f, 0.f, 0.f, 0.f};
@@ -405,37 +430,33 @@ __global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call
 #pragma unroll
             for (int d = 0; d < NS / 2; d++) {
               const int f = (q * 4 * RT + NS * n) / 2 + d;
-              o.w[d] = v[f / 4].w[f % 4];
+              o.w[d] = wv[f / 4].w[f % 4];
             }
             acc = mma(o, ur[p][n], acc);
           }
 #pragma unroll
         for (int i = 0; i < 4; i++) out[4 * q + i] = id == a ? sc * (back * acc[i]) : out[4 * q + i];
       }
-    };
-    const int next = cb + WAVES;
-    if (next < last) {  // the next outputs' operands, in flight through this step
-      if (mine) load_b(wn, a0, next);
-      load_base(bn, next);
-    }
-    if (mine) add(wv, a0, sc0);
-    for (uint64_t todo = rest; todo;) {
-      const int a = pick(todo);
-      load_b(wv, a, cb);
-      add(wv, a, c.scale[a]);
-    }
-    if (in && (TOK == 16 || col == 0)) {
+    if (done) {
+      if (in && (TOK == 16 || col == 0)) {
 #pragma unroll
-      for (int i = 0; i < 16; i++) out[i] += bv.at(i);
+        for (int i = 0; i < 16; i++) out[i] += bv.at(i);
 #pragma unroll
-      for (int i = 0; i < 16; i++) bv.set(i, out[i]);
-      Y *yr = c.y + row * c.y_stride + 64 * cb + 16 * g;
-      if (64 * cb + 64 <= c.d_out) bv.store(yr);
-      else bv.store_part(yr, c.d_out - 64 * cb - 16 * g);
+        for (int i = 0; i < 16; i++) bv.set(i, out[i]);
+        Y *yr = c.y + row * c.y_stride + 64 * cb + 16 * g;
+        if (64 * cb + 64 <= c.d_out) bv.store(yr);
+        else bv.store_part(yr, c.d_out - 64 * cb - 16 * g);
+      }
+      if (!more) break;
+#pragma unroll
+      for (int i = 0; i < 16; i++) out[i] = 0.0f;
+      bv = bn;
     }
 #pragma unroll
     for (int j = 0; j < 2 * RT; j++) wv[j] = wn[j];
-    bv = bn;
+    cb = cb1;
+    a = a1;
+    sc = sc1;
   }
 }
 
@@ -494,7 +515,8 @@ void launch(const hy3x_adapters *h, const int32_t *ids, const void *x, int64_t x
   const int tiles = single ? T : (T + 15) / 16;
   const int slices = std::max(1, std::min(c.nb, TARGET_BLOCKS / tiles));
   c.per = (c.nb + slices - 1) / slices;
-  const dim3 grid(tiles, (c.nb + c.per - 1) / c.per), block(64 * waves_for(single ? 1 : 16, h->rp / 16));
+  c.slices = (c.nb + c.per - 1) / c.per;
+  const dim3 grid((uint32_t)tiles * c.slices), block(64 * waves_for(single ? 1 : 16, h->rp / 16));
 #define HY3X_ADAPTERS(RT)                                    \
   if (h->rp == 16 * RT) {                                    \
     if (single)                                              \
