@@ -54,25 +54,15 @@ typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef _Float16 h4v __attribute__((ext_vector_type(4)));
 typedef short s4v __attribute__((ext_vector_type(4)));
 
-// Waves of a block, and blocks that the slices are made for.
-#ifndef NW1
-#define NW1 16
-#endif
-#ifndef NW16
-#define NW16 8
-#endif
 #ifndef TB
 #define TB 256
 #endif
-#ifndef R4
-#define R4 2
-#endif
+constexpr int waves_for(int TOK, int RT) { return RT == 1 || (RT == 2 && TOK == 16) ? 16 : 8; }
 #ifndef SMT
 #define SMT 256
 #endif
-constexpr int waves_for(int TOK, int RT) { return TOK == 1 && RT <= 2 ? NW1 : NW16; }
 constexpr int SINGLE_MAX_T = SMT;   // up to this many tokens a block takes one token
-constexpr int TARGET_BLOCKS = TB;
+constexpr int TARGET_BLOCKS = TB;  // blocks that the slices are made for
 
 __device__ __forceinline__ float elem(float v) { return v; }
 __device__ __forceinline__ float elem(__half v) { return __half2float(v); }
@@ -110,7 +100,17 @@ struct Run {
     }
   }
   __device__ __forceinline__ void load(const T *p) { __builtin_memcpy(w, p, sizeof(w)); }
-  __device__ __forceinline__ void store(T *p) const { __builtin_memcpy(p, w, sizeof(w)); }
+  // Stores past the caches (non-temporal). Plain ones fill the L2s with y, whose
+  // write-back then ends the kernel: 4096 x 4096 outputs at rank 64 49.8 us with
+  // plain stores, 36.1 with these; a kernel that reads y next is not slower for it
+  // (32 x 1536 to 4096 x 4096).
+  __device__ __forceinline__ void store(T *p) const {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+#pragma unroll
+    for (int k = 0; k < N * (int)sizeof(T) / 16; k++)
+      __builtin_nontemporal_store((u4){w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]},
+                                  (u4 *)p + k);
+  }
   // elements c .. of a row of n (n >= 1), zeros beyond it: every load in bounds
   // and none waiting for another
   __device__ __forceinline__ void load_part(const T *row, int c, int n) {
@@ -156,15 +156,13 @@ __device__ __forceinline__ f4v mma(const Run<W, 8> &a, const Run<float, 8> &b, f
   return c;
 }
 
-template <class X, class Y>
 struct Call {
   const uint16_t *a, *b;
   const float *scale;
   int count, kt, nb, d_in, d_out;  // kt = kp / 32, nb = np / 64
   const int32_t *ids;
-  const X *x;
-  const Y *base;
-  Y *y;
+  const void *x, *base;  // rows in the kernel's X and Y
+  void *y;
   int64_t x_stride, base_stride, y_stride;
   int T, slices, per;  // per: 64-output blocks of a slice
 };
@@ -189,78 +187,70 @@ constexpr int parts_for() {
   return __is_same(W, __half) && sizeof(Y) == 2 ? 2 : 3;
 }
 
-constexpr int steps_for(int TOK, int RT, int x_size) {
-  return RT == 8 ? 1 : x_size == 2 ? (RT == 1 ? 4 : RT == 2 && TOK == 1 ? 2 : RT == 2 ? 4 : R4) : 2;
-}
+// The tokens of a wave's columns: 16 consecutive ones, or one in all of them.
+// Columns past the last token read row 0, for nothing.
+struct Tokens {
+  int64_t row;
+  bool in;
+  int id;         // this column's adapter, -1: none
+  uint64_t mine;  // lanes below 16 whose column has one
 
-template <class W, class X, class Y, int RT, int TOK>
-__global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call<X, Y> c) {
-  constexpr int WAVES = waves_for(TOK, RT);
-  constexpr int RP = 16 * RT, PITCH = RP + 4;  // floats per token in LDS
-  constexpr int PARTS = parts_for<W, Y>();
-  // 32-element steps of d_in per group; two groups are in flight
-  constexpr int U = steps_for(TOK, RT, sizeof(X));
-  __shared__ __align__(16) float part[WAVES][TOK][PITCH];
-  __shared__ __align__(16) float u[TOK][PITCH];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
-  // each XCD on a contiguous run of (tokens, slice) items: the slices of one
-  // tile share x and A in its L2, neighbouring tiles their adapters
-  const uint32_t n = gridDim.x, xcd = blockIdx.x % 8;
-  const uint32_t item = xcd * (n / 8) + min(xcd, n % 8) + blockIdx.x / 8;
-  const uint32_t tile = item / c.slices, slice = item % c.slices;
-  const int64_t tok = (int64_t)tile * TOK + (TOK == 1 ? 0 : col);
-  const bool in = tok < c.T;
-  const int64_t row = in ? tok : 0;  // columns past the last token read row 0, for nothing
-  int id = c.ids[row];
-
-  // step n of this wave: pairs of 32 (128 bytes of a two-byte row) in turn over the waves
-  const int full = c.d_in / 32;
-  auto step = [&](int n) { return 2 * WAVES * (n >> 1) + 2 * wave + (n & 1); };
-  const X *xr = c.x + row * c.x_stride;
-  Run<X, 8> xv[U], xn[U];
-  auto load_x = [&](Run<X, 8>(&v)[U], int n0) {
-#pragma unroll
-    for (int i = 0; i < U; i++) v[i].load(xr + 32 * min(step(n0 + i), full - 1) + 8 * g);
-  };
-  // what does not need the token's adapter is asked for first: x, and the base
-  // of the first 64 outputs
-  if (full) load_x(xv, 0);
-  const int last = min(c.nb, (int)(slice + 1) * c.per), cb0 = slice * c.per + wave;
-  const Y *br = c.base ? c.base + row * c.base_stride : nullptr;
-  auto load_base = [&](Run<Y, 16> &v, int cb) {
-    if (br && 64 * cb + 64 <= c.d_out) v.load(br + 64 * cb + 16 * g);
-    else if (br) v.load_part(br, 64 * cb + 16 * g, c.d_out);
-    else
-#pragma unroll
-      for (int i = 0; i < 16; i++) v.set(i, 0.0f);
-  };
-  Run<Y, 16> bv, bn;
-  if (cb0 < last) load_base(bv, cb0);
-
-  if (!in || id >= c.count) id = -1;
-  const uint64_t mine = __ballot(id >= 0 && g == 0);  // tokens with an adapter
-  auto pick = [&](uint64_t &todo) {  // the next adapter of those tokens
+  __device__ __forceinline__ void find(int64_t token, int T, const int32_t *ids) {
+    in = token < T;
+    row = in ? token : 0;
+    id = ids[row];
+  }
+  __device__ __forceinline__ void settle(int count) {
+    if (!in || id >= count) id = -1;
+    mine = __ballot(id >= 0) & 0xffffu;
+  }
+  // the next adapter of the tokens in todo
+  __device__ __forceinline__ int pick(uint64_t &todo) const {
     const int a = __builtin_amdgcn_readlane(id, __ffsll((long long)todo) - 1);
     todo &= ~__ballot(id == a);
     return a;
-  };
-  uint64_t rest = mine;
-  const int a0 = mine ? pick(rest) : 0;
-  Run<W, 8> wv[2 * RT], wn[2 * RT];
-  auto load_b = [&](Run<W, 8>(&v)[2 * RT], int a, int cb) {
-    const W *bw = (const W *)c.b + (((int64_t)a * c.nb + cb) * 2 * RT * 64 + lane) * 8;
-#pragma unroll
-    for (int j = 0; j < 2 * RT; j++) v[j].load(bw + j * 512);
-  };
+  }
+};
 
-  // u, rank 16 r + 4 g + i of token col in acc[r][i]: groups of U steps, and in
-  // each the adapters of these tokens one after another
-  // (DOT: this lane's eight elements of rank 16 r + col, in acc[r][0])
-  constexpr bool DOT = TOK == 1 && sizeof(X) == 4;
+// This wave's part of u of its tokens, rank 16 r + 4 g + i of its column in
+// acc[r][i]: d_in in steps of 32, pairs of them (128 bytes of a two-byte row) in
+// turn over WAVES waves, U steps to a group, two groups in flight; in each group
+// the adapters of these tokens one after another.
+// DOT: by fp32 products instead of MFMAs (one token), this lane's eight elements
+// of a step for rank 16 r + col in acc[r][0].
+template <class W, class X, int RT, int WAVES, int U, bool DOT>
+struct Shrink {
+  Run<X, 8> xv[U];
+  const X *xr;
   f4v acc[RT];
+  int full, kt, d_in, lane, wave;  // full: whole steps, kt: all steps
+
+  __device__ __forceinline__ int step(int n) const {
+    return 2 * WAVES * (n >> 1) + 2 * wave + (n & 1);
+  }
+  __device__ __forceinline__ void load_x(Run<X, 8> (&v)[U], int n0) const {
 #pragma unroll
-  for (int r = 0; r < RT; r++) acc[r] = f4v{0.f, 0.f, 0.f, 0.f};
-  auto product = [](const Run<W, 8> &a, const Run<X, 8> &b, f4v v) {
+    for (int i = 0; i < U; i++)
+      v[i].load(xr + 32 * min(step(n0 + i), full - 1) + 8 * (lane >> 4));
+  }
+  // x of the first group, which needs no adapter yet
+  __device__ __forceinline__ void begin(const Call &c, const Tokens &tk, int w) {
+    lane = threadIdx.x & 63;
+    wave = w;
+    d_in = c.d_in;
+    full = d_in / 32;
+    kt = c.kt;
+    xr = (const X *)c.x + tk.row * c.x_stride;
+#pragma unroll
+    for (int r = 0; r < RT; r++) acc[r] = f4v{0.f, 0.f, 0.f, 0.f};
+    if (full) load_x(xv, 0);
+  }
+  __device__ __forceinline__ void load_a(Run<W, 8> (&v)[RT], const W *a, int step) const {
+    const W *aw = a + ((int64_t)step * RT * 64 + lane) * 8;
+#pragma unroll
+    for (int r = 0; r < RT; r++) v[r].load(aw + 512 * r);
+  }
+  static __device__ __forceinline__ f4v product(const Run<W, 8> &a, const Run<X, 8> &b, f4v v) {
     if constexpr (DOT) {
 #pragma unroll
       for (int j = 0; j < 8; j++) v[0] = __builtin_fmaf(a.at(j), b.at(j), v[0]);
@@ -268,115 +258,91 @@ __global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call
     } else {
       return mma(a, b, v);
     }
-  };
-  auto load_a = [&](Run<W, 8>(&v)[RT], int a, int kt) {
-    const W *aw = (const W *)c.a + (((int64_t)a * c.kt + kt) * RT * 64 + lane) * 8;
+  }
+  // N steps of adapter a's weights for the columns that use it
+  template <int N, class Live>
+  __device__ __forceinline__ void add(const Run<W, 8> (&av)[N][RT], const Run<X, 8> (&x)[N],
+                                      const Tokens &tk, int a, Live live) {
+    f4v sum[RT];
 #pragma unroll
-    for (int r = 0; r < RT; r++) v[r].load(aw + 512 * r);
-  };
-  if (mine && step(0) < full) {
-    Run<W, 8> av[U][RT], an[U][RT];
-    auto load_group = [&](Run<W, 8>(&v)[U][RT], int a, int n0) {
+    for (int r = 0; r < RT; r++) sum[r] = acc[r];
 #pragma unroll
-      for (int i = 0; i < U; i++) load_a(v[i], a, min(step(n0 + i), full - 1));
-    };
-    int n0 = 0, a = a0;
-    uint64_t todo = rest;
-    load_group(av, a, 0);
-    for (;;) {
-      // the next adapter of this group, or the first of the next group: in
-      // flight through this one's products
-      const int n1 = todo ? n0 : n0 + U;
-      const bool more = step(n1) < full;
-      int a1 = a0;
-      if (todo) a1 = pick(todo);
-      else todo = rest;
-      if (more) {
-        load_group(an, a1, n1);
-        if (n1 != n0) load_x(xn, n1);
+    for (int i = 0; i < N; i++)
+      if (live(i)) {
+#pragma unroll
+        for (int r = 0; r < RT; r++) sum[r] = product(av[i][r], x[i], sum[r]);
       }
-      __builtin_amdgcn_sched_barrier(0);
-      f4v sum[RT];
 #pragma unroll
-      for (int r = 0; r < RT; r++) sum[r] = acc[r];
+    for (int r = 0; r < RT; r++)
 #pragma unroll
-      for (int i = 0; i < U; i++)
-        if (step(n0 + i) < full) {
+      for (int i = 0; i < 4; i++) acc[r][i] = tk.id == a ? sum[r][i] : acc[r][i];
+  }
+  __device__ __forceinline__ void run(const Call &c, const Tokens &tk) {
+    uint64_t rest = tk.mine;
+    if (!rest) return;
+    const int64_t size = (int64_t)kt * RT * 512;  // elements of one adapter's A
+    const W *base = (const W *)c.a;
+    const int a0 = tk.pick(rest);
+    if (step(0) < full) {
+      Run<X, 8> xn[U];
+      Run<W, 8> av[U][RT], an[U][RT];
+      auto load_group = [&](Run<W, 8>(&v)[U][RT], int a, int n0) {
 #pragma unroll
-          for (int r = 0; r < RT; r++) sum[r] = product(av[i][r], xv[i], sum[r]);
+        for (int i = 0; i < U; i++) load_a(v[i], base + a * size, min(step(n0 + i), full - 1));
+      };
+      int n0 = 0, a = a0;
+      uint64_t todo = rest;
+      load_group(av, a, 0);
+      for (;;) {
+        // the next adapter of this group, or the first of the next group
+        const int n1 = todo ? n0 : n0 + U;
+        const bool more = step(n1) < full;
+        int a1 = a0;
+        if (todo) a1 = tk.pick(todo);
+        else todo = rest;
+        if (more) {
+          load_group(an, a1, n1);
+          if (n1 != n0) load_x(xn, n1);
         }
+        __builtin_amdgcn_sched_barrier(0);  // these loads before the products
+        add<U>(av, xv, tk, a, [&](int i) { return step(n0 + i) < full; });
+        if (!more) break;
 #pragma unroll
-      for (int r = 0; r < RT; r++)
+        for (int i = 0; i < U; i++) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[r][i] = id == a ? sum[r][i] : acc[r][i];
-      if (!more) break;
-#pragma unroll
-      for (int i = 0; i < U; i++) {
-#pragma unroll
-        for (int r = 0; r < RT; r++) av[i][r] = an[i][r];
-        if (n1 != n0) xv[i] = xn[i];
+          for (int r = 0; r < RT; r++) av[i][r] = an[i][r];
+          if (n1 != n0) xv[i] = xn[i];
+        }
+        n0 = n1;
+        a = a1;
       }
-      n0 = n1;
-      a = a1;
     }
-  }
-  if (full < c.kt && wave == WAVES - 1) {  // the last, part step of an odd d_in
-    Run<X, 8> xt;
-    xt.load_part(xr, 32 * full + 8 * g, c.d_in);
-    for (uint64_t todo = mine; todo;) {
-      const int a = pick(todo);
-      Run<W, 8> av[RT];
-      load_a(av, a, full);
-#pragma unroll
-      for (int r = 0; r < RT; r++) {
-        const f4v sum = product(av[r], xt, acc[r]);
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[r][i] = id == a ? sum[i] : acc[r][i];
+    if (full < kt && wave == WAVES - 1) {  // the last, part step of an odd d_in
+      Run<X, 8> xt[1];
+      xt[0].load_part(xr, 32 * full + 8 * (lane >> 4), d_in);
+      for (uint64_t todo = tk.mine; todo;) {
+        const int a = tk.pick(todo);
+        Run<W, 8> av[1][RT];
+        load_a(av[0], base + a * size, full);
+        add<1>(av, xt, tk, a, [](int) { return true; });
       }
     }
   }
-  if (mine && cb0 < last) load_b(wv, a0, cb0);
-  if (mine) {  // of the block: every wave has the same tokens
-    if constexpr (DOT) {
-#pragma unroll
-      for (int r = 0; r < RT; r++) {
-        float v = acc[r][0] + __shfl_xor(acc[r][0], 16, 64);
-        v += __shfl_xor(v, 32, 64);
-        if (g == 0) part[wave][0][16 * r + col] = v;
-      }
-    } else if (TOK == 16 || col == 0)
-#pragma unroll
-      for (int r = 0; r < RT; r++)
-        *reinterpret_cast<f4v *>(&part[wave][TOK == 1 ? 0 : col][16 * r + 4 * g]) = acc[r];
-    __syncthreads();
-    for (int i = tid; i < TOK * RP; i += 64 * WAVES) {
-      const int t = i / RP, r = i % RP;
-      float sum = 0.0f;
-#pragma unroll
-      for (int w = 0; w < WAVES; w++) sum += part[w][t][r];
-      u[t][r] = sum;
-    }
-    __syncthreads();
-  }
+};
 
-  // this lane's token: ranks 4 RT g .. of its u, in parts
-  constexpr int NS = RT == 1 ? 4 : 8, NV = 4 * RT / NS;  // elements and count of MFMA operands
-  Run<W, NS> ur[PARTS][NV];
-  float back = 1.0f;  // 2^e
-  {
-    __align__(16) float v[4 * RT];
-    float top = 0.0f;
-    if (mine)
-#pragma unroll
-      for (int r = 0; r < RT; r++)
-        *reinterpret_cast<f4v *>(&v[4 * r]) =
-            *reinterpret_cast<const f4v *>(&u[TOK == 1 ? 0 : col][4 * RT * g + 4 * r]);
-    else
-#pragma unroll
-      for (int r = 0; r < 4 * RT; r++) v[r] = 0.0f;
-#pragma unroll
-    for (int r = 0; r < 4 * RT; r++) top = fmaxf(top, fabsf(v[r]));
+// u of a lane's token, ranks 4 RT g + s, as MFMA operands in PARTS parts.
+template <class W, int RT, int PARTS>
+struct Parts {
+  static constexpr int NS = RT == 1 ? 4 : 8, NV = 4 * RT / NS;  // elements, operands
+  Run<W, NS> p[PARTS][NV];
+  float back;  // 2^e
+
+  __device__ __forceinline__ void split(float (&v)[4 * RT]) {
+    back = 1.0f;
     if (__is_same(W, __half)) {
+      float top = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 4 * RT; r++) top = fmaxf(top, fabsf(v[r]));
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const int e = top < INFINITY ? max((int)(__float_as_uint(top) >> 23) - 127 - 14, -126) : 0;
@@ -388,76 +354,189 @@ __global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call
     for (int r = 0; r < 4 * RT; r++) {
       const bool finite = fabsf(v[r]) < INFINITY;
 #pragma unroll
-      for (int p = 0; p < PARTS; p++) {
-        const float h = finite ? part_of(v[r], (W *)nullptr) : p ? 0.0f : v[r];
-        ur[p][r / NS].set(r % NS, h);
+      for (int q = 0; q < PARTS; q++) {
+        const float h = finite ? part_of(v[r], (W *)nullptr) : q ? 0.0f : v[r];
+        p[q][r / NS].set(r % NS, h);
         v[r] -= finite ? h : 0.0f;
       }
     }
   }
-
-  // 64 outputs of each token after another, and for each the adapters of these
-  // tokens; the next step's operands in flight through this one's products
-  if (cb0 >= last) return;
-  float out[16];
+  // outputs 16 g + 4 q + i of a block of 64 in acc[i]
+  __device__ __forceinline__ f4v product(const Run<W, 8> (&b)[2 * RT], int q) const {
+    f4v acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 16; i++) out[i] = 0.0f;
-  int cb = cb0, a = a0;
-  uint64_t todo = rest;
-  float sc = c.scale[a0];
-  for (;;) {
-    const int cb1 = todo ? cb : cb + WAVES;
-    const bool more = cb1 < last, done = !todo;
-    int a1 = a0;
-    if (todo) a1 = pick(todo);
-    else todo = rest;
-    float sc1 = sc;
-    if (more) {
-      if (mine) load_b(wn, a1, cb1);
-      if (rest) sc1 = c.scale[a1];
-      if (done) load_base(bn, cb1);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    if (mine)
+    for (int k = PARTS - 1; k >= 0; k--)
 #pragma unroll
-      for (int q = 0; q < 4; q++) {
-        f4v acc = {0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < NV; n++) {
+        Run<W, NS> o;  // elements q 4 RT + NS n .. of the lane's 16 RT
 #pragma unroll
-        for (int p = PARTS - 1; p >= 0; p--)
-#pragma unroll
-          for (int n = 0; n < NV; n++) {
-            Run<W, NS> o;  // elements q 4 RT + NS n .. of the lane's 16 RT
-#pragma unroll
-            for (int d = 0; d < NS / 2; d++) {
-              const int f = (q * 4 * RT + NS * n) / 2 + d;
-              o.w[d] = wv[f / 4].w[f % 4];
-            }
-            acc = mma(o, ur[p][n], acc);
-          }
-#pragma unroll
-        for (int i = 0; i < 4; i++) out[4 * q + i] = id == a ? sc * (back * acc[i]) : out[4 * q + i];
+        for (int d = 0; d < NS / 2; d++) {
+          const int f = (q * 4 * RT + NS * n) / 2 + d;
+          o.w[d] = b[f / 4].w[f % 4];
+        }
+        acc = mma(o, p[k][n], acc);
       }
-    if (done) {
-      if (in && (TOK == 16 || col == 0)) {
+    return acc;
+  }
+};
+
+// The outputs cb0, cb0 + WAVES, .. (blocks of 64) below `last` of the wave's
+// tokens, and for each the adapters of these tokens one after another; the next
+// step's operands in flight through this one's products.
+template <class W, class Y, int RT, int WAVES>
+struct Expand {
+  Run<Y, 16> bv, bn;
+  Run<W, 8> wv[2 * RT], wn[2 * RT];
+  const Y *br;
+
+  __device__ __forceinline__ void load_base(const Call &c, Run<Y, 16> &v, int cb) const {
+    const int c0 = 64 * cb + 16 * ((threadIdx.x & 63) >> 4);
+    if (br && 64 * cb + 64 <= c.d_out) v.load(br + c0);
+    else if (br) v.load_part(br, c0, c.d_out);
+    else
+#pragma unroll
+      for (int i = 0; i < 16; i++) v.set(i, 0.0f);
+  }
+  __device__ __forceinline__ void load_b(const Call &c, Run<W, 8> (&v)[2 * RT], int a,
+                                         int cb) const {
+    const W *bw = (const W *)c.b +
+                  (((int64_t)a * c.nb + cb) * 2 * RT * 64 + (threadIdx.x & 63)) * 8;
+#pragma unroll
+    for (int j = 0; j < 2 * RT; j++) v[j].load(bw + j * 512);
+  }
+  // the base of the first outputs, which needs no adapter yet
+  __device__ __forceinline__ void begin(const Call &c, const Tokens &tk, int cb0, int last) {
+    br = c.base ? (const Y *)c.base + tk.row * c.base_stride : nullptr;
+    if (cb0 < last) load_base(c, bv, cb0);
+  }
+  // B of the first outputs and adapter
+  __device__ __forceinline__ void ahead(const Call &c, const Tokens &tk, int cb0, int last) {
+    uint64_t rest = tk.mine;
+    if (rest && cb0 < last) load_b(c, wv, tk.pick(rest), cb0);
+  }
+  template <class P>
+  __device__ __forceinline__ void run(const Call &c, const Tokens &tk, const P &u, int cb0,
+                                      int last, bool stores) {
+    if (cb0 >= last) return;
+    uint64_t rest = tk.mine;
+    const int a0 = rest ? tk.pick(rest) : 0;
+    float out[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) out[i] = 0.0f;
+    int cb = cb0, a = a0;
+    uint64_t todo = rest;
+    float sc = c.scale[a0];
+    for (;;) {
+      const int cb1 = todo ? cb : cb + WAVES;
+      const bool more = cb1 < last, done = !todo;
+      int a1 = a0;
+      if (todo) a1 = tk.pick(todo);
+      else todo = rest;
+      float sc1 = sc;
+      if (more) {
+        if (tk.mine) load_b(c, wn, a1, cb1);
+        if (rest) sc1 = c.scale[a1];
+        if (done) load_base(c, bn, cb1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (tk.mine)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const f4v acc = u.product(wv, q);
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            out[4 * q + i] = tk.id == a ? sc * (u.back * acc[i]) : out[4 * q + i];
+        }
+      if (done) {
+        const int c0 = 64 * cb + 16 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
         for (int i = 0; i < 16; i++) out[i] += bv.at(i);
 #pragma unroll
         for (int i = 0; i < 16; i++) bv.set(i, out[i]);
-        Y *yr = c.y + row * c.y_stride + 64 * cb + 16 * g;
-        if (64 * cb + 64 <= c.d_out) bv.store(yr);
-        else bv.store_part(yr, c.d_out - 64 * cb - 16 * g);
+        if (tk.in && stores) {
+          Y *yr = (Y *)c.y + tk.row * c.y_stride + c0;
+          if (64 * cb + 64 > c.d_out) bv.store_part(yr, c.d_out - c0);
+          else bv.store(yr);
+        }
+        if (!more) break;
+#pragma unroll
+        for (int i = 0; i < 16; i++) out[i] = 0.0f;
+        bv = bn;
       }
-      if (!more) break;
 #pragma unroll
-      for (int i = 0; i < 16; i++) out[i] = 0.0f;
-      bv = bn;
+      for (int j = 0; j < 2 * RT; j++) wv[j] = wn[j];
+      cb = cb1;
+      a = a1;
+      sc = sc1;
     }
-#pragma unroll
-    for (int j = 0; j < 2 * RT; j++) wv[j] = wn[j];
-    cb = cb1;
-    a = a1;
-    sc = sc1;
   }
+};
+
+// Launch order -> item: each XCD on a contiguous run of (tokens, slice) items,
+// so that the slices of some tokens share x and A in its L2, and neighbouring
+// tokens their adapters.
+__device__ __forceinline__ uint32_t item_of(uint32_t block, uint32_t n) {
+  const uint32_t xcd = block % 8;
+  return xcd * (n / 8) + min(xcd, n % 8) + block / 8;
+}
+
+// Steps of a group by register budget: 128 registers a lane with 16 waves, 256
+// with 8.
+constexpr int steps_for(int waves, int RT, int x_size) {
+  return RT == 8 ? 1 : x_size == 4 || RT == 4 || (RT == 2 && waves == 16) ? 2 : 4;
+}
+
+template <class W, class X, class Y, int RT, int TOK>
+__global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call c) {
+  constexpr int WAVES = waves_for(TOK, RT);
+  constexpr int RP = 16 * RT, PITCH = RP + 4;  // floats per token in LDS
+  constexpr bool DOT = TOK == 1 && sizeof(X) == 4;
+  __shared__ __align__(16) float part[WAVES][TOK][PITCH];
+  __shared__ __align__(16) float u[TOK][PITCH];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+  const int col = lane & 15, at = TOK == 1 ? 0 : col;  // at: the column's token of the block
+  const uint32_t item = item_of(blockIdx.x, gridDim.x), tile = item / c.slices;
+  const int slice = item % c.slices;
+  const int last = min(c.nb, (slice + 1) * c.per), cb0 = slice * c.per + wave;
+  Tokens tk;
+  tk.find((int64_t)tile * TOK + at, c.T, c.ids);
+  Shrink<W, X, RT, WAVES, steps_for(WAVES, RT, sizeof(X)), DOT> sh;
+  sh.begin(c, tk, wave);
+  Expand<W, Y, RT, WAVES> ex;
+  ex.begin(c, tk, cb0, last);
+  tk.settle(c.count);
+  sh.run(c, tk);
+  ex.ahead(c, tk, cb0, last);
+  Parts<W, RT, parts_for<W, Y>()> pu;
+  if (tk.mine) {  // of the block: every wave has the same tokens
+    if constexpr (DOT) {
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
+        float s = sh.acc[r][0] + __shfl_xor(sh.acc[r][0], 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        if (g == 0) part[wave][0][16 * r + col] = s;
+      }
+    } else if (TOK == 16 || col == 0)
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+        *reinterpret_cast<f4v *>(&part[wave][at][16 * r + 4 * g]) = sh.acc[r];
+    __syncthreads();
+    for (int i = tid; i < TOK * RP; i += 64 * WAVES) {
+      const int t = i / RP, r = i % RP;
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; w++) s += part[w][t][r];
+      u[t][r] = s;
+    }
+    __syncthreads();
+    __align__(16) float v[4 * RT];
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+      *reinterpret_cast<f4v *>(&v[4 * r]) =
+          *reinterpret_cast<const f4v *>(&u[at][4 * RT * g + 4 * r]);
+    pu.split(v);
+  }
+  ex.run(c, tk, pu, cb0, last, TOK == 16 || col == 0);
 }
 
 // A and B of one adapter into the layouts above, a thread per 16 bytes.
@@ -494,7 +573,7 @@ template <class W, class X, class Y>
 void launch(const hy3x_adapters *h, const int32_t *ids, const void *x, int64_t x_stride,
             const void *base, int64_t base_stride, void *y, int64_t y_stride, int T,
             hipStream_t st) {
-  Call<X, Y> c;
+  Call c;
   c.a = h->a;
   c.b = h->b;
   c.scale = h->scale;
@@ -504,26 +583,27 @@ void launch(const hy3x_adapters *h, const int32_t *ids, const void *x, int64_t x
   c.d_in = h->d_in;
   c.d_out = h->d_out;
   c.ids = ids;
-  c.x = (const X *)x;
-  c.base = (const Y *)base;
-  c.y = (Y *)y;
+  c.x = x;
+  c.base = base;
+  c.y = y;
   c.x_stride = x_stride;
   c.base_stride = base_stride;
   c.y_stride = y_stride;
   c.T = T;
+  auto slice = [&](int tiles) {
+    const int slices = std::max(1, std::min(c.nb, TARGET_BLOCKS / tiles));
+    c.per = (c.nb + slices - 1) / slices;
+    c.slices = (c.nb + c.per - 1) / c.per;
+    return dim3((uint32_t)tiles * c.slices);
+  };
   const bool single = T <= SINGLE_MAX_T;
-  const int tiles = single ? T : (T + 15) / 16;
-  const int slices = std::max(1, std::min(c.nb, TARGET_BLOCKS / tiles));
-  c.per = (c.nb + slices - 1) / slices;
-  c.slices = (c.nb + c.per - 1) / c.per;
-  const dim3 grid((uint32_t)tiles * c.slices), block(64 * waves_for(single ? 1 : 16, h->rp / 16));
-#define HY3X_ADAPTERS(RT)                                    \
-  if (h->rp == 16 * RT) {                                    \
-    if (single)                                              \
-      k_adapters<W, X, Y, RT, 1><<<grid, block, 0, st>>>(c); \
-    else                                                     \
-      k_adapters<W, X, Y, RT, 16><<<grid, block, 0, st>>>(c); \
-    return;                                                  \
+#define HY3X_ADAPTERS(RT)                                                                       \
+  if (h->rp == 16 * RT) {                                                                       \
+    if (single)                                                                                 \
+      k_adapters<W, X, Y, RT, 1><<<slice(T), 64 * waves_for(1, RT), 0, st>>>(c);                \
+    else                                                                                        \
+      k_adapters<W, X, Y, RT, 16><<<slice((T + 15) / 16), 64 * waves_for(16, RT), 0, st>>>(c);  \
+    return;                                                                                     \
   }
   HY3X_ADAPTERS(1)
   HY3X_ADAPTERS(2)
