@@ -85,6 +85,13 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
+// Lane i's value, i the same in all lanes.
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int i) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, i);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), i);
+  return (uint64_t)hi << 32 | lo;
+}
+
 // One row as its wave reads it.
 template <class T>
 struct Row {
@@ -166,7 +173,7 @@ __device__ __forceinline__ int groups64(const hy3x_route_spec &spec, const Row<T
   const uint64_t best = !live ? GONE<uint64_t> : ordered(top2 && live > 1 ? b0 + b1 : b0);
   int before = 0;
   for (int g = 0; g < spec.n_group; g++) {
-    const uint64_t o = __shfl(best, g << L.shift, 64);
+    const uint64_t o = lane_of(best, g << L.shift);
     before += o > best || (o == best && g < L.group);
   }
   return before;
@@ -219,16 +226,16 @@ __device__ __forceinline__ float margin(bool softmax, float most, float key) {
 }
 
 // Weights of the chosen experts (lane k: the k-th) and the row's outputs.
-// sum: the softmax's. fp32, except where a score lies near or below its normal
+// sum: the softmax's; live, l: the expert is not masked, its logit. fp32, except where a score lies near or below its normal
 // numbers.
 template <class T>
 __device__ __forceinline__ void finish(const hy3x_route_spec &spec, const Row<T> &row,
-                                       const Lanes &L, float sum, int mine, int64_t t,
-                                       int32_t *ids, float *w) {
+                                       const Lanes &L, float sum, int mine, bool live, float l,
+                                       int64_t t, int32_t *ids, float *w) {
   static_assert(HY3X_ROUTE_MAX_K <= 16, "a row of 16 lanes holds the chosen");
   const int lane = L.lane, K = spec.k;
-  const bool live = lane < K && !row.masked(mine);
-  const float x = live ? row.logit(mine) - (row.softmax ? row.top : 0.0f) : 0.0f;
+  live = live && lane < K;
+  const float x = live ? l - (row.softmax ? row.top : 0.0f) : 0.0f;
   float v = 0.0f;
   if (__ballot(x < -80.0f)) {
     const double s64 = sum64(row, L);
@@ -353,6 +360,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_route_experts(
   // rounds of the largest key left: lane k receives the k-th and its expert
   uint32_t my_key = GONE<uint32_t>;
   int mine = 0;
+  float my_l = 0.0f;  // its logit
   auto round = [&](int k) {
     uint32_t v = key[0];
 #pragma unroll
@@ -409,15 +417,19 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_route_experts(
 #pragma unroll
     for (int j = 0; j < V; j++) {
       const bool hit = (uint32_t)__shfl((int)key[j], from, 64) == my_key;
+      const float lj = __shfl(l[j], from, 64);
+      my_l = hit && seen == nth ? lj : my_l;
       slot = hit && seen == nth ? j : slot;
       seen += hit;
     }
     mine = __shfl(L.first, from, 64) + slot;
   } else {
     for (int k = 0; k < K; k++) kth = round(k);
+    my_l = row.logit(mine);
 #pragma unroll
     for (int j = 0; j < V; j++) head = max(head, key[j]);
   }
+  bool live = my_key > MASKED<uint32_t>;
   if (bias) {
     // close to the next chosen, or left over and close to the last
     const float edge = margin(softmax, most, number(kth));
@@ -435,7 +447,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_route_experts(
           for (int j = 0; j < V; j++) key[j] = e == L.first + j && j < L.n ? GONE<uint32_t> : key[j];
         }
       // experts of the same logit and bias are equal in any arithmetic
-      const float lm = row.logit(mine), bm = bias[mine];
+      const float lm = my_l, bm = bias[mine];
       const float ln = __shfl(lm, lane + 1, 64), bn = __shfl(bm, lane + 1, 64);
       const float lk = __shfl(lm, K - 1, 64), bk = __shfl(bm, K - 1, 64);
       bool any = close && (lm != ln || bm != bn);
@@ -454,16 +466,18 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_route_experts(
           const uint64_t k64 = lane < n ? row.key64(mine, s64) : GONE<uint64_t>;
           int rank = lane < n ? 0 : lane;
           for (int i = 0; i < n; i++) {
-            const uint64_t o = __shfl(k64, i, 64);
-            const int oe = __shfl(mine, i, 64);
+            const uint64_t o = lane_of(k64, i);
+            const int oe = __builtin_amdgcn_readlane(mine, i);
             if (lane < n) rank += o > k64 || (o == k64 && oe < mine);
           }
           mine = __builtin_amdgcn_ds_permute(4 * rank, mine);
         }
+        my_l = row.logit(mine);
+        live = !row.masked(mine);
       }
     }
   }
-  finish(spec, row, L, sum, mine, t, ids, w);
+  finish(spec, row, L, sum, mine, live, my_l, t, ids, w);
 }
 
 template <class T>
