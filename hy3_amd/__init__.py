@@ -261,6 +261,8 @@ class Adapters:
         if not on_device:
             a, b = np.ascontiguousarray(a), np.ascontiguousarray(b)
             assert a.nbytes == 2 * self.rank * self.d_in and b.nbytes == 2 * self.rank * self.d_out
+        elif hasattr(a, "is_contiguous"):
+            assert a.is_contiguous() and b.is_contiguous()
         _check(lib().hy3x_adapters_set(self._h, index, _ptr(a), _ptr(b), scale,
                                        1 if on_device else 0))
 

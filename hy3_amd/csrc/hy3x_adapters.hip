@@ -159,7 +159,7 @@ __device__ __forceinline__ f4v mma(const Run<W, 8> &a, const Run<float, 8> &b, f
 struct Call {
   const uint16_t *a, *b;
   const float *scale;
-  int count, kt, nb, d_in, d_out;  // kt = kp / 32, nb = np / 64
+  int count, rank, kt, nb, d_in, d_out;  // kt = kp / 32, nb = np / 64
   const int32_t *ids;
   const void *x, *base;  // rows in the kernel's X and Y
   void *y;
@@ -526,7 +526,7 @@ __global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call
       float s = 0.0f;
 #pragma unroll
       for (int w = 0; w < WAVES; w++) s += part[w][t][r];
-      u[t][r] = s;
+      u[t][r] = r < c.rank ? s : 0.0f;  // an infinite x makes NaNs of the padding's zeros
     }
     __syncthreads();
     __align__(16) float v[4 * RT];
@@ -539,15 +539,17 @@ __global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call
   ex.run(c, tk, pu, cb0, last, TOK == 16 || col == 0);
 }
 
-// A and B of one adapter into the layouts above, a thread per 16 bytes.
+// A, B and scale of one adapter into the handle, a thread per 16 bytes.
 __global__ __launch_bounds__(256) void k_pack_adapter(const uint16_t *__restrict__ a,
                                                       const uint16_t *__restrict__ b, int rank,
                                                       int d_in, int d_out, int rp, int kt, int nb,
                                                       uint16_t *__restrict__ pa,
-                                                      uint16_t *__restrict__ pb) {
+                                                      uint16_t *__restrict__ pb,
+                                                      float scale, float *__restrict__ pscale) {
   const int rt = rp / 16, na = kt * rt * 64, nbl = nb * 2 * rt * 64;
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i >= na + nbl) return;
+  if (i == 0) *pscale = scale;
   uint16_t v[8];
   if (i < na) {
     const int lane = i & 63, r = 16 * ((i >> 6) % rt) + lane % 16;
@@ -578,6 +580,7 @@ void launch(const hy3x_adapters *h, const int32_t *ids, const void *x, int64_t x
   c.b = h->b;
   c.scale = h->scale;
   c.count = h->count;
+  c.rank = h->rank;
   c.kt = h->kp / 32;
   c.nb = h->np / 64;
   c.d_in = h->d_in;
@@ -754,9 +757,9 @@ int hy3x_adapters_set(hy3x_adapters *h, int index, const void *a, const void *b,
   const int n = (kt + 2 * ob) * (h->rp / 16) * 64;
   k_pack_adapter<<<(n + 255) / 256, 256>>>(
       (const uint16_t *)a, (const uint16_t *)b, h->rank, h->d_in, h->d_out, h->rp, kt, ob,
-      h->a + (size_t)index * h->rp * h->kp, h->b + (size_t)index * h->rp * h->np);
+      h->a + (size_t)index * h->rp * h->kp, h->b + (size_t)index * h->rp * h->np, scale,
+      h->scale + index);
   OP_HIP_TRY(hipGetLastError());
-  OP_HIP_TRY(hipMemcpy(h->scale + index, &scale, sizeof(float), hipMemcpyHostToDevice));
   OP_HIP_TRY(hipDeviceSynchronize());
   return HY3X_OK;
 }

@@ -549,14 +549,25 @@ extern "C" int hy3x_route_experts(const hy3x_route_spec *spec, const void *logit
     return op_fail(HY3X_E_ARG, "logits type %d unknown", type);
   if (T < 0 || T > HY3X_ROUTE_MAX_TOKENS)
     return op_fail(HY3X_E_ARG, "T=%d outside [0,%d]", T, HY3X_ROUTE_MAX_TOKENS);
-  if (row_stride < spec->n_expert)
-    return op_fail(HY3X_E_ARG, "row_stride %lld below n_expert %d", (long long)row_stride,
-                   spec->n_expert);
+  if (row_stride < spec->n_expert || row_stride > (int64_t)1 << 32)
+    return op_fail(HY3X_E_ARG, "row_stride %lld outside [n_expert %d, 2^32]",
+                   (long long)row_stride, spec->n_expert);
   if (T == 0) return HY3X_OK;
   if (!logits || !ids || !w) return op_fail(HY3X_E_ARG, "NULL logits, ids or w");
   const size_t size = type == HY3X_F32 ? 4 : 2;
   if ((uintptr_t)logits % size || (uintptr_t)bias % 4 || (uintptr_t)ids % 4 || (uintptr_t)w % 4)
     return op_fail(HY3X_E_ARG, "a pointer is not aligned to its elements");
+  // no output may lie on anything else
+  struct Span {
+    uintptr_t at, end;
+    Span(const void *p, int64_t bytes) : at((uintptr_t)p), end(at + (p ? (uintptr_t)bytes : 0)) {}
+    bool meets(const Span &o) const { return at < o.end && o.at < end; }
+  };
+  const int64_t chosen = (int64_t)T * spec->k * 4;
+  const Span in(logits, ((int64_t)(T - 1) * row_stride + spec->n_expert) * (int64_t)size),
+      by(bias, 4 * spec->n_expert), i(ids, chosen), o(w, chosen);
+  if (i.meets(in) || i.meets(by) || i.meets(o) || o.meets(in) || o.meets(by))
+    return op_fail(HY3X_E_ARG, "ids or w overlaps another buffer");
   launch_route(*spec, logits, type, row_stride, bias, T, ids, w, (hipStream_t)stream);
   OP_HIP_TRY(hipGetLastError());
   return HY3X_OK;

@@ -305,7 +305,7 @@ typedef struct hy3x_route_spec {
  *    row with nothing left gets the first k experts with weights 0.
  *  - A logit of +inf counts as the largest finite value of its type.
  * logits: device [T rows of E elements], `type` HY3X_F32 / F16 / BF16, rows
- * row_stride elements apart (>= E); bias: device fp32 [E] or NULL; ids, w:
+ * row_stride elements apart (E .. 2^32); bias: device fp32 [E] or NULL; ids, w:
  * device, dense, overlapping nothing else. T = 0 does nothing. No allocation,
  * no scratch: calls on any streams may overlap, and a call may be captured
  * into a graph. stream: a hipStream_t of the current device (NULL = default
@@ -342,9 +342,12 @@ int hy3x_adapters_set(hy3x_adapters *adapters, int index, const void *a, const v
  * (same pointer and stride: added in place); otherwise y may overlap neither x
  * nor base (rows of one wider buffer may lie between each other).
  * x: device [T x d_in], x_type HY3X_F32 or the handle's type; base, y: device
- * [T x d_out], y_type HY3X_F32 or the handle's type; strides in elements, at
- * least the row length. Sums are fp32; y is rounded once; tokens do not affect
- * each other's results, whatever their adapters hold. T = 0 does nothing. The
+ * [T x d_out], y_type HY3X_F32 or the handle's type; strides in elements, from
+ * the row length to 2^32. Sums are fp32; y is rounded once; tokens do not affect
+ * each other's results, whatever their adapters hold. Up to 256 tokens each takes
+ * its own adapter at the same cost; more run in tiles of 16 consecutive tokens
+ * that cost as much again for each further adapter in them, so keep a request's
+ * tokens together. T = 0 does nothing. The
  * handle's device must be current. No allocation, no scratch: calls on one
  * handle may overlap, and a call may be captured into a graph.
  * stream: a hipStream_t of the handle's device (NULL = default stream).

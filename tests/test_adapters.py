@@ -217,6 +217,53 @@ def test_tokens_do_not_affect_each_other(torch, dtype, T):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rank", [1, 5, 16])
+def test_infinities_as_the_formula_has_them(torch, dtype, rank):
+    """An infinite x: each output infinite or NaN as in 64 bits, ranks padded or not."""
+    s = Setup(torch, 2, rank, 70, 66, dtype)
+    for T in (4, 300):
+        for xt, yt in io_types(dtype):
+            x, base, ids = s.inputs(T, xt, yt)
+            ids = ids.clamp(min=0)
+            x[:, 7] = float("inf")
+            with np.errstate(invalid="ignore"):
+                want, _ = s.expect(x, base, ids)
+            got = s.apply(x, base, ids, xt, yt).double().numpy()
+            assert np.array_equal(np.isnan(got), np.isnan(want))
+            assert np.array_equal(got[~np.isnan(got)], want[~np.isnan(want)])
+    s.h.close()
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_2_31(torch):
+    """Adapters, rows of x and rows of y more than 2^31 elements from the first."""
+    h = H.Adapters(4200, 128, 4096, 64, "bf16")  # 2.2e9 elements of A
+    g = torch.Generator().manual_seed(1)
+    a = (torch.randn(128, 4096, generator=g) / 64).bfloat16()
+    b = torch.randn(64, 128, generator=g).bfloat16()
+    h.set(4199, a.cuda(), b.cuda(), 1.0, on_device=True)
+    step = (1 << 31) + 8
+    x, y = torch.randn(2, 4096, generator=g).bfloat16(), torch.empty(2, 64)
+    buf = torch.empty(step + 4096, dtype=torch.bfloat16, device="cuda")
+    out = torch.empty(step + 64, dtype=torch.bfloat16, device="cuda")
+    buf[:4096], buf[step:] = x[0].cuda(), x[1].cuda()
+    for ids in ([4199, 4199], [0, 4199]):
+        h.apply(torch.tensor(ids, dtype=torch.int32).cuda(), buf, out, 2, x_stride=step,
+                y_stride=step)
+        torch.cuda.synchronize()
+        y[0], y[1] = out[:64].cpu().float(), out[step:].cpu().float()
+        u = x.double() @ a.double().t()
+        want = u @ b.double().t()
+        S = (x.double().abs() @ a.double().abs().t()) @ b.double().abs().t()
+        tol = (4096 / 32 + 128 + 48) * HALF * S + 2.0 ** -8 * want.abs()
+        if ids[0] == 0:
+            want[0], tol[0] = 0.0, 0.0
+        assert ((y.double() - want).abs() <= tol).all()
+    h.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_wide_range(torch, dtype):
     """Rows of very large and very small values: u keeps fp32's range between the
     two products, whatever the weights' type holds."""

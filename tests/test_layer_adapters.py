@@ -251,6 +251,35 @@ def test_without_an_adapter_the_block_is_as_it_was(block, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 6])
+def test_no_adapters_set(block, T):
+    x = C.inputs(0xAA, T)
+    y0, ids0, _, _ = block.run(x)
+    y, ids, _, _ = block.run(x, [0] * T)  # ids name adapters of no projection
+    assert np.array_equal(y, y0) and np.array_equal(ids, ids0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 9, 64])
+def test_rule_on_the_static_scratch_and_the_gemv_path(block, T):
+    torch, layer = block.torch, block.layer
+    x = C.inputs(0xAB, T)
+    layer.set_routing(H.RouteSpec(E, 1, "softmax", 4, 2, "top2"))
+    y0, ids0, wpre0, _ = block.run(x)
+    xd = torch.from_numpy(x.copy()).cuda()
+    layer.forward_static(xd.data_ptr(), T)
+    torch.cuda.synchronize()
+    ids, wpre, _ = layer.last_routing()
+    assert np.array_equal(xd.cpu().numpy(), y0)
+    assert np.array_equal(ids, ids0) and np.array_equal(wpre, wpre0)
+    if not block.shared_q8:
+        layer.set_path(1)
+        y1, ids1, wpre1, _ = block.run(x)
+        assert np.array_equal(ids1, ids0) and np.array_equal(wpre1, wpre0)
+        assert O.rel_l2(y1 - x, y0 - x) <= TOL
+
+
+@pytest.mark.gpu
 def test_residual_and_two_layers_with_one_scratch(torch):
     b = Block(torch)
     other = H.MoELayer(0, share_scratch_with=b.layer)

@@ -78,12 +78,17 @@ def test_argument_refusals():
                                       bias, T, ids, w, None)
     assert call(spec=None) == -1
     assert call(dtype=3) == -1 and call(dtype=-1) == -1
-    assert call(stride=191) == -1
+    assert call(stride=191) == -1 and call(stride=(1 << 32) + 1) == -1
     assert call(T=-1) == -1 and call(T=(1 << 24) + 1) == -1
     assert call(logits=None) == -1 and call(ids=None) == -1 and call(w=None) == -1
     assert call(logits=4098) == -1 and call(bias=4097) == -1
     assert call(ids=4097) == -1 and call(w=4098) == -1
     assert b"aligned" in lib.hy3x_last_error()
+    far = dict(ids=1 << 20, w=2 << 20)  # 8 x 4 bytes each
+    for bad in (dict(w=(1 << 20) + 28), dict(ids=4096 + 188 * 4), dict(w=4096), dict(logits=(2 << 20) + 4),
+                dict(bias=(1 << 20) - 4), dict(T=3, ids=4096 + 2 * 192 * 4)):
+        assert call(**dict(far, **bad)) == -1, bad
+        assert b"overlaps" in lib.hy3x_last_error()
     for field in ("score", "group_score"):
         bad = H.RouteSpec(**GOOD)
         setattr(bad, field, 2)
@@ -236,6 +241,20 @@ def test_keys_closer_than_fp32(torch):
         for groups, best in ((1, "max"), (8, "max"), (8, "top2")):
             check(torch, H.RouteSpec(E, 8, score, groups, max(1, groups // 2), best), logits, "f32",
                   bias)
+
+
+@pytest.mark.gpu
+def test_rows_more_than_2_31_elements_apart(torch):
+    E, stride, k = 192, (1 << 31) + 5, 8
+    logits = make(torch, 2, E, "bf16", 4)
+    buf = torch.empty(stride + E, dtype=torch.bfloat16, device="cuda")
+    buf[:E], buf[stride:] = logits[0].cuda(), logits[1].cuda()
+    ids = torch.empty(2, k, dtype=torch.int32, device="cuda")
+    w = torch.empty(2, k, device="cuda")
+    H.route_experts(H.RouteSpec(E, k), buf, 2, ids, w, dtype="bf16", row_stride=stride)
+    torch.cuda.synchronize()
+    want, _ = run(torch, H.RouteSpec(E, k), logits, "bf16")
+    assert np.array_equal(ids.cpu().numpy(), want)
 
 
 @pytest.mark.gpu
