@@ -7,7 +7,10 @@
 // One launch: a block takes TOK tokens and a slice of their outputs, and forms
 // u for itself, so nothing passes between blocks: no scratch memory, no second
 // launch, no order of blocks in the results. Its waves split d_in, join their
-// parts of u in LDS, then split the outputs.
+// parts of u in LDS, then split the outputs. (Two launches over scratch, the
+// parts of u by blocks of their own and A and B read for 32 tokens at a time,
+// measured 39.0 us against 36.1 at 4096 x 4096 outputs of rank 64, 18.9 against
+// 17.4 at 512 tokens in fp32.)
 //
 // TOK = 16: 16 consecutive tokens, the columns of every MFMA. The adapters that
 // occur among them are taken one after another: each forms its products for all
@@ -16,8 +19,18 @@
 // token in every column.
 //
 // Products. u: v_mfma_f32_16x16x32_{f16,bf16} (rows = 16 ranks, columns =
-// tokens) where x has the weights' type, v_mfma_f32_16x16x4_f32 where x is
-// fp32. B u: v_mfma_f32_16x16x4_f32, as u has fp32's range and precision.
+// tokens) where x has the weights' type; where x is fp32, v_mfma_f32_16x16x4_f32,
+// or fp32 FMAs for one token. B u: the two-byte MFMAs on u in two or three parts
+// (Parts), which keep fp32's range and precision.
+//
+// What bounds it (us of the kernel, inputs and weights from HBM, MI355X): many
+// tokens the bytes of x, base and y, 16-token tiles with two adapters last (4096
+// x 4096 outputs of 4096 inputs, rank 64: 36 us for 111 MB, 3.1 TB/s; rank 16,
+// 2000 tokens: 16.3 us for 53 MB, 3.2 TB/s); up to 256 decoded tokens the adapters'
+// weights (256 tokens, 128 adapters: 13.7 us for 40 MB, 2.9 TB/s); a few tokens
+// four loads that wait for each other, ids, A, B, the store (32 tokens: 6.0 us;
+// one token beside the router: 6.0 us); fp32 x the fp32 MFMAs (512 tokens, 1536
+// inputs, rank 32: 16.2 us).
 //
 // Weights as the MFMAs read them, one coalesced 16-byte load per lane:
 //   A  [count][kp / 32][rank tile][lane][8]: rank 16 rt + lane % 16, k = 32 kt
@@ -54,15 +67,21 @@ typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef _Float16 h4v __attribute__((ext_vector_type(4)));
 typedef short s4v __attribute__((ext_vector_type(4)));
 
-#ifndef TB
-#define TB 256
-#endif
+// Waves of a block: 16 where 128 registers a lane hold the operands in flight
+// (512 tokens, fp32, rank 32: 16.9 us with 8 waves, 15.6 with 16; one token beside
+// the router 9.0 and 7.8), 8 above.
 constexpr int waves_for(int TOK, int RT) { return RT == 1 || (RT == 2 && TOK == 16) ? 16 : 8; }
-#ifndef SMT
-#define SMT 256
-#endif
-constexpr int SINGLE_MAX_T = SMT;   // up to this many tokens a block takes one token
-constexpr int TARGET_BLOCKS = TB;  // blocks that the slices are made for
+// Up to this many tokens, one per CU, a block takes one token and the order of the
+// adapters does not matter; above, tiles of 16. us, one token per block and tiles,
+// 4096 -> 4096 of rank 16 in bf16, every token another adapter | runs of 100:
+//   64 tokens 7.0 and 38.9 | 6.6 and 8.1     256: 13.2 and 39.5 | 10.2 and 9.8
+//   320 (a second round of blocks): 21.0 and 38.9 | 18.4 and 10.4
+//   1024: 45.1 and 44.2 | 36.6 and 12.6
+constexpr int SINGLE_MAX_T = 256;
+// Blocks that the outputs are sliced for: one per CU. More slices form u again
+// (512 blocks: 32 decoded tokens 10.2 us against 6.4, 512 in fp32 25.8 against
+// 17.8, 2000 20.6 against 18.7, 4096 of rank 64 48.5 against 42.2).
+constexpr int TARGET_BLOCKS = 256;
 
 __device__ __forceinline__ float elem(float v) { return v; }
 __device__ __forceinline__ float elem(__half v) { return __half2float(v); }
