@@ -399,29 +399,69 @@ struct Parts {
   }
 };
 
+// Where a lane's 16 outputs of a block of 64 lie: two-byte ones in one run of 16
+// (32 bytes), fp32 ones in four runs of 4, 16 apart, so that the four lanes of a
+// token write 64 bytes at a time (4096 x 4096 fp32 outputs, rank 64: 67.0 us, in one
+// run of 64 bytes per lane 76.0; the same without adapters 33.1 and 63.7).
+template <class Y>
+struct Place {
+  static constexpr int RUN = sizeof(Y) == 4 ? 4 : 16, N = 16 / RUN;
+  static __device__ __forceinline__ int col(int g, int k) {  // of run k
+    return sizeof(Y) == 4 ? 16 * k + 4 * g : 16 * g;
+  }
+};
+
 // The outputs cb0, cb0 + WAVES, .. (blocks of 64) below `last` of the wave's
 // tokens, and for each the adapters of these tokens one after another; the next
 // step's operands in flight through this one's products.
 template <class W, class Y, int RT, int WAVES>
 struct Expand {
-  Run<Y, 16> bv, bn;
+  using P = Place<Y>;
+  using Piece = Run<Y, P::RUN>;
+  Piece bv[P::N], bn[P::N];
   Run<W, 8> wv[2 * RT], wn[2 * RT];
   const Y *br;
 
-  __device__ __forceinline__ void load_base(const Call &c, Run<Y, 16> &v, int cb) const {
-    const int c0 = 64 * cb + 16 * ((threadIdx.x & 63) >> 4);
-    if (br && 64 * cb + 64 <= c.d_out) v.load(br + c0);
-    else if (br) v.load_part(br, c0, c.d_out);
-    else
+  __device__ __forceinline__ void load_base(const Call &c, Piece (&v)[P::N], int cb) const {
+    const int g = (threadIdx.x & 63) >> 4;
+    const bool whole = 64 * cb + 64 <= c.d_out;
 #pragma unroll
-      for (int i = 0; i < 16; i++) v.set(i, 0.0f);
+    for (int k = 0; k < P::N; k++) {
+      const int c0 = 64 * cb + P::col(g, k);
+      if (br && whole) v[k].load(br + c0);
+      else if (br) v[k].load_part(br, c0, c.d_out);
+      else
+#pragma unroll
+        for (int i = 0; i < P::RUN; i++) v[k].set(i, 0.0f);
+    }
   }
+  // B's rows as the MFMAs of these places read them: row m of MFMA q is output
+  // 16 (m / 4) + 4 q + m % 4, as B is laid out, or output 16 q + m, which lies with
+  // lane 4 q + m % 4 as its part m / 4
   __device__ __forceinline__ void load_b(const Call &c, Run<W, 8> (&v)[2 * RT], int a,
                                          int cb) const {
-    const W *bw = (const W *)c.b +
-                  (((int64_t)a * c.nb + cb) * 2 * RT * 64 + (threadIdx.x & 63)) * 8;
+    const int lane = threadIdx.x & 63;
+    const W *bw = (const W *)c.b + ((int64_t)a * c.nb + cb) * 2 * RT * 512;
+    if constexpr (sizeof(Y) == 2) {
 #pragma unroll
-    for (int j = 0; j < 2 * RT; j++) v[j].load(bw + j * 512);
+      for (int j = 0; j < 2 * RT; j++) v[j].load(bw + j * 512 + lane * 8);
+    } else {
+      const int part = (lane & 15) >> 2;
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const int from = (lane & 48) + 4 * q + (lane & 3);
+        if constexpr (RT == 1) {
+          Run<W, 4> h;
+          h.load(bw + (part >> 1) * 512 + from * 8 + (part & 1) * 4);
+          v[q / 2].w[q % 2 * 2] = h.w[0];
+          v[q / 2].w[q % 2 * 2 + 1] = h.w[1];
+        } else {
+#pragma unroll
+          for (int j = 0; j < RT / 2; j++)
+            v[q * (RT / 2) + j].load(bw + (part * (RT / 2) + j) * 512 + from * 8);
+        }
+      }
+    }
   }
   // the base of the first outputs, which needs no adapter yet
   __device__ __forceinline__ void begin(const Call &c, const Tokens &tk, int cb0, int last) {
@@ -433,8 +473,8 @@ struct Expand {
     uint64_t rest = tk.mine;
     if (rest && cb0 < last) load_b(c, wv, tk.pick(rest), cb0);
   }
-  template <class P>
-  __device__ __forceinline__ void run(const Call &c, const Tokens &tk, const P &u, int cb0,
+  template <class U>
+  __device__ __forceinline__ void run(const Call &c, const Tokens &tk, const U &u, int cb0,
                                       int last, bool stores) {
     if (cb0 >= last) return;
     uint64_t rest = tk.mine;
@@ -467,20 +507,25 @@ struct Expand {
             out[4 * q + i] = tk.id == a ? sc * (u.back * acc[i]) : out[4 * q + i];
         }
       if (done) {
-        const int c0 = 64 * cb + 16 * ((threadIdx.x & 63) >> 4);
+        const int g = (threadIdx.x & 63) >> 4;
+        Y *yr = (Y *)c.y + tk.row * c.y_stride;
 #pragma unroll
-        for (int i = 0; i < 16; i++) out[i] += bv.at(i);
+        for (int k = 0; k < P::N; k++) {
+          float sum[P::RUN];
 #pragma unroll
-        for (int i = 0; i < 16; i++) bv.set(i, out[i]);
-        if (tk.in && stores) {
-          Y *yr = (Y *)c.y + tk.row * c.y_stride + c0;
-          if (64 * cb + 64 > c.d_out) bv.store_part(yr, c.d_out - c0);
-          else bv.store(yr);
+          for (int i = 0; i < P::RUN; i++) sum[i] = out[P::RUN * k + i] + bv[k].at(i);
+#pragma unroll
+          for (int i = 0; i < P::RUN; i++) bv[k].set(i, sum[i]);
+          const int c0 = 64 * cb + P::col(g, k);
+          if (!tk.in || !stores) continue;
+          if (64 * cb + 64 > c.d_out) bv[k].store_part(yr + c0, c.d_out - c0);
+          else bv[k].store(yr + c0);
         }
         if (!more) break;
 #pragma unroll
         for (int i = 0; i < 16; i++) out[i] = 0.0f;
-        bv = bn;
+#pragma unroll
+        for (int k = 0; k < P::N; k++) bv[k] = bn[k];
       }
 #pragma unroll
       for (int j = 0; j < 2 * RT; j++) wv[j] = wn[j];
