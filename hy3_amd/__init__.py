@@ -213,7 +213,7 @@ class RouteSpec(ctypes.Structure):
 
 
 def _dev(a):
-    """_ptr of device memory, a tensor first: a small call's host time counts."""
+    """_ptr of device memory, a tensor first: the host's share of a small call counts."""
     try:
         return a.data_ptr()
     except AttributeError:
@@ -223,10 +223,16 @@ def _dev(a):
 def route_experts(spec, logits, T, ids, w, dtype="f32", row_stride=None, bias=None, stream=None):
     """ids [T x k] (int32) and w [T x k] (fp32) of T rows of logits in device memory
     (hy3x_route_experts)."""
-    rc = (_lib or lib()).hy3x_route_experts(
-        ctypes.byref(spec), _dev(logits), DTYPES[dtype],
-        spec.n_expert if row_stride is None else row_stride,
-        None if bias is None else _dev(bias), T, _dev(ids), _dev(w), stream)
+    if row_stride is None:
+        row_stride = spec.n_expert
+    if bias is not None:
+        bias = _dev(bias)
+    try:  # tensors, without a call of _dev for each
+        logits, ids, w = logits.data_ptr(), ids.data_ptr(), w.data_ptr()
+    except AttributeError:
+        logits, ids, w = _dev(logits), _dev(ids), _dev(w)
+    rc = (_lib or lib()).hy3x_route_experts(ctypes.byref(spec), logits, DTYPES[dtype], row_stride,
+                                            bias, T, ids, w, stream)
     if rc:
         _check(rc)
 
@@ -271,12 +277,17 @@ class Adapters:
         """y[t] = base[t] + the product of adapter ids[t] with x[t], on device memory
         (hy3x_adapters_apply). Types default to the adapters', strides to dense rows; no
         base: 0."""
-        rc = self._apply(
-            self._h, _dev(ids), _dev(x), DTYPES[x_dtype or self.dtype],
-            self.d_in if x_stride is None else x_stride, None if base is None else _dev(base),
-            self.d_out if base_stride is None else base_stride, _dev(y),
-            DTYPES[y_dtype or self.dtype], self.d_out if y_stride is None else y_stride, T,
-            stream)
+        if base is not None:
+            base = _dev(base)
+        try:  # tensors, without a call of _dev for each
+            ids, x, y = ids.data_ptr(), x.data_ptr(), y.data_ptr()
+        except AttributeError:
+            ids, x, y = _dev(ids), _dev(x), _dev(y)
+        rc = self._apply(self._h, ids, x, DTYPES[x_dtype or self.dtype],
+                         self.d_in if x_stride is None else x_stride, base,
+                         self.d_out if base_stride is None else base_stride, y,
+                         DTYPES[y_dtype or self.dtype],
+                         self.d_out if y_stride is None else y_stride, T, stream)
         if rc:
             _check(rc)
 
