@@ -217,12 +217,33 @@ def _dev(a):
     try:
         return a.data_ptr()
     except AttributeError:
+        if isinstance(a, np.ndarray):
+            raise TypeError("host memory where the kernels read device memory") from None
         return _ptr(a)
 
 
-def route_experts(spec, logits, T, ids, w, dtype="f32", row_stride=None, bias=None, stream=None):
+_KINDS = {"torch.float32": "f32", "torch.float16": "f16", "torch.bfloat16": "bf16"}
+
+
+def _kind(a, default, **others):
+    """The element type of a: a tensor's own, on the GPU and of a type that the operators
+    know, a pointer's the default. The others, name = (tensor, type): checked too."""
+    for name, (t, want) in others.items():
+        if hasattr(t, "data_ptr") and (not t.is_cuda or str(t.dtype) != "torch." + want):
+            raise TypeError(f"{name}: {t.dtype} on {t.device}, not {want} on the GPU")
+    if not hasattr(a, "data_ptr"):
+        return default
+    if not a.is_cuda or str(a.dtype) not in _KINDS:
+        raise TypeError(f"{a.dtype} on {a.device}, not f32, f16 or bf16 on the GPU")
+    return _KINDS[str(a.dtype)]
+
+
+def route_experts(spec, logits, T, ids, w, dtype=None, row_stride=None, bias=None, stream=None):
     """ids [T x k] (int32) and w [T x k] (fp32) of T rows of logits in device memory
-    (hy3x_route_experts)."""
+    (hy3x_route_experts). Without a dtype: the logits' own (of a pointer, "f32"), and the
+    tensors' types and places are checked, which takes the host about 1 us."""
+    if dtype is None:
+        dtype = _kind(logits, "f32", ids=(ids, "int32"), w=(w, "float32"), bias=(bias, "float32"))
     if row_stride is None:
         row_stride = spec.n_expert
     if bias is not None:
@@ -267,26 +288,33 @@ class Adapters:
         if not on_device:
             a, b = np.ascontiguousarray(a), np.ascontiguousarray(b)
             assert a.nbytes == 2 * self.rank * self.d_in and b.nbytes == 2 * self.rank * self.d_out
-        elif hasattr(a, "is_contiguous"):
-            assert a.is_contiguous() and b.is_contiguous()
-        _check(lib().hy3x_adapters_set(self._h, index, _ptr(a), _ptr(b), scale,
-                                       1 if on_device else 0))
+        else:
+            for t, n in ((a, self.rank * self.d_in), (b, self.rank * self.d_out)):
+                if hasattr(t, "data_ptr"):
+                    assert _kind(t, None) == self.dtype and t.numel() == n and t.is_contiguous()
+        a, b = (_dev(a), _dev(b)) if on_device else (_ptr(a), _ptr(b))
+        _check(lib().hy3x_adapters_set(self._h, index, a, b, scale, 1 if on_device else 0))
 
     def apply(self, ids, x, y, T, base=None, x_dtype=None, y_dtype=None, x_stride=None,
               base_stride=None, y_stride=None, stream=None):
         """y[t] = base[t] + the product of adapter ids[t] with x[t], on device memory
-        (hy3x_adapters_apply). Types default to the adapters', strides to dense rows; no
-        base: 0."""
+        (hy3x_adapters_apply). Types default to the tensors' own (of pointers, the adapters'),
+        which are then checked, as in route_experts; strides to dense rows; no base: 0."""
+        if x_dtype is None or y_dtype is None:
+            x_dtype = x_dtype or _kind(x, self.dtype, ids=(ids, "int32"))
+            y_dtype = y_dtype or _kind(y, self.dtype)
+            if base is not None and _kind(base, y_dtype) != y_dtype:
+                raise TypeError(f"base: {base.dtype}, y: {y_dtype}")
         if base is not None:
             base = _dev(base)
         try:  # tensors, without a call of _dev for each
             ids, x, y = ids.data_ptr(), x.data_ptr(), y.data_ptr()
         except AttributeError:
             ids, x, y = _dev(ids), _dev(x), _dev(y)
-        rc = self._apply(self._h, ids, x, DTYPES[x_dtype or self.dtype],
+        rc = self._apply(self._h, ids, x, DTYPES[x_dtype],
                          self.d_in if x_stride is None else x_stride, base,
                          self.d_out if base_stride is None else base_stride, y,
-                         DTYPES[y_dtype or self.dtype],
+                         DTYPES[y_dtype],
                          self.d_out if y_stride is None else y_stride, T, stream)
         if rc:
             _check(rc)
@@ -435,6 +463,8 @@ class MoELayer:
     def set_adapters(self, projection, adapters=None):
         """Adapters beside "router", "gate", "up" or "down" for forward_adapters, or none
         (hy3x_layer_set_adapters)."""
+        if adapters is not None and not adapters._h:
+            raise HY3XError("the adapters are closed")
         _check(lib().hy3x_layer_set_adapters(self._h, self.PROJECTIONS.index(projection),
                                              None if adapters is None else adapters._h))
         self._adapters = dict(getattr(self, "_adapters", {}), **{projection: adapters})
@@ -444,7 +474,7 @@ class MoELayer:
         """The block for tokens with adapters of their own, adapter_ids [T] int32 in device
         memory (hy3x_layer_forward_adapters)."""
         _check(lib().hy3x_layer_forward_adapters(self._h, x_dev_ptr, attn_dev_ptr,
-                                                 _ptr(adapter_ids), T, K, scale, stream))
+                                                 _dev(adapter_ids), T, K, scale, stream))
 
     def last_shape(self):
         """(T, K) of the last forward."""

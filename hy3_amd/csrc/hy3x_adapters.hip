@@ -847,6 +847,9 @@ int hy3x_adapters_apply(const hy3x_adapters *h, const int32_t *ids, const void *
   const int64_t xs = x_type == HY3X_F32 ? 4 : 2, ys = y_type == HY3X_F32 ? 4 : 2;
   if ((uintptr_t)ids % 4 || (uintptr_t)x % xs || (uintptr_t)y % ys || (uintptr_t)base % ys)
     return op_fail(HY3X_E_ARG, "a pointer is not aligned to its elements");
+  const uintptr_t i0 = (uintptr_t)ids, y0 = (uintptr_t)y;
+  if (i0 < y0 + (uintptr_t)(((T - 1) * y_stride + h->d_out) * ys) && y0 < i0 + (uintptr_t)T * 4)
+    return op_fail(HY3X_E_ARG, "y overlaps ids");
   if (overlap(x, x_stride * xs, h->d_in * xs, y, y_stride * ys, h->d_out * ys, T))
     return op_fail(HY3X_E_ARG, "y overlaps x");
   if (base && !(base == y && (base_stride == y_stride || T == 1)) &&

@@ -21,8 +21,16 @@
 // 64-bit keys, a lane each, and are ranked by counting (experts of the same
 // logit and bias need none: they are equal). A row with more candidates than
 // lanes is decided by 64-bit keys throughout (choose64). Groups whose scores are
-// that close at the border are scored in 64 bits (groups64). Without a bias the keys are the logits, which
-// are exact: no margin, and ties are ties.
+// that close at the border are scored in 64 bits (groups64). Without a bias the
+// keys are the logits, which are exact: no margin, and ties are ties.
+//
+// What bounds it (us of the kernel, MI355X): few rows the load and k rounds that
+// wait for each other (one row of 192: 3.0 us; 512: 4.4, its end a row with
+// candidates); many rows vector instructions, not bytes (4096 rows of 256 in 8
+// groups: 8.9 us, about 640 a row; 16383 of 251: 18.3 us, 518 a row, 10 MB). With
+// 64-bit keys for every row these were 8.2, 10.2, 22.8 and 48.7. A wave per row
+// in blocks of 4 waves: blocks of 1, 8 or 16 are no faster; waves that take rows in
+// turn, the next row's loads in flight, 10.4 and 22.4 at 4096 and 16383.
 #include <hip/hip_bf16.h>
 #include <math.h>
 
@@ -183,8 +191,7 @@ __device__ __forceinline__ int groups64(const hy3x_route_spec &spec, const Row<T
 // rows with more candidates than lanes. It forms every key again in each round
 // and keeps none.
 template <class T>
-__device__ __forceinline__ int choose64(const hy3x_route_spec spec, const Row<T> row,
-                                                  int v) {
+__device__ __forceinline__ int choose64(const hy3x_route_spec &spec, const Row<T> &row, int v) {
   const Lanes L(spec, v);
   const double sum = sum64(row, L);
   const bool stays = spec.n_group == 1 || groups64(spec, row, v) < spec.topk_group;
@@ -226,8 +233,8 @@ __device__ __forceinline__ float margin(bool softmax, float most, float key) {
 }
 
 // Weights of the chosen experts (lane k: the k-th) and the row's outputs.
-// sum: the softmax's; live, l: the expert is not masked, its logit. fp32, except where a score lies near or below its normal
-// numbers.
+// sum: the softmax's; live, l: the expert is not masked, its logit. fp32, except
+// where a score lies near or below its normal numbers.
 template <class T>
 __device__ __forceinline__ void finish(const hy3x_route_spec &spec, const Row<T> &row,
                                        const Lanes &L, float sum, int mine, bool live, float l,

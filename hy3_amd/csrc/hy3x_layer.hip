@@ -788,6 +788,9 @@ int hy3x_layer_forward_adapters(hy3x_layer *L, float *x, const float *attn_out,
   if ((uintptr_t)adapter_ids % 4) return fail(HY3X_E_ARG, "adapter_ids is not aligned");
   if (x && attn_out && T > 0 && overlaps(x, attn_out, T))
     return fail(HY3X_E_ARG, "attn_out overlaps x");
+  const uintptr_t i0 = (uintptr_t)adapter_ids, x0 = (uintptr_t)x;
+  if (x && T > 0 && i0 < x0 + (uintptr_t)T * D * sizeof(float) && x0 < i0 + (uintptr_t)T * 4)
+    return fail(HY3X_E_ARG, "adapter_ids overlaps x");
   return forward_impl(L, &L->own, &L->scratch_mem->owner, x, attn_out, T, K, scale, stream,
                       adapter_ids);
 }

@@ -340,7 +340,7 @@ int hy3x_adapters_set(hy3x_adapters *adapters, int index, const void *a, const v
  * int32[T]); a token whose id is outside [0, count) (-1, by convention) has no
  * adapter: y[t] = base[t]. base NULL: 0 in its place. base may be y itself
  * (same pointer and stride: added in place); otherwise y may overlap neither x
- * nor base (rows of one wider buffer may lie between each other).
+ * nor base (rows of one wider buffer may lie between each other), and never ids.
  * x: device [T x d_in], x_type HY3X_F32 or the handle's type; base, y: device
  * [T x d_out], y_type HY3X_F32 or the handle's type; strides in elements, from
  * the row length to 2^32. Sums are fp32; y is rounded once; tokens do not affect
@@ -382,10 +382,10 @@ int hy3x_layer_set_adapters(hy3x_layer *layer, int projection, const hy3x_adapte
 
 /* hy3x_layer_forward_residual (attn_out NULL: hy3x_layer_forward) for a batch
  * whose tokens use different adapters: token t of every adapted projection uses
- * adapter adapter_ids[t] (device int32[T]; outside the table: none, the block as
- * it is). Router adapters act before the routing, gate's and up's before SwiGLU,
- * down's on the fp32 SwiGLU product. A single token runs on the MFMA tiles.
- * Otherwise as hy3x_layer_forward; the other forwards use no adapters. */
+ * adapter adapter_ids[t] (device int32[T], apart from x; outside the table: none,
+ * the block as it is). Router adapters act before the routing, gate's and up's
+ * before SwiGLU, down's on the fp32 SwiGLU product. A single token runs on the
+ * MFMA tiles. Otherwise as hy3x_layer_forward; the other forwards use no adapters. */
 int hy3x_layer_forward_adapters(hy3x_layer *layer, float *x, const float *attn_out,
                                 const int32_t *adapter_ids, int T, int K, float scale,
                                 void *stream);

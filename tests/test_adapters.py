@@ -32,6 +32,25 @@ def test_null_refusals():
     assert lib.hy3x_adapters_apply(None, 4096, 4096, 0, 64, None, 64, 8192, 0, 64, 1, None) == -1
 
 
+def test_host_memory_refusals():
+    import torch
+    h = H.Adapters.__new__(H.Adapters)  # no GPU, no handle: refused before it is used
+    h._h, h.rank, h.d_in, h.d_out, h.dtype = None, 8, 64, 96, "bf16"
+    x = torch.zeros(1, 64, dtype=torch.bfloat16)
+    ids = torch.zeros(1, dtype=torch.int32)
+    for args in ((ids, 4096, 8192), (4096, x, 8192), (4096, 8192, x),
+                 (ids.numpy(), 4096, 8192), (4096, np.zeros(64, np.float32), 8192)):
+        h._apply = None
+        with pytest.raises(TypeError):
+            h.apply(*args, 1)
+    with pytest.raises(TypeError):
+        h.apply(4096, 8192, 16384, 1, base=x)
+    with pytest.raises(TypeError):
+        h.set(0, np.zeros((8, 64), np.uint16), np.zeros((96, 8), np.uint16), on_device=True)
+    with pytest.raises(TypeError):
+        h.set(0, torch.zeros(8, 64, dtype=torch.bfloat16), 4096, on_device=True)
+
+
 # ---------------------------------------------------------------- on the GPU
 @pytest.fixture(scope="module")
 def torch():
@@ -338,6 +357,46 @@ def test_apply_refusals(torch):
     assert lib.hy3x_adapters_set(h._h, 0, None, p, 1.0, 1) == -1
     torch.cuda.synchronize()
     h.close()
+
+
+@pytest.mark.gpu
+def test_y_on_its_ids_is_refused(torch):
+    h = H.Adapters(2, 8, 64, 96, "bf16")
+    buf = torch.zeros(1 << 14, device="cuda")
+    y = buf.data_ptr() + 8192
+
+    def call(ids, T=4):
+        return H.lib().hy3x_adapters_apply(h._h, ids, y + 32768, 2, 64, None, 96, y, 2, 96, T, None)
+    for ids in (y, y - 12, y + 4 * 96 * 2 - 4):
+        assert call(ids) == -1 and b"ids" in H.lib().hy3x_last_error()
+    assert call(y - 16) == 0 and call(y + 4 * 96 * 2) == 0
+    torch.cuda.synchronize()
+    h.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("io", ["same", "f32"])
+def test_types_of_tensors(torch, io):
+    s = Setup(torch, 2, 8, 64, 96, "f16")
+    t = torch.float32 if io == "f32" else torch.float16
+    x = torch.randn(3, 64, generator=s.g).to(t).cuda()
+    ids = torch.tensor([1, 0, 1], dtype=torch.int32, device="cuda")
+    y, named = torch.zeros(3, 96, dtype=t, device="cuda"), torch.zeros(3, 96, dtype=t, device="cuda")
+    kind = "f32" if io == "f32" else "f16"
+    s.h.apply(ids, x, named, 3, x_dtype=kind, y_dtype=kind)
+    s.h.apply(ids, x, y, 3)  # the tensors' own types
+    torch.cuda.synchronize()
+    assert torch.equal(y, named) and y.abs().max() > 0
+    with pytest.raises(H.HY3XError, match="type"):
+        s.h.apply(ids, x.bfloat16(), y, 3)
+    for bad in (dict(ids=ids.long()), dict(x=x.double()), dict(y=y.double()),
+                dict(base=y.bfloat16())):
+        with pytest.raises(TypeError):
+            s.h.apply(**dict(dict(ids=ids, x=x, y=y, T=3), **bad))
+    with pytest.raises(AssertionError):
+        s.h.set(0, torch.zeros(8, 64, device="cuda"), torch.zeros(96, 8, device="cuda"),
+                on_device=True)
+    s.h.close()
 
 
 @pytest.mark.gpu

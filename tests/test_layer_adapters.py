@@ -366,6 +366,21 @@ def test_refusals(block):
 
 
 @pytest.mark.gpu
+def test_ids_on_x_and_closed_adapters_are_refused(block):
+    torch, layer = block.torch, block.layer
+    x = torch.zeros(4, D, device="cuda")
+    for at in (x.data_ptr(), x.data_ptr() - 12, x.data_ptr() + 4 * (4 * D - 1)):
+        with pytest.raises(H.HY3XError, match="adapter_ids overlaps x"):
+            layer.forward_adapters(x.data_ptr(), at, 4)
+    with pytest.raises(TypeError):
+        layer.forward_adapters(x.data_ptr(), np.zeros(4, np.int32), 4)
+    h = H.Adapters(1, 8, D, E, "f16")
+    h.close()
+    with pytest.raises(H.HY3XError, match="closed"):
+        layer.set_adapters("router", h)
+
+
+@pytest.mark.gpu
 def test_kernel_names_and_replays(block):
     torch, layer = block.torch, block.layer
     block.use(("gate",))

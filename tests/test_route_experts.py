@@ -70,6 +70,18 @@ def test_spec_refusals(change, word):
         H.route_experts(spec, 4096, 1, 4096, 4096)
 
 
+def test_host_memory_refusals():
+    import torch
+    spec = H.RouteSpec(**GOOD)
+    logits, ids, w = torch.zeros(1, 192), torch.zeros(1, 8, dtype=torch.int32), torch.zeros(1, 8)
+    for args in ((logits, 1, 4096, 4096), (4096, 1, ids, 4096), (4096, 1, 4096, w),
+                 (logits.numpy(), 1, 4096, 4096), (4096, 1, ids.numpy(), 4096)):
+        with pytest.raises(TypeError):
+            H.route_experts(spec, *args)
+    with pytest.raises(TypeError):
+        H.route_experts(spec, 4096, 1, 4096, 4096, bias=w)
+
+
 def test_argument_refusals():
     lib, spec = H.lib(), H.RouteSpec(**GOOD)
 
@@ -255,6 +267,25 @@ def test_rows_more_than_2_31_elements_apart(torch):
     torch.cuda.synchronize()
     want, _ = run(torch, H.RouteSpec(E, k), logits, "bf16")
     assert np.array_equal(ids.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_types_of_tensors(torch, dtype):
+    spec = H.RouteSpec(192, 8)
+    logits = make(torch, 5, 192, dtype, 3)
+    want = run(torch, spec, logits, dtype)
+    logits, bias = logits.cuda(), torch.zeros(192, dtype=torch.float64, device="cuda")
+    ids = torch.zeros(5, 8, dtype=torch.int32, device="cuda")
+    w = torch.zeros(5, 8, device="cuda")
+    H.route_experts(spec, logits, 5, ids, w)  # the logits' own type
+    torch.cuda.synchronize()
+    assert np.array_equal(ids.cpu().numpy(), want[0])
+    assert np.array_equal(w.cpu().numpy(), want[1])
+    for bad in (dict(ids=ids.long()), dict(w=w.double()), dict(logits=logits.double()),
+                dict(bias=bias)):
+        with pytest.raises(TypeError):
+            H.route_experts(spec, **dict(dict(logits=logits, T=5, ids=ids, w=w), **bad))
 
 
 @pytest.mark.gpu
