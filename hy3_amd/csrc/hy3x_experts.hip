@@ -88,8 +88,9 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   v = max(v, (uint32_t)dppi<DPP_XOR2>((int)v));
   v = max(v, (uint32_t)dppi<DPP_HALF_MIRROR>((int)v));
   v = max(v, (uint32_t)dppi<DPP_MIRROR>((int)v));
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, DPP_BCAST15, 0xA, 0xF, false));
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, DPP_BCAST31, 0xC, 0xF, false));
+  // 0 where a row takes no broadcast: one instruction with the maximum
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, DPP_BCAST15, 0xA, 0xF, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, DPP_BCAST31, 0xC, 0xF, false));
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
@@ -402,23 +403,25 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_route_experts(
         q[j] = max(x, y);
         q[j + 1] = min(x, y);
       }
-    int from = 0, nth = 0;  // the lane, and how many equal keys it gave before
+    int where = 0;  // the lane, and 64 times how many equal keys it gave before
     int last = -1, again = 0;
     for (int k = 0; k < K; k++) {
       const uint32_t M = wave_max(q[0]);
       const int wl = __builtin_ctzll(__ballot(q[0] == M));
 #pragma unroll
-      for (int j = 0; j < V; j++)
-        q[j] = lane == wl ? (j + 1 < V ? q[j + 1] : GONE<uint32_t>) : q[j];
-      again = M == kth && wl == last ? again + 1 : 0;
+      for (int j = 0; j < V; j++) {
+        const uint32_t own = q[j], up = j + 1 < V ? q[j + 1] : GONE<uint32_t>;
+        q[j] = lane == wl ? up : own;
+      }
+      again = M == kth && wl == last ? again + 64 : 0;
       kth = M;
       last = wl;
       if (lane == k) {
         my_key = M;
-        from = wl;
-        nth = again;
+        where = wl + again;
       }
     }
+    const int from = where & 63, nth = where >> 6;
     head = q[0];
     int seen = 0, slot = 0;
 #pragma unroll
