@@ -157,8 +157,8 @@ __device__ __forceinline__ double sum64(const Row<T> &row, const Lanes &L) {
 
 // How many groups come ahead of this lane's, by 64-bit scores.
 template <class T>
-__device__ __forceinline__ int groups64(const hy3x_route_spec &spec, const Row<T> &row, int v) {
-  const Lanes L(spec, v);
+__device__ __forceinline__ int groups64(const hy3x_route_spec &spec, const Row<T> &row,
+                                        const Lanes &L) {
   const bool top2 = spec.group_score == HY3X_GROUP_TOP2;
   const double sum = sum64(row, L);
   double b0 = -INFINITY, b1 = -INFINITY;
@@ -192,10 +192,10 @@ __device__ __forceinline__ int groups64(const hy3x_route_spec &spec, const Row<T
 // rows with more candidates than lanes. It forms every key again in each round
 // and keeps none.
 template <class T>
-__device__ __forceinline__ int choose64(const hy3x_route_spec &spec, const Row<T> &row, int v) {
-  const Lanes L(spec, v);
+__device__ __forceinline__ int choose64(const hy3x_route_spec &spec, const Row<T> &row,
+                                        const Lanes &L) {
   const double sum = sum64(row, L);
-  const bool stays = spec.n_group == 1 || groups64(spec, row, v) < spec.topk_group;
+  const bool stays = spec.n_group == 1 || groups64(spec, row, L) < spec.topk_group;
   uint32_t taken = 0;
   int mine = 0;
   for (int k = 0; k < spec.k; k++) {
@@ -264,7 +264,7 @@ __device__ __forceinline__ void finish(const hy3x_route_spec &spec, const Row<T>
 }
 
 template <class T, int V>
-__global__ __launch_bounds__(64 * ROUTE_WAVES) void k_route_experts(
+__global__ __launch_bounds__(64 * ROUTE_WAVES, V > 1 && V <= 4 ? 8 : 1) void k_route_experts(
     const hy3x_route_spec spec, const T *__restrict__ logits, int64_t stride,
     const float *__restrict__ bias, int n_row, int32_t *__restrict__ ids, float *__restrict__ w) {
   const int lane = threadIdx.x & 63;
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_route_experts(
         const uint32_t in = at(spec.topk_group - 1), out = at(spec.topk_group);
         if (out > MASKED<uint32_t> &&
             !(number(in) - number(out) > 2.0f * margin(softmax, most, number(in))))
-          before = groups64(spec, row, V);
+          before = groups64(spec, row, L);
       }
       const bool stays = L.group < G && before < spec.topk_group;
 #pragma unroll
@@ -462,7 +462,8 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_route_experts(
       const float lk = __shfl(lm, K - 1, 64), bk = __shfl(bm, K - 1, 64);
       bool any = close && (lm != ln || bm != bn);
 #pragma unroll
-      for (int j = 0; j < V; j++) any |= left(key[j]) && (l[j] != lk || b[j] != bk);
+      for (int j = 0; j < V; j++)
+        if (left(key[j])) any |= l[j] != lk || bias[L.first + j] != bk;
       if (__ballot(any)) {
         // candidates: the k chosen and all that lies close to the last of them
         int n = K;
@@ -470,7 +471,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_route_experts(
                          !(number(kth) - number(M) > edge);)
           n++;
         if (n == 64) {
-          mine = choose64(spec, row, V);
+          mine = choose64(spec, row, L);
         } else {
           const double s64 = sum64(row, L);
           const uint64_t k64 = lane < n ? row.key64(mine, s64) : GONE<uint64_t>;
