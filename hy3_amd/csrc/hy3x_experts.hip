@@ -115,14 +115,15 @@ struct Row {
   __device__ __forceinline__ bool masked(int e) const {
     return !(to_f32(logits[e]) > -Limits<T>::max) || (bias && !(bias[e] > -INFINITY));
   }
-  // the score, in 64 bits; sum: the softmax's
-  __device__ __forceinline__ double score64(int e, double sum) const {
-    return softmax ? exp((double)logit(e) - (double)top) / sum
-                   : 1.0 / (1.0 + exp(-(double)logit(e)));
+  // the score of logit l, in 64 bits; sum: the softmax's
+  __device__ __forceinline__ double score64(float l, double sum) const {
+    const double x = softmax ? (double)l - (double)top : -(double)l;
+    const double e = exp(x);
+    return softmax ? e / sum : 1.0 / (1.0 + e);
   }
   __device__ __forceinline__ uint64_t key64(int e, double sum) const {
     if (masked(e)) return MASKED<uint64_t>;
-    return ordered(bias ? score64(e, sum) + (double)bias[e] : (double)logit(e));
+    return ordered(bias ? score64(logit(e), sum) + (double)bias[e] : (double)logit(e));
   }
 };
 
@@ -140,35 +141,69 @@ struct Lanes {
   }
 };
 
+// This lane's logits one after another, NaN for masked ones and slots without an
+// expert: l as the kernel holds it, moved up (no indexed registers), or, of many,
+// read again.
+template <class T, int V>
+struct Each {
+  static constexpr bool HELD = V <= 8;
+  float c[HELD ? V : 1];
+  const Row<T> &row;
+  const Lanes &L;
+  int j = 0;
+  __device__ __forceinline__ Each(const Row<T> &r, const Lanes &lanes, const float (&l)[V])
+      : row(r), L(lanes) {
+#pragma unroll
+    for (int i = 0; i < (HELD ? V : 0); i++) c[i] = l[i];
+  }
+  __device__ __forceinline__ float next() {
+    if constexpr (HELD) {
+      const float x = c[0];
+#pragma unroll
+      for (int i = 0; i + 1 < V; i++) c[i] = c[i + 1];
+      return x;
+    } else {
+      const int e = L.first + j;
+      return j++ < L.n && !row.masked(e) ? row.logit(e) : NAN;
+    }
+  }
+};
+
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
 
-template <class T>
-__device__ __forceinline__ double sum64(const Row<T> &row, const Lanes &L) {
+template <class T, int V>
+__device__ __forceinline__ double sum64(const Row<T> &row, const Lanes &L, const float (&l)[V]) {
+  if (!row.softmax) return 0.0;
   double sum = 0.0;
-  if (row.softmax)
-    for (int j = 0; j < L.n; j++)
-      if (!row.masked(L.first + j)) sum += exp((double)row.logit(L.first + j) - (double)row.top);
+  Each<T, V> each(row, L, l);
+#pragma unroll 1  // one copy of exp in the code
+  for (int j = 0; j < V; j++) {
+    const float x = each.next();
+    if (x == x) sum += exp((double)x - (double)row.top);
+  }
   return wave_sum64(sum);
 }
 
 // How many groups come ahead of this lane's, by 64-bit scores.
-template <class T>
+template <class T, int V>
 __device__ __forceinline__ int groups64(const hy3x_route_spec &spec, const Row<T> &row,
-                                        const Lanes &L) {
+                                        const Lanes &L, const float (&l)[V]) {
   const bool top2 = spec.group_score == HY3X_GROUP_TOP2;
-  const double sum = sum64(row, L);
+  const double sum = sum64(row, L, l);
   double b0 = -INFINITY, b1 = -INFINITY;
   int live = 0;
-  for (int j = 0; j < L.n; j++) {
-    const int e = L.first + j;
-    if (row.masked(e)) continue;
+  Each<T, V> each(row, L, l);
+#pragma unroll 1
+  for (int j = 0; j < V; j++) {
+    const float x = each.next();
+    if (x != x) continue;
     const double s = !top2 && !row.bias
-                         ? (double)row.logit(e)
-                         : row.score64(e, sum) + (row.bias ? (double)row.bias[e] : 0.0);
+                         ? (double)x
+                         : row.score64(x, sum) + (row.bias ? (double)row.bias[L.first + j] : 0.0);
     b1 = fmax(b1, fmin(b0, s));
     b0 = fmax(b0, s);
     live++;
@@ -191,11 +226,11 @@ __device__ __forceinline__ int groups64(const hy3x_route_spec &spec, const Row<T
 // The choice by 64-bit keys alone, lane k < K returning the k-th expert: for
 // rows with more candidates than lanes. It forms every key again in each round
 // and keeps none.
-template <class T>
+template <class T, int V>
 __device__ __forceinline__ int choose64(const hy3x_route_spec &spec, const Row<T> &row,
-                                        const Lanes &L) {
-  const double sum = sum64(row, L);
-  const bool stays = spec.n_group == 1 || groups64(spec, row, L) < spec.topk_group;
+                                        const Lanes &L, const float (&l)[V]) {
+  const double sum = sum64(row, L, l);
+  const bool stays = spec.n_group == 1 || groups64(spec, row, L, l) < spec.topk_group;
   uint32_t taken = 0;
   int mine = 0;
   for (int k = 0; k < spec.k; k++) {
@@ -234,20 +269,20 @@ __device__ __forceinline__ float margin(bool softmax, float most, float key) {
 }
 
 // Weights of the chosen experts (lane k: the k-th) and the row's outputs.
-// sum: the softmax's; live, l: the expert is not masked, its logit. fp32, except
-// where a score lies near or below its normal numbers.
-template <class T>
+// ls: the lane's logits; sum: the softmax's; live, l: the expert is not masked, its
+// logit. fp32, except where a score lies near or below its normal numbers.
+template <class T, int V>
 __device__ __forceinline__ void finish(const hy3x_route_spec &spec, const Row<T> &row,
-                                       const Lanes &L, float sum, int mine, bool live, float l,
-                                       int64_t t, int32_t *ids, float *w) {
+                                       const Lanes &L, const float (&ls)[V], float sum,
+                                       int mine, bool live, float l, int64_t t, int32_t *ids, float *w) {
   static_assert(HY3X_ROUTE_MAX_K <= 16, "a row of 16 lanes holds the chosen");
   const int lane = L.lane, K = spec.k;
   live = live && lane < K;
   const float x = live ? l - (row.softmax ? row.top : 0.0f) : 0.0f;
   float v = 0.0f;
   if (__ballot(x < -80.0f)) {
-    const double s64 = sum64(row, L);
-    double s = live ? row.score64(mine, s64) : 0.0;
+    const double s64 = sum64(row, L, ls);
+    double s = live ? row.score64(l, s64) : 0.0;
     if (spec.renorm) s /= wave_sum64(s) + 1e-20;
     v = (float)(s * (double)spec.scale);
   } else {
@@ -303,7 +338,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, V > 1 && V <= 4 ? 8 : 1) void k_r
 #pragma unroll
     for (int j = 0; j < V; j++) {
       on[j] = j < L.n && l[j] > -Limits<T>::max && b[j] > -INFINITY;
-      l[j] = fminf(l[j], Limits<T>::max);
+      l[j] = on[j] ? fminf(l[j], Limits<T>::max) : NAN;
     }
     if (softmax) {
       uint32_t top = 0;
@@ -357,7 +392,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, V > 1 && V <= 4 ? 8 : 1) void k_r
         const uint32_t in = at(spec.topk_group - 1), out = at(spec.topk_group);
         if (out > MASKED<uint32_t> &&
             !(number(in) - number(out) > 2.0f * margin(softmax, most, number(in))))
-          before = groups64(spec, row, L);
+          before = groups64(spec, row, L, l);
       }
       const bool stays = L.group < G && before < spec.topk_group;
 #pragma unroll
@@ -457,13 +492,16 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, V > 1 && V <= 4 ? 8 : 1) void k_r
           for (int j = 0; j < V; j++) key[j] = e == L.first + j && j < L.n ? GONE<uint32_t> : key[j];
         }
       // experts of the same logit and bias are equal in any arithmetic
+      if constexpr (V <= 8)
+#pragma unroll
+        for (int j = 0; j < V; j++) b[j] = bias[min(L.first + j, spec.n_expert - 1)];
       const float lm = my_l, bm = bias[mine];
       const float ln = __shfl(lm, lane + 1, 64), bn = __shfl(bm, lane + 1, 64);
       const float lk = __shfl(lm, K - 1, 64), bk = __shfl(bm, K - 1, 64);
       bool any = close && (lm != ln || bm != bn);
 #pragma unroll
       for (int j = 0; j < V; j++)
-        if (left(key[j])) any |= l[j] != lk || bias[L.first + j] != bk;
+        if (left(key[j])) any |= l[j] != lk || (V <= 8 ? b[j] : bias[L.first + j]) != bk;
       if (__ballot(any)) {
         // candidates: the k chosen and all that lies close to the last of them
         int n = K;
@@ -471,9 +509,9 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, V > 1 && V <= 4 ? 8 : 1) void k_r
                          !(number(kth) - number(M) > edge);)
           n++;
         if (n == 64) {
-          mine = choose64(spec, row, L);
+          mine = choose64(spec, row, L, l);
         } else {
-          const double s64 = sum64(row, L);
+          const double s64 = sum64(row, L, l);
           const uint64_t k64 = lane < n ? row.key64(mine, s64) : GONE<uint64_t>;
           int rank = lane < n ? 0 : lane;
           for (int i = 0; i < n; i++) {
@@ -488,7 +526,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, V > 1 && V <= 4 ? 8 : 1) void k_r
       }
     }
   }
-  finish(spec, row, L, sum, mine, live, my_l, t, ids, w);
+  finish(spec, row, L, l, sum, mine, live, my_l, t, ids, w);
 }
 
 template <class T>
