@@ -9,8 +9,7 @@
 // launch, no order of blocks in the results. Its waves split d_in, join their
 // parts of u in LDS, then split the outputs. (Two launches over scratch, the
 // parts of u by blocks of their own and A and B read for 32 tokens at a time,
-// measured 39.0 us against 36.1 at 4096 x 4096 outputs of rank 64, 18.9 against
-// 17.4 at 512 tokens in fp32.)
+// measured 39.0 us against 36.1 at 4096 x 4096 outputs of rank 64.)
 //
 // TOK = 16: 16 consecutive tokens, the columns of every MFMA. The adapters that
 // occur among them are taken one after another: each forms its products for all
@@ -18,19 +17,21 @@
 // meets another adapter's values (not even their infinities). TOK = 1: one
 // token in every column.
 //
-// Products. u: v_mfma_f32_16x16x32_{f16,bf16} (rows = 16 ranks, columns =
-// tokens) where x has the weights' type; where x is fp32, v_mfma_f32_16x16x4_f32,
-// or fp32 FMAs for one token. B u: the two-byte MFMAs on u in two or three parts
-// (Parts), which keep fp32's range and precision.
+// Products: v_mfma_f32_16x16x32_{f16,bf16} (rows = 16 ranks, columns = tokens).
+// fp32 x meets A in three two-byte parts (Split), or in fp32 FMAs for one token;
+// u meets B in two or three (Parts). The parts keep fp32's range and precision.
+// (v_mfma_f32_16x16x4_f32 on fp32 x: 512 tokens of 4096 inputs 52.6 us at rank 64,
+// 24.3 in parts, 19.2 and 15.3 at rank 16.)
 //
 // What bounds it (us of the kernel, inputs and weights from HBM, MI355X): many
 // tokens the bytes of x, base and y, 16-token tiles with two adapters last (4096
 // x 4096 outputs of 4096 inputs, rank 64: 36 us for 111 MB, 3.1 TB/s; rank 16,
 // 2000 tokens: 16.3 us for 53 MB, 3.2 TB/s); up to 256 decoded tokens the adapters'
 // weights (256 tokens, 128 adapters: 13.7 us for 40 MB, 2.9 TB/s); a few tokens
-// four loads that wait for each other, ids, A, B, the store (32 tokens: 6.0 us;
-// one token beside the router: 6.0 us); fp32 x the fp32 MFMAs (512 tokens, 1536
-// inputs, rank 32: 16.2 us).
+// four loads that wait for each other, ids, A, B, the store (32 tokens: 6.1 us;
+// one token beside the router: 6.2 us), and the same in few tiles (512 tokens,
+// 1536 fp32 inputs, 4096 fp32 outputs, rank 32: 13.1 us for 20 MB, 2.2 of it the
+// tiles with two adapters).
 //
 // Weights as the MFMAs read them, one coalesced 16-byte load per lane:
 //   A  [count][kp / 32][rank tile][lane][8]: rank 16 rt + lane % 16, k = 32 kt
@@ -45,6 +46,7 @@
 
 #include <algorithm>
 #include <new>
+#include <type_traits>
 
 #include "../../include/hy3x_moe.h"
 #include "hy3x_common.h"
@@ -68,7 +70,7 @@ typedef _Float16 h4v __attribute__((ext_vector_type(4)));
 typedef short s4v __attribute__((ext_vector_type(4)));
 
 // Waves of a block: 16 where 128 registers a lane hold the operands in flight
-// (512 tokens, fp32, rank 32: 16.9 us with 8 waves, 15.6 with 16; one token beside
+// (512 tokens, fp32, rank 32: 12.6 us with 8 waves, 12.1 with 16; one token beside
 // the router 9.0 and 7.8), 8 above.
 constexpr int waves_for(int TOK, int RT) { return RT == 1 || (RT == 2 && TOK == 16) ? 16 : 8; }
 // Up to this many tokens, one per CU, a block takes one token and the order of the
@@ -79,8 +81,8 @@ constexpr int waves_for(int TOK, int RT) { return RT == 1 || (RT == 2 && TOK == 
 //   1024: 45.1 and 44.2 | 36.6 and 12.6
 constexpr int SINGLE_MAX_T = 256;
 // Blocks that the outputs are sliced for: one per CU. More slices form u again
-// (512 blocks: 32 decoded tokens 10.2 us against 6.4, 512 in fp32 25.8 against
-// 17.8, 2000 20.6 against 18.7, 4096 of rank 64 48.5 against 42.2).
+// (512 blocks: 32 decoded tokens 9.8 us against 6.1, 512 in fp32 19.1 against
+// 13.1, 2000 22.4 against 16.4, 4096 of rank 64 45.0 against 36.2).
 constexpr int TARGET_BLOCKS = 256;
 
 __device__ __forceinline__ float elem(float v) { return v; }
@@ -167,14 +169,6 @@ __device__ __forceinline__ f4v mma(const Run<__hip_bfloat16, 4> &a,
   return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4v, a),
                                                    __builtin_bit_cast(s4v, b), c, 0, 0, 0);
 }
-template <class W>
-__device__ __forceinline__ f4v mma(const Run<W, 8> &a, const Run<float, 8> &b, f4v c) {
-#pragma unroll
-  for (int j = 0; j < 8; j++)
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.at(j), b.at(j), c, 0, 0, 0);
-  return c;
-}
-
 struct Call {
   const uint16_t *a, *b;
   const float *scale;
@@ -205,6 +199,92 @@ template <class W, class Y>
 constexpr int parts_for() {
   return __is_same(W, __half) && sizeof(Y) == 2 ? 2 : 3;
 }
+
+// N steps of a token's fp32 x as three two-byte operands each, which hold its 24
+// bits: x = 2^e (p0 + p1 + p2). bf16 has fp32's range, and e = 0. fp16: e grows
+// with the largest |x| so far, which lies below 2^(e + 15), and what was summed
+// before is scaled along; parts reach down to 2^-24, 2^-39 of the largest.
+template <class W>
+struct Wide {
+  Run<W, 8> p[3];
+};
+template <class W>
+struct Split {
+  int e = -126;
+  template <int N, int RT>
+  __device__ __forceinline__ void operator()(const Run<float, 8> (&x)[N], Wide<W> (&out)[N],
+                                             f4v (&acc)[RT]) {
+    float v[N][8], top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        v[i][j] = x[i].at(j);
+        top = fmaxf(top, fabsf(v[i][j]));
+      }
+    const bool odd = __ballot(top == INFINITY);
+    if (odd) {
+      top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          top = fabsf(v[i][j]) < INFINITY ? fmaxf(top, fabsf(v[i][j])) : top;
+    }
+    if constexpr (__is_same(W, __half)) {
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const int at = max((int)(__float_as_uint(top) >> 23) - 127 - 14, e);
+      if (__ballot(at != e)) {
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[r][i] = __builtin_amdgcn_ldexpf(acc[r][i], e - at);
+        e = at;
+      }
+      const float by = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+      for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[i][j] *= by;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+      for (int q = 0; q < 3; q++) {
+        float h[8];
+#pragma unroll
+        for (int d = 0; d < 4; d++) {
+          if constexpr (__is_same(W, __half)) {
+            const auto two = __builtin_amdgcn_cvt_pkrtz(v[i][2 * d], v[i][2 * d + 1]);
+            out[i].p[q].w[d] = __builtin_bit_cast(uint32_t, two);
+            h[2 * d] = (float)two[0];
+            h[2 * d + 1] = (float)two[1];
+          } else {
+            const uint32_t lo = __float_as_uint(v[i][2 * d]), hi = __float_as_uint(v[i][2 * d + 1]);
+            out[i].p[q].w[d] = __builtin_amdgcn_perm(hi, lo, 0x07060302);
+            h[2 * d] = __uint_as_float(lo & 0xffff0000u);
+            h[2 * d + 1] = __uint_as_float(hi & 0xffff0000u);
+          }
+        }
+        if (q == 2) break;
+        if (odd)  // an infinity is its first part, the others 0
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            if (fabsf(v[i][j]) == INFINITY) v[i][j] = h[j] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[i][j] -= h[j];
+      }
+  }
+  template <int RT>
+  __device__ __forceinline__ void end(f4v (&acc)[RT]) const {
+    if constexpr (__is_same(W, __half))
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[r][i] = __builtin_amdgcn_ldexpf(acc[r][i], e);
+  }
+};
 
 // The tokens of a wave's columns: 16 consecutive ones, or one in all of them.
 // Columns past the last token read row 0, for nothing.
@@ -237,9 +317,13 @@ struct Tokens {
 // the adapters of these tokens one after another.
 // DOT: by fp32 products instead of MFMAs (one token), this lane's eight elements
 // of a step for rank 16 r + col in acc[r][0].
+// SPLIT: fp32 x as three two-byte parts (Split).
 template <class W, class X, int RT, int WAVES, int U, bool DOT>
 struct Shrink {
+  static constexpr bool SPLIT = sizeof(X) == 4 && !DOT;
+  using XO = std::conditional_t<SPLIT, Wide<W>, Run<X, 8>>;  // x as the products read it
   Run<X, 8> xv[U];
+  Split<W> parts;
   const X *xr;
   f4v acc[RT];
   int full, kt, d_in, lane, wave;  // full: whole steps, kt: all steps
@@ -269,8 +353,20 @@ struct Shrink {
 #pragma unroll
     for (int r = 0; r < RT; r++) v[r].load(aw + 512 * r);
   }
-  static __device__ __forceinline__ f4v product(const Run<W, 8> &a, const Run<X, 8> &b, f4v v) {
-    if constexpr (DOT) {
+  // x of a group, loaded, as operands
+  template <int N>
+  __device__ __forceinline__ void take(const Run<X, 8> (&x)[N], XO (&o)[N]) {
+    if constexpr (SPLIT) parts(x, o, acc);
+    else
+#pragma unroll
+      for (int i = 0; i < N; i++) o[i] = x[i];
+  }
+  static __device__ __forceinline__ f4v product(const Run<W, 8> &a, const XO &b, f4v v) {
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int k = 2; k >= 0; k--) v = mma(a, b.p[k], v);
+      return v;
+    } else if constexpr (DOT) {
 #pragma unroll
       for (int j = 0; j < 8; j++) v[0] = __builtin_fmaf(a.at(j), b.at(j), v[0]);
       return v;
@@ -280,7 +376,7 @@ struct Shrink {
   }
   // N steps of adapter a's weights for the columns that use it
   template <int N, class Live>
-  __device__ __forceinline__ void add(const Run<W, 8> (&av)[N][RT], const Run<X, 8> (&x)[N],
+  __device__ __forceinline__ void add(const Run<W, 8> (&av)[N][RT], const XO (&x)[N],
                                       const Tokens &tk, int a, Live live) {
     f4v sum[RT];
 #pragma unroll
@@ -304,6 +400,7 @@ struct Shrink {
     const int a0 = tk.pick(rest);
     if (step(0) < full) {
       Run<X, 8> xn[U];
+      XO xo[U];
       Run<W, 8> av[U][RT], an[U][RT];
       auto load_group = [&](Run<W, 8>(&v)[U][RT], int a, int n0) {
 #pragma unroll
@@ -312,6 +409,7 @@ struct Shrink {
       int n0 = 0, a = a0;
       uint64_t todo = rest;
       load_group(av, a, 0);
+      take(xv, xo);
       for (;;) {
         // the next adapter of this group, or the first of the next group
         const int n1 = todo ? n0 : n0 + U;
@@ -324,28 +422,30 @@ struct Shrink {
           if (n1 != n0) load_x(xn, n1);
         }
         __builtin_amdgcn_sched_barrier(0);  // these loads before the products
-        add<U>(av, xv, tk, a, [&](int i) { return step(n0 + i) < full; });
+        add<U>(av, xo, tk, a, [&](int i) { return step(n0 + i) < full; });
         if (!more) break;
 #pragma unroll
-        for (int i = 0; i < U; i++) {
+        for (int i = 0; i < U; i++)
 #pragma unroll
           for (int r = 0; r < RT; r++) av[i][r] = an[i][r];
-          if (n1 != n0) xv[i] = xn[i];
-        }
+        if (n1 != n0) take(xn, xo);
         n0 = n1;
         a = a1;
       }
     }
     if (full < kt && wave == WAVES - 1) {  // the last, part step of an odd d_in
       Run<X, 8> xt[1];
+      XO xo[1];
       xt[0].load_part(xr, 32 * full + 8 * (lane >> 4), d_in);
+      take(xt, xo);
       for (uint64_t todo = tk.mine; todo;) {
         const int a = tk.pick(todo);
         Run<W, 8> av[1][RT];
         load_a(av[0], base + a * size, full);
-        add<1>(av, xt, tk, a, [](int) { return true; });
+        add<1>(av, xo, tk, a, [](int) { return true; });
       }
     }
+    if constexpr (SPLIT) parts.end(acc);
   }
 };
 
@@ -545,9 +645,10 @@ __device__ __forceinline__ uint32_t item_of(uint32_t block, uint32_t n) {
 }
 
 // Steps of a group by register budget: 128 registers a lane with 16 waves, 256
-// with 8.
-constexpr int steps_for(int waves, int RT, int x_size) {
-  return RT == 8 ? 1 : x_size == 4 || RT == 4 || (RT == 2 && waves == 16) ? 2 : 4;
+// with 8; split: fp32 x in three parts.
+constexpr int steps_for(int waves, int RT, int x_size, bool split) {
+  if (RT == 8 || (RT == 2 && split)) return 1;
+  return x_size == 4 || RT == 4 || (RT == 2 && waves == 16) ? 2 : 4;
 }
 
 template <class W, class X, class Y, int RT, int TOK>
@@ -564,7 +665,7 @@ __global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call
   const int last = min(c.nb, (slice + 1) * c.per), cb0 = slice * c.per + wave;
   Tokens tk;
   tk.find((int64_t)tile * TOK + at, c.T, c.ids);
-  Shrink<W, X, RT, WAVES, steps_for(WAVES, RT, sizeof(X)), DOT> sh;
+  Shrink<W, X, RT, WAVES, steps_for(WAVES, RT, sizeof(X), sizeof(X) == 4 && !DOT), DOT> sh;
   sh.begin(c, tk, wave);
   Expand<W, Y, RT, WAVES> ex;
   ex.begin(c, tk, cb0, last);

@@ -254,6 +254,60 @@ def test_infinities_as_the_formula_has_them(torch, dtype, rank):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rank", [3, 24, 60, 128])
+def test_fp32_x_of_a_wide_range(torch, dtype, rank):
+    """Elements of one row 2^-24 to 2^24, rising, falling and mixed along d_in. In tiles
+    fp16 parts of x reach down to 2^-38 of the row's largest (2^-24 of a unit whose 2^14
+    it reaches): sum |A| of that on top, through B."""
+    s = Setup(torch, 2, rank, 4096 + 40, 70, dtype)
+    for T in (6, 300):
+        x, base, ids = s.inputs(T, "f32", "f32", mixed=False)
+        powers = 2.0 ** torch.linspace(-24, 24, s.h.d_in)
+        order = torch.randperm(s.h.d_in, generator=s.g)
+        for t in range(T):
+            x[t] *= (powers, powers.flip(0), powers[order])[t % 3]
+        base = base * 0.0
+        want, tol = s.expect(x, base, ids)
+        for t, i in enumerate(ids.tolist()):
+            if T > 256 and dtype == "f16" and i >= 0:
+                A, B = s.a[i].double().abs(), s.b[i].double().abs()
+                low = 2.0 ** -38 * x[t].abs().max().item()
+                tol[t] += s.scale[i] * low * (B @ A.sum(1)).numpy()
+        got = s.apply(x, base, ids, "f32", "f32").double().numpy()
+        assert (np.abs(got - want) <= tol).all()
+    s.h.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rank", [1, 20, 50])
+def test_fp32_x_with_infinities_among_large_values(torch, dtype, rank):
+    """An infinity early or late in a row whose finite values rise to fp32's largest:
+    as in 64 bits; a NaN stays with its token."""
+    s = Setup(torch, 1, rank, 4096 + 5, 33, dtype)
+    for T in (4, 290):
+        for at in (3, 2000, 4100):
+            x, base, ids = s.inputs(T, "f32", "f32")
+            ids = ids * 0
+            x *= 2.0 ** torch.linspace(-60, 100, s.h.d_in)
+            x[:, at] = float("inf")
+            x[1] = torch.randn(s.h.d_in, generator=s.g)  # finite
+            x[2] = 0.0
+            x[2, at] = float("nan")
+            x[3] = 0.0
+            with np.errstate(invalid="ignore"):
+                want, tol = s.expect(x, base, ids)
+            got = s.apply(x, base, ids, "f32", "f32").double().numpy()
+            assert np.array_equal(np.isnan(got), np.isnan(want))
+            some = np.isfinite(want)
+            assert some[1].all() and some[3].all()
+            assert np.array_equal(got[~some & ~np.isnan(want)], want[~some & ~np.isnan(want)])
+            assert (np.abs(got[some] - want[some]) <= tol[some]).all()
+    s.h.close()
+
+
+@pytest.mark.gpu
 def test_offsets_beyond_2_31(torch):
     """Adapters, rows of x and rows of y more than 2^31 elements from the first."""
     h = H.Adapters(4200, 128, 4096, 64, "bf16")  # 2.2e9 elements of A
