@@ -14,7 +14,8 @@
 // TOK = 16: 16 consecutive tokens, the columns of every MFMA. The adapters that
 // occur among them are taken one after another: each forms its products for all
 // 16 columns, and the columns of its own tokens are selected, so a token never
-// meets another adapter's values (not even their infinities). TOK = 1: one
+// meets another adapter's values (not even their infinities). Where several blocks
+// share a tile's outputs its adapters can be dealt to them (deal_for). TOK = 1: one
 // token in every column.
 //
 // Products: v_mfma_f32_16x16x32_{f16,bf16} (rows = 16 ranks, columns = tokens).
@@ -178,6 +179,7 @@ struct Call {
   void *y;
   int64_t x_stride, base_stride, y_stride;
   int T, slices, per;  // per: 64-output blocks of a slice
+  uint64_t deal;       // deal_for
 };
 
 // v in PARTS parts of W's precision, largest first: v = 2^e (p0 + p1 + ..).
@@ -308,6 +310,26 @@ struct Tokens {
     const int a = __builtin_amdgcn_readlane(id, __ffsll((long long)todo) - 1);
     todo &= ~__ballot(id == a);
     return a;
+  }
+  // Several adapters in a tile whose outputs `slices` blocks share: dealt to parts
+  // (deal_for), each with its share of the slices. This block then has the tokens
+  // of one part. Returns the number of parts.
+  __device__ __forceinline__ int deal(uint64_t table, int slices, int slice) {
+    uint64_t todo = mine;
+    int n = 0, at = 0;  // adapters, this column's
+    while (todo) {
+      const int next = pick(todo);
+      at = id == next ? n : at;
+      n++;
+    }
+    const int parts = n ? (int)(table >> (4 * n - 4) & 15) + 1 : 1;
+    if (parts == 1) return 1;
+    if (at % parts != slice % parts) {  // without an adapter: of part 0
+      in = false;
+      id = -1;
+    }
+    mine = __ballot(id >= 0) & 0xffffu;
+    return parts;
   }
 };
 
@@ -565,7 +587,7 @@ struct Expand {
   }
   // the base of the first outputs, which needs no adapter yet
   __device__ __forceinline__ void begin(const Call &c, const Tokens &tk, int cb0, int last) {
-    br = c.base ? (const Y *)c.base + tk.row * c.base_stride : nullptr;
+    br = c.base && tk.in ? (const Y *)c.base + tk.row * c.base_stride : nullptr;
     if (cb0 < last) load_base(c, bv, cb0);
   }
   // B of the first outputs and adapter
@@ -662,7 +684,7 @@ __global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call
   const int col = lane & 15, at = TOK == 1 ? 0 : col;  // at: the column's token of the block
   const uint32_t item = item_of(blockIdx.x, gridDim.x), tile = item / c.slices;
   const int slice = item % c.slices;
-  const int last = min(c.nb, (slice + 1) * c.per), cb0 = slice * c.per + wave;
+  int last = min(c.nb, (slice + 1) * c.per), cb0 = slice * c.per + wave;
   Tokens tk;
   tk.find((int64_t)tile * TOK + at, c.T, c.ids);
   Shrink<W, X, RT, WAVES, steps_for(WAVES, RT, sizeof(X), sizeof(X) == 4 && !DOT), DOT> sh;
@@ -670,6 +692,16 @@ __global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call
   Expand<W, Y, RT, WAVES> ex;
   ex.begin(c, tk, cb0, last);
   tk.settle(c.count);
+  if (TOK > 1 && c.slices > 1) {
+    const int parts = tk.deal(c.deal, c.slices, slice);
+    if (parts > 1) {
+      const int blocks = (c.slices - 1 - slice % parts) / parts + 1;
+      const int per = (c.nb + blocks - 1) / blocks;
+      last = min(c.nb, (slice / parts + 1) * per);
+      cb0 = slice / parts * per + wave;
+      ex.begin(c, tk, cb0, last);
+    }
+  }
   sh.run(c, tk);
   ex.ahead(c, tk, cb0, last);
   Parts<W, RT, parts_for<W, Y>()> pu;
@@ -736,6 +768,34 @@ __global__ __launch_bounds__(256) void k_pack_adapter(const uint16_t *__restrict
   }
 }
 
+// Into how many parts the n = 1 .. 16 adapters of a tile are dealt (less one, in 4
+// bits each), so that a block forms u of fewer adapters, for more outputs: the
+// number with the fewest bytes for the block that has the most. a: of one A, b: of
+// one B, io: of a tile's base and y, whose tokens may be uneven by 6; 32 KB an
+// adapter and 200 KB for the base's first loads again stand for their latencies (a
+// CU takes about 100 KB a us). us, not dealt and dealt: 512 tokens of 4096 fp32
+// inputs, 1536 outputs, rank 64, two adapters in some tiles 24.0 and 18.7, eight in
+// every tile 75.2 and 22.9; 2000 tokens, 4096 x 4096, rank 64 27.0 and 23.9; rank
+// 16, which stays at one part, 15.9 and 17.0.
+uint64_t deal_for(int slices, float a, float b, float io) {
+  uint64_t table = 0;
+  for (int n = 2; n <= 16; n++) {
+    int parts = 1;
+    float least = n * (a + b / slices + 32e3f) + io / slices;
+    for (int p = 2; p <= std::min(n, slices); p++) {
+      const int m = (n + p - 1) / p;  // adapters of a part
+      const float q = slices / p, tokens = std::min(16, 16 * m / n + 6);
+      const float bytes = m * (a + b / q + 32e3f) + io / q * tokens / 16 + 200e3f;
+      if (bytes < least) {
+        parts = p;
+        least = bytes;
+      }
+    }
+    table |= (uint64_t)(parts - 1) << (4 * n - 4);
+  }
+  return table;
+}
+
 template <class W, class X, class Y>
 void launch(const hy3x_adapters *h, const int32_t *ids, const void *x, int64_t x_stride,
             const void *base, int64_t base_stride, void *y, int64_t y_stride, int T,
@@ -762,6 +822,9 @@ void launch(const hy3x_adapters *h, const int32_t *ids, const void *x, int64_t x
     const int slices = std::max(1, std::min(c.nb, TARGET_BLOCKS / tiles));
     c.per = (c.nb + slices - 1) / slices;
     c.slices = (c.nb + c.per - 1) / c.per;
+    c.deal = c.slices == 1 ? 0
+                           : deal_for(c.slices, 2.0f * h->kp * h->rp, 2.0f * h->np * h->rp,
+                                      32.0f * c.d_out * sizeof(Y));
     return dim3((uint32_t)tiles * c.slices);
   };
   const bool single = T <= SINGLE_MAX_T;

@@ -194,6 +194,28 @@ def test_many_tokens(torch, dtype, T, rank, mixed):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("d_out", [64, 130, 1000, 2048])
+@pytest.mark.parametrize("count,rank", [(2, 16), (3, 40), (20, 7)])
+def test_tiles_of_several_adapters(torch, dtype, d_out, count, rank):
+    """Tiles whose adapters are dealt to the slices of their outputs: fewer slices than
+    adapters, as many, more; tokens without one among them, in place too."""
+    s = Setup(torch, count, rank, 320, d_out, dtype)
+    for i, T in enumerate((257, 400, 1040)):
+        xt, yt = io_types(dtype)[(i + rank) % 4]
+        s.check(T, xt, yt, mixed=True, in_place=i % 2 == 0, pads=(3, 5, 2))
+    x, base, ids = s.inputs(300, "f32", dtype)
+    ids[:16], ids[16:32], ids[32:40] = -1, 1, 0  # tiles of none, of one, of some
+    want, tol = s.expect(x, base, ids)
+    got = s.apply(x, base, ids, "f32", dtype)
+    assert (np.abs(got.double().numpy() - want) <= tol).all()
+    for at in (33, 200, 299):  # with other neighbours the same bits
+        other = torch.where(torch.arange(300) == at, ids, (ids + 1) % count).int()
+        assert torch.equal(s.apply(x, base, other, "f32", dtype)[at], got[at])
+    s.h.close()
+
+
+@pytest.mark.gpu
 def test_ids_outside_the_table_have_no_adapter(torch):
     s = Setup(torch, 3, 8, 64, 64, "bf16")
     x, base, _ = s.inputs(6, "bf16", "bf16")
