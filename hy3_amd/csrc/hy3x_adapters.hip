@@ -26,13 +26,13 @@
 //
 // What bounds it (us of the kernel, inputs and weights from HBM, MI355X): many
 // tokens the bytes of x, base and y, 16-token tiles with two adapters last (4096
-// x 4096 outputs of 4096 inputs, rank 64: 36 us for 111 MB, 3.1 TB/s; rank 16,
-// 2000 tokens: 16.3 us for 53 MB, 3.2 TB/s); up to 256 decoded tokens the adapters'
-// weights (256 tokens, 128 adapters: 13.7 us for 40 MB, 2.9 TB/s); a few tokens
-// four loads that wait for each other, ids, A, B, the store (32 tokens: 6.1 us;
-// one token beside the router: 6.2 us), and the same in few tiles (512 tokens,
-// 1536 fp32 inputs, 4096 fp32 outputs, rank 32: 13.1 us for 20 MB, 2.2 of it the
-// tiles with two adapters).
+// x 4096 outputs of 4096 inputs, rank 64: 34.9 us for 111 MB, 3.2 TB/s, 25.6 where
+// no tile has two; rank 16, 2000 tokens: 16.4 us for 53 MB, 3.2 TB/s); up to 256
+// decoded tokens the adapters' weights (256 tokens, 128 adapters: 14.0 us for 40 MB,
+// 2.9 TB/s); a few tokens four loads that wait for each other, ids, A, B, the store
+// (32 tokens: 6.0 us; one token beside the router: 6.2 us), and the same in few
+// tiles (512 tokens, 1536 fp32 inputs, 4096 fp32 outputs, rank 32: 12.9 us for 20
+// MB, 2 of it the tiles with two adapters).
 //
 // Weights as the MFMAs read them, one coalesced 16-byte load per lane:
 //   A  [count][kp / 32][rank tile][lane][8]: rank 16 rt + lane % 16, k = 32 kt

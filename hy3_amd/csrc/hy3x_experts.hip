@@ -25,12 +25,14 @@
 // keys are the logits, which are exact: no margin, and ties are ties.
 //
 // What bounds it (us of the kernel, MI355X): few rows the load and k rounds that
-// wait for each other (one row of 192: 3.0 us; 512: 4.4, its end a row with
+// wait for each other (one row of 192: 2.7 us; 512: 4.2, its end a row with
 // candidates); many rows vector instructions, not bytes (4096 rows of 256 in 8
-// groups: 8.9 us, about 640 a row; 16383 of 251: 18.3 us, 518 a row, 10 MB). With
-// 64-bit keys for every row these were 8.2, 10.2, 22.8 and 48.7. A wave per row
-// in blocks of 4 waves: blocks of 1, 8 or 16 are no faster; waves that take rows in
-// turn, the next row's loads in flight, 10.4 and 22.4 at 4096 and 16383.
+// groups: 8.1 us, 507 a row; 16383 of 251: 15.6 us, 401 a row, 10 MB). With 64-bit
+// keys for every row these were 8.2, 10.2, 22.8 and 48.7. A wave per row in blocks
+// of 4 waves: blocks of 1, 8 or 16 are no faster; waves that take rows in turn, the
+// next row's loads in flight, were slower (10.4 against 9.3 at 4096 rows, 22.4
+// against 18.8 at 16383). 64 registers, 8 waves a SIMD, where lanes hold 2 to 4
+// experts: 16.5 us against 17.0 with 72.
 #include <hip/hip_bf16.h>
 #include <math.h>
 
