@@ -346,13 +346,13 @@ int hy3x_adapters_set(hy3x_adapters *adapters, int index, const void *a, const v
  * the row length to 2^32. Sums are fp32 (fp16 adapters: what lies below 2^-38 of
  * a token's largest A x, or above 256 tokens of its largest fp32 x, may not count);
  * y is rounded once; tokens do not affect each other's results, whatever their
- * adapters hold. Up to 256 tokens each takes its own adapter at the same cost;
- * more run in tiles of 16 consecutive tokens that read each adapter occurring in
- * them, so keep a request's tokens together, and give the single-token requests of
- * a batch a call of their own. T = 0 does nothing. The handle's device must be
- * current. No allocation, no scratch: calls on one handle may overlap, and a call
- * may be captured into a graph. stream: a hipStream_t of the handle's device
- * (NULL = default stream). Asynchronous. */
+ * adapters hold. Up to 256 tokens each takes its own adapter (neighbours with the
+ * same one share its reads); more run in tiles of 16 consecutive tokens that read
+ * each adapter occurring in them, so keep a request's tokens together, and give the
+ * single-token requests of a batch a call of their own. T = 0 does nothing. The
+ * handle's device must be current. No allocation, no scratch: calls on one handle
+ * may overlap, and a call may be captured into a graph. stream: a hipStream_t of
+ * the handle's device (NULL = default stream). Asynchronous. */
 int hy3x_adapters_apply(const hy3x_adapters *adapters, const int32_t *ids, const void *x,
                         int x_type, int64_t x_stride, const void *base, int64_t base_stride,
                         void *y, int y_type, int64_t y_stride, int T, void *stream);
