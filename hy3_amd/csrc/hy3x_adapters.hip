@@ -205,7 +205,7 @@ constexpr int parts_for() {
 // N steps of a token's fp32 x as three two-byte operands each, which hold its 24
 // bits: x = 2^e (p0 + p1 + p2). bf16 has fp32's range, and e = 0. fp16: e grows
 // with the largest |x| so far, which lies below 2^(e + 15), and what was summed
-// before is scaled along; parts reach down to 2^-24, 2^-39 of the largest.
+// before is scaled along; parts reach down to 2^-24, at most 2^-38 of the largest.
 template <class W>
 struct Wide {
   Run<W, 8> p[3];

@@ -276,7 +276,8 @@ __device__ __forceinline__ float margin(bool softmax, float most, float key) {
 template <class T, int V>
 __device__ __forceinline__ void finish(const hy3x_route_spec &spec, const Row<T> &row,
                                        const Lanes &L, const float (&ls)[V], float sum,
-                                       int mine, bool live, float l, int64_t t, int32_t *ids, float *w) {
+                                       int mine, bool live, float l, int64_t t, int32_t *ids,
+                                       float *w) {
   static_assert(HY3X_ROUTE_MAX_K <= 16, "a row of 16 lanes holds the chosen");
   const int lane = L.lane, K = spec.k;
   live = live && lane < K;
@@ -425,7 +426,8 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, V > 1 && V <= 4 ? 8 : 1) void k_r
     }
     return M;
   };
-  uint32_t kth = GONE<uint32_t>, head = GONE<uint32_t>;  // the last chosen; this lane's largest left
+  uint32_t kth = GONE<uint32_t>;   // the last chosen
+  uint32_t head = GONE<uint32_t>;  // this lane's largest left
   if constexpr (V <= 8) {
     // each lane's keys sorted once: a round is the maximum of the heads, and
     // its lane's keys move up; the expert is found from the unsorted keys
@@ -491,7 +493,8 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, V > 1 && V <= 4 ? 8 : 1) void k_r
         for (int k = 0; k < K; k++) {
           const int e = __builtin_amdgcn_readlane(mine, k);
 #pragma unroll
-          for (int j = 0; j < V; j++) key[j] = e == L.first + j && j < L.n ? GONE<uint32_t> : key[j];
+          for (int j = 0; j < V; j++)
+            key[j] = e == L.first + j && j < L.n ? GONE<uint32_t> : key[j];
         }
       // experts of the same logit and bias are equal in any arithmetic
       if constexpr (V <= 8)

@@ -457,7 +457,7 @@ def test_types_of_tensors(torch, io):
     t = torch.float32 if io == "f32" else torch.float16
     x = torch.randn(3, 64, generator=s.g).to(t).cuda()
     ids = torch.tensor([1, 0, 1], dtype=torch.int32, device="cuda")
-    y, named = torch.zeros(3, 96, dtype=t, device="cuda"), torch.zeros(3, 96, dtype=t, device="cuda")
+    y, named = (torch.zeros(3, 96, dtype=t, device="cuda") for _ in range(2))
     kind = "f32" if io == "f32" else "f16"
     s.h.apply(ids, x, named, 3, x_dtype=kind, y_dtype=kind)
     s.h.apply(ids, x, y, 3)  # the tensors' own types
