@@ -21,8 +21,9 @@
 // 64-bit keys, a lane each, and are ranked by counting (experts of the same
 // logit and bias need none: they are equal). A row with more candidates than
 // lanes is decided by 64-bit keys throughout (choose64). Groups whose scores are
-// that close at the border are scored in 64 bits (groups64). Without a bias the
-// keys are the logits, which are exact: no margin, and ties are ties.
+// that close at the border, or are sums that cancel, are scored in 64 bits
+// (groups64). Without a bias the keys are the logits, which are exact: no
+// margin, and ties are ties.
 //
 // What bounds it (us of the kernel, MI355X): few rows the load and k rounds that
 // wait for each other (one row of 192: 2.7 us; 512: 4.2, its end a row with
@@ -381,7 +382,14 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, V > 1 && V <= 4 ? 8 : 1) void k_r
         a1 = max(max(a1, o1), min(a0, o0));
         a0 = max(a0, o0);
       }
-      if (top2 && a1 > MASKED<uint32_t>) a0 = ordered(number(a0) + number(a1));
+      // A sum rounds as its two keys do, so margin() of the sum covers it unless they
+      // cancel: a steering bias of +1e6 and one of -1e6 leave a sum of 1 off by 0.1.
+      bool cancel = false;
+      if (top2 && a1 > MASKED<uint32_t>) {
+        const float k0 = number(a0), k1 = number(a1), both = k0 + k1;
+        cancel = fabsf(k0) + fabsf(k1) > fabsf(both) + most;
+        a0 = ordered(both);
+      }
       int before = 0;  // groups ahead of this lane's
       for (int g = 0; g < G; g++) {
         const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)a0, g << L.shift);
@@ -393,8 +401,9 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, V > 1 && V <= 4 ? 8 : 1) void k_r
               (int)a0, __builtin_ctzll(__ballot(L.group < G && before == place)));
         };
         const uint32_t in = at(spec.topk_group - 1), out = at(spec.topk_group);
-        if (out > MASKED<uint32_t> &&
-            !(number(in) - number(out) > 2.0f * margin(softmax, most, number(in))))
+        if (__ballot(cancel) ||
+            (out > MASKED<uint32_t> &&
+             !(number(in) - number(out) > 2.0f * margin(softmax, most, number(in)))))
           before = groups64(spec, row, L, l);
       }
       const bool stays = L.group < G && before < spec.topk_group;

@@ -317,3 +317,17 @@ def test_streams_and_graph(torch):
         torch.cuda.synchronize()
         assert np.array_equal(ids[0].cpu().numpy(), want[0])
         assert np.array_equal(w[0].cpu().numpy(), want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("span", [12.0, 1e4, 1e6, 3e7])
+@pytest.mark.parametrize("E,groups,kept", [(64, 32, 5), (192, 8, 4), (256, 16, 8), (1000, 20, 5)])
+def test_sums_of_two_that_cancel(torch, score, span, E, groups, kept):
+    """One expert of each group pinned by a large bias, the others held off by its
+    negative: a group's score is what is left of the two, far below their rounding in
+    fp32, and the groups still come in the order of 64 bits."""
+    logits = make(torch, 60, E, "f32", 21)
+    bias = np.full(E, -span, np.float32)
+    bias[np.arange(groups) * (E // groups) + np.arange(groups) % (E // groups)] = span
+    check(torch, H.RouteSpec(E, 5, score, groups, kept, "top2"), logits, "f32", bias)
