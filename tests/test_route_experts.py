@@ -331,3 +331,64 @@ def test_sums_of_two_that_cancel(torch, score, span, E, groups, kept):
     bias = np.full(E, -span, np.float32)
     bias[np.arange(groups) * (E // groups) + np.arange(groups) % (E // groups)] = span
     check(torch, H.RouteSpec(E, 5, score, groups, kept, "top2"), logits, "f32", bias)
+
+
+# Lanes that hold 8 experts, and those that hold more and read their logits again:
+# without groups 512 (8 a lane), 320 (5), 1024 (16); 1000 in 20 groups (25 of 32), 1024 in
+# 64 groups (16), 360 in 3 (8).
+WIDE = [(320, 1, 1), (512, 1, 1), (1024, 1, 1), (360, 3, 2), (1000, 20, 7), (1024, 64, 9)]
+
+
+def check_wide(torch, spec, logits, dtype, bias=None, pad=0):
+    """check() with the weights' tolerance for lanes of up to 32 experts: the argument
+    (reach), exp (4), the softmax's sum of 32 a lane and 64 lanes (32 + 6) of terms off by
+    (1.5 |x| + 4) roundings of themselves (at most 11 of the sum of 1024, as |x| exp(-|x|)
+    falls), the renormalisation (18), the scale (1)."""
+    info = torch.finfo(logits.dtype)
+    want, w, reach = oracle(spec, logits.float().numpy(), bias, info.min, info.max)
+    ids, got = run(torch, spec, logits, dtype, bias, pad)
+    assert np.array_equal(ids, want)
+    tol = (72 + reach[:, None]) * HALF * np.abs(w) + 2.0 ** -149 * abs(spec.scale)
+    assert (np.abs(got - w) <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("E,groups,kept", WIDE)
+def test_rows_of_wide_lanes(torch, dtype, score, E, groups, kept):
+    for i, (best, bias, renorm) in enumerate([("max", True, True), ("top2", True, False),
+                                              ("max", False, False), ("top2", False, True)]):
+        spec = H.RouteSpec(E, 16 - i, score, groups, kept, best, renorm, 2.5)
+        check_wide(torch, spec, make(torch, 70, E, dtype, 10 * i + E), dtype,
+                   bias_of(E, i, 0.1 if score == "sigmoid" else 0.01) if bias else None,
+                   pad=(0, 3, 8, 1)[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("best", ["max", "top2"])
+@pytest.mark.parametrize("E,groups,kept", WIDE)
+def test_special_rows_of_wide_lanes(torch, dtype, score, best, E, groups, kept):
+    logits = special_rows(E, dtype, torch)
+    odd = bias_of(E, 1)
+    odd[0], odd[E // 3], odd[E - 1] = -np.inf, np.nan, np.inf
+    near = (0.5 + np.arange(E) * 2.0 ** -24).astype(np.float32)
+    for bias in (None, np.zeros(E, np.float32), odd, near):
+        for renorm in (True, False):
+            spec = H.RouteSpec(E, 7, score, groups, kept, best, renorm, 2.0)
+            check_wide(torch, spec, logits, dtype, bias)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("E,groups,kept", WIDE + [(192, 1, 1), (256, 8, 4)])
+def test_more_near_ties_than_lanes(torch, score, E, groups, kept):
+    """Every expert within fp32's margin of every other: more candidates than a wave has
+    lanes, all of them in the order of 64 bits."""
+    g = torch.Generator().manual_seed(E)
+    logits = -4.0 + torch.randint(-40, 41, (12, E), generator=g) * 2.0 ** -20
+    bias = np.full(E, 0.75, np.float32)
+    for best in ("max", "top2"):
+        check_wide(torch, H.RouteSpec(E, 8, score, groups, kept, best), logits, "f32", bias)
