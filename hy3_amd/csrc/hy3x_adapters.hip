@@ -20,7 +20,7 @@
 //
 // Products: v_mfma_f32_16x16x32_{f16,bf16} (rows = 16 ranks, columns = tokens).
 // fp32 x meets A in three two-byte parts (Split), or in fp32 FMAs for one token;
-// u meets B in two or three (Parts). The parts keep fp32's range and precision.
+// u meets B in three too (Parts). The parts keep fp32's range and precision.
 // (v_mfma_f32_16x16x4_f32 on fp32 x: 512 tokens of 4096 inputs 52.6 us at rank 64,
 // 24.3 in parts, 19.2 and 15.3 at rank 16.)
 //
@@ -182,7 +182,7 @@ struct Call {
   uint64_t deal;       // deal_for
 };
 
-// v in PARTS parts of W's precision, largest first: v = 2^e (p0 + p1 + ..).
+// v in parts of W's precision, largest first: v = 2^e (p0 + p1 + p2).
 // fp16 parts are of v 2^-e with e chosen so that the row's largest |v| lies in
 // [2^14, 2^15): the parts keep 11 bits each, down to 2^-24 2^-14 of the
 // largest. bf16 has fp32's range, and e = 0. An infinity or NaN is its first
@@ -194,13 +194,9 @@ __device__ __forceinline__ float part_of(float v, __hip_bfloat16 *) {
   return __uint_as_float(__float_as_uint(v) & 0xffff0000u);
 }
 
-// Three parts hold all 24 bits of an fp32 u. Two fp16 parts hold 20 bits of
-// each value, an error that an fp16 y's rounding (11 bits) covers also where
-// the base cancels most of the product; two bf16 parts would hold 14.
-template <class W, class Y>
-constexpr int parts_for() {
-  return __is_same(W, __half) && sizeof(Y) == 2 ? 2 : 3;
-}
+// Parts of u: three, which hold all 24 bits of an fp32 value. Two fp16 parts hold 22
+// and cut the rest off, which an fp16 y shows where the base cancels the product.
+constexpr int PARTS = 3;
 
 // N steps of a token's fp32 x as three two-byte operands each, which hold its 24
 // bits: x = 2^e (p0 + p1 + p2). bf16 has fp32's range, and e = 0. fp16: e grows
@@ -471,8 +467,8 @@ struct Shrink {
   }
 };
 
-// u of a lane's token, ranks 4 RT g + s, as MFMA operands in PARTS parts.
-template <class W, int RT, int PARTS>
+// u of a lane's token, ranks 4 RT g + s, as MFMA operands in parts.
+template <class W, int RT>
 struct Parts {
   static constexpr int NS = RT == 1 ? 4 : 8, NV = 4 * RT / NS;  // elements, operands
   Run<W, NS> p[PARTS][NV];
@@ -704,7 +700,7 @@ __global__ __launch_bounds__(64 * waves_for(TOK, RT)) void k_adapters(const Call
   }
   sh.run(c, tk);
   ex.ahead(c, tk, cb0, last);
-  Parts<W, RT, parts_for<W, Y>()> pu;
+  Parts<W, RT> pu;
   if (tk.mine) {  // of the block: every wave has the same tokens
     if constexpr (DOT) {
 #pragma unroll

@@ -505,3 +505,28 @@ def test_streams_and_graph(torch, T):
         torch.cuda.synchronize()
         assert torch.equal(y.cpu(), want[i])
     s.h.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T", [1, 60, 300])
+@pytest.mark.parametrize("rank,d_in", [(2, 2), (5, 40), (64, 200), (128, 33)])
+def test_all_bits_of_the_product_reach_y(torch, dtype, T, rank, d_in):
+    """One rank's u is x[0] = 1 + 2^-11 + (4 j + 3) 2^-23, all 24 bits of fp32, another's 1.
+    B of 1 and -2^-11 and a base of -1 leave the lowest bits, which y's type holds: every
+    sum is a multiple of 2^-23 below 2, so every step is exact, and y too."""
+    t = dtype_of(torch, dtype)
+    h = H.Adapters(1, rank, d_in, 70, dtype)
+    a, b = torch.zeros(rank, d_in, dtype=t), torch.zeros(70, rank, dtype=t)
+    a[0, 0], a[rank - 1, 1] = 1.0, 1.0
+    b[:, 0], b[:, rank - 1] = 1.0, -2.0 ** -11
+    h.set(0, a.cuda(), b.cuda(), 1.0, on_device=True)
+    low = (4.0 * (torch.arange(T) % 61) + 3.0) * 2.0 ** -23  # 8 bits
+    x = torch.zeros(T, d_in)
+    x[:, 0], x[:, 1] = 1.0 + 2.0 ** -11 + low, 1.0
+    ids, base = torch.zeros(T, dtype=torch.int32).cuda(), torch.full((T, 70), -1.0, dtype=t).cuda()
+    y = torch.zeros_like(base)
+    h.apply(ids, x.cuda(), y, T, base=base)
+    torch.cuda.synchronize()
+    assert torch.equal(y.float().cpu(), low[:, None].expand(T, 70))
+    h.close()
