@@ -597,9 +597,10 @@ struct Expand {
     if (cb0 >= last) return;
     uint64_t rest = tk.mine;
     const int a0 = rest ? tk.pick(rest) : 0;
+    // -0: what a token without an adapter adds to its base, a base of -0 included
     float out[16];
 #pragma unroll
-    for (int i = 0; i < 16; i++) out[i] = 0.0f;
+    for (int i = 0; i < 16; i++) out[i] = -0.0f;
     int cb = cb0, a = a0;
     uint64_t todo = rest;
     float sc = c.scale[a0];
@@ -641,7 +642,7 @@ struct Expand {
         }
         if (!more) break;
 #pragma unroll
-        for (int i = 0; i < 16; i++) out[i] = 0.0f;
+        for (int i = 0; i < 16; i++) out[i] = -0.0f;
 #pragma unroll
         for (int k = 0; k < P::N; k++) bv[k] = bn[k];
       }

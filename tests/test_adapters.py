@@ -530,3 +530,27 @@ def test_all_bits_of_the_product_reach_y(torch, dtype, T, rank, d_in):
     torch.cuda.synchronize()
     assert torch.equal(y.float().cpu(), low[:, None].expand(T, 70))
     h.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T", [3, 300])
+def test_a_token_without_an_adapter_keeps_its_base(torch, dtype, T):
+    """Bit for bit: zeros of either sign, infinities, the smallest and the largest; 0
+    where there is no base."""
+    s = Setup(torch, 2, 8, 64, 72, dtype)
+    for xt, yt in io_types(dtype):
+        x, base, _ = s.inputs(T, xt, yt)
+        info = torch.finfo(base.dtype)
+        base[:, ::8], base[:, 1::8], base[:, 2::8] = -0.0, 0.0, float("-inf")
+        base[:, 3::8], base[:, 4::8], base[:, 5::8] = info.max, info.min, info.smallest_normal
+        ids = torch.full((T,), -1, dtype=torch.int32)
+        kind = {4: torch.int32, 2: torch.int16}[base.element_size()]
+        for i in ([], [1], list(range(0, T, 2))):  # alone, and beside tokens with one
+            ids[i] = 1
+            got = s.apply(x, base, ids, xt, yt)
+            rest = [t for t in range(T) if ids[t] < 0]
+            assert torch.equal(got[rest].view(kind), base[rest].view(kind))
+            none = s.apply(x, base, ids, xt, yt, none=True)
+            assert (none[rest].view(kind) == 0).all()
+    s.h.close()
