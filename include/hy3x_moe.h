@@ -346,7 +346,10 @@ int hy3x_adapters_set(hy3x_adapters *adapters, int index, const void *a, const v
  * the row length to 2^32. Sums are fp32 (fp16 adapters: what lies below 2^-38 of
  * a token's largest A x, or above 256 tokens of its largest fp32 x, may not count);
  * y is rounded once; tokens do not affect each other's results, whatever their
- * adapters hold. Up to 256 tokens each takes its own adapter (neighbours with the
+ * adapters hold. A weight that is infinite or NaN makes the outputs that it enters
+ * infinite or NaN, but which of the two is not specified: the products meet x and
+ * A x in parts, some of them 0, and 0 inf is NaN where the formula has inf. An
+ * infinite x gives what the formula gives. Up to 256 tokens each takes its own adapter (neighbours with the
  * same one share its reads); more run in tiles of 16 consecutive tokens that read
  * each adapter occurring in them, so keep a request's tokens together, and give the
  * single-token requests of a batch a call of their own. T = 0 does nothing. The

@@ -554,3 +554,30 @@ def test_a_token_without_an_adapter_keeps_its_base(torch, dtype, T):
             none = s.apply(x, base, ids, xt, yt, none=True)
             assert (none[rest].view(kind) == 0).all()
     s.h.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T", [5, 256, 257])
+@pytest.mark.parametrize("rank", [1, 20, 128])
+def test_infinite_weights(torch, dtype, T, rank):
+    """An infinite or NaN element of B makes its own output so, one of A every output of
+    its adapter's tokens, whether by infinity or NaN; all others are as they should be."""
+    s = Setup(torch, 3, rank, 70, 66, dtype)
+    inf, nan = float("inf"), float("nan")
+    s.b[0, 9, rank - 1], s.b[0, 65, 0], s.b[0, 30, 0] = inf, -inf, nan
+    s.a[1, rank - 1, 69] = inf
+    for i in (0, 1):
+        s.load(i)
+    for xt, yt in io_types(dtype):
+        x, base, ids = s.inputs(T, xt, yt)
+        ids[0], ids[1], ids[2] = 0, 1, 2
+        x[3:] = x[3:].round()  # zeros among them: 0 inf is NaN in any arithmetic
+        with np.errstate(invalid="ignore"):
+            want, tol = s.expect(x, base, ids)
+        got = s.apply(x, base, ids, xt, yt).double().numpy()
+        fine = np.isfinite(want)
+        assert np.array_equal(np.isfinite(got), fine)
+        assert (~fine[0]).sum() == 3 and not fine[1].any() and fine[2].all()
+        assert (np.abs(got[fine] - want[fine]) <= tol[fine]).all()
+    s.h.close()
