@@ -213,7 +213,9 @@ class RouteSpec(ctypes.Structure):
 
 
 def _dev(a):
-    """_ptr of device memory, a tensor first: the host's share of a small call counts."""
+    """_ptr of device memory: an array is refused."""
+    if type(a) is int:
+        return a
     try:
         return a.data_ptr()
     except AttributeError:
@@ -222,38 +224,51 @@ def _dev(a):
         return _ptr(a)
 
 
-_KINDS = {"torch.float32": "f32", "torch.float16": "f16", "torch.bfloat16": "bf16"}
+_KINDS = {"torch.float32": "f32", "torch.float16": "f16", "torch.bfloat16": "bf16",
+          "torch.int32": "i32"}
+_kind_of = {}  # a torch dtype, once met: its name here
 
 
-def _kind(a, default, **others):
-    """The element type of a: a tensor's own, on the GPU and of a type that the operators
-    know, a pointer's the default. The others, name = (tensor, type): checked too."""
-    for name, (t, want) in others.items():
-        if hasattr(t, "data_ptr") and (not t.is_cuda or str(t.dtype) != "torch." + want):
-            raise TypeError(f"{name}: {t.dtype} on {t.device}, not {want} on the GPU")
-    if not hasattr(a, "data_ptr"):
-        return default
-    if not a.is_cuda or str(a.dtype) not in _KINDS:
-        raise TypeError(f"{a.dtype} on {a.device}, not f32, f16 or bf16 on the GPU")
-    return _KINDS[str(a.dtype)]
+def _met(a):
+    """The name of a tensor's element type, the first time it is met; of a pointer None."""
+    if hasattr(a, "data_ptr"):
+        _kind_of[a.dtype] = kind = _KINDS.get(str(a.dtype), "other")
+        return kind
+    _dev(a)  # refuses an array
+
+
+def _typed(name, a, want=None):
+    """The element type of a tensor on the GPU, checked: `want`, or one of DTYPES; of a
+    pointer `want`. A named type is checked as well: the kernels would read host memory, or
+    other elements, without a word."""
+    if type(a) is int:
+        return want
+    try:
+        kind = _kind_of[a.dtype]
+    except (AttributeError, KeyError):
+        kind = _met(a)
+        if kind is None:
+            return want
+    if not a.is_cuda or (kind != want if want else kind not in DTYPES):
+        raise TypeError(f"{name}: {a.dtype} on {a.device}, not {want or 'f32, f16 or bf16'} "
+                        "on the GPU")
+    return kind
 
 
 def route_experts(spec, logits, T, ids, w, dtype=None, row_stride=None, bias=None, stream=None):
     """ids [T x k] (int32) and w [T x k] (fp32) of T rows of logits in device memory
-    (hy3x_route_experts). Without a dtype: the logits' own (of a pointer, "f32"), and the
-    tensors' types and places are checked, which takes the host about 1 us."""
-    if dtype is None:
-        dtype = _kind(logits, "f32", ids=(ids, "int32"), w=(w, "float32"), bias=(bias, "float32"))
+    (hy3x_route_experts): tensors, whose types and places are checked, or pointers. Without
+    a dtype: the logits' own (of a pointer, "f32")."""
+    dtype = _typed("logits", logits, dtype) or "f32"
+    _typed("ids", ids, "i32")
+    _typed("w", w, "f32")
     if row_stride is None:
         row_stride = spec.n_expert
     if bias is not None:
+        _typed("bias", bias, "f32")
         bias = _dev(bias)
-    try:  # tensors, without a call of _dev for each
-        logits, ids, w = logits.data_ptr(), ids.data_ptr(), w.data_ptr()
-    except AttributeError:
-        logits, ids, w = _dev(logits), _dev(ids), _dev(w)
-    rc = (_lib or lib()).hy3x_route_experts(ctypes.byref(spec), logits, DTYPES[dtype], row_stride,
-                                            bias, T, ids, w, stream)
+    rc = (_lib or lib()).hy3x_route_experts(ctypes.byref(spec), _dev(logits), DTYPES[dtype],
+                                            row_stride, bias, T, _dev(ids), _dev(w), stream)
     if rc:
         _check(rc)
 
@@ -289,31 +304,27 @@ class Adapters:
             a, b = np.ascontiguousarray(a), np.ascontiguousarray(b)
             assert a.nbytes == 2 * self.rank * self.d_in and b.nbytes == 2 * self.rank * self.d_out
         else:
-            for t, n in ((a, self.rank * self.d_in), (b, self.rank * self.d_out)):
+            for name, t, n in (("a", a, self.rank * self.d_in), ("b", b, self.rank * self.d_out)):
                 if hasattr(t, "data_ptr"):
-                    assert _kind(t, None) == self.dtype and t.numel() == n and t.is_contiguous()
+                    assert _typed(name, t) == self.dtype and t.numel() == n and t.is_contiguous()
         a, b = (_dev(a), _dev(b)) if on_device else (_ptr(a), _ptr(b))
         _check(lib().hy3x_adapters_set(self._h, index, a, b, scale, 1 if on_device else 0))
 
     def apply(self, ids, x, y, T, base=None, x_dtype=None, y_dtype=None, x_stride=None,
               base_stride=None, y_stride=None, stream=None):
         """y[t] = base[t] + the product of adapter ids[t] with x[t], on device memory
-        (hy3x_adapters_apply). Types default to the tensors' own (of pointers, the adapters'),
-        which are then checked, as in route_experts; strides to dense rows; no base: 0."""
-        if x_dtype is None or y_dtype is None:
-            x_dtype = x_dtype or _kind(x, self.dtype, ids=(ids, "int32"))
-            y_dtype = y_dtype or _kind(y, self.dtype)
-            if base is not None and _kind(base, y_dtype) != y_dtype:
-                raise TypeError(f"base: {base.dtype}, y: {y_dtype}")
+        (hy3x_adapters_apply): tensors, whose types and places are checked, or pointers.
+        Types default to the tensors' own (of pointers, the adapters'); strides to dense
+        rows; no base: 0."""
+        _typed("ids", ids, "i32")
+        x_dtype = _typed("x", x, x_dtype) or self.dtype
+        y_dtype = _typed("y", y, y_dtype) or self.dtype
         if base is not None:
+            _typed("base", base, y_dtype)
             base = _dev(base)
-        try:  # tensors, without a call of _dev for each
-            ids, x, y = ids.data_ptr(), x.data_ptr(), y.data_ptr()
-        except AttributeError:
-            ids, x, y = _dev(ids), _dev(x), _dev(y)
-        rc = self._apply(self._h, ids, x, DTYPES[x_dtype],
+        rc = self._apply(self._h, _dev(ids), _dev(x), DTYPES[x_dtype],
                          self.d_in if x_stride is None else x_stride, base,
-                         self.d_out if base_stride is None else base_stride, y,
+                         self.d_out if base_stride is None else base_stride, _dev(y),
                          DTYPES[y_dtype],
                          self.d_out if y_stride is None else y_stride, T, stream)
         if rc:
