@@ -138,6 +138,11 @@ def _ptr(a):
         return None
     if type(a) is int:
         return a
+    try:  # as it mostly is, in as few calls as can be
+        if _kind_of[a.dtype] == want and a.is_cuda and a.numel() >= n and a.is_contiguous():
+            return a.data_ptr()
+    except (AttributeError, KeyError):
+        pass
     if isinstance(a, np.ndarray):
         assert a.flags["C_CONTIGUOUS"]
         return a.ctypes.data
@@ -239,36 +244,87 @@ def _met(a):
 
 def _typed(name, a, want=None):
     """The element type of a tensor on the GPU, checked: `want`, or one of DTYPES; of a
-    pointer `want`. A named type is checked as well: the kernels would read host memory, or
+    pointer None. A named type is checked as well: the kernels would read host memory, or
     other elements, without a word."""
-    if type(a) is int:
-        return want
     try:
         kind = _kind_of[a.dtype]
     except (AttributeError, KeyError):
         kind = _met(a)
         if kind is None:
-            return want
+            return None
     if not a.is_cuda or (kind != want if want else kind not in DTYPES):
         raise TypeError(f"{name}: {a.dtype} on {a.device}, not {want or 'f32, f16 or bf16'} "
                         "on the GPU")
     return kind
 
 
+def _flat(name, a, want, n):
+    """Pointer of n elements of type `want` in device memory: of a tensor, which has to
+    hold them one after another, or as given."""
+    if type(a) is int:
+        return a
+    try:  # as it mostly is, in as few calls as can be
+        if _kind_of[a.dtype] == want and a.is_cuda and a.numel() >= n and a.is_contiguous():
+            return a.data_ptr()
+    except (AttributeError, KeyError):
+        pass
+    if _typed(name, a, want) and (a.numel() < n or not a.is_contiguous()):
+        raise ValueError(f"{name}: {tuple(a.shape)}, strides {a.stride()}: not {n} elements "
+                         "one after another")
+    return _dev(a)
+
+
+def _rows(name, a, want, T, width, stride):
+    """Pointer, element type and row stride (elements) of T rows of `width` elements in
+    device memory. A tensor has its own type, and where no stride is named its own stride;
+    its memory has to hold the rows. Of a pointer: as named, dense rows."""
+    if type(a) is int:
+        return a, want, width if stride is None else stride
+    try:  # rows of the named type and stride, in as few calls as can be
+        if _kind_of[a.dtype] == want and a.is_cuda:
+            shape = a.shape
+            if shape[-1] == width and (
+                    stride in (None, width) and a.is_contiguous() and a.numel() >= T * width
+                    or len(shape) == 2 and shape[0] >= T and a.stride() == (stride, 1)):
+                return a.data_ptr(), want, width if stride is None else stride
+    except (AttributeError, KeyError, IndexError):
+        pass
+    kind = _typed(name, a, want)
+    if kind is None:
+        return _dev(a), want, width if stride is None else stride
+    if a.is_contiguous():
+        if stride is None:
+            if a.ndim > 1 and a.shape[-1] != width:
+                raise ValueError(f"{name}: {tuple(a.shape)}, not rows of {width}")
+            stride = width
+        if a.numel() >= (T - 1) * stride + width or T < 1:
+            return a.data_ptr(), kind, stride
+    else:
+        if a.shape[-1] > 1 and a.stride(-1) != 1:
+            raise ValueError(f"{name}: strides {a.stride()}: a row's elements lie apart")
+        if stride is None:
+            if a.ndim != 2 or a.shape[1] != width or a.shape[0] < T:
+                raise ValueError(f"{name}: {tuple(a.shape)}, not {T} rows of {width}")
+            stride = a.stride(0) if T > 1 else width
+    # a named stride may go beyond the tensor itself, in the buffer that it is a part of
+    held = a.untyped_storage().nbytes() // a.element_size() - a.storage_offset()
+    if held < (T - 1) * stride + width and T > 0:
+        raise ValueError(f"{name}: {tuple(a.shape)} does not hold {T} rows of {width}, "
+                         f"{stride} apart")
+    return a.data_ptr(), kind, stride
+
+
 def route_experts(spec, logits, T, ids, w, dtype=None, row_stride=None, bias=None, stream=None):
     """ids [T x k] (int32) and w [T x k] (fp32) of T rows of logits in device memory
-    (hy3x_route_experts): tensors, whose types and places are checked, or pointers. Without
-    a dtype: the logits' own (of a pointer, "f32")."""
-    dtype = _typed("logits", logits, dtype) or "f32"
-    _typed("ids", ids, "i32")
-    _typed("w", w, "f32")
-    if row_stride is None:
-        row_stride = spec.n_expert
+    (hy3x_route_experts): tensors, whose types, places and sizes are checked, or pointers.
+    Without a dtype and row_stride: the logits' own (of a pointer, "f32" and dense rows)."""
+    logits, dtype, row_stride = _rows("logits", logits, dtype, T, spec.n_expert, row_stride)
+    n = T * spec.k
     if bias is not None:
-        _typed("bias", bias, "f32")
-        bias = _dev(bias)
-    rc = (_lib or lib()).hy3x_route_experts(ctypes.byref(spec), _dev(logits), DTYPES[dtype],
-                                            row_stride, bias, T, _dev(ids), _dev(w), stream)
+        bias = _flat("bias", bias, "f32", spec.n_expert)
+    rc = (_lib or lib()).hy3x_route_experts(ctypes.byref(spec), logits, DTYPES[dtype or "f32"],
+                                            row_stride, bias, T, _flat("ids", ids, "i32", n),
+                                            _flat("w", w, "f32", n), stream)
     if rc:
         _check(rc)
 
@@ -313,20 +369,16 @@ class Adapters:
     def apply(self, ids, x, y, T, base=None, x_dtype=None, y_dtype=None, x_stride=None,
               base_stride=None, y_stride=None, stream=None):
         """y[t] = base[t] + the product of adapter ids[t] with x[t], on device memory
-        (hy3x_adapters_apply): tensors, whose types and places are checked, or pointers.
-        Types default to the tensors' own (of pointers, the adapters'); strides to dense
-        rows; no base: 0."""
-        _typed("ids", ids, "i32")
-        x_dtype = _typed("x", x, x_dtype) or self.dtype
-        y_dtype = _typed("y", y, y_dtype) or self.dtype
+        (hy3x_adapters_apply): tensors, whose types, places and sizes are checked, or
+        pointers. Types and strides default to the tensors' own (of pointers, the adapters'
+        type and dense rows); no base: 0."""
+        x, x_dtype, x_stride = _rows("x", x, x_dtype, T, self.d_in, x_stride)
+        y, y_dtype, y_stride = _rows("y", y, y_dtype, T, self.d_out, y_stride)
+        y_dtype = y_dtype or self.dtype
         if base is not None:
-            _typed("base", base, y_dtype)
-            base = _dev(base)
-        rc = self._apply(self._h, _dev(ids), _dev(x), DTYPES[x_dtype],
-                         self.d_in if x_stride is None else x_stride, base,
-                         self.d_out if base_stride is None else base_stride, _dev(y),
-                         DTYPES[y_dtype],
-                         self.d_out if y_stride is None else y_stride, T, stream)
+            base, _, base_stride = _rows("base", base, y_dtype, T, self.d_out, base_stride)
+        rc = self._apply(self._h, _flat("ids", ids, "i32", T), x, DTYPES[x_dtype or self.dtype],
+                         x_stride, base, base_stride or 0, y, DTYPES[y_dtype], y_stride, T, stream)
         if rc:
             _check(rc)
 

@@ -111,3 +111,105 @@ def test_pointers_have_the_named_or_the_default_type(calls, handle):
     handle.apply(4096, 8192, 16384, 5, x_dtype="f32", base=32768)
     assert [c[3] for c in calls[2:]] == [H.DTYPES["bf16"], H.DTYPES["f32"]]
     assert [c[8] for c in calls[2:]] == [H.DTYPES["bf16"]] * 2
+
+
+# ---------------------------------------------------------------- strides and sizes
+def part(rows, wide, cols, at=0, dtype=torch.float32):
+    """Columns of a wider buffer."""
+    return OnGPU(torch.zeros(rows, wide, dtype=dtype)[:, at:at + cols])
+
+
+def test_route_takes_the_rows_as_they_lie(calls):
+    wide, one = part(5, 256, 192, 3), part(1, 256, 192)
+    H.route_experts(SPEC, **route_args(logits=wide))
+    H.route_experts(SPEC, **route_args(logits=wide, row_stride=256))
+    H.route_experts(SPEC, **route_args(logits=wide, T=2))
+    H.route_experts(SPEC, **route_args(logits=one, T=1))
+    H.route_experts(SPEC, **route_args(logits=on_gpu(5 * 192)))          # dense, flat
+    H.route_experts(SPEC, **route_args(logits=on_gpu(5, 1, 192)))        # dense, more axes
+    H.route_experts(SPEC, **route_args(logits=on_gpu(5, 256), row_stride=256))
+    H.route_experts(SPEC, **route_args(logits=part(1, 5 * 256, 192), row_stride=256))
+    H.route_experts(SPEC, **route_args(logits=on_gpu(5, 192), T=0))
+    assert [c[3] for c in calls] == [256, 256, 256, 192, 192, 192, 256, 256, 192]
+    assert calls[0][1] == wide.data_ptr()
+    # one row for all tokens: its stride of 0 reaches the library, which refuses it
+    for named in ({}, dict(row_stride=0), dict(dtype="f32"), dict(dtype="f32", row_stride=0)):
+        H.route_experts(SPEC, **route_args(logits=OnGPU(torch.zeros(1, 192).expand(5, 192))), **named)
+        assert calls[-1][3] == 0
+    # one expert: a column of anything
+    H.route_experts(H.RouteSpec(1, 1), OnGPU(torch.zeros(5, 3)[:, 1:2]),
+                    5, on_gpu(5, dtype=I32), on_gpu(5))
+    assert calls[-1][3] == 3
+
+
+@pytest.mark.parametrize("named", [{}, dict(dtype="f32")])
+def test_route_refuses_rows_that_are_not_there(calls, named):
+    for bad in (dict(logits=on_gpu(4, 192)), dict(logits=on_gpu(5, 256)), dict(logits=on_gpu(5, 96)),
+                dict(logits=OnGPU(torch.zeros(192, 5).t())), dict(logits=part(5, 256, 191)),
+                dict(logits=part(4, 256, 192)), dict(logits=OnGPU(torch.zeros(5, 384)[:, ::2])),
+                dict(logits=OnGPU(torch.zeros(5, 384)[:, ::2]), row_stride=384),
+                dict(logits=on_gpu(5, 192), row_stride=193), dict(logits=on_gpu(5 * 192 - 1)),
+                dict(logits=part(5, 256, 192, 64), row_stride=257),
+                dict(logits=OnGPU(torch.zeros(5, 2, 400)[:, :, :192])),
+                dict(ids=on_gpu(5, 7, dtype=I32)), dict(ids=part(5, 16, 8, dtype=I32)),
+                dict(ids=on_gpu(4, 8, dtype=I32)), dict(w=on_gpu(39)), dict(w=part(5, 9, 8)),
+                dict(bias=on_gpu(191)), dict(bias=OnGPU(torch.zeros(384)[::2])), dict(T=6)):
+        with pytest.raises(ValueError):
+            H.route_experts(SPEC, **route_args(**bad), **named)
+    assert not calls
+
+
+def test_apply_takes_the_rows_as_they_lie(calls, handle):
+    x, base = part(5, 100, 64, 7, BF16), part(5, 200, 96, 0, BF16)
+    y = part(5, 300, 96, 5, BF16)
+    handle.apply(**apply_args(x=x, base=base, y=y))
+    handle.apply(**apply_args(x=x, base=y, y=y, x_stride=100, y_stride=300))
+    handle.apply(**apply_args(ids=on_gpu(9, dtype=I32)))
+    assert [(c[4], c[9]) for c in calls] == [(100, 300), (100, 300), (64, 96)]
+    assert [c[6] for c in calls[:2]] == [200, 300] and calls[2][5] is None
+    assert (calls[0][2], calls[0][5], calls[0][7]) == (x.data_ptr(), base.data_ptr(), y.data_ptr())
+    handle.apply(4096, 8192, 16384, 5, base=32768)
+    assert (calls[-1][4], calls[-1][6], calls[-1][9]) == (64, 96, 96)
+
+
+@pytest.mark.parametrize("named", [{}, dict(x_dtype="bf16", y_dtype="bf16")])
+def test_apply_refuses_rows_that_are_not_there(calls, handle, named):
+    for bad in (dict(ids=on_gpu(4, dtype=I32)), dict(ids=OnGPU(torch.zeros(10, dtype=I32)[::2])),
+                dict(x=on_gpu(4, 64, dtype=BF16)), dict(x=on_gpu(5, 65, dtype=BF16)),
+                dict(x=OnGPU(torch.zeros(64, 5, dtype=BF16).t())), dict(x=part(4, 100, 64, dtype=BF16)),
+                dict(x_stride=65), dict(y=on_gpu(5, 95, dtype=BF16)), dict(y_stride=97),
+                dict(y=part(5, 100, 95, dtype=BF16)), dict(base=on_gpu(4, 96, dtype=BF16)),
+                dict(base=on_gpu(5, 97, dtype=BF16)), dict(base=on_gpu(5, 96, dtype=BF16), base_stride=98),
+                dict(base=on_gpu(1, 96, dtype=BF16)), dict(T=6)):
+        with pytest.raises(ValueError):
+            handle.apply(**apply_args(**bad), **named)
+    assert not calls
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 7])
+def test_parts_of_wider_buffers_on_the_gpu(T):
+    assert torch.cuda.is_available(), "no GPU"
+    g = torch.Generator().manual_seed(T)
+    wide = torch.randn(T, 256, generator=g).cuda()
+    got, want = ([torch.zeros(T, 8, dtype=I32, device="cuda"), torch.zeros(T, 8, device="cuda")]
+                 for _ in range(2))
+    H.route_experts(SPEC, wide[:, 20:212], T, *got)
+    H.route_experts(SPEC, wide[:, 20:212].contiguous(), T, *want)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    h = H.Adapters(2, 8, 64, 96)
+    for i in range(2):
+        h.set(i, torch.randn(8, 64, generator=g).bfloat16().cuda(),
+              torch.randn(96, 8, generator=g).bfloat16().cuda(), on_device=True)
+    x = torch.randn(T, 80, generator=g).bfloat16().cuda()[:, 3:67]
+    base = torch.randn(T, 100, generator=g).bfloat16().cuda()[:, 1:97]
+    y = torch.full((T, 120), 5.0, dtype=BF16, device="cuda")
+    ids = (torch.arange(T) % 3 - 1).int().cuda()
+    dense = torch.zeros(T, 96, dtype=BF16, device="cuda")
+    h.apply(ids, x, y[:, 7:103], T, base=base)
+    h.apply(ids, x.contiguous(), dense, T, base=base.contiguous())
+    torch.cuda.synchronize()
+    assert torch.equal(y[:, 7:103], dense)
+    assert (y[:, :7] == 5.0).all() and (y[:, 103:] == 5.0).all()
+    h.close()
