@@ -535,9 +535,10 @@ class MoELayer:
     def forward_adapters(self, x_dev_ptr, adapter_ids, T, attn_dev_ptr=None, K=K_MAX,
                          scale=ROUTE_SCALE, stream=None):
         """The block for tokens with adapters of their own, adapter_ids [T] int32 in device
-        memory (hy3x_layer_forward_adapters)."""
-        _check(lib().hy3x_layer_forward_adapters(self._h, x_dev_ptr, attn_dev_ptr,
-                                                 _dev(adapter_ids), T, K, scale, stream))
+        memory, a tensor (checked) or a pointer (hy3x_layer_forward_adapters)."""
+        ids = _flat("adapter_ids", adapter_ids, "i32", T)
+        _check(lib().hy3x_layer_forward_adapters(self._h, x_dev_ptr, attn_dev_ptr, ids, T, K,
+                                                 scale, stream))
 
     def last_shape(self):
         """(T, K) of the last forward."""

@@ -213,3 +213,34 @@ def test_parts_of_wider_buffers_on_the_gpu(T):
     assert torch.equal(y[:, 7:103], dense)
     assert (y[:, :7] == 5.0).all() and (y[:, 103:] == 5.0).all()
     h.close()
+
+
+# ---------------------------------------------------------------- the layer's adapters
+@pytest.fixture
+def layer(calls, monkeypatch):
+    L = H.MoELayer.__new__(H.MoELayer)
+    L._h = None
+
+    def record(*args):
+        calls.append(args)
+        return 0
+    for name in ("forward", "forward_static", "forward_residual", "forward_adapters",
+                 "set_adapters", "time_stage"):
+        setattr(H._lib, "hy3x_layer_" + name, record)
+    setattr(H._lib, "hy3x_layers_time_stage", record)
+    return L
+
+
+def test_layer_adapter_ids(calls, layer):
+    ids = on_gpu(6, dtype=I32)
+    layer.forward_adapters(4096, ids, 5)
+    layer.forward_adapters(4096, 8192, 5)
+    assert [c[3] for c in calls] == [ids.data_ptr(), 8192]
+    for bad in (torch.zeros(5, dtype=I32), on_gpu(5, dtype=torch.int64), on_gpu(5),
+                np.zeros(5, np.int32)):
+        with pytest.raises(TypeError):
+            layer.forward_adapters(4096, bad, 5)
+    for bad in (on_gpu(4, dtype=I32), OnGPU(torch.zeros(10, dtype=I32)[::2])):
+        with pytest.raises(ValueError):
+            layer.forward_adapters(4096, bad, 5)
+    assert len(calls) == 2
