@@ -184,6 +184,8 @@ def gguf_check_layer(path, layer_index):
 def layers_time_stage(layers, stage, reps, stream=None):
     """Mean µs per launch of one stage's kernels replayed over `layers` in rotation
     (hy3x_layers_time_stage)."""
+    for L in layers:
+        _still_open(L._ran)
     arr = (P * len(layers))(*[L._h for L in layers])
     us = ctypes.c_float()
     _check(lib().hy3x_layers_time_stage(arr, len(layers), MoELayer.STAGES.index(stage), reps,
@@ -383,6 +385,14 @@ class Adapters:
             _check(rc)
 
 
+def _still_open(adapters):
+    """Refuses adapters that were closed after a layer received them: it holds their
+    address."""
+    for a in adapters:
+        if not a._h:
+            raise HY3XError("adapters that the layer uses are closed")
+
+
 class MoELayer:
     """One Hy3 MoE FFN layer resident on the current HIP device."""
 
@@ -483,6 +493,7 @@ class MoELayer:
     def time_stage(self, stage, reps, stream=None):
         """Mean µs per launch of one stage's kernels, replayed `reps` times back to
         back after the last forward (hy3x_layer_time_stage)."""
+        _still_open(self._ran)
         us = ctypes.c_float()
         _check(lib().hy3x_layer_time_stage(self._h, self.STAGES.index(stage), reps, stream,
                                            ctypes.byref(us)))
@@ -504,19 +515,24 @@ class MoELayer:
     def forward(self, x_dev_ptr, T, K=K_MAX, scale=ROUTE_SCALE, stream=None):
         """In-place MoE block on device memory x[T x 4096] (fp32)."""
         _check(lib().hy3x_layer_forward(self._h, x_dev_ptr, T, K, scale, stream))
+        self._ran = ()
 
     def forward_static(self, x_dev_ptr, T, K=K_MAX, scale=ROUTE_SCALE, stream=None):
         """forward() on the library's static per-GPU scratch: no allocation
         (hy3x_layer_forward_static; T <= 64)."""
         _check(lib().hy3x_layer_forward_static(self._h, x_dev_ptr, T, K, scale, stream))
+        self._ran = ()
 
     def forward_residual(self, x_dev_ptr, attn_dev_ptr, T, K=K_MAX, scale=ROUTE_SCALE,
                          stream=None):
         """x += attn_out, then the MoE block, in one forward (hy3x_layer_forward_residual)."""
         _check(lib().hy3x_layer_forward_residual(self._h, x_dev_ptr, attn_dev_ptr, T, K, scale,
                                                  stream))
+        self._ran = ()
 
     PROJECTIONS = ("router", "gate", "up", "down")
+    _adapters = {}  # projection -> Adapters or None, as set
+    _ran = ()       # the adapters of the last forward, which a replay of it launches again
 
     def set_routing(self, spec=None):
         """Route by `spec` (a RouteSpec; its k and scale are each forward's), or by the
@@ -530,15 +546,18 @@ class MoELayer:
             raise HY3XError("the adapters are closed")
         _check(lib().hy3x_layer_set_adapters(self._h, self.PROJECTIONS.index(projection),
                                              None if adapters is None else adapters._h))
-        self._adapters = dict(getattr(self, "_adapters", {}), **{projection: adapters})
+        self._adapters = dict(self._adapters, **{projection: adapters})
 
     def forward_adapters(self, x_dev_ptr, adapter_ids, T, attn_dev_ptr=None, K=K_MAX,
                          scale=ROUTE_SCALE, stream=None):
         """The block for tokens with adapters of their own, adapter_ids [T] int32 in device
         memory, a tensor (checked) or a pointer (hy3x_layer_forward_adapters)."""
         ids = _flat("adapter_ids", adapter_ids, "i32", T)
+        held = tuple(a for a in self._adapters.values() if a is not None)
+        _still_open(held)
         _check(lib().hy3x_layer_forward_adapters(self._h, x_dev_ptr, attn_dev_ptr, ids, T, K,
                                                  scale, stream))
+        self._ran = held
 
     def last_shape(self):
         """(T, K) of the last forward."""

@@ -393,3 +393,23 @@ def test_kernel_names_and_replays(block):
             assert layer.time_stage(stage, 2) >= 0.0
     layer.forward(x.data_ptr(), 400)
     assert layer.last_kernel("gateup").startswith("mfma_wide::")
+
+
+@pytest.mark.gpu
+def test_adapters_closed_while_set_are_refused(block):
+    torch, layer = block.torch, block.layer
+    x = torch.from_numpy(C.inputs(0xAC, 6).copy()).cuda()
+    ids = torch.zeros(6, dtype=torch.int32, device="cuda")
+    h = H.Adapters(1, 8, D, F, "f16")
+    layer.set_adapters("up", h)
+    layer.forward_adapters(x.data_ptr(), ids, 6)
+    torch.cuda.synchronize()
+    h.close()
+    with pytest.raises(H.HY3XError, match="closed"):
+        layer.forward_adapters(x.data_ptr(), ids, 6)
+    with pytest.raises(H.HY3XError, match="closed"):
+        layer.time_stage("gateup", 1)
+    layer.set_adapters("up", None)
+    layer.forward_adapters(x.data_ptr(), ids, 6)  # none set: the block as it is
+    assert layer.time_stage("gateup", 1) >= 0.0
+    torch.cuda.synchronize()

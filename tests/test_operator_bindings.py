@@ -244,3 +244,64 @@ def test_layer_adapter_ids(calls, layer):
         with pytest.raises(ValueError):
             layer.forward_adapters(4096, bad, 5)
     assert len(calls) == 2
+
+
+def open_handle():
+    h = H.Adapters.__new__(H.Adapters)
+    h._h = 4096
+    return h
+
+
+def closed(h):
+    h._h = None  # as close() leaves it
+
+
+def test_closed_adapters_of_a_layer(calls, layer):
+    """Closed after they were set: refused by every call that would launch them."""
+    gate, down = open_handle(), open_handle()
+    try:
+        layer.set_adapters("gate", gate)
+        layer.set_adapters("down", down)
+        layer.forward_adapters(4096, 8192, 5)
+        layer.time_stage("gateup", 1)
+        closed(gate)
+        n = len(calls)
+        for call in (lambda: layer.forward_adapters(4096, 8192, 5),
+                     lambda: layer.time_stage("gateup", 1),
+                     lambda: H.layers_time_stage([layer], "gateup", 1)):
+            with pytest.raises(H.HY3XError, match="closed"):
+                call()
+        layer.set_adapters("gate", None)  # the last forward's replay still has it
+        with pytest.raises(H.HY3XError, match="closed"):
+            layer.time_stage("combine", 1)
+        assert len(calls) == n + 1
+        layer.forward_adapters(4096, 8192, 5)
+        layer.time_stage("gateup", 1)
+        for run in (lambda: layer.forward(4096, 5), lambda: layer.forward_static(4096, 5),
+                    lambda: layer.forward_residual(4096, 8192, 5)):
+            closed(down)
+            with pytest.raises(H.HY3XError, match="closed"):
+                layer.forward_adapters(4096, 16384, 5)
+            run()  # uses no adapters, and nor does its replay
+            layer.time_stage("gateup", 1)
+            down._h = 4096
+    finally:
+        closed(gate), closed(down)
+
+
+def test_a_layer_keeps_the_adapters_of_its_last_forward(layer):
+    import gc
+    import weakref
+    h = open_handle()
+    alive = weakref.ref(h)
+    h.close = lambda: None
+    layer.set_adapters("up", h)
+    layer.forward_adapters(4096, 8192, 5)
+    layer.set_adapters("up", None)
+    del h
+    gc.collect()
+    assert alive() is not None  # its replay launches them
+    closed(alive())
+    layer.forward(4096, 5)
+    gc.collect()
+    assert alive() is None
