@@ -355,16 +355,26 @@ class Adapters:
         except Exception:
             pass
 
+    _NAMES = {"f16": "float16", "bf16": "bfloat16"}
+
     def set(self, index, a, b, scale=1.0, on_device=False):
         """Adapter `index`: a [rank x d_in], b [d_out x rank], two-byte elements of the
-        handle's type (arrays of them, or device memory with on_device)."""
+        handle's type (arrays of them, or of their bits as 16-bit integers; device memory
+        with on_device: contiguous tensors of the type, or pointers)."""
         if not on_device:
             a, b = np.ascontiguousarray(a), np.ascontiguousarray(b)
-            assert a.nbytes == 2 * self.rank * self.d_in and b.nbytes == 2 * self.rank * self.d_out
-        else:
-            for name, t, n in (("a", a, self.rank * self.d_in), ("b", b, self.rank * self.d_out)):
-                if hasattr(t, "data_ptr"):
-                    assert _typed(name, t) == self.dtype and t.numel() == n and t.is_contiguous()
+        for name, m, shape in (("a", a, (self.rank, self.d_in)), ("b", b, (self.d_out, self.rank))):
+            if on_device and not hasattr(m, "data_ptr"):
+                continue  # a pointer
+            axes = [n for n in m.shape if n != 1]
+            if axes not in ([n for n in shape if n != 1], [shape[0] * shape[1]]):
+                raise ValueError(f"{name}: {tuple(m.shape)}, not {shape}")
+            if on_device:
+                assert _typed(name, m) == self.dtype
+                if not m.is_contiguous():
+                    raise ValueError(f"{name}: not contiguous")
+            elif m.dtype.name not in ("int16", "uint16", self._NAMES[self.dtype]):
+                raise TypeError(f"{name}: {m.dtype}, not {self.dtype} or its bits")
         a, b = (_dev(a), _dev(b)) if on_device else (_ptr(a), _ptr(b))
         _check(lib().hy3x_adapters_set(self._h, index, a, b, scale, 1 if on_device else 0))
 

@@ -305,3 +305,30 @@ def test_a_layer_keeps_the_adapters_of_its_last_forward(layer):
     layer.forward(4096, 5)
     gc.collect()
     assert alive() is None
+
+
+# ---------------------------------------------------------------- weights
+def test_set_takes_weights_of_its_own_type_and_shape(calls, handle):
+    a, b = np.zeros((8, 64), np.uint16), np.zeros((96, 8), np.int16)
+    handle.set(1, a, b)
+    handle.set(1, a.ravel(), b.ravel())
+    handle.set(1, a[None], b[:, None])
+    handle.set(1, on_gpu(8, 64, dtype=BF16), on_gpu(96, 8, dtype=BF16), on_device=True)
+    handle.set(1, 4096, 8192, on_device=True)
+    assert calls[-1][2:4] == (4096, 8192) and len(calls) == 5
+    for bad in ((a.astype(np.float16), b), (a, b.astype(np.float16)), (a.astype(np.float32), b),
+                (a.astype(np.uint8), b)):
+        with pytest.raises(TypeError):
+            handle.set(1, *bad)
+    for bad in ((a.T, b), (a, b.T), (a[:7], b), (a, b[:95]), (a.reshape(4, 128), b),
+                (a[:, :32].astype(np.uint32), b)):
+        with pytest.raises(ValueError):
+            handle.set(1, *bad)
+    ad, bd = torch.zeros(8, 64, dtype=BF16), torch.zeros(96, 8, dtype=BF16)
+    for bad in ((OnGPU(ad.t().contiguous()), OnGPU(bd)), (OnGPU(ad), OnGPU(bd.t().contiguous())),
+                (OnGPU(torch.zeros(64, 8, dtype=BF16).t()), OnGPU(bd)), (OnGPU(ad[:7]), OnGPU(bd))):
+        with pytest.raises(ValueError):
+            handle.set(1, *bad, on_device=True)
+    handle.dtype = "f16"
+    handle.set(1, a.astype(np.float16), b)
+    assert len(calls) == 6
