@@ -138,11 +138,6 @@ def _ptr(a):
         return None
     if type(a) is int:
         return a
-    try:  # as it mostly is, in as few calls as can be
-        if _kind_of[a.dtype] == want and a.is_cuda and a.numel() >= n and a.is_contiguous():
-            return a.data_ptr()
-    except (AttributeError, KeyError):
-        pass
     if isinstance(a, np.ndarray):
         assert a.flags["C_CONTIGUOUS"]
         return a.ctypes.data

@@ -332,3 +332,12 @@ def test_set_takes_weights_of_its_own_type_and_shape(calls, handle):
     handle.dtype = "f16"
     handle.set(1, a.astype(np.float16), b)
     assert len(calls) == 6
+
+
+def test_pointers_of_what_the_binding_takes(calls):
+    H.route_experts(SPEC, **route_args())  # has met fp32 and int32 tensors
+    for t in (torch.zeros(3), torch.zeros(3, dtype=I32), torch.zeros(3, dtype=torch.uint8)):
+        assert H._ptr(t) == H._dev(t) == t.data_ptr()
+    n = np.zeros(3, np.float32)
+    assert H._ptr(n) == n.ctypes.data and H._ptr(np.int64(4096)) == H._dev(np.int64(4096)) == 4096
+    assert H._ptr(None) is H._dev(None) is None and H._ptr(4096) == H._dev(4096) == 4096
