@@ -13,6 +13,7 @@ gpu_ffn_moe (hy3_gpu.cu:706-738) and its upload in hy3_gpu_init
 """
 import ctypes
 import os
+import sys
 
 import numpy as np
 
@@ -239,10 +240,24 @@ def _met(a):
     _dev(a)  # refuses an array
 
 
+_gpus = None  # how many GPUs this process sees, once counted
+
+
+def _here():
+    """Index of the current device, where the kernels run."""
+    global _gpus
+    if _gpus is None:
+        torch = sys.modules.get("torch")
+        if torch is None:
+            return 0  # no tensors either
+        _gpus = torch.cuda.device_count()
+    return sys.modules["torch"].cuda.current_device() if _gpus > 1 else 0
+
+
 def _typed(name, a, want=None):
-    """The element type of a tensor on the GPU, checked: `want`, or one of DTYPES; of a
-    pointer None. A named type is checked as well: the kernels would read host memory, or
-    other elements, without a word."""
+    """The element type of a tensor on the current device, checked: `want`, or one of
+    DTYPES; of a pointer None. A named type is checked as well: the kernels would read host
+    memory, another GPU's, or other elements, without a word."""
     try:
         kind = _kind_of[a.dtype]
     except (AttributeError, KeyError):
@@ -252,16 +267,19 @@ def _typed(name, a, want=None):
     if not a.is_cuda or (kind != want if want else kind not in DTYPES):
         raise TypeError(f"{name}: {a.dtype} on {a.device}, not {want or 'f32, f16 or bf16'} "
                         "on the GPU")
+    if a.get_device() != _here():
+        raise ValueError(f"{name}: on {a.device}, the current device is {_here()}")
     return kind
 
 
-def _flat(name, a, want, n):
-    """Pointer of n elements of type `want` in device memory: of a tensor, which has to
-    hold them one after another, or as given."""
+def _flat(name, a, want, n, here):
+    """Pointer of n elements of type `want` in the memory of device `here`, the current
+    one: of a tensor, which has to hold them one after another, or as given."""
     if type(a) is int:
         return a
     try:  # as it mostly is, in as few calls as can be
-        if _kind_of[a.dtype] == want and a.is_cuda and a.numel() >= n and a.is_contiguous():
+        if (_kind_of[a.dtype] == want and a.get_device() == here and a.numel() >= n
+                and a.is_contiguous()):
             return a.data_ptr()
     except (AttributeError, KeyError):
         pass
@@ -271,14 +289,15 @@ def _flat(name, a, want, n):
     return _dev(a)
 
 
-def _rows(name, a, want, T, width, stride):
+def _rows(name, a, want, T, width, stride, here):
     """Pointer, element type and row stride (elements) of T rows of `width` elements in
-    device memory. A tensor has its own type, and where no stride is named its own stride;
-    its memory has to hold the rows. Of a pointer: as named, dense rows."""
+    the memory of device `here`, the current one. A tensor has its own type, and where no
+    stride is named its own stride; its memory has to hold the rows. Of a pointer: as
+    named, dense rows."""
     if type(a) is int:
         return a, want, width if stride is None else stride
     try:  # rows of the named type and stride, in as few calls as can be
-        if _kind_of[a.dtype] == want and a.is_cuda:
+        if _kind_of[a.dtype] == want and a.get_device() == here:
             shape = a.shape
             if shape[-1] == width and (
                     stride in (None, width) and a.is_contiguous() and a.numel() >= T * width
@@ -315,13 +334,14 @@ def route_experts(spec, logits, T, ids, w, dtype=None, row_stride=None, bias=Non
     """ids [T x k] (int32) and w [T x k] (fp32) of T rows of logits in device memory
     (hy3x_route_experts): tensors, whose types, places and sizes are checked, or pointers.
     Without a dtype and row_stride: the logits' own (of a pointer, "f32" and dense rows)."""
-    logits, dtype, row_stride = _rows("logits", logits, dtype, T, spec.n_expert, row_stride)
+    here = _here()
+    logits, dtype, row_stride = _rows("logits", logits, dtype, T, spec.n_expert, row_stride, here)
     n = T * spec.k
     if bias is not None:
-        bias = _flat("bias", bias, "f32", spec.n_expert)
+        bias = _flat("bias", bias, "f32", spec.n_expert, here)
     rc = (_lib or lib()).hy3x_route_experts(ctypes.byref(spec), logits, DTYPES[dtype or "f32"],
-                                            row_stride, bias, T, _flat("ids", ids, "i32", n),
-                                            _flat("w", w, "f32", n), stream)
+                                            row_stride, bias, T, _flat("ids", ids, "i32", n, here),
+                                            _flat("w", w, "f32", n, here), stream)
     if rc:
         _check(rc)
 
@@ -379,13 +399,15 @@ class Adapters:
         (hy3x_adapters_apply): tensors, whose types, places and sizes are checked, or
         pointers. Types and strides default to the tensors' own (of pointers, the adapters'
         type and dense rows); no base: 0."""
-        x, x_dtype, x_stride = _rows("x", x, x_dtype, T, self.d_in, x_stride)
-        y, y_dtype, y_stride = _rows("y", y, y_dtype, T, self.d_out, y_stride)
+        here = _here()
+        ids = _flat("ids", ids, "i32", T, here)
+        x, x_dtype, x_stride = _rows("x", x, x_dtype, T, self.d_in, x_stride, here)
+        y, y_dtype, y_stride = _rows("y", y, y_dtype, T, self.d_out, y_stride, here)
         y_dtype = y_dtype or self.dtype
         if base is not None:
-            base, _, base_stride = _rows("base", base, y_dtype, T, self.d_out, base_stride)
-        rc = self._apply(self._h, _flat("ids", ids, "i32", T), x, DTYPES[x_dtype or self.dtype],
-                         x_stride, base, base_stride or 0, y, DTYPES[y_dtype], y_stride, T, stream)
+            base, _, base_stride = _rows("base", base, y_dtype, T, self.d_out, base_stride, here)
+        rc = self._apply(self._h, ids, x, DTYPES[x_dtype or self.dtype], x_stride, base,
+                         base_stride or 0, y, DTYPES[y_dtype], y_stride, T, stream)
         if rc:
             _check(rc)
 
@@ -557,7 +579,7 @@ class MoELayer:
                          scale=ROUTE_SCALE, stream=None):
         """The block for tokens with adapters of their own, adapter_ids [T] int32 in device
         memory, a tensor (checked) or a pointer (hy3x_layer_forward_adapters)."""
-        ids = _flat("adapter_ids", adapter_ids, "i32", T)
+        ids = _flat("adapter_ids", adapter_ids, "i32", T, _here())
         held = tuple(a for a in self._adapters.values() if a is not None)
         _still_open(held)
         _check(lib().hy3x_layer_forward_adapters(self._h, x_dev_ptr, attn_dev_ptr, ids, T, K,

@@ -341,3 +341,42 @@ def test_pointers_of_what_the_binding_takes(calls):
     n = np.zeros(3, np.float32)
     assert H._ptr(n) == n.ctypes.data and H._ptr(np.int64(4096)) == H._dev(np.int64(4096)) == 4096
     assert H._ptr(None) is H._dev(None) is None and H._ptr(4096) == H._dev(4096) == 4096
+
+
+# ---------------------------------------------------------------- devices
+class OnOther(OnGPU):
+    device = "cuda:1"
+
+    def get_device(self):
+        return 1
+
+
+@pytest.mark.parametrize("named", [False, True])
+def test_tensors_of_another_device(calls, handle, layer, monkeypatch, named):
+    """Refused unless their device is the current one, where the kernels run."""
+    monkeypatch.setattr(H, "_gpus", 2)
+    now = [0]
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    kinds = dict(dtype="f32") if named else {}
+    types = dict(x_dtype="bf16", y_dtype="bf16") if named else {}
+    route = route_args(bias=on_gpu(192))
+    apply = apply_args(base=on_gpu(5, 96, dtype=BF16))
+    H.route_experts(SPEC, **route, **kinds)
+    handle.apply(**apply, **types)
+    for name in ("logits", "ids", "w", "bias"):
+        with pytest.raises(ValueError, match="current device"):
+            H.route_experts(SPEC, **dict(route, **{name: OnOther(route[name].t)}), **kinds)
+    for name in ("ids", "x", "y", "base"):
+        with pytest.raises(ValueError, match="current device"):
+            handle.apply(**dict(apply, **{name: OnOther(apply[name].t)}), **types)
+    a, b = torch.zeros(8, 64, dtype=BF16), torch.zeros(96, 8, dtype=BF16)
+    with pytest.raises(ValueError, match="current device"):
+        handle.set(0, OnGPU(a), OnOther(b), on_device=True)
+    with pytest.raises(ValueError, match="current device"):
+        layer.forward_adapters(4096, OnOther(apply["ids"].t), 5)
+    assert len(calls) == 2
+    now[0] = 1
+    H.route_experts(SPEC, **{k: OnOther(v.t) if k != "T" else v for k, v in route.items()}, **kinds)
+    with pytest.raises(ValueError, match="current device"):
+        H.route_experts(SPEC, **route, **kinds)
+    assert len(calls) == 3
