@@ -413,3 +413,28 @@ def test_adapters_closed_while_set_are_refused(block):
     layer.forward_adapters(x.data_ptr(), ids, 6)  # none set: the block as it is
     assert layer.time_stage("gateup", 1) >= 0.0
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [30, 400, 1300])
+@pytest.mark.parametrize("runs", [1, 20])
+def test_a_long_batch_against_the_definition(block, T, runs):
+    """Tokens from all over a batch in adapter tiles of 16 and in the wide expert tiles,
+    each with an adapter of its own or in requests: the experts are ones that the 64-bit
+    keys allow, and the outputs those of the definition for these experts and weights."""
+    x = C.inputs(0xAD, T)
+    adapter = [(t * 7 // runs) % 5 - 1 for t in range(T)]
+    used = ("router", "gate", "up", "down")
+    block.use(used)
+    y, ids, wpre, w = block.run(x, adapter)
+    at = sorted({0, 1, T // 3, T // 2, T - 17, T - 1})  # first and last tiles, tails
+    ad = [adapter[t] for t in at]
+    s, lg = block.logits(x[at], ad, used)
+    sig = 1.0 / (1.0 + np.exp(-lg))
+    near_choice(ids[at], sig + block.cpu.bias.astype(np.float64), 8)
+    want = np.take_along_axis(sig, ids[at], 1)
+    want = want / (want.sum(1, keepdims=True) + 1e-20)
+    assert (np.abs(wpre[at] - want) <= 2e-5).all()
+    out = block.expect(x[at], s, ad, ids[at], w[at].astype(np.float64), used)
+    for i, t in enumerate(at):
+        assert O.rel_l2(y[t] - x[t], out[i]) <= TOL
