@@ -304,6 +304,9 @@ typedef struct hy3x_route_spec {
  *    group score; a group of masked experts comes after every other group. A
  *    row with nothing left gets the first k experts with weights 0.
  *  - A logit of +inf counts as the largest finite value of its type.
+ *  - The weights are fp32 arithmetic, of 64-bit scores only where a score lies near
+ *    or below fp32's normal numbers: each is off by at most (72 + |l_e - max l|, of
+ *    sigmoid |l_e|) 2^-24 of itself, by about one 2^-24 on average.
  * logits: device [T rows of E elements], `type` HY3X_F32 / F16 / BF16, rows
  * row_stride elements apart (E .. 2^32); bias: device fp32 [E] or NULL; ids, w:
  * device, dense, overlapping nothing else. T = 0 does nothing. No allocation,
@@ -349,13 +352,14 @@ int hy3x_adapters_set(hy3x_adapters *adapters, int index, const void *a, const v
  * adapters hold. A weight that is infinite or NaN makes the outputs that it enters
  * infinite or NaN, but which of the two is not specified: the products meet x and
  * A x in parts, some of them 0, and 0 inf is NaN where the formula has inf. An
- * infinite x gives what the formula gives. Up to 256 tokens each takes its own adapter (neighbours with the
- * same one share its reads); more run in tiles of 16 consecutive tokens that read
- * each adapter occurring in them, so keep a request's tokens together, and give the
- * single-token requests of a batch a call of their own. T = 0 does nothing. The
- * handle's device must be current. No allocation, no scratch: calls on one handle
- * may overlap, and a call may be captured into a graph. stream: a hipStream_t of
- * the handle's device (NULL = default stream). Asynchronous. */
+ * infinite x gives what the formula gives. Up to 256 tokens each takes its own
+ * adapter (neighbours with the same one share its reads); more run in tiles of 16
+ * consecutive tokens that read each adapter occurring in them, so keep a request's
+ * tokens together, and give the single-token requests beside long ones a call of
+ * their own (all of them one call). T = 0 does nothing. The handle's device must be
+ * current. No allocation, no scratch: calls on one handle may overlap, and a call
+ * may be captured into a graph. stream: a hipStream_t of the handle's device (NULL =
+ * default stream). Asynchronous. */
 int hy3x_adapters_apply(const hy3x_adapters *adapters, const int32_t *ids, const void *x,
                         int x_type, int64_t x_stride, const void *base, int64_t base_stride,
                         void *y, int y_type, int64_t y_stride, int T, void *stream);
