@@ -11,6 +11,9 @@
 // parts of u by blocks of their own and A and B read for 32 tokens at a time,
 // measured 39.0 us against 36.1 at 4096 x 4096 outputs of rank 64.)
 //
+// Figures in pairs or in braces compare two forms of one step, measured together
+// when it was chosen; what the kernel takes as it stands is under "What bounds it".
+//
 // TOK = 16: 16 consecutive tokens, the columns of every MFMA. The adapters that
 // occur among them are taken one after another: each forms its products for all
 // 16 columns, and the columns of its own tokens are selected, so a token never
@@ -22,16 +25,18 @@
 // fp32 x meets A in three two-byte parts (Split), or in fp32 FMAs for one token;
 // u meets B in three too (Parts). The parts keep fp32's range and precision.
 // (v_mfma_f32_16x16x4_f32 on fp32 x: 512 tokens of 4096 inputs 52.6 us at rank 64,
-// 24.3 in parts, 19.2 and 15.3 at rank 16.)
+// 24.3 in parts, 19.2 and 15.3 at rank 16; before tiles dealt their adapters.)
 //
-// What bounds it (us of the kernel, inputs and weights from HBM, MI355X): many
-// tokens the bytes of x, base and y, 16-token tiles with two adapters last (4096
-// x 4096 outputs of 4096 inputs, rank 64: 34.9 us for 111 MB, 3.2 TB/s, 25.6 where
-// no tile has two; rank 16, 2000 tokens: 16.4 us for 53 MB, 3.2 TB/s); up to 256
+// What bounds it (us of the kernel, inputs and weights from HBM, MI355X; a copy
+// reaches 5.2 TB/s): many tokens the bytes of x, base and y only in part, 13.0 us for
+// 4096 x 4096 fp16 outputs of 4096 inputs without an adapter; with them each tile's
+// chain of x, A, LDS, B and y, and the tiles with several adapters, which end last
+// (rank 64: 36.2 us for 111 MB, 3.1 TB/s, 58 with two in every tile; rank 16, 2000
+// tokens: 16.3 us for 53 MB, 3.2 TB/s, 14.0 where no tile has two); up to 256
 // decoded tokens the adapters' weights (256 tokens, 128 adapters: 14.0 us for 40 MB,
 // 2.9 TB/s); a few tokens four loads that wait for each other, ids, A, B, the store
-// (32 tokens: 6.0 us; one token beside the router: 6.2 us), and the same in few
-// tiles (512 tokens, 1536 fp32 inputs, 4096 fp32 outputs, rank 32: 12.9 us for 20
+// (32 tokens: 6.1 us; one token beside the router: 6.2 us), and the same in few
+// tiles (512 tokens, 1536 fp32 inputs, 4096 fp32 outputs, rank 32: 13.3 us for 20
 // MB, 2 of it the tiles with two adapters).
 //
 // Weights as the MFMAs read them, one coalesced 16-byte load per lane:
@@ -75,11 +80,15 @@ typedef short s4v __attribute__((ext_vector_type(4)));
 // the router 9.0 and 7.8), 8 above.
 constexpr int waves_for(int TOK, int RT) { return RT == 1 || (RT == 2 && TOK == 16) ? 16 : 8; }
 // Up to this many tokens, one per CU, a block takes one token and the order of the
-// adapters does not matter; above, tiles of 16. us, one token per block and tiles,
-// 4096 -> 4096 of rank 16 in bf16, every token another adapter | runs of 100:
-//   64 tokens 7.0 and 38.9 | 6.6 and 8.1     256: 13.2 and 39.5 | 10.2 and 9.8
-//   320 (a second round of blocks): 21.0 and 38.9 | 18.4 and 10.4
-//   1024: 45.1 and 44.2 | 36.6 and 12.6
+// adapters does not matter; above, tiles of 16. The ids are on the device, so T alone
+// decides. us, one token per block | tiles, 4096 -> 4096 of rank 16 in bf16, every
+// token another of 128 adapters, and runs of 100 tokens with one:
+//   256 tokens         14.3 | 39.5 (not dealt)   10.2 | 9.8
+//   320 (a second round of blocks) 21.0 | 20.9   18.4 | 10.9
+//   1024               45.1 | 35.0               36.6 | 13.7
+// What neither serves are single tokens beside long runs: their tiles of up to 16
+// adapters end long after the others (2000 tokens, 64 of them single: 45.0 us, in
+// two calls 22.6; 4096 of rank 64, 256 single: 210 and 81).
 constexpr int SINGLE_MAX_T = 256;
 // Blocks that the outputs are sliced for: one per CU. More slices form u again
 // (512 blocks: 32 decoded tokens 9.8 us against 6.1, 512 in fp32 19.1 against
@@ -520,7 +529,9 @@ struct Parts {
 // Where a lane's 16 outputs of a block of 64 lie: two-byte ones in one run of 16
 // (32 bytes), fp32 ones in four runs of 4, 16 apart, so that the four lanes of a
 // token write 64 bytes at a time (4096 x 4096 fp32 outputs, rank 64: 67.0 us, in one
-// run of 64 bytes per lane 76.0; the same without adapters 33.1 and 63.7).
+// run of 64 bytes per lane 76.0; the same without adapters 33.1 and 63.7). Half a line
+// at a time past the caches is still more than y: 512 x 4096 outputs, 8.4 MB, write
+// 11.9 MB by the counters, two-byte ones 1.07 to 1.1 times y.
 template <class Y>
 struct Place {
   static constexpr int RUN = sizeof(Y) == 4 ? 4 : 16, N = 16 / RUN;

@@ -26,9 +26,11 @@
 // margin, and ties are ties.
 //
 // What bounds it (us of the kernel, MI355X): few rows the load and k rounds that
-// wait for each other (one row of 192: 2.7 us; 512: 4.2, its end a row with
-// candidates); many rows vector instructions, not bytes (4096 rows of 256 in 8
-// groups: 8.1 us, 507 a row; 16383 of 251: 15.6 us, 401 a row, 10 MB). With 64-bit
+// wait for each other (one row of 192: 2.8 us; 512: 4.2, its end a row with
+// candidates); 4096 rows, 4 a SIMD, still this latency: of 8.2 us for 256 experts in
+// 8 groups the 512 vector instructions a row are 3.4, the others the groups' shuffles
+// and lane reads, the rounds and the rows with candidates; 16383 rows of 251 mostly
+// vector instructions (401 a row, 10.7 us of 15.9), not bytes (8 MB). With 64-bit
 // keys for every row these were 8.2, 10.2, 22.8 and 48.7. A wave per row in blocks
 // of 4 waves: blocks of 1, 8 or 16 are no faster; waves that take rows in turn, the
 // next row's loads in flight, were slower (10.4 against 9.3 at 4096 rows, 22.4
