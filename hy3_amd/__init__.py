@@ -20,7 +20,7 @@ import numpy as np
 __all__ = ["lib", "lib_path", "MoELayer", "HY3XError", "D_MODEL", "D_FF", "N_EXPERT",
            "K_MAX", "Q4K_MATRIX_BYTES", "ROUTE_SCALE", "SHARED", "synth_key",
            "synth_normal", "synth_uniform_sym", "synth_zipf_bias", "RouteSpec", "route_experts",
-           "Adapters"]
+           "Adapters", "Linear4", "logprobs", "logprobs_workspace"]
 
 D_MODEL = 4096
 D_FF = 1536
@@ -85,6 +85,12 @@ _SIGS = {
     "hy3x_adapters_destroy": (I32, [P]),
     "hy3x_adapters_set": (I32, [P, I32, P, P, F32, I32]),
     "hy3x_adapters_apply": (I32, [P, P, P, I32, I64, P, I64, P, I32, I64, I32, P]),
+    "hy3x_linear4_create": (I32, [ctypes.POINTER(P), I32, I32, I32, I32]),
+    "hy3x_linear4_destroy": (I32, [P]),
+    "hy3x_linear4_set": (I32, [P, P, P, P, I32]),
+    "hy3x_linear4_apply": (I32, [P, P, I32, I64, P, I64, P, I32, I64, I32, P]),
+    "hy3x_logprobs_workspace": (I64, [I32, I32, I32]),
+    "hy3x_logprobs": (I32, [P, I32, I64, I32, P, I32, I32, P, P, P, P, P, I64, P]),
     "hy3x_synth_layer_experts": (I32, [P, U64, U32]),
     "hy3x_synth_quantize_q4k": (I32, [P, P, I64, P]),
     "hy3x_synth_key": (U64, [U64, U32, U32, U32]),
@@ -228,7 +234,7 @@ def _dev(a):
 
 
 _KINDS = {"torch.float32": "f32", "torch.float16": "f16", "torch.bfloat16": "bf16",
-          "torch.int32": "i32"}
+          "torch.int32": "i32", "torch.uint8": "u8"}
 _kind_of = {}  # a torch dtype, once met: its name here
 
 
@@ -410,6 +416,128 @@ class Adapters:
                          base_stride or 0, y, DTYPES[y_dtype], y_stride, T, stream)
         if rc:
             _check(rc)
+
+
+class Linear4:
+    """A projection [d_out x d_in] of 4-bit weights with a scale (and a zero point) for each
+    group of a row's weights, resident on the current HIP device (hy3x_linear4_*)."""
+
+    def __init__(self, d_out, d_in, group=128, dtype="bf16"):
+        h = P()
+        _check(lib().hy3x_linear4_create(ctypes.byref(h), d_out, d_in, group, DTYPES[dtype]))
+        self._h = h
+        self._apply = lib().hy3x_linear4_apply
+        self.d_out, self.d_in, self.group, self.dtype = d_out, d_in, group, dtype
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().hy3x_linear4_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def set(self, q, scales, zeros=None, on_device=False):
+        """The weights: q [d_out x ceil(d_in / 2)] bytes (an even weight in the low four
+        bits), scales [d_out x groups] of the handle's type, zeros [d_out x groups] bytes of
+        0 to 16 (None: 8 everywhere). Arrays (of the scales or of their bits as 16-bit
+        integers), or device memory with on_device: contiguous tensors, or pointers."""
+        per_group = (self.d_out, -(-self.d_in // self.group))
+        given = [("q", q, (self.d_out, -(-self.d_in // 2)), ("uint8",), "u8"),
+                 ("scales", scales, per_group,
+                  ("int16", "uint16", Adapters._NAMES[self.dtype]), self.dtype),
+                 ("zeros", zeros, per_group, ("uint8",), "u8")]
+        args, held = [], []
+        for name, m, shape, host, device in given:
+            if m is None and name == "zeros":
+                args.append(None)
+                continue
+            if on_device:
+                if hasattr(m, "data_ptr"):
+                    _typed(name, m, device)
+                    if not m.is_contiguous():
+                        raise ValueError(f"{name}: not contiguous")
+                args.append(_dev(m))
+            else:
+                m = np.ascontiguousarray(m)
+                if m.dtype.name not in host:
+                    raise TypeError(f"{name}: {m.dtype}, not {' or '.join(host)}")
+                held.append(m)
+                args.append(m.ctypes.data)
+            if hasattr(m, "shape"):
+                axes = [n for n in m.shape if n != 1]
+                if axes not in ([n for n in shape if n != 1], [shape[0] * shape[1]]):
+                    raise ValueError(f"{name}: {tuple(m.shape)}, not {shape}")
+        _check(lib().hy3x_linear4_set(self._h, *args, 1 if on_device else 0))
+
+    def apply(self, x, y, T, base=None, x_dtype=None, y_dtype=None, x_stride=None,
+              base_stride=None, y_stride=None, stream=None):
+        """y[t] = base[t] + W x[t] on device memory (hy3x_linear4_apply): tensors of f32, f16
+        or bf16, whose types, places and sizes are checked, or pointers. Types and strides
+        default to the tensors' own (of pointers, the scales' type and dense rows); no base:
+        0."""
+        here = _here()
+        x, x_dtype, x_stride = _rows("x", x, x_dtype, T, self.d_in, x_stride, here)
+        y, y_dtype, y_stride = _rows("y", y, y_dtype, T, self.d_out, y_stride, here)
+        y_dtype = y_dtype or self.dtype
+        if base is not None:
+            base, _, base_stride = _rows("base", base, y_dtype, T, self.d_out, base_stride, here)
+        rc = self._apply(self._h, x, DTYPES[x_dtype or self.dtype], x_stride, base,
+                         base_stride or 0, y, DTYPES[y_dtype], y_stride, T, stream)
+        if rc:
+            _check(rc)
+
+
+def logprobs_workspace(T, vocab, top=0):
+    """Bytes of workspace that logprobs needs for T rows of `vocab` logits and `top`
+    alternatives; 0: none (hy3x_logprobs_workspace)."""
+    n = lib().hy3x_logprobs_workspace(T, vocab, top)
+    if n < 0:
+        _check(n)
+    return n
+
+
+def logprobs(logits, tokens, T, logp, entropy=None, top_ids=None, top_logp=None, vocab=None,
+             top=None, dtype=None, row_stride=None, workspace=None, stream=None):
+    """logp [T] of the given tokens [T] (int32), and where given the entropy [T] and the most
+    probable tokens top_ids [T x top] (int32) and their top_logp, of T rows of logits in
+    device memory (hy3x_logprobs): tensors, whose types, places and sizes are checked, or
+    pointers. Without them: vocab and top are those of the tensors' last axes, dtype and
+    row_stride the logits' own (of a pointer, "f32" and dense rows; vocab is named then).
+    workspace: a byte tensor of logprobs_workspace(T, vocab, top), or a pointer to as many."""
+    here = _here()
+    if vocab is None:
+        if not hasattr(logits, "data_ptr"):
+            raise ValueError("vocab: not named, and logits is a pointer")
+        vocab = logits.shape[-1]
+    if top_ids is None or top_logp is None:
+        if top_ids is not top_logp or top:
+            raise ValueError("top_ids and top_logp belong together")
+        top = 0
+    elif top is None:
+        if not hasattr(top_ids, "data_ptr"):
+            raise ValueError("top: not named, and top_ids is a pointer")
+        top = top_ids.shape[-1]
+    logits, dtype, row_stride = _rows("logits", logits, dtype, T, vocab, row_stride, here)
+    tokens = _flat("tokens", tokens, "i32", T, here)
+    logp = _flat("logp", logp, "f32", T, here)
+    if entropy is not None:
+        entropy = _flat("entropy", entropy, "f32", T, here)
+    if top:
+        top_ids = _flat("top_ids", top_ids, "i32", T * top, here)
+        top_logp = _flat("top_logp", top_logp, "f32", T * top, here)
+    room = 0
+    if workspace is not None:
+        room = logprobs_workspace(T, vocab, top)
+        workspace = _flat("workspace", workspace, "u8", room, here)
+    rc = (_lib or lib()).hy3x_logprobs(logits, DTYPES[dtype or "f32"], row_stride, vocab, tokens,
+                                       T, top, logp, entropy, top_ids if top else None,
+                                       top_logp if top else None, workspace, room, stream)
+    if rc:
+        _check(rc)
 
 
 def _still_open(adapters):

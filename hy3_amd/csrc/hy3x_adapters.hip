@@ -865,20 +865,6 @@ void launch_types(const hy3x_adapters *h, const int32_t *ids, const void *x, boo
     launch<W, W, W>(h, ids, x, x_stride, base, base_stride, y, y_stride, T, st);
 }
 
-// Whether T rows of a_row bytes, a_step apart from a, and T rows of b share a
-// byte. Rows of one wider buffer (equal steps) may lie between each other.
-bool overlap(const void *a, int64_t a_step, int64_t a_row, const void *b, int64_t b_step,
-             int64_t b_row, int T) {
-  const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
-  const uintptr_t a1 = a0 + (uintptr_t)((T - 1) * a_step + a_row);
-  const uintptr_t b1 = b0 + (uintptr_t)((T - 1) * b_step + b_row);
-  if (a1 <= b0 || b1 <= a0) return false;
-  if (a_step != b_step || T == 1) return true;
-  const int64_t off = (int64_t)((b0 >= a0 ? b0 - a0 : a0 - b0) % (uintptr_t)a_step);
-  const int64_t ab = b0 >= a0 ? off : (a_step - off) % a_step;  // b's place in a's rows
-  return ab < a_row || ab + b_row > a_step;
-}
-
 }  // namespace
 
 AdaptersShape adapters_shape(const hy3x_adapters *h) { return {h->d_in, h->d_out, h->device}; }
@@ -1022,10 +1008,10 @@ int hy3x_adapters_apply(const hy3x_adapters *h, const int32_t *ids, const void *
   const uintptr_t i0 = (uintptr_t)ids, y0 = (uintptr_t)y;
   if (i0 < y0 + (uintptr_t)(((T - 1) * y_stride + h->d_out) * ys) && y0 < i0 + (uintptr_t)T * 4)
     return op_fail(HY3X_E_ARG, "y overlaps ids");
-  if (overlap(x, x_stride * xs, h->d_in * xs, y, y_stride * ys, h->d_out * ys, T))
+  if (rows_overlap(x, x_stride * xs, h->d_in * xs, y, y_stride * ys, h->d_out * ys, T))
     return op_fail(HY3X_E_ARG, "y overlaps x");
   if (base && !(base == y && (base_stride == y_stride || T == 1)) &&
-      overlap(base, base_stride * ys, h->d_out * ys, y, y_stride * ys, h->d_out * ys, T))
+      rows_overlap(base, base_stride * ys, h->d_out * ys, y, y_stride * ys, h->d_out * ys, T))
     return op_fail(HY3X_E_ARG, "y overlaps base without being base");
   const int rc = check_device(h);
   if (rc) return rc;

@@ -364,6 +364,81 @@ int hy3x_adapters_apply(const hy3x_adapters *adapters, const int32_t *ids, const
                         int x_type, int64_t x_stride, const void *base, int64_t base_stride,
                         void *y, int y_type, int64_t y_stride, int T, void *stream);
 
+/* ---- products of 4-bit weights ------------------------------------------------
+ * One projection W [d_out x d_in] of 4-bit weights with a scale, and perhaps a zero
+ * point, for each `group` consecutive weights of a row:
+ *   W[n][k] = scale[n][k / group] * (q[n][k] - zero[n][k / group])
+ * for the projections around the block (attention's, a dense layer's, the LM head),
+ * whose product adapters can then stand beside. */
+typedef struct hy3x_linear4 hy3x_linear4;
+#define HY3X_LINEAR4_MAX_OUT (1 << 20)
+#define HY3X_LINEAR4_MAX_IN 65536
+#define HY3X_LINEAR4_MAX_TOKENS (1 << 24)
+
+/* A matrix on the current device, without weights until they are set. group: 32, 64
+ * or 128 (the last group of a row may be shorter); type HY3X_F16 or HY3X_BF16: the
+ * elements of the scales. Device memory: d_out d_in / 2 bytes and 3 for each group
+ * (d_out rounded up to 16, d_in to 128, the groups of a row to those of 512). */
+int hy3x_linear4_create(hy3x_linear4 **out, int d_out, int d_in, int group, int type);
+int hy3x_linear4_destroy(hy3x_linear4 *weights);
+/* The weights: q, bytes [d_out x (d_in + 1) / 2], weight k of a row in byte k / 2, an
+ * even k in the low four bits; scales [d_out x (d_in + group - 1) / group] in the
+ * handle's type; zeros, bytes of the same shape, 0 to 16 (HY3X_E_ARG above, and the
+ * handle keeps what it had), or NULL: 8 everywhere. Dense, row-major (host pointers, or
+ * device pointers with src_on_device != 0; copied and laid out for the kernels). Waits
+ * for the device before and after the copy. */
+int hy3x_linear4_set(hy3x_linear4 *weights, const void *q, const void *scales, const void *zeros,
+                     int src_on_device);
+/* y[t] = base[t] + W x[t] for T tokens. base NULL: 0 in its place. base may be y itself
+ * (same pointer and stride: added in place); otherwise y may overlap neither x nor base
+ * (rows of one wider buffer may lie between each other). x: device [T x d_in], base, y:
+ * device [T x d_out], x_type and y_type each HY3X_F32, HY3X_F16 or HY3X_BF16; strides in
+ * elements, from the row length to 2^32. x and the integers q and zero meet exactly, in
+ * fp32 sums, which the scales multiply group by group; y is rounded once. Tokens do not
+ * affect each other's results. An x that is infinite or NaN makes its token's outputs
+ * infinite or NaN (as the formula does), but which of the two is not specified: q x and
+ * zero x may meet as sums, and inf - inf is NaN where the formula has inf. The same
+ * holds for sums of 16 |x| beyond fp32's range. T = 0 does nothing. The handle's device
+ * must be current. No allocation, no scratch: calls on one handle may overlap, and a
+ * call may be captured into a graph. HY3X_E_STATE before hy3x_linear4_set. stream: a
+ * hipStream_t of the handle's device (NULL = default stream). Asynchronous. */
+int hy3x_linear4_apply(const hy3x_linear4 *weights, const void *x, int x_type, int64_t x_stride,
+                       const void *base, int64_t base_stride, void *y, int y_type,
+                       int64_t y_stride, int T, void *stream);
+
+/* ---- log-probabilities of tokens ----------------------------------------------
+ * Of rows of logits over a vocabulary: the log-probability of each row's given token,
+ * the row's entropy, and its most probable tokens. */
+#define HY3X_LOGPROBS_MAX_VOCAB (1 << 24)
+#define HY3X_LOGPROBS_MAX_TOP 32
+#define HY3X_LOGPROBS_MAX_TOKENS (1 << 24)
+
+/* Bytes of workspace that hy3x_logprobs needs for T rows of V logits and n_top
+ * alternatives (0 where it needs none), or a negative HY3X_E* code. */
+int64_t hy3x_logprobs_workspace(int T, int V, int n_top);
+/* With p = softmax of a row of V logits:
+ *   logp[t]     = log p[tokens[t]]; 0 where tokens[t] is outside [0, V) (a row of padding);
+ *   entropy[t]  = -sum p log p, in nats (NULL: not wanted);
+ *   top_ids, top_logp [T x n_top]: the n_top most probable tokens in falling order of
+ *     their logits, equal ones by the lower index (n_top 0: not wanted).
+ *  - Masked tokens: a logit that is NaN, -inf or the lowest finite value of its type.
+ *    They have p = 0 and log p = -inf and come after every other token, in index order.
+ *    A row with nothing left has logp -inf, entropy 0 and tokens 0 .. n_top - 1.
+ *  - A logit of +inf counts as the largest finite value of its type.
+ *  - fp32 exponentials, whose sums over a row are joined in 64 bits.
+ * logits: device [T rows of V elements], `type` HY3X_F32 / F16 / BF16, rows row_stride
+ * elements apart (V .. 2^32); tokens: device int32[T]; outputs: device, dense, overlapping
+ * nothing else (logits are a range from their first to their last element). workspace:
+ * device memory of at least hy3x_logprobs_workspace bytes, aligned to 16, for this call
+ * alone until it has run (calls in order on one stream may share one, and so may the
+ * replays of a captured one; calls that may overlap need one each); its contents are of
+ * no account before and after. NULL where 0 bytes are needed. T = 0 does nothing. No
+ * allocation: a call may be captured into a graph. stream: a hipStream_t of the current
+ * device (NULL = default stream). Asynchronous. */
+int hy3x_logprobs(const void *logits, int type, int64_t row_stride, int V, const int32_t *tokens,
+                  int T, int n_top, float *logp, float *entropy, int32_t *top_ids, float *top_logp,
+                  void *workspace, int64_t workspace_bytes, void *stream);
+
 /* ---- the layer with a routing rule of its own, and with adapters -------------- */
 /* From the next forward on, every forward of this layer routes by this rule
  * instead of the built-in one (NULL: the built-in one again): n_expert 192,
