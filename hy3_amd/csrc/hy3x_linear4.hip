@@ -1,32 +1,13 @@
-// hy3x_linear4.hip -- products of 4-bit weights with a scale, and perhaps a
-// zero point, for each group of a row's weights (hy3x_linear4_*):
-//
-//   W[n][k] = s[n][k / group] (q[n][k] - z[n][k / group])
-//   y[t][n] = base[t][n] + sum_k W[n][k] x[t][k]        (fp32 sums, y rounded once)
-//
-// Products: v_mfma_f32_16x16x32_{bf16,f16}, rows = tokens, columns = 16 rows of
-// W. The integers q and -z are exact in both types, so a group's sum
-// sum_k x (q - z) is the fp32 accumulator of its MFMAs, and its scale is one FMA.
-// fp32 x meets them as three bf16 parts (hi + mid + lo, 24 bits), each a row of
-// the MFMA.
-//
-// Weights as the MFMAs read them:
-//   q  [row tile][chunk of 128 k][lane][4 dwords]: dword j of lane l holds k =
-//      128 c + 32 j + 8 (l / 16) + i of row 16 rt + l % 16, element i < 4 in the
-//      low half of byte i, i >= 4 in the high half of byte i - 4: both halves are
-//      bytes q, which v_cvt_scalef32_pk_{bf16,f16}_fp8 turns into the numbers q,
-//      as e4m3 bytes below 16 stand for q 2^-9;
-//   s  [row tile][quad of chunks][row][4 GP] (GP groups in a chunk), 0 beyond d_in
-//      and d_out; z the same, in bytes.
+// hy3x_linear4.hip -- products of 4-bit weights with group scales (hy3x_linear4_*):
+// the handle, its weights' layout and the entry points. The kernels are hy3x_linear4.h's.
 #include <hip/hip_bf16.h>
-#include <string.h>
+#include <hip/hip_fp16.h>
 
 #include <algorithm>
 #include <new>
 
-#include "../../include/hy3x_moe.h"
-#include "hy3x_common.h"
 #include "hy3x_error.h"
+#include "hy3x_linear4.h"
 #include "hy3x_ops.h"
 
 struct hy3x_linear4 {
@@ -41,194 +22,6 @@ struct hy3x_linear4 {
 namespace hy3x {
 namespace {
 
-typedef float f4v __attribute__((ext_vector_type(4)));
-typedef uint32_t u4v __attribute__((ext_vector_type(4)));
-typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
-typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
-typedef _Float16 h2v __attribute__((ext_vector_type(2)));
-typedef _Float16 h8v __attribute__((ext_vector_type(8)));
-
-// The MFMAs' operand type for x: its own two-byte type, bf16 parts of fp32.
-template <class X>
-struct Op;
-template <>
-struct Op<__half> {
-  static constexpr int PARTS = 1;
-  static __device__ __forceinline__ f4v mma(u4v a, u4v b, f4v c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a),
-                                                  __builtin_bit_cast(h8v, b), c, 0, 0, 0);
-  }
-  template <bool HI>
-  static __device__ __forceinline__ uint32_t ints(uint32_t bytes) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes, 512.0f, HI));
-  }
-  static __device__ __forceinline__ uint32_t both(float v) {  // v in both halves
-    return 0x10001u * __builtin_bit_cast(uint16_t, (_Float16)v);
-  }
-};
-template <>
-struct Op<__hip_bfloat16> {
-  static constexpr int PARTS = 1;
-  static __device__ __forceinline__ f4v mma(u4v a, u4v b, f4v c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, a),
-                                                   __builtin_bit_cast(bf8v, b), c, 0, 0, 0);
-  }
-  template <bool HI>
-  static __device__ __forceinline__ uint32_t ints(uint32_t bytes) {
-    return __builtin_bit_cast(uint32_t,
-                              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(bytes, 512.0f, HI));
-  }
-  static __device__ __forceinline__ uint32_t both(float v) {  // exact: at most 8 bits
-    return (__float_as_uint(v) >> 16) * 0x10001u;
-  }
-};
-template <>
-struct Op<float> : Op<__hip_bfloat16> {
-  static constexpr int PARTS = 3;
-};
-
-// 8 weights of a lane as an operand.
-template <class X>
-__device__ __forceinline__ u4v weights(uint32_t w) {
-  const uint32_t lo = w & 0x0f0f0f0fu, hi = w >> 4 & 0x0f0f0f0fu;
-  return (u4v){Op<X>::template ints<false>(lo), Op<X>::template ints<true>(lo),
-               Op<X>::template ints<false>(hi), Op<X>::template ints<true>(hi)};
-}
-
-// Part p of v in bf16: v = p0 + p1 + p2. An infinity is its first part, the
-// others 0.
-__device__ __forceinline__ float trunc16(float v) {
-  return __uint_as_float(__float_as_uint(v) & 0xffff0000u);
-}
-__device__ __forceinline__ uint32_t part_of(float v, int p) {
-  const float a = trunc16(v), r = fabsf(v) == INFINITY ? 0.0f : v - a, b = trunc16(r);
-  return __float_as_uint(p == 0 ? a : p == 1 ? b : p == 2 ? r - b : 0.0f) >> 16;
-}
-
-// Elements k .. k + 7 of a row of n as an operand, zeros beyond it.
-template <class X>
-__device__ __forceinline__ u4v operand(const X *row, int k, int n, int part) {
-  u4v out;
-  if constexpr (sizeof(X) == 2) {
-    if (k + 8 <= n) {
-      __builtin_memcpy(&out, row + k, 16);
-    } else {
-      uint16_t e[8];
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        __builtin_memcpy(&e[j], row + min(k + j, n - 1), 2);
-        if (k + j >= n) e[j] = 0;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; j++) out[j] = e[2 * j] | (uint32_t)e[2 * j + 1] << 16;
-    }
-  } else {
-    float e[8];
-    if (k + 8 <= n) {
-      __builtin_memcpy(e, row + k, 32);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        e[j] = row[min(k + j, n - 1)];
-        if (k + j >= n) e[j] = 0.0f;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      out[j] = part_of(e[2 * j], part) | part_of(e[2 * j + 1], part) << 16;
-  }
-  return out;
-}
-
-struct Call {
-  const u4v *q;
-  const uint16_t *s;
-  const uint8_t *z;  // NULL: 8 everywhere
-  int d_out, d_in, tiles, chunks, quads;
-  bool s16;  // scales are fp16
-  const void *x, *base;
-  void *y;
-  int64_t x_stride, base_stride, y_stride;
-  int T, y_type;
-};
-
-__device__ __forceinline__ float scale_of(uint32_t bits, bool s16) {
-  return s16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)bits) : __uint_as_float(bits << 16);
-}
-
-__device__ __forceinline__ float load_y(const void *p, int64_t at, int type) {
-  if (type == HY3X_F32) return ((const float *)p)[at];
-  if (type == HY3X_F16) return __half2float(((const __half *)p)[at]);
-  return __bfloat162float(((const __hip_bfloat16 *)p)[at]);
-}
-__device__ __forceinline__ void store_y(void *p, int64_t at, int type, float v) {
-  if (type == HY3X_F32) ((float *)p)[at] = v;
-  else if (type == HY3X_F16) ((__half *)p)[at] = __float2half(v);
-  else ((__hip_bfloat16 *)p)[at] = __float2bfloat16(v);
-}
-
-constexpr int WAVES = 4;
-
-// One row tile and one token tile at a time; the waves split the quads.
-template <class X, int GP>
-__global__ __launch_bounds__(64 * WAVES) void k_linear4(Call c) {
-  constexpr int TT = Op<X>::PARTS == 1 ? 16 : 4;  // tokens of a tile
-  __shared__ float red[WAVES][4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, h = lane >> 4;
-  const int token_tiles = (c.T + TT - 1) / TT;
-  const int64_t all = (int64_t)token_tiles * c.tiles;
-  for (int64_t item = blockIdx.x; item < all; item += gridDim.x) {
-    const int rt = (int)(item % c.tiles);
-    const int64_t t0 = item / c.tiles * TT;
-    const int part = TT == 4 ? col & 3 : 0;
-    const int64_t t = min(t0 + (TT == 4 ? col >> 2 : col), (int64_t)c.T - 1);
-    const X *row = (const X *)c.x + t * c.x_stride;
-    f4v acc = {0, 0, 0, 0};
-    for (int qd = wave; qd < c.quads; qd += WAVES) {
-      const size_t at = (((size_t)rt * c.quads + qd) * 16 + col) * (4 * GP);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int ch = 4 * qd + i;
-        if (ch >= c.chunks) break;
-        const u4v w = c.q[((size_t)rt * c.chunks + ch) * 64 + lane];
-#pragma unroll
-        for (int g = 0; g < GP; g++) {
-          const float s = scale_of(c.s[at + i * GP + g], c.s16);
-          const uint32_t zz = Op<X>::both(c.z ? -(float)c.z[at + i * GP + g] : -8.0f);
-          const u4v z = {zz, zz, zz, zz};
-          f4v d = {0, 0, 0, 0};
-#pragma unroll
-          for (int j = g * 4 / GP; j < (g + 1) * 4 / GP; j++) {
-            const u4v a = operand(row, 128 * ch + 32 * j + 8 * h, c.d_in, part);
-            d = Op<X>::mma(a, weights<X>(w[j]), d);
-            d = Op<X>::mma(a, z, d);
-          }
-#pragma unroll
-          for (int r = 0; r < 4; r++) acc[r] = fmaf(s, d[r], acc[r]);
-        }
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < 4; r++) red[wave][r][lane] = acc[r];
-    __syncthreads();
-    // thread: register r of a lane
-    const int r = wave;
-    float v = 0.0f;
-    if (TT == 16) {
-      for (int w = 0; w < WAVES; w++) v += red[w][r][lane];
-    } else if (r == 0) {
-      for (int w = 0; w < WAVES; w++) v += red[w][0][lane] + (red[w][1][lane] + red[w][2][lane]);
-    }
-    const int64_t token = t0 + (TT == 16 ? 4 * h + r : h);
-    const int n = 16 * rt + col;
-    if ((TT == 16 || r == 0) && token < c.T && n < c.d_out) {
-      if (c.base) v += load_y(c.base, token * c.base_stride + n, c.y_type);
-      store_y(c.y, token * c.y_stride + n, c.y_type, v);
-    }
-    __syncthreads();
-  }
-}
-
 // q [d_out x ceil(d_in / 2)] bytes (element k in byte k / 2, even k low), scales and
 // zeros [d_out x groups] to the kernels' layout.
 __global__ __launch_bounds__(256) void k_pack_q(const uint8_t *q, int d_out, int d_in, int chunks,
@@ -237,7 +30,7 @@ __global__ __launch_bounds__(256) void k_pack_q(const uint8_t *q, int d_out, int
   if (i >= n) return;
   const int j = (int)(i & 3), lane = (int)(i >> 2 & 63);
   const int64_t tile = i >> 8;
-  const int64_t row = tile / chunks * 16 + (lane & 15);
+  const int64_t row = linear4_row(tile / chunks, lane & 15);
   const int k0 = (int)(tile % chunks) * 128 + 32 * j + 8 * (lane >> 4);
   uint32_t w = 0;
   if (row < d_out)
@@ -255,25 +48,16 @@ __global__ __launch_bounds__(256) void k_pack_s(const uint16_t *s, const uint8_t
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // a group
   if (i >= n) return;
   const int64_t tile = i / (64 * gp);
-  const int64_t row = tile / quads * 16 + i / (4 * gp) % 16;
+  const int64_t row = linear4_row(tile / quads, (int)(i / (4 * gp) % 16));
   const int64_t g = tile % quads * (4 * gp) + i % (4 * gp);
   const bool in = row < d_out && g < groups;
   so[i] = in ? s[row * groups + g] : 0;
   if (z) zo[i] = in ? z[row * groups + g] : 0;
+  else if (i < 64 * gp) zo[i] = 8;  // one quad for all
 }
 __global__ __launch_bounds__(256) void k_check_zeros(const uint8_t *z, int64_t n, int *bad) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
     if (z[i] > 16) *bad = 1;
-}
-
-template <class X>
-void launch(const Call &c, int group, hipStream_t st) {
-  constexpr int TT = Op<X>::PARTS == 1 ? 16 : 4;
-  const int64_t all = (int64_t)((c.T + TT - 1) / TT) * c.tiles;
-  const dim3 grid((uint32_t)std::min<int64_t>(all, 1 << 20)), block(64 * WAVES);
-  if (group == 128) k_linear4<X, 1><<<grid, block, 0, st>>>(c);
-  else if (group == 64) k_linear4<X, 2><<<grid, block, 0, st>>>(c);
-  else k_linear4<X, 4><<<grid, block, 0, st>>>(c);
 }
 
 }  // namespace
@@ -297,8 +81,9 @@ int hy3x_linear4_create(hy3x_linear4 **out, int d_out, int d_in, int group, int 
   *out = nullptr;
   if (d_out < 1 || d_out > HY3X_LINEAR4_MAX_OUT)
     return op_fail(HY3X_E_ARG, "d_out %d outside [1,%d]", d_out, HY3X_LINEAR4_MAX_OUT);
-  if (d_in < 1 || d_in > HY3X_LINEAR4_MAX_IN)
-    return op_fail(HY3X_E_ARG, "d_in %d outside [1,%d]", d_in, HY3X_LINEAR4_MAX_IN);
+  if (d_in < HY3X_LINEAR4_MIN_IN || d_in > HY3X_LINEAR4_MAX_IN)
+    return op_fail(HY3X_E_ARG, "d_in %d outside [%d,%d]", d_in, HY3X_LINEAR4_MIN_IN,
+                   HY3X_LINEAR4_MAX_IN);
   if (group != 32 && group != 64 && group != 128)
     return op_fail(HY3X_E_ARG, "group %d is none of 32, 64, 128", group);
   if (type != HY3X_F16 && type != HY3X_BF16)
@@ -309,7 +94,7 @@ int hy3x_linear4_create(hy3x_linear4 **out, int d_out, int d_in, int group, int 
   h->d_in = d_in;
   h->group = group;
   h->type = type;
-  h->tiles = (d_out + 15) / 16;
+  h->tiles = (d_out + 63) / 64 * 4;
   h->chunks = (d_in + 127) / 128;
   h->quads = (h->chunks + 3) / 4;
   const hipError_t e = hipGetDevice(&h->device);
@@ -421,15 +206,18 @@ int hy3x_linear4_apply(const hy3x_linear4 *h, const void *x, int x_type, int64_t
     return op_fail(HY3X_E_ARG, "y overlaps base without being base");
   const int rc = check_device(h);
   if (rc) return rc;
-  Call c;
+  Linear4Call c;
   c.q = (const u4v *)h->q;
   c.s = h->s;
-  c.z = h->zeros ? h->z : nullptr;
+  c.z = h->z;
+  c.z_quad = h->zeros ? 64 * (128 / h->group) : 0;
+  c.z_tile = c.z_quad * h->quads;
   c.d_out = h->d_out;
   c.d_in = h->d_in;
   c.tiles = h->tiles;
   c.chunks = h->chunks;
   c.quads = h->quads;
+  c.group = h->group;
   c.s16 = h->type == HY3X_F16;
   c.x = x;
   c.base = base;
@@ -440,9 +228,9 @@ int hy3x_linear4_apply(const hy3x_linear4 *h, const void *x, int x_type, int64_t
   c.T = T;
   c.y_type = y_type;
   const hipStream_t st = (hipStream_t)stream;
-  if (x_type == HY3X_F32) launch<float>(c, h->group, st);
-  else if (x_type == HY3X_F16) launch<__half>(c, h->group, st);
-  else launch<__hip_bfloat16>(c, h->group, st);
+  if (x_type == HY3X_F32) launch_linear4<float>(c, st);
+  else if (x_type == HY3X_F16) launch_linear4<__half>(c, st);
+  else launch_linear4<__hip_bfloat16>(c, st);
   OP_HIP_TRY(hipGetLastError());
   return HY3X_OK;
 }

@@ -1,0 +1,628 @@
+// hy3x_linear4_kernels.h -- kernels of the products of 4-bit weights (the
+// mathematics and the weights' layout: hy3x_linear4.h).
+//
+// Products: v_mfma_f32_16x16x32_{bf16,f16}, rows = tokens, columns = 16 rows of W.
+// The integers are exact in both types, so a group's sum is the fp32 accumulator of
+// its MFMAs, and its scale is one FMA. fp32 x meets them as three bf16 parts.
+#pragma once
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include <algorithm>
+
+#include "hy3x_dma.h"
+#include "hy3x_linear4.h"
+
+namespace hy3x {
+namespace linear4 {
+
+typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef short s2v __attribute__((ext_vector_type(2)));
+
+// The MFMAs' operand type for x: its own two-byte type, bf16 parts of fp32.
+template <class X>
+struct Op;
+template <>
+struct Op<__half> {
+  static constexpr int PARTS = 1;
+  static __device__ __forceinline__ f4v mma(u4v a, u4v b, f4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a),
+                                                  __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+  }
+  // two bytes below 16 (the low or the high ones) as numbers: as e4m3 they stand for
+  // 2^-9 of themselves
+  template <bool HI>
+  static __device__ __forceinline__ uint32_t ints(uint32_t bytes) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes, 512.0f, HI));
+  }
+  static __device__ __forceinline__ uint32_t both(float v) {  // v in both halves
+    return 0x10001u * __builtin_bit_cast(uint16_t, (_Float16)v);
+  }
+};
+template <>
+struct Op<__hip_bfloat16> {
+  static constexpr int PARTS = 1;
+  static __device__ __forceinline__ f4v mma(u4v a, u4v b, f4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, a),
+                                                   __builtin_bit_cast(bf8v, b), c, 0, 0, 0);
+  }
+  template <bool HI>
+  static __device__ __forceinline__ uint32_t ints(uint32_t bytes) {
+    return __builtin_bit_cast(uint32_t,
+                              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(bytes, 512.0f, HI));
+  }
+  static __device__ __forceinline__ uint32_t both(float v) {  // exact: at most 8 bits
+    return (__float_as_uint(v) >> 16) * 0x10001u;
+  }
+};
+template <>
+struct Op<float> : Op<__hip_bfloat16> {
+  static constexpr int PARTS = 3;
+};
+
+// 8 weights q of a lane as an operand, in the order of k.
+template <class X>
+__device__ __forceinline__ u4v weights(uint32_t w) {
+  const uint32_t lo = w & 0x0f0f0f0fu, hi = w >> 4 & 0x0f0f0f0fu;
+  return (u4v){Op<X>::template ints<false>(lo), Op<X>::template ints<true>(lo),
+               Op<X>::template ints<false>(hi), Op<X>::template ints<true>(hi)};
+}
+
+// Part p of v in bf16: v = p0 + p1 + p2. An infinity is its first part, the
+// others 0.
+__device__ __forceinline__ float trunc16(float v) {
+  return __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+}
+__device__ __forceinline__ float part_of(float v, int p) {
+  const float a = trunc16(v), r = fabsf(v) == INFINITY ? 0.0f : v - a, b = trunc16(r);
+  return p == 0 ? a : p == 1 ? b : p == 2 ? r - b : 0.0f;
+}
+__device__ __forceinline__ uint32_t pair16(float lo, float hi) {  // their upper halves
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302);
+}
+
+// Elements k .. k + 7 of a row. Loads are 16 bytes at the elements' own alignment.
+template <class X>
+struct Eight {
+  uint32_t w[2 * sizeof(X)];
+  __device__ __forceinline__ void load(const X *row, int k) {
+    __builtin_memcpy(w, row + k, sizeof(w));
+  }
+  // of a row of n (n >= 8), zeros beyond it: its last 8, moved down
+  __device__ __forceinline__ void load_within(const X *row, int k, int n) {
+    load(row, min(k, n - 8));
+    const int by = min(max(k + 8 - n, 0), 8);
+    if constexpr (sizeof(X) == 4) {
+#pragma unroll
+      for (int s = 1; s <= 8; s *= 2)
+#pragma unroll
+        for (int j = 0; j < 8; j++) w[j] = by & s ? (j + s < 8 ? w[j + s] : 0) : w[j];
+    } else {
+      uint64_t lo = w[0] | (uint64_t)w[1] << 32, hi = w[2] | (uint64_t)w[3] << 32;
+      const int bits = 16 * (by & 3);
+      if (by & 8) lo = hi = 0;
+      lo = by & 4 ? hi : lo;
+      hi = by & 4 ? 0 : hi;
+      lo = lo >> bits | (hi << 1) << (63 - bits);
+      hi >>= bits;
+      w[0] = (uint32_t)lo;
+      w[1] = (uint32_t)(lo >> 32);
+      w[2] = (uint32_t)hi;
+      w[3] = (uint32_t)(hi >> 32);
+    }
+  }
+  // as an operand (part `part` of fp32), in the order of k
+  __device__ __forceinline__ u4v operand(int part) const {
+    u4v out;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if constexpr (sizeof(X) == 4)
+        out[j] = pair16(part_of(__uint_as_float(w[2 * j]), part),
+                        part_of(__uint_as_float(w[2 * j + 1]), part));
+      else out[j] = w[j];
+    }
+    return out;
+  }
+};
+
+__device__ __forceinline__ float scale_of(uint32_t bits, bool s16) {
+  return s16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)bits) : __uint_as_float(bits << 16);
+}
+
+template <class Y>
+constexpr int type_of() {
+  return __is_same(Y, float) ? HY3X_F32 : __is_same(Y, __half) ? HY3X_F16 : HY3X_BF16;
+}
+__device__ __forceinline__ float load_y(const void *p, int64_t at, int type) {
+  if (type == HY3X_F32) return ((const float *)p)[at];
+  if (type == HY3X_F16) return __half2float(((const __half *)p)[at]);
+  return __bfloat162float(((const __hip_bfloat16 *)p)[at]);
+}
+__device__ __forceinline__ void store_y(void *p, int64_t at, int type, float v) {
+  if (type == HY3X_F32) ((float *)p)[at] = v;
+  else if (type == HY3X_F16) ((__half *)p)[at] = __float2half(v);
+  else ((__hip_bfloat16 *)p)[at] = __float2bfloat16(v);
+}
+__device__ __forceinline__ void put(const Linear4Call &c, int64_t token, int n, float v) {
+  if (c.base) v += load_y(c.base, token * c.base_stride + n, c.y_type);
+  store_y(c.y, token * c.y_stride + n, c.y_type, v);
+}
+// N outputs that follow each other, in one store
+template <class Y, int N>
+__device__ __forceinline__ void put_run(const Linear4Call &c, int64_t token, int n,
+                                        const float (&v)[N]) {
+  Y e[N];
+  float b[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) b[i] = 0.0f;
+  if (c.base) {
+    __builtin_memcpy(e, (const Y *)c.base + token * c.base_stride + n, sizeof(e));
+#pragma unroll
+    for (int i = 0; i < N; i++) b[i] = load_y(&e[i], 0, type_of<Y>());
+  }
+#pragma unroll
+  for (int i = 0; i < N; i++) store_y(&e[i], 0, type_of<Y>(), v[i] + b[i]);
+  __builtin_memcpy((Y *)c.y + token * c.y_stride + n, e, sizeof(e));
+}
+
+// A quad's scales and zero points of one row: 4 GP of each.
+template <int GP>
+struct Groups {
+  uint32_t s[2 * GP], z[GP];
+  __device__ __forceinline__ void load(const Linear4Call &c, int rt, int qd, int row) {
+    __builtin_memcpy(s, __builtin_assume_aligned(
+        c.s + (((size_t)rt * c.quads + qd) * 16 + row) * (4 * GP), 8 * GP), sizeof(s));
+    __builtin_memcpy(z, __builtin_assume_aligned(
+        c.z + ((size_t)rt * c.z_tile + (size_t)qd * c.z_quad + row * (4 * GP)), 4 * GP), sizeof(z));
+  }
+  __device__ __forceinline__ float scale(int g, bool s16) const {
+    return scale_of(s[g / 2] >> (16 * (g & 1)) & 0xffffu, s16);
+  }
+  __device__ __forceinline__ float zero(int g) const { return (float)(z[g / 4] >> (8 * (g & 3)) & 255); }
+};
+
+// ---- few tokens ---------------------------------------------------------------
+// A block's waves split the quads of every row of W; each holds its part of x as
+// operands for as long as the block lasts, and the weights stream past, a row tile at
+// a time, RING of them in flight. The waves' sums meet in LDS.
+//
+// Operands are the integers q; what the zero points take off, z sum x, is formed from
+// sums of x over the groups, which the MFMAs find (times a matrix of ones) while the
+// first weights are on their way.
+//
+// Tokens: one tile of 16 (fp32: of 4, whose three parts are rows 4 t + p). Token t is row
+// 4 (t % 4) + t / 4, so that up to 4 tokens end in one register of the accumulator: NR of
+// its 4 are used.
+
+// Waves of a block, at most: the registers of a SIMD are enough for 4, or for 2 with a
+// ring or with fp32 on its way to parts.
+template <class X, int RING>
+constexpr int few_waves() {
+  return RING == 1 && Op<X>::PARTS == 1 ? 16 : 8;
+}
+
+template <int HQ, int GP>
+struct FewWeights {
+  u4v q[HQ][4];
+  Groups<GP> g[HQ];
+  __device__ __forceinline__ void load(const Linear4Call &c, int rt, int wave, int waves,
+                                       int lane) {
+#pragma unroll
+    for (int i = 0; i < HQ; i++) {
+      const int qd = min(wave + i * waves, c.quads - 1);
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        q[i][j] = __builtin_nontemporal_load(
+            &c.q[((size_t)rt * c.chunks + min(4 * qd + j, c.chunks - 1)) * 64 + lane]);
+      g[i].load(c, rt, qd, lane & 15);
+    }
+  }
+};
+
+template <class X, int GP, int HQ, int NR, int RING>
+__global__ __launch_bounds__((64 * few_waves<X, RING>()), (few_waves<X, RING>() / 4)) void k_linear4_few(
+    Linear4Call c) {
+  constexpr bool SPLIT = Op<X>::PARTS == 3;
+  constexpr int TT = SPLIT ? 4 : 16, OUT = SPLIT ? 1 : NR;  // sums of a lane
+  constexpr int REGS = SPLIT ? 3 : NR, WAVES = few_waves<X, RING>();
+  __shared__ float red[RING == 1 ? 1 : 2][WAVES][OUT][64];
+  __shared__ f4v sums[WAVES][HQ * 4 * GP][4];  // of x over the groups: registers of 4 rows
+  const int lane = threadIdx.x & 63, col = lane & 15, h = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+
+  // this lane's row of A: token and part
+  const int part = SPLIT ? col & 3 : 0, token = SPLIT ? col >> 2 : 4 * (col & 3) + (col >> 2);
+  u4v a[HQ][4][4];
+  FewWeights<HQ, GP> ring[RING];
+  {
+    const X *row = (const X *)c.x + (int64_t)min(token, c.T - 1) * c.x_stride;
+#pragma unroll
+    for (int i = 0; i < HQ; i++) {
+      const int k0 = 512 * (wave + i * waves);
+      const bool whole = k0 + 512 <= c.d_in;
+#pragma unroll
+      for (int ch = 0; ch < 4; ch++) {
+        Eight<X> e[4];
+        if (whole) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) e[j].load(row, k0 + 128 * ch + 32 * j + 8 * h);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            e[j].load_within(row, k0 + 128 * ch + 32 * j + 8 * h, c.d_in);
+        }
+        if (i == 0 && ch == (SPLIT ? 0 : 3)) ring[0].load(c, blockIdx.x, wave, waves, lane);
+#pragma unroll
+        for (int j = 0; j < 4; j++) a[i][ch][j] = e[j].operand(part);
+        if (SPLIT) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+#pragma unroll
+  for (int p = 1; p < RING; p++)
+    if (blockIdx.x + p * gridDim.x < (uint32_t)c.tiles)
+      ring[p].load(c, blockIdx.x + p * gridDim.x, wave, waves, lane);
+  const uint32_t one = Op<X>::both(1.0f);
+#pragma unroll
+  for (int i = 0; i < HQ; i++)
+#pragma unroll
+    for (int g = 0; g < 4 * GP; g++) {
+      f4v d = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = g * 4 / GP; j < (g + 1) * 4 / GP; j++)
+        d = Op<X>::mma(a[i][j / 4][j % 4], (u4v){one, one, one, one}, d);
+      if (col == 0) sums[wave][i * 4 * GP + g][h] = d;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+
+  auto tile = [&](const FewWeights<HQ, GP> &w, int rt, int turn) {
+    float acc[REGS];
+#pragma unroll
+    for (int r = 0; r < REGS; r++) acc[r] = 0.0f;
+    asm volatile("" ::: "memory");  // the sums stay in LDS from tile to tile
+#pragma unroll
+    for (int i = 0; i < HQ; i++)
+#pragma unroll
+      for (int g = 0; g < 4 * GP; g++) {  // groups of the quad
+        f4v d = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = g * 4 / GP; j < (g + 1) * 4 / GP; j++)  // 32 k of the quad's 512
+          d = Op<X>::mma(a[i][j / 4][j % 4], weights<X>(w.q[i][j / 4][j % 4]), d);
+        const float s = w.g[i].scale(g, c.s16), z = w.g[i].zero(g);
+        const float *x = (const float *)&sums[wave][i * 4 * GP + g][h];
+#pragma unroll
+        for (int r = 0; r < REGS; r++) acc[r] = fmaf(s, fmaf(-z, x[r], d[r]), acc[r]);
+        if (g % GP == GP - 1) __builtin_amdgcn_sched_barrier(0);  // registers of one chunk
+      }
+#pragma unroll
+    for (int r = 0; r < OUT; r++)
+      red[turn & 1][wave][r][lane] = SPLIT ? acc[0] + (acc[REGS / 2] + acc[REGS - 1]) : acc[r];
+  };
+  auto join = [&](int rt, int turn) {
+    __syncthreads();
+    // 64 sums at a time, by waves in turn; two buffers: a wave that writes the other one
+    // has passed this barrier, and one that writes this one the next
+    for (int o = (wave + waves - turn % waves) % waves; o < OUT; o += waves) {
+      const int64_t t = SPLIT ? h : 4 * o + h;
+      const int n = (int)linear4_row(rt, col);
+      float v = 0.0f;
+#pragma unroll 4
+      for (int w = 0; w < waves; w++) v += red[turn & 1][w][o][lane];
+      if (t < c.T && n < c.d_out) put(c, t, n, v);
+    }
+  };
+  if constexpr (RING == 1) {
+    tile(ring[0], blockIdx.x, 0);
+    join(blockIdx.x, 0);
+  } else {
+    int turn = 0;
+    for (int rt0 = blockIdx.x; rt0 < c.tiles; rt0 += RING * gridDim.x) {
+#pragma unroll
+      for (int p = 0; p < RING; p++, turn++) {
+        const int rt = rt0 + p * gridDim.x;
+        if (p && rt >= c.tiles) return;
+        tile(ring[p], rt, turn);
+        if (rt + RING * (int)gridDim.x < c.tiles)
+          ring[p].load(c, rt + RING * gridDim.x, wave, waves, lane);
+        join(rt, turn);
+      }
+    }
+  }
+}
+
+// ---- many tokens --------------------------------------------------------------
+// A block takes 16 RT WN rows of W and 16 CT tokens; WK of its waves share a row's k,
+// a chunk of 128 each at a time. x goes through LDS in the operands' order, a step ahead:
+// copied there as it is (DMA: rows of whole chunks, aligned to 16 bytes), or by way of
+// registers (fp32 becomes its three parts). Weights go straight to the lanes that use
+// them, and a chunk's operands stay in registers while its token tiles pass.
+//
+// Operands are the integers q. What the zero points take off, s z sum x, follows a step
+// behind: the waves that share a chunk find the sums of its token tiles, a few each, on
+// the MFMAs (x times ones), and leave them in LDS for all.
+template <class X, int GP, int RT, int CT, int WN, int WK, bool DMA>
+__global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c) {
+  constexpr int PARTS = Op<X>::PARTS, THREADS = 64 * WN * WK;
+  constexpr int PIECES = WK * CT * 256 / THREADS;  // runs of 8 elements a thread loads a step
+  static_assert(PIECES * THREADS == WK * CT * 256 && !(DMA && PARTS > 1), "whole pieces");
+  constexpr int XS = WK * PARTS * CT * 256, BUFS = DMA ? 2 : 1;
+  constexpr int RED = WK > 1 ? (WK - 1) * WN * RT * CT * 64 : 1;
+  __shared__ u4v lds[BUFS * XS > RED ? BUFS * XS : RED];
+  __shared__ f4v sums[2][WK][CT][GP][4];  // of x over a chunk's groups
+  const int lane = threadIdx.x & 63, col = lane & 15, h = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = wave / WK, wk = wave % WK;
+  // XCDs take blocks in turn: each gets a run of neighbouring tiles, token tiles first
+  const uint32_t token_tiles = (c.T + 16 * CT - 1) / (16 * CT);
+  const uint32_t per = gridDim.x / 8, left = gridDim.x % 8;
+  const uint32_t xcd = blockIdx.x % 8, item = xcd * per + min(xcd, left) + blockIdx.x / 8;
+  const int rt0 = (int)(item / token_tiles) * (RT * WN) + wn * RT;
+  const int64_t t0 = (int64_t)(item % token_tiles) * (16 * CT);
+
+  // piece p of a step: [wk][ct][j][lane], run j of 32 k and (lane / 16) of 8 of a token
+  const X *const x0 = (const X *)c.x + t0 * c.x_stride;
+  const X *from[DMA ? 1 : PIECES];
+  uint32_t offset[DMA ? PIECES : 1];
+#pragma unroll
+  for (int i = 0; i < PIECES; i++) {
+    const int p = threadIdx.x + i * THREADS;
+    const int64_t at = min((int64_t)(p / 256 % CT) * 16 + p % 16, c.T - 1 - t0) * c.x_stride;
+    if constexpr (DMA)
+      offset[i] = (uint32_t)(2 * (at + p / (256 * CT) * 128 + p / 64 % 4 * 32 + p % 64 / 16 * 8));
+    else from[i] = x0 + at;
+  }
+  Eight<X> ex[DMA ? 1 : PIECES];
+  auto fetch = [&](int step) {
+    if constexpr (DMA) {
+#pragma unroll
+      for (int i = 0; i < PIECES; i++)
+        dma16_s(x0 + (size_t)step * (WK * 128), offset[i],
+                lds_addr(&lds[(step & 1) * XS + i * THREADS + 64 * wave]));
+    } else {
+      const bool whole = (step + 1) * (WK * 128) <= c.d_in;
+#pragma unroll
+      for (int i = 0; i < PIECES; i++) {
+        const int p = threadIdx.x + i * THREADS;
+        const int k = (step * WK + p / (256 * CT)) * 128 + p / 64 % 4 * 32 + p % 64 / 16 * 8;
+        if (whole) ex[i].load(from[i], k);
+        else ex[i].load_within(from[i], k, c.d_in);
+      }
+    }
+  };
+  struct Weights {
+    u4v q[RT];
+    uint32_t s[RT][(GP + 1) / 2], z[RT];
+    __device__ __forceinline__ void load(const Linear4Call &c, int rt0, int chunk, int lane) {
+      const int ch = min(chunk, c.chunks - 1);
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
+        const int rt = min(rt0 + r, c.tiles - 1);
+        q[r] = c.q[((size_t)rt * c.chunks + ch) * 64 + lane];
+        const uint32_t at = (lane & 15) * (4 * GP);
+        const uint16_t *sp = c.s + ((size_t)rt * c.quads + (ch >> 2)) * (64 * GP) + (ch & 3) * GP;
+        const uint8_t *zp = c.z + (size_t)rt * c.z_tile + (size_t)(ch >> 2) * c.z_quad + (ch & 3) * GP;
+        if constexpr (GP == 1) {
+          s[r][0] = sp[at];
+          z[r] = zp[at];
+        } else if constexpr (GP == 2) {
+          s[r][0] = *(const uint32_t *)(sp + at);
+          z[r] = *(const uint16_t *)(zp + at);
+        } else {
+          const uint2 v = *(const uint2 *)(sp + at);
+          s[r][0] = v.x;
+          s[r][1] = v.y;
+          z[r] = *(const uint32_t *)(zp + at);
+        }
+      }
+    }
+  };
+  Weights next;
+  float acc[RT][CT][4], off[GP][RT];  // off: -s z of the chunk before
+#pragma unroll
+  for (int r = 0; r < RT; r++) {
+#pragma unroll
+    for (int t = 0; t < CT; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[r][t][i] = 0.0f;
+#pragma unroll
+    for (int g = 0; g < GP; g++) off[g][r] = 0.0f;
+  }
+  if (wn == 0)
+    for (int i = lane; i < CT * GP * 4; i += 64) (&sums[1][wk][0][0][0])[i] = (f4v){0, 0, 0, 0};
+
+  const int steps = (c.chunks + WK - 1) / WK;
+  fetch(0);
+  next.load(c, rt0, wk, lane);
+  for (int step = 0; step < steps; step++) {
+    if constexpr (DMA) {
+      wait_copies_and_barrier<0>();
+    } else {
+      if (step) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < PIECES; i++) {
+        const int p = threadIdx.x + i * THREADS;
+#pragma unroll
+        for (int q = 0; q < PARTS; q++)
+          lds[(p / (256 * CT) * PARTS + q) * (256 * CT) + p % (256 * CT)] = ex[i].operand(q);
+      }
+      __syncthreads();
+    }
+    u4v b[4][RT];
+    float s[GP][RT], z[GP][RT];
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+#pragma unroll
+      for (int g = 0; g < GP; g++) {
+        s[g][r] = scale_of(next.s[r][g / 2] >> (16 * (g & 1)) & 0xffffu, c.s16);
+        z[g][r] = (float)(next.z[r] >> (8 * g) & 255);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) b[j][r] = weights<X>(next.q[r][j]);
+    }
+    if (step + 1 < steps) {
+      fetch(step + 1);
+      next.load(c, rt0, (step + 1) * WK + wk, lane);
+    }
+    // a chunk beyond d_in meets zeros of x
+    const u4v *xs = &lds[(DMA ? (step & 1) * XS : 0) + wk * (PARTS * CT * 256) + lane];
+    {  // the sums of this wave's share of the token tiles
+      const uint32_t one = Op<X>::both(1.0f);
+#pragma unroll
+      for (int o = 0; o < (CT + WN - 1) / WN; o++) {
+        const int t = wn + o * WN;
+        if (CT % WN && t >= CT) break;
+#pragma unroll
+        for (int g = 0; g < GP; g++) {
+          f4v d = {0, 0, 0, 0};
+#pragma unroll
+          for (int j = g * 4 / GP; j < (g + 1) * 4 / GP; j++)
+#pragma unroll
+            for (int q = 0; q < PARTS; q++)
+              d = Op<X>::mma(xs[(q * CT + t) * 256 + j * 64], (u4v){one, one, one, one}, d);
+          if (col == 0) sums[step & 1][wk][t][g][h] = d;
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < CT; t++) {
+#pragma unroll
+      for (int g = 0; g < GP; g++) {
+        f4v d[RT];
+#pragma unroll
+        for (int r = 0; r < RT; r++) d[r] = (f4v){0, 0, 0, 0};
+#pragma unroll
+        for (int j = g * 4 / GP; j < (g + 1) * 4 / GP; j++)
+#pragma unroll
+          for (int q = 0; q < PARTS; q++) {
+            const u4v a = xs[(q * CT + t) * 256 + j * 64];
+#pragma unroll
+            for (int r = 0; r < RT; r++) d[r] = Op<X>::mma(a, b[j][r], d[r]);
+          }
+        const f4v before = sums[~step & 1][wk][t][g][h];
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            acc[r][t][i] = fmaf(off[g][r], before[i], acc[r][t][i]);
+            acc[r][t][i] = fmaf(s[g][r], d[r][i], acc[r][t][i]);
+          }
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < GP; g++)
+#pragma unroll
+      for (int r = 0; r < RT; r++) off[g][r] = -s[g][r] * z[g][r];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < CT; t++)
+#pragma unroll
+    for (int g = 0; g < GP; g++) {
+      const f4v before = sums[~steps & 1][wk][t][g][h];
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[r][t][i] = fmaf(off[g][r], before[i], acc[r][t][i]);
+    }
+  if constexpr (WK > 1) {  // the waves' parts of k
+    if (wk)
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int t = 0; t < CT; t++)
+          lds[(((wk - 1) * WN + wn) * RT * CT + r * CT + t) * 64 + lane] =
+              __builtin_bit_cast(u4v, *(f4v *)acc[r][t]);
+    __syncthreads();
+    if (wk) return;
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+      for (int t = 0; t < CT; t++)
+        for (int w = 1; w < WK; w++) {
+          const f4v o = __builtin_bit_cast(
+              f4v, lds[(((w - 1) * WN + wn) * RT * CT + r * CT + t) * 64 + lane]);
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[r][t][i] += o[i];
+        }
+  }
+  const int n = (int)linear4_row(rt0, col);
+#pragma unroll
+  for (int t = 0; t < CT; t++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int64_t token = t0 + 16 * t + 4 * h + i;
+      if (token >= c.T) continue;
+      float v[RT];
+#pragma unroll
+      for (int r = 0; r < RT; r++) v[r] = acc[r][t][i];
+      if (n + RT <= c.d_out) {
+        if (c.y_type == HY3X_F32) put_run<float>(c, token, n, v);
+        else if (c.y_type == HY3X_F16) put_run<__half>(c, token, n, v);
+        else put_run<__hip_bfloat16>(c, token, n, v);
+      } else {
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+          if (n + r < c.d_out) put(c, token, n + r, v[r]);
+      }
+    }
+}
+
+template <class X, int GP, int RT, int CT, int WN, int WK, bool DMA>
+void many(const Linear4Call &c, hipStream_t st) {
+  const int64_t blocks = (int64_t)((c.T + 16 * CT - 1) / (16 * CT)) *
+                         ((c.tiles + RT * WN - 1) / (RT * WN));
+  k_linear4_many<X, GP, RT, CT, WN, WK, DMA><<<(uint32_t)blocks, 64 * WN * WK, 0, st>>>(c);
+}
+template <class X, int GP, int HQ, int NR, int RING>
+void few(const Linear4Call &c, int waves, int blocks, hipStream_t st) {
+  k_linear4_few<X, GP, HQ, NR, RING><<<blocks, 64 * waves, 0, st>>>(c);
+}
+// Where all row tiles fit the card at once each has a block, and no ring.
+template <class X, int GP, int NR>
+bool few(const Linear4Call &c, hipStream_t st) {
+  constexpr int ONCE = few_waves<X, 1>(), RING = few_waves<X, 2>();
+  if (c.quads <= ONCE && (int64_t)c.tiles * c.quads <= 256 * ONCE)
+    few<X, GP, 1, NR, 1>(c, c.quads, c.tiles, st);
+  else if (c.quads <= RING)
+    few<X, GP, 1, NR, 3>(c, c.quads, std::min(c.tiles, 256), st);
+  else if (c.quads <= 2 * RING)
+    few<X, GP, 2, NR, 2>(c, (c.quads + 1) / 2, std::min(c.tiles, 256), st);
+  else
+    return false;
+  return true;
+}
+
+template <class X, int GP>
+void launch_group(const Linear4Call &c, hipStream_t st) {
+  constexpr bool SPLIT = Op<X>::PARTS == 3;
+  if (c.T <= 4) {
+    if (few<X, GP, 1>(c, st)) return;
+  } else if (!SPLIT && c.T <= 16) {
+    if (few<X, GP, SPLIT ? 1 : 4>(c, st)) return;
+  }
+  if (c.T <= 16) return many<X, GP, 1, 1, 1, 8, false>(c, st);
+  if (c.T <= 32) return many<X, GP, 2, 2, 2, 2, false>(c, st);
+  const int64_t big = (int64_t)((c.T + 63) / 64) * ((c.tiles + 15) / 16);
+  if (big >= 256) {
+    if constexpr (!SPLIT)  // 32-bit offsets of 64 rows
+      if (c.d_in % 128 == 0 && (uintptr_t)c.x % 16 == 0 && c.x_stride % 8 == 0 &&
+          c.x_stride <= 1 << 24)
+        return many<X, GP, 4, 4, 4, 1, true>(c, st);
+    return many<X, GP, 4, 4, 4, 1, false>(c, st);
+  }
+  return many<X, GP, 2, 2, 2, 2, false>(c, st);
+}
+
+}  // namespace linear4
+
+template <class X>
+void launch_linear4(const Linear4Call &c, hipStream_t st) {
+  if (c.group == 128) linear4::launch_group<X, 1>(c, st);
+  else if (c.group == 64) linear4::launch_group<X, 2>(c, st);
+  else linear4::launch_group<X, 4>(c, st);
+}
+
+}  // namespace hy3x

@@ -372,13 +372,14 @@ int hy3x_adapters_apply(const hy3x_adapters *adapters, const int32_t *ids, const
  * whose product adapters can then stand beside. */
 typedef struct hy3x_linear4 hy3x_linear4;
 #define HY3X_LINEAR4_MAX_OUT (1 << 20)
+#define HY3X_LINEAR4_MIN_IN 8
 #define HY3X_LINEAR4_MAX_IN 65536
 #define HY3X_LINEAR4_MAX_TOKENS (1 << 24)
 
 /* A matrix on the current device, without weights until they are set. group: 32, 64
  * or 128 (the last group of a row may be shorter); type HY3X_F16 or HY3X_BF16: the
  * elements of the scales. Device memory: d_out d_in / 2 bytes and 3 for each group
- * (d_out rounded up to 16, d_in to 128, the groups of a row to those of 512). */
+ * (d_out rounded up to 64, d_in to 128, the groups of a row to those of 512). */
 int hy3x_linear4_create(hy3x_linear4 **out, int d_out, int d_in, int group, int type);
 int hy3x_linear4_destroy(hy3x_linear4 *weights);
 /* The weights: q, bytes [d_out x (d_in + 1) / 2], weight k of a row in byte k / 2, an
