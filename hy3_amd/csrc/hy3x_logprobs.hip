@@ -11,16 +11,20 @@
 // to it (a larger maximum scales them down), in fp32; lanes, waves and the parts of a row
 // meet in 64 bits. Few rows are split into parts, which a second launch joins.
 //
-// The most probable tokens: a wave keeps its best in falling order, one a lane, and looks
-// at single logits only where one of 64 lanes has met a batch whose maximum passes the
-// last of them. The first batch would put every logit there: a bound is found first, with
-// at least as many lanes at or above it as tokens are wanted.
+// The most probable tokens: a lane remembers the largest maximum of its batches, which
+// batch it was, and the second largest. When all have been met, a value is found that as
+// many lanes' maxima reach as tokens are wanted. The batches of the lanes above it are
+// read again (all of a lane's where its second reaches it too), and what reaches it,
+// little more than is wanted, is ranked: a candidate's place is the number of better
+// ones. Rows where too many logits reach it (equal ones) are gone through again, the
+// wave's best in its lanes.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
 #include <algorithm>
 
 #include "../../include/hy3x_moe.h"
+#include "hy3x_common.h"
 #include "hy3x_error.h"
 #include "hy3x_ops.h"
 
@@ -53,17 +57,13 @@ struct Type<__hip_bfloat16> {
 constexpr float FAR = 200.0f;
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int MAX_PARTS = 64;  // of a row: a lane for each in k_join
-constexpr int NO_ID = 0x7fffffff;
 
 struct Stats {  // of a part of a row; m: the type's lowest value where all is masked
   double S, E;
-  float m;
-  int unused[3];
+  float m, unused;
 };
-struct Entry {
-  float v;
-  int id;
-};
+// A logit and its index as one number: the better one is the larger one. 0: none.
+typedef unsigned long long Entry;
 
 struct Call {
   const void *logits;
@@ -76,73 +76,128 @@ struct Call {
   Entry *lists;   // [T x parts x top]
 };
 
-__device__ __forceinline__ bool better(float v, int id, float w, int jd) {
-  return v > w || (v == w && id < jd);
+template <int CTRL>
+__device__ __forceinline__ double moved(double v) {  // between lanes of 16
+  const long long b = __double_as_longlong(v);
+  const uint32_t lo = dppi<CTRL>((int)b), hi = dppi<CTRL>((int)(b >> 32));
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  const long long b = __double_as_longlong(v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)b, lane),
+                 hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
 }
 __device__ __forceinline__ float lane_value(float v, int lane) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
+__device__ __forceinline__ double sum_of_wave(double v) {
+  v += moved<DPP_XOR1>(v);
+  v += moved<DPP_XOR2>(v);
+  v += moved<DPP_HALF_MIRROR>(v);
+  v += moved<DPP_MIRROR>(v);
+  return (lane_value(v, 0) + lane_value(v, 16)) + (lane_value(v, 32) + lane_value(v, 48));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, dpp<DPP_XOR1>(v));
+  v = fmaxf(v, dpp<DPP_XOR2>(v));
+  v = fmaxf(v, dpp<DPP_HALF_MIRROR>(v));
+  v = fmaxf(v, dpp<DPP_MIRROR>(v));
+  return fmaxf(fmaxf(lane_value(v, 0), lane_value(v, 16)),
+               fmaxf(lane_value(v, 32), lane_value(v, 48)));
+}
 
-// Integers in the order of the floats, -0 as 0; the float just below one.
+// Integers in the order of the floats, -0 as 0; the float of one, and the one just below.
 __device__ __forceinline__ int order_of(float v) {
   const int b = __float_as_int(v + 0.0f);
   return b ^ (b >> 31 & 0x7fffffff);
 }
-__device__ __forceinline__ float below(int order) {
-  int o = order - 1;
-  if (o == -1) o = -2;  // -0
+__device__ __forceinline__ float in_order(int o) {
   return __int_as_float(o ^ (o >> 31 & 0x7fffffff));
 }
-// A value that at least n of the wave's v reach (-inf if fewer are finite): bisected, in
-// their order.
+__device__ __forceinline__ float below(int o) {
+  return in_order(o == 0 ? -2 : o - 1);  // -1 stands for -0
+}
+__device__ __forceinline__ Entry entry(float v, int id) {
+  return (Entry)((uint32_t)order_of(v) ^ 0x80000000u) << 32 | (uint32_t)~id;
+}
+__device__ __forceinline__ float value_of(Entry e) {
+  return in_order((int)((uint32_t)(e >> 32) ^ 0x80000000u));
+}
+__device__ __forceinline__ int id_of(Entry e) { return (int)~(uint32_t)e; }
+// How many of n entries in LDS are better.
+__device__ __forceinline__ int better_than(Entry e, const Entry *all, int n) {
+  int place = 0, k = 0;
+  for (; k + 8 <= n; k += 8) {
+    Entry o[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) o[j] = all[k + j];
+#pragma unroll
+    for (int j = 0; j < 8; j++) place += o[j] > e;
+  }
+  for (; k < n; k++) place += all[k] > e;
+  return place;
+}
+
+// A value that at least n of the wave's v reach (-inf if fewer are finite), near the
+// largest such: its place in their order, quartered.
 __device__ __forceinline__ int reached_by(float v, int n) {
   const int k = order_of(v), none = order_of(-INFINITY);
   if (__popcll(__ballot(k > none)) < n) return none;
-  int lo = none, hi = order_of(INFINITY);
-  for (int i = 0; i < 20; i++) {
+  int lo = order_of(-wave_max(-v)), hi = order_of(wave_max(v));
+  for (int i = 0; i < 6; i++) {
     const int mid = (lo & hi) + ((lo ^ hi) >> 1);
-    if (__popcll(__ballot(k >= mid)) >= n) lo = mid;
-    else hi = mid;
+    const int low = (lo & mid) + ((lo ^ mid) >> 1), high = (mid & hi) + ((mid ^ hi) >> 1);
+    const int a = __popcll(__ballot(k >= low)), b = __popcll(__ballot(k >= mid)),
+              c = __popcll(__ballot(k >= high));
+    hi = a < n ? low : b < n ? mid : c < n ? high : hi;
+    lo = c >= n ? high : b >= n ? mid : a >= n ? low : lo;
   }
   return lo;
 }
 
+constexpr int MAX_TOP = HY3X_LOGPROBS_MAX_TOP;
+constexpr int CANDIDATES = 512;
+constexpr int AGAIN = 1024;  // batches of a lane that are read again
+constexpr int ROUND = 8;  // logits of a lane that are ranked at once
+struct Ranking {          // a wave's, in LDS
+  Entry all[MAX_TOP + 64 * ROUND], sorted[MAX_TOP];
+};
+
 // The wave's best in falling order, one a lane.
 struct Best {
-  float v = -INFINITY, last;  // last: what a logit has to pass
-  int id = NO_ID;
-  __device__ __forceinline__ void put(float x, int i, int n, int lane) {
-    const int at = __popcll(__ballot(better(v, id, x, i)));
-    if (at >= n) return;
-    const float up = __int_as_float(
-        __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x138, 0xf, 0xf, false));
-    const int upi = __builtin_amdgcn_update_dpp(0, id, 0x138, 0xf, 0xf, false);
-    v = lane < at ? v : lane == at ? x : up;
-    id = lane < at ? id : lane == at ? i : upi;
-    last = fmaxf(last, lane_value(v, n - 1));
+  Entry e = 0;
+  float last;  // what a logit has to pass
+  int size = 0;
+  // with `more` entries from room.all[MAX_TOP] on, the best n
+  __device__ __forceinline__ void rank(Ranking &room, int more, int n, int lane) {
+    if (lane < size) room.all[MAX_TOP - size + lane] = e;
+    const Entry *all = room.all + MAX_TOP - size;
+    const int count = size + more;
+    for (int c = 0; c < count; c += 64) {
+      const Entry o = all[min(c + lane, count - 1)];
+      const int place = better_than(o, all, count);
+      if (c + lane < count && place < n) room.sorted[place] = o;
+    }
+    size = min(count, n);
+    e = room.sorted[lane % MAX_TOP];
+    if (lane >= size) e = 0;
+    if (size == n) last = lane_value(value_of(e), n - 1);
   }
 };
 
-// S and E of lanes, relative to their own maxima, to sums over the wave relative to the
-// wave's.
-__device__ __forceinline__ void meet(float &m, double &S, double &E) {
-  float top = m;
-  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-  const double d = fmax((double)m - top, (double)-FAR), f = exp(d);
-  E = (E + S * d) * f;
+// A lane's maximum and sums relative to it, to sums relative to `top`.
+__device__ __forceinline__ void rescale(float m, float top, float &S, float &E) {
+  const float d = fmaxf(m - top, -FAR), f = __expf(d);
+  E = fmaf(S, d, E) * f;
   S *= f;
-  for (int o = 32; o; o >>= 1) {
-    S += __shfl_xor(S, o, 64);
-    E += __shfl_xor(E, o, 64);
-  }
-  m = top;
 }
 
-// The row's results from its statistics and its candidates (value, id; -inf: none), which
-// stand in LDS. Every thread of the block calls it.
+// The row's results from its statistics and its candidates, which stand in LDS (some may
+// be none). Every thread of the block calls it.
 template <class X>
-__device__ void finish(const Call &c, int t, float m, double S, double E, float given,
-                       const Entry *cand, int n_cand) {
+__device__ void finish(const Call &c, int t, int token, float given, float m, double S, double E,
+                       const Entry *cand, int n_cand, int live) {
   const X *row = (const X *)c.logits + t * c.stride;
   const bool some = m > -Type<X>::HIGH;
   const double lse = some ? log(S) : 0.0;
@@ -150,28 +205,21 @@ __device__ void finish(const Call &c, int t, float m, double S, double E, float 
     return l > -Type<X>::HIGH ? (float)(((double)fminf(l, Type<X>::HIGH) - m) - lse) : -INFINITY;
   };
   if (threadIdx.x == 0) {
-    const int token = c.tokens[t];
     c.logp[t] = token >= 0 && token < c.V ? logp(given) : 0.0f;
     if (c.entropy) c.entropy[t] = some ? (float)(lse - E / S) : 0.0f;
   }
   if (!c.top) return;
-  __shared__ int live;
-  if (threadIdx.x == 0) live = 0;
-  __syncthreads();
   for (int i = threadIdx.x; i < n_cand; i += blockDim.x) {
     const Entry e = cand[i];
-    if (e.id == NO_ID) continue;
-    int rank = 0;
-    for (int j = 0; j < n_cand; j++) rank += better(cand[j].v, cand[j].id, e.v, e.id);
-    atomicAdd(&live, 1);
-    if (rank < c.top) {
-      c.top_ids[(int64_t)t * c.top + rank] = e.id;
-      c.top_logp[(int64_t)t * c.top + rank] = logp(e.v);
+    if (!e) continue;
+    const int place = better_than(e, cand, n_cand);
+    if (place < c.top) {
+      c.top_ids[(int64_t)t * c.top + place] = id_of(e);
+      c.top_logp[(int64_t)t * c.top + place] = logp(value_of(e));
     }
   }
-  __syncthreads();
   // masked tokens in the places that are left, in index order
-  if (live < c.top && threadIdx.x < 64) {
+  if (threadIdx.x < 64) {
     int at = live;
     for (int v = 0; v < c.V && at < c.top; v += 64) {
       const int id = v + threadIdx.x;
@@ -188,128 +236,209 @@ __device__ void finish(const Call &c, int t, float m, double S, double E, float 
 }
 
 template <class X>
-__device__ __forceinline__ float given_logit(const Call &c, int t) {
-  const int token = c.tokens[t];
+__device__ __forceinline__ float given_logit(const Call &c, int t, int token) {
   return elem(((const X *)c.logits)[t * c.stride + min(max(token, 0), c.V - 1)]);
+}
+
+// A lane's logits of a batch: U times N that follow each other.
+template <class X>
+struct Batch {
+  static constexpr int N = 16 / sizeof(X), U = 4, COUNT = N * U, SIZE = THREADS * COUNT;
+  uint32_t w[U][4];
+  // index of logit j in the batch
+  static __device__ __forceinline__ int place(int j, int tid) {
+    return (j / N * THREADS + tid) * N + j % N;
+  }
+  // of the batch from `at`; what lies beyond `end` is masked
+  __device__ __forceinline__ void load(const X *row, int at, int end, int tid) {
+    if (at + SIZE <= end) {
+#pragma unroll
+      for (int u = 0; u < U; u++) __builtin_memcpy(w[u], row + at + place(u * N, tid), 16);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int k = at + place(u * N, tid);
+        if (k + N <= end) {
+          __builtin_memcpy(w[u], row + k, 16);
+        } else {
+          X e[N];
+#pragma unroll
+          for (int i = 0; i < N; i++) {
+            const uint32_t none = Type<X>::MASKED;
+            __builtin_memcpy(&e[i], &none, sizeof(X));
+            if (k + i < end) e[i] = row[k + i];
+          }
+          __builtin_memcpy(w[u], e, 16);
+        }
+      }
+    }
+  }
+  // logit j; +inf as the largest finite value where the caller says that there is one
+  __device__ __forceinline__ float at(int j) const {
+    const uint32_t x = sizeof(X) == 4 ? w[j / 4][j % 4] : w[j / 8][j % 8 / 2];
+    if constexpr (sizeof(X) == 4) return __uint_as_float(x);
+    else return elem(__builtin_bit_cast(X, (uint16_t)(x >> (16 * (j & 1)))));
+  }
+};
+
+// The waves' best of a part, through its batches, whatever there is.
+template <class X>
+__device__ void best_of_all(const X *row, int first, int end, int n, Ranking &room, Entry *cand) {
+  using B = Batch<X>;
+  const int tid = threadIdx.x, lane = tid & 63;
+  Best best;
+  best.last = -Type<X>::HIGH;
+  for (int at = first; at < end; at += B::SIZE) {
+    B batch;
+    batch.load(row, at, end, tid);
+    float v[B::COUNT], top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < B::COUNT; j++) {
+      v[j] = batch.at(j) > Type<X>::HIGH ? Type<X>::HIGH : batch.at(j);
+      top = fmaxf(top, v[j]);
+    }
+    const uint64_t over = __ballot(top > best.last);
+    if (!over) continue;
+    // an equal logit of a later batch has a higher index and comes after the last
+    float last = best.last;
+    if (__popcll(over) >= n) last = fmaxf(last, below(reached_by(top, n)));
+    for (int round = 0; round < B::COUNT / ROUND; round++) {
+      int more = 0;
+#pragma unroll
+      for (int j = 0; j < ROUND; j++) {
+        float x = v[j];
+        int id = at + B::place(j, tid);
+#pragma unroll
+        for (int r = 1; r < B::COUNT / ROUND; r++) {
+          x = round == r ? v[r * ROUND + j] : x;
+          id = round == r ? at + B::place(r * ROUND + j, tid) : id;
+        }
+        const uint64_t hits = __ballot(x > last);
+        if (x > last)
+          room.all[MAX_TOP + more + __popcll(hits & ((1ull << lane) - 1))] = entry(x, id);
+        more += __popcll(hits);
+      }
+      if (more) best.rank(room, more, n, lane);
+    }
+  }
+  if (lane < n) cand[tid / 64 * n + lane] = best.e;
 }
 
 // A part of a row.
 template <class X, bool TOP>
 __global__ __launch_bounds__(THREADS) void k_logprobs(Call c) {
-  constexpr int N = 16 / sizeof(X), U = sizeof(X) == 4 ? 4 : 2, BATCH = THREADS * N * U;
+  using B = Batch<X>;
   constexpr float HIGH = Type<X>::HIGH;
-  __shared__ Stats part[WAVES];
-  __shared__ Entry cand[TOP ? WAVES * HY3X_LOGPROBS_MAX_TOP : 1];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ float high[WAVES], reach[WAVES];
+  __shared__ double sums[WAVES][2];
+  __shared__ Entry cand[TOP ? CANDIDATES : 1];
+  __shared__ Ranking room[TOP ? WAVES : 1];
+  __shared__ int again[TOP ? AGAIN : 1];  // batch of the part and thread
+  __shared__ int n_cand, n_again;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int t = blockIdx.x / c.parts, p = blockIdx.x % c.parts;
   const int first = p * c.part, end = min(c.V, first + c.part);
   const X *row = (const X *)c.logits + t * c.stride;
-  const float given = c.parts == 1 ? given_logit<X>(c, t) : 0.0f;
+  const int token = c.parts == 1 ? c.tokens[t] : 0;
+  const float given = c.parts == 1 ? given_logit<X>(c, t, token) : 0.0f;
 
-  struct Raw {
-    uint32_t w[U][4];
-    __device__ __forceinline__ void load(const X *row, int at, int end, int tid) {
-      if (at + BATCH <= end) {
-#pragma unroll
-        for (int u = 0; u < U; u++)
-          __builtin_memcpy(w[u], row + at + (u * THREADS + tid) * N, 16);
-      } else {
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-          const int k = at + (u * THREADS + tid) * N;
-          if (k + N <= end) {
-            __builtin_memcpy(w[u], row + k, 16);
-          } else {
-            X e[N];
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-              const uint32_t none = Type<X>::MASKED;
-              __builtin_memcpy(&e[i], &none, sizeof(X));
-              if (k + i < end) e[i] = row[k + i];
-            }
-            __builtin_memcpy(w[u], e, 16);
-          }
-        }
-      }
-    }
-    __device__ __forceinline__ float at(int j) const {
-      const uint32_t x = sizeof(X) == 4 ? w[j / 4][j % 4] : w[j / 8][j % 8 / 2];
-      if constexpr (sizeof(X) == 4) return __uint_as_float(x);
-      else return elem(__builtin_bit_cast(X, (uint16_t)(x >> (16 * (j & 1)))));
-    }
-  };
-  Raw next;
+  B next;
   next.load(row, first, end, tid);
   float m = -HIGH, S = 0.0f, E = 0.0f;
-  Best best;
-  best.last = -HIGH;
-  for (int at = first; at < end; at += BATCH) {
-    float v[N * U];
+  float best = -INFINITY, second = -INFINITY;  // of the batches' maxima
+  int best_at = first;
+  for (int at = first; at < end; at += B::SIZE) {
+    float v[B::COUNT];
 #pragma unroll
-    for (int j = 0; j < N * U; j++) v[j] = next.at(j);
-    if (at + BATCH < end) next.load(row, at + BATCH, end, tid);
+    for (int j = 0; j < B::COUNT; j++) v[j] = next.at(j);
+    if (at + B::SIZE < end) next.load(row, at + B::SIZE, end, tid);
     float top = -INFINITY;  // not NaN where all of them are
 #pragma unroll
-    for (int j = 0; j < N * U; j++) top = fmaxf(top, v[j]);
+    for (int j = 0; j < B::COUNT; j++) top = fmaxf(top, v[j]);
     if (__ballot(top > HIGH)) {  // +inf
 #pragma unroll
-      for (int j = 0; j < N * U; j++) v[j] = v[j] > HIGH ? HIGH : v[j];
+      for (int j = 0; j < B::COUNT; j++) v[j] = v[j] > HIGH ? HIGH : v[j];
       top = fminf(top, HIGH);
     }
-    if constexpr (TOP) {
-      if (at == first) {
-        const int bound = reached_by(top, c.top);
-        if (bound != order_of(-INFINITY)) best.last = fmaxf(best.last, below(bound));
-      }
-      if (__ballot(top > best.last)) {
-        const float last = best.last;  // a later batch's equals have higher indices
-#pragma unroll
-        for (int j = 0; j < N * U; j++) {
-          uint64_t hits = __ballot(v[j] > last);
-          while (hits) {
-            const int l = __builtin_ctzll(hits);
-            hits &= hits - 1;
-            best.put(lane_value(v[j], l),
-                     at + (j / N * THREADS + 64 * wave + l) * N + j % N, c.top, lane);
-          }
-        }
-      }
+    if (TOP) {
+      second = fmaxf(second, fminf(best, top));
+      best_at = top > best ? at : best_at;
+      best = fmaxf(best, top);
     }
-    const float to = fmaxf(m, top), d = fmaxf(m - to, -FAR), f = __expf(d);
-    E = fmaf(S, d, E) * f;
-    S *= f;
+    const float to = fmaxf(m, top);
+    rescale(m, to, S, E);
     m = to;
 #pragma unroll
-    for (int j = 0; j < N * U; j++) {
+    for (int j = 0; j < B::COUNT; j++) {
       const float x = fmaxf(v[j] - m, -FAR), e = __expf(x);
       S += e;
       E = fmaf(e, x, E);
     }
   }
-  double Sd = S, Ed = E;
-  meet(m, Sd, Ed);
-  if (lane == 0) part[wave] = {Sd, Ed, m, {}};
-  if (TOP && lane < c.top) cand[wave * c.top + lane] = {best.v, best.id};
+  // the block's maximum, then the sums
+  const float wave_high = wave_max(m);  // every lane takes part
+  if (lane == 0) high[wave] = wave_high;
+  if (TOP) {
+    const int bound = reached_by(best, (c.top + WAVES - 1) / WAVES);
+    if (lane == 0) reach[wave] = in_order(bound);
+    if (tid == 0) n_cand = n_again = 0;
+  }
   __syncthreads();
-  m = part[lane % WAVES].m;
-  Sd = lane < WAVES ? part[lane % WAVES].S : 0.0;
-  Ed = lane < WAVES ? part[lane % WAVES].E : 0.0;
-  meet(m, Sd, Ed);
+  float top = high[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; w++) top = fmaxf(top, high[w]);
+  rescale(m, top, S, E);
+  const double Sw = sum_of_wave((double)S), Ew = sum_of_wave((double)E);
+  if (lane == 0) sums[wave][0] = Sw, sums[wave][1] = Ew;
+  if (TOP) {
+    float bound = reach[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; w++) bound = fminf(bound, reach[w]);
+    bound = fmaxf(bound, below(order_of(-HIGH) + 2));  // of what is not masked
+    if (best >= bound) {
+      const bool all = second >= bound;
+      const int batches = all ? (end - first + B::SIZE - 1) / B::SIZE : 1;
+      const int at = all ? 0 : (best_at - first) / B::SIZE, to = atomicAdd(&n_again, batches);
+      for (int i = 0; i < batches && to + i < AGAIN; i++) again[to + i] = (at + i) * THREADS + tid;
+    }
+    __syncthreads();
+    const int items = min(n_again, AGAIN) * B::COUNT;
+#pragma unroll 4
+    for (int i = tid; i < items; i += THREADS) {
+      const int a = again[i / B::COUNT];
+      const int id = first + a / THREADS * B::SIZE + B::place(i % B::COUNT, a % THREADS);
+      const float x = id < end ? elem(row[id]) : -INFINITY;
+      if (x >= bound) {
+        const int to = atomicAdd(&n_cand, 1);
+        if (to < CANDIDATES) cand[to] = entry(fminf(x, HIGH), id);
+      }
+    }
+  }
+  __syncthreads();
+  double Sd = 0.0, Ed = 0.0;
+#pragma unroll
+  for (int w = 0; w < WAVES; w++) Sd += sums[w][0], Ed += sums[w][1];
+  int count = TOP ? n_cand : 0, live = count;
+  if (TOP && (count > CANDIDATES || n_again > AGAIN)) {
+    __syncthreads();
+    best_of_all<X>(row, first, end, c.top, room[wave], cand);
+    count = WAVES * c.top;
+    __syncthreads();
+    live = better_than(0, cand, count);
+  }
   if (c.parts == 1) {
-    finish<X>(c, t, m, Sd, Ed, given, cand, TOP ? WAVES * c.top : 0);
+    finish<X>(c, t, token, given, top, Sd, Ed, cand, count, live);
     return;
   }
-  if (tid == 0) c.stats[blockIdx.x] = {Sd, Ed, m, {}};
-  if (TOP && tid < WAVES * c.top) {
-    const Entry e = cand[tid];
-    int rank = 0;
-    for (int j = 0; j < WAVES * c.top; j++) {
-      // empty places are equal: in the order of the threads
-      const Entry o = cand[j];
-      rank += better(o.v, o.id, e.v, e.id) || (o.v == e.v && o.id == e.id && j < tid);
+  if (tid == 0) c.stats[blockIdx.x] = {Sd, Ed, top, 0.0f};
+  if (TOP) {
+    Entry *list = c.lists + (int64_t)blockIdx.x * c.top;
+    for (int i = tid; i < count; i += THREADS) {
+      const Entry e = cand[i];
+      const int place = better_than(e, cand, count);
+      if (e && place < c.top) list[place] = e;
     }
-    if (rank < c.top) c.lists[(int64_t)blockIdx.x * c.top + rank] = e;
+    if (tid < c.top && tid >= live) list[tid] = 0;
   }
 }
 
@@ -319,26 +448,28 @@ __global__ __launch_bounds__(THREADS) void k_join(Call c) {
   __shared__ Entry cand[MAX_PARTS * HY3X_LOGPROBS_MAX_TOP];
   __shared__ int n_cand;
   const int t = blockIdx.x, lane = threadIdx.x & 63;
-  const float given = given_logit<X>(c, t);
+  const int token = c.tokens[t];
+  const float given = given_logit<X>(c, t, token);
   const bool in = lane < c.parts;
   const Stats part = c.stats[(int64_t)t * c.parts + (in ? lane : 0)];
-  float m = part.m;
-  double S = in ? part.S : 0.0, E = in ? part.E : 0.0;
-  meet(m, S, E);
+  const float m = wave_max(part.m);
+  const float d = fmaxf(part.m - m, -FAR), f = in ? __expf(d) : 0.0f;
+  const double S = sum_of_wave(part.S * f), E = sum_of_wave((part.E + part.S * d) * f);
   if (threadIdx.x == 0) n_cand = 0;
   __syncthreads();
   if (c.top) {
     // at least c.top candidates reach what `lists` of the lists' `deep` first ones reach
     const Entry *all = c.lists + (int64_t)t * c.parts * c.top;
     const int deep = (c.top + c.parts - 1) / c.parts, lists = (c.top + deep - 1) / deep;
-    const int bound = reached_by(in ? all[lane * c.top + deep - 1].v : -INFINITY, lists);
+    const Entry first = in ? all[lane * c.top + deep - 1] : 0;
+    const int bound = reached_by(first ? value_of(first) : -INFINITY, lists);
     for (int i = threadIdx.x; i < c.parts * c.top; i += THREADS) {
       const Entry e = all[i];
-      if (e.id != NO_ID && order_of(e.v) >= bound) cand[atomicAdd(&n_cand, 1)] = e;
+      if (e && order_of(value_of(e)) >= bound) cand[atomicAdd(&n_cand, 1)] = e;
     }
     __syncthreads();
   }
-  finish<X>(c, t, m, S, E, given, cand, n_cand);
+  finish<X>(c, t, token, given, m, S, E, cand, n_cand, n_cand);
 }
 
 // Parts of a row: enough blocks for the card, of no less than PART logits each.

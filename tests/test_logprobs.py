@@ -158,6 +158,14 @@ def test_rows(torch, T, kind):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", list(NAMES))
+@pytest.mark.parametrize("T,V", [(1, 100), (1, 30000), (40, 5000), (1100, 700)])
+def test_negative_logits(torch, T, V, kind):
+    l = logits(torch, T, V, kind, V) - 60.0
+    check(torch, Call(torch, l, given(torch, T, V, 1), 12)())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(NAMES))
 def test_the_head_s_vocabulary(torch, kind):
     for T in (1, 2, 9):
         check(torch, Call(torch, logits(torch, T, 120832, kind, T), given(torch, T, 120832, T), 32)())
