@@ -55,7 +55,6 @@ struct Type<__hip_bfloat16> {
 // e^(-FAR) is 0 in fp32: what lies further below a maximum counts as this far, so that a
 // masked logit, -inf or NaN (which max passes over), adds 0 to both sums.
 constexpr float FAR = 200.0f;
-constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int MAX_PARTS = 64;  // of a row: a lane for each in k_join
 
 struct Stats {  // of a part of a row; m: the type's lowest value where all is masked
@@ -157,9 +156,9 @@ __device__ __forceinline__ int reached_by(float v, int n) {
 }
 
 constexpr int MAX_TOP = HY3X_LOGPROBS_MAX_TOP;
-constexpr int CANDIDATES = 512;
-constexpr int AGAIN = 1024;  // batches of a lane that are read again
-constexpr int ROUND = 8;  // logits of a lane that are ranked at once
+constexpr int CANDIDATES = 384;
+constexpr int AGAIN = 512;  // batches of a lane that are read again
+constexpr int ROUND = 4;  // logits of a lane that are ranked at once
 struct Ranking {          // a wave's, in LDS
   Entry all[MAX_TOP + 64 * ROUND], sorted[MAX_TOP];
 };
@@ -241,9 +240,10 @@ __device__ __forceinline__ float given_logit(const Call &c, int t, int token) {
 }
 
 // A lane's logits of a batch: U times N that follow each other.
-template <class X>
+template <class X, int WAVES>
 struct Batch {
-  static constexpr int N = 16 / sizeof(X), U = 4, COUNT = N * U, SIZE = THREADS * COUNT;
+  static constexpr int THREADS = 64 * WAVES, N = 16 / sizeof(X), U = sizeof(X) == 4 ? 4 : 2;
+  static constexpr int COUNT = N * U, SIZE = THREADS * COUNT;
   uint32_t w[U][4];
   // index of logit j in the batch
   static __device__ __forceinline__ int place(int j, int tid) {
@@ -282,9 +282,9 @@ struct Batch {
 };
 
 // The waves' best of a part, through its batches, whatever there is.
-template <class X>
+template <class X, int WAVES>
 __device__ void best_of_all(const X *row, int first, int end, int n, Ranking &room, Entry *cand) {
-  using B = Batch<X>;
+  using B = Batch<X, WAVES>;
   const int tid = threadIdx.x, lane = tid & 63;
   Best best;
   best.last = -Type<X>::HIGH;
@@ -325,9 +325,10 @@ __device__ void best_of_all(const X *row, int first, int end, int n, Ranking &ro
 }
 
 // A part of a row.
-template <class X, bool TOP>
-__global__ __launch_bounds__(THREADS) void k_logprobs(Call c) {
-  using B = Batch<X>;
+template <class X, bool TOP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_logprobs(Call c) {
+  using B = Batch<X, WAVES>;
+  constexpr int THREADS = B::THREADS;
   constexpr float HIGH = Type<X>::HIGH;
   __shared__ float high[WAVES], reach[WAVES];
   __shared__ double sums[WAVES][2];
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(THREADS) void k_logprobs(Call c) {
   int count = TOP ? n_cand : 0, live = count;
   if (TOP && (count > CANDIDATES || n_again > AGAIN)) {
     __syncthreads();
-    best_of_all<X>(row, first, end, c.top, room[wave], cand);
+    best_of_all<X, WAVES>(row, first, end, c.top, room[wave], cand);
     count = WAVES * c.top;
     __syncthreads();
     live = better_than(0, cand, count);
@@ -443,48 +444,71 @@ __global__ __launch_bounds__(THREADS) void k_logprobs(Call c) {
 }
 
 // The parts of a row.
+constexpr int JOIN = 256;  // threads
 template <class X>
-__global__ __launch_bounds__(THREADS) void k_join(Call c) {
+__global__ __launch_bounds__(JOIN) void k_join(Call c) {
   __shared__ Entry cand[MAX_PARTS * HY3X_LOGPROBS_MAX_TOP];
   __shared__ int n_cand;
   const int t = blockIdx.x, lane = threadIdx.x & 63;
-  const int token = c.tokens[t];
-  const float given = given_logit<X>(c, t, token);
   const bool in = lane < c.parts;
   const Stats part = c.stats[(int64_t)t * c.parts + (in ? lane : 0)];
+  // at least c.top candidates reach what `lists` of the lists' `deep` first ones reach
+  const Entry *all = c.lists + (int64_t)t * c.parts * c.top;
+  const int count = c.parts * c.top;
+  const int deep = (c.top + c.parts - 1) / c.parts, lists = c.top ? (c.top + deep - 1) / deep : 0;
+  Entry mine[MAX_PARTS * MAX_TOP / JOIN], first = 0;  // on their way together
+  if (c.top) {
+    if (in) first = all[lane * c.top + deep - 1];
+#pragma unroll
+    for (int i = 0; i < MAX_PARTS * MAX_TOP / JOIN; i++) {
+      const int at = threadIdx.x + i * JOIN;
+      mine[i] = 0;
+      if (at < count) mine[i] = all[at];
+    }
+  }
+  const int token = c.tokens[t];
+  const float given = given_logit<X>(c, t, token);
   const float m = wave_max(part.m);
   const float d = fmaxf(part.m - m, -FAR), f = in ? __expf(d) : 0.0f;
   const double S = sum_of_wave(part.S * f), E = sum_of_wave((part.E + part.S * d) * f);
   if (threadIdx.x == 0) n_cand = 0;
   __syncthreads();
   if (c.top) {
-    // at least c.top candidates reach what `lists` of the lists' `deep` first ones reach
-    const Entry *all = c.lists + (int64_t)t * c.parts * c.top;
-    const int deep = (c.top + c.parts - 1) / c.parts, lists = (c.top + deep - 1) / deep;
-    const Entry first = in ? all[lane * c.top + deep - 1] : 0;
     const int bound = reached_by(first ? value_of(first) : -INFINITY, lists);
-    for (int i = threadIdx.x; i < c.parts * c.top; i += THREADS) {
-      const Entry e = all[i];
-      if (e && order_of(value_of(e)) >= bound) cand[atomicAdd(&n_cand, 1)] = e;
-    }
+#pragma unroll
+    for (int i = 0; i < MAX_PARTS * MAX_TOP / JOIN; i++)
+      if (mine[i] && order_of(value_of(mine[i])) >= bound) cand[atomicAdd(&n_cand, 1)] = mine[i];
     __syncthreads();
   }
   finish<X>(c, t, token, given, m, S, E, cand, n_cand, n_cand);
 }
 
-// Parts of a row: enough blocks for the card, of no less than PART logits each.
+// Rows in parts: few rows over a long vocabulary, whose parts then have no less than PART
+// logits. us of whole rows (8 waves each) and of parts and their join, fp32 with 5
+// alternatives: one row of 32003 8.3 and 9.8, of 64000 11.0 and 9.9, of 120832 15.7 and
+// 9.9; 64 rows of 64000 13.1 and 14.0, of 120832 18.0 and 17.4; 100 of 120832 19.0, 19.7.
 constexpr int PART = 2048, BLOCKS = 1024;
 int parts_of(int T, int V) {
-  const int most = std::min(MAX_PARTS, (V + PART - 1) / PART);
-  return std::max(1, std::min(most, BLOCKS / std::max(T, 1)));
+  if (T < 1 || (int64_t)(90 - T) * V < 3000000) return 1;
+  return std::min({MAX_PARTS, (V + PART - 1) / PART, BLOCKS / T});
 }
+// Whole rows: 8 waves each where the rows are too few for all of the card's, and long.
+// us with 4 waves and with 8, 5 alternatives: fp32 16 rows of 16000 7.6 and 7.8, of 32003
+// 9.0 and 9.0, of 64000 13.3 and 12.1; bf16 256 of 120832 30.7 and 20.6, 333 of 32003 14.5
+// and 14.4, 511 of 50021 20.4 and 21.5, 2048 of 120832 108 and 113.
+constexpr int EIGHT_T = 384, EIGHT_V = 24576;
 
+template <class X, int WAVES>
+void launch_waves(const Call &c, hipStream_t st) {
+  const uint32_t blocks = (uint32_t)c.T * c.parts;
+  if (c.top) k_logprobs<X, true, WAVES><<<blocks, 64 * WAVES, 0, st>>>(c);
+  else k_logprobs<X, false, WAVES><<<blocks, 64 * WAVES, 0, st>>>(c);
+}
 template <class X>
 void launch(const Call &c, hipStream_t st) {
-  const uint32_t blocks = (uint32_t)c.T * c.parts;
-  if (c.top) k_logprobs<X, true><<<blocks, THREADS, 0, st>>>(c);
-  else k_logprobs<X, false><<<blocks, THREADS, 0, st>>>(c);
-  if (c.parts > 1) k_join<X><<<c.T, THREADS, 0, st>>>(c);
+  if (c.parts == 1 && c.T < EIGHT_T && c.V >= EIGHT_V) launch_waves<X, 8>(c, st);
+  else launch_waves<X, 4>(c, st);
+  if (c.parts > 1) k_join<X><<<c.T, JOIN, 0, st>>>(c);
 }
 
 }  // namespace
