@@ -302,13 +302,17 @@ def _rows(name, a, want, T, width, stride, here):
     named, dense rows."""
     if type(a) is int:
         return a, want, width if stride is None else stride
-    try:  # rows of the named type and stride, in as few calls as can be
-        if _kind_of[a.dtype] == want and a.get_device() == here:
+    try:  # rows of the named type and stride or of its own, in as few calls as can be
+        kind = _kind_of[a.dtype]
+        if (kind == want or want is None and kind in DTYPES) and a.get_device() == here:
             shape = a.shape
-            if shape[-1] == width and (
-                    stride in (None, width) and a.is_contiguous() and a.numel() >= T * width
-                    or len(shape) == 2 and shape[0] >= T and a.stride() == (stride, 1)):
-                return a.data_ptr(), want, width if stride is None else stride
+            if shape[-1] == width:
+                if stride in (None, width) and a.is_contiguous() and a.numel() >= T * width:
+                    return a.data_ptr(), kind, width if stride is None else stride
+                if len(shape) == 2 and shape[0] >= T:
+                    own, one = a.stride()
+                    if one == 1 and (own == stride or stride is None and T > 1):
+                        return a.data_ptr(), kind, own
     except (AttributeError, KeyError, IndexError):
         pass
     kind = _typed(name, a, want)
@@ -509,33 +513,35 @@ def logprobs(logits, tokens, T, logp, entropy=None, top_ids=None, top_logp=None,
     row_stride the logits' own (of a pointer, "f32" and dense rows; vocab is named then).
     workspace: a byte tensor of logprobs_workspace(T, vocab, top), or a pointer to as many."""
     here = _here()
-    if vocab is None:
-        if not hasattr(logits, "data_ptr"):
-            raise ValueError("vocab: not named, and logits is a pointer")
-        vocab = logits.shape[-1]
-    if top_ids is None or top_logp is None:
-        if top_ids is not top_logp or top:
-            raise ValueError("top_ids and top_logp belong together")
-        top = 0
-    elif top is None:
-        if not hasattr(top_ids, "data_ptr"):
-            raise ValueError("top: not named, and top_ids is a pointer")
-        top = top_ids.shape[-1]
+    try:
+        if vocab is None:
+            vocab = logits.shape[-1]
+        if top is None:
+            top = 0 if top_ids is None else top_ids.shape[-1]
+    except AttributeError:
+        raise ValueError("vocab or top: not named, and not a tensor's") from None
     logits, dtype, row_stride = _rows("logits", logits, dtype, T, vocab, row_stride, here)
     tokens = _flat("tokens", tokens, "i32", T, here)
     logp = _flat("logp", logp, "f32", T, here)
     if entropy is not None:
         entropy = _flat("entropy", entropy, "f32", T, here)
     if top:
+        if top_ids is None or top_logp is None:
+            raise ValueError("top_ids and top_logp belong together")
         top_ids = _flat("top_ids", top_ids, "i32", T * top, here)
         top_logp = _flat("top_logp", top_logp, "f32", T * top, here)
+    elif top_ids is not None or top_logp is not None:
+        raise ValueError("top_ids and top_logp hold no alternatives")
     room = 0
     if workspace is not None:
-        room = logprobs_workspace(T, vocab, top)
-        workspace = _flat("workspace", workspace, "u8", room, here)
+        if type(workspace) is int:
+            room = logprobs_workspace(T, vocab, top)
+        else:
+            room = workspace.numel()
+            workspace = _flat("workspace", workspace, "u8", room, here)
     rc = (_lib or lib()).hy3x_logprobs(logits, DTYPES[dtype or "f32"], row_stride, vocab, tokens,
-                                       T, top, logp, entropy, top_ids if top else None,
-                                       top_logp if top else None, workspace, room, stream)
+                                       T, top, logp, entropy, top_ids, top_logp, workspace, room,
+                                       stream)
     if rc:
         _check(rc)
 

@@ -302,7 +302,7 @@ def test_a_missing_workspace_is_refused(torch):
         with pytest.raises(H.HY3XError, match="workspace"):
             call()
         call.ws = torch.empty(room - 1, dtype=torch.uint8, device="cuda")
-        with pytest.raises(ValueError, match="workspace"):
+        with pytest.raises(H.HY3XError, match="workspace"):
             call()
 
 
