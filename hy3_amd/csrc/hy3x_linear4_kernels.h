@@ -71,13 +71,12 @@ __device__ __forceinline__ u4v weights(uint32_t w) {
                Op<X>::template ints<false>(hi), Op<X>::template ints<true>(hi)};
 }
 
-// Part p of v in bf16: v = p0 + p1 + p2. An infinity is its first part, the
-// others 0.
+// Part p of v in bf16: v = p0 + p1 + p2 (of an infinity the others are NaN).
 __device__ __forceinline__ float trunc16(float v) {
   return __uint_as_float(__float_as_uint(v) & 0xffff0000u);
 }
 __device__ __forceinline__ float part_of(float v, int p) {
-  const float a = trunc16(v), r = fabsf(v) == INFINITY ? 0.0f : v - a, b = trunc16(r);
+  const float a = trunc16(v), r = v - a, b = trunc16(r);
   return p == 0 ? a : p == 1 ? b : p == 2 ? r - b : 0.0f;
 }
 __device__ __forceinline__ uint32_t pair16(float lo, float hi) {  // their upper halves
@@ -334,22 +333,25 @@ __global__ __launch_bounds__((64 * few_waves<X, RING>()), (few_waves<X, RING>() 
 }
 
 // ---- many tokens --------------------------------------------------------------
-// A block takes 16 RT WN rows of W and 16 CT tokens; WK of its waves share a row's k,
-// a chunk of 128 each at a time. x goes through LDS in the operands' order, a step ahead:
-// copied there as it is (DMA: rows of whole chunks, aligned to 16 bytes), or by way of
-// registers (fp32 becomes its three parts). Weights go straight to the lanes that use
-// them, and a chunk's operands stay in registers while its token tiles pass.
+// A block takes 16 RT WN rows of W and 16 CT tokens; WK of its waves share a row's k, a
+// run of its chunks each, one a step. x goes through LDS in the operands' order, a step
+// ahead: copied there as it is (DMA: rows of whole chunks, aligned to 16 bytes), or by way
+// of registers (fp32 becomes its three parts). Weights go straight to the lanes that use
+// them, and a chunk's operands stay in registers while its token tiles pass; scales and
+// zero points come for several chunks at once, as every load costs the same address cycles.
 //
 // Operands are the integers q. What the zero points take off, s z sum x, follows a step
-// behind: the waves that share a chunk find the sums of its token tiles, a few each, on
-// the MFMAs (x times ones), and leave them in LDS for all.
+// behind: the waves that share a chunk find the sums of its token tiles on the MFMAs (x
+// times ones), each those of the tiles that it comes to first, and leave them in LDS.
 template <class X, int GP, int RT, int CT, int WN, int WK, bool DMA>
 __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c) {
   constexpr int PARTS = Op<X>::PARTS, THREADS = 64 * WN * WK;
   constexpr int PIECES = WK * CT * 256 / THREADS;  // runs of 8 elements a thread loads a step
   static_assert(PIECES * THREADS == WK * CT * 256 && !(DMA && PARTS > 1), "whole pieces");
+  static_assert(CT % WN == 0 || WN % CT == 0, "a wave's own token tiles");
   constexpr int XS = WK * PARTS * CT * 256, BUFS = DMA ? 2 : 1;
   constexpr int RED = WK > 1 ? (WK - 1) * WN * RT * CT * 64 : 1;
+  constexpr int SQ = 4 / GP;  // chunks of a quad whose scales come in one load: 4 groups
   __shared__ u4v lds[BUFS * XS > RED ? BUFS * XS : RED];
   __shared__ f4v sums[2][WK][CT][GP][4];  // of x over a chunk's groups
   const int lane = threadIdx.x & 63, col = lane & 15, h = lane >> 4;
@@ -361,7 +363,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c)
   const uint32_t xcd = blockIdx.x % 8, item = xcd * per + min(xcd, left) + blockIdx.x / 8;
   const int rt0 = (int)(item / token_tiles) * (RT * WN) + wn * RT;
   const int64_t t0 = (int64_t)(item % token_tiles) * (16 * CT);
-
+  const int steps = (c.chunks + WK - 1) / WK;  // wave wk's chunks: from steps wk on
   // piece p of a step: [wk][ct][j][lane], run j of 32 k and (lane / 16) of 8 of a token
   const X *const x0 = (const X *)c.x + t0 * c.x_stride;
   const X *from[DMA ? 1 : PIECES];
@@ -370,56 +372,49 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c)
   for (int i = 0; i < PIECES; i++) {
     const int p = threadIdx.x + i * THREADS;
     const int64_t at = min((int64_t)(p / 256 % CT) * 16 + p % 16, c.T - 1 - t0) * c.x_stride;
-    if constexpr (DMA)
-      offset[i] = (uint32_t)(2 * (at + p / (256 * CT) * 128 + p / 64 % 4 * 32 + p % 64 / 16 * 8));
+    if constexpr (DMA) offset[i] = (uint32_t)(2 * (at + p / 64 % 4 * 32 + p % 64 / 16 * 8));
     else from[i] = x0 + at;
   }
   Eight<X> ex[DMA ? 1 : PIECES];
   auto fetch = [&](int step) {
     if constexpr (DMA) {
 #pragma unroll
-      for (int i = 0; i < PIECES; i++)
-        dma16_s(x0 + (size_t)step * (WK * 128), offset[i],
+      for (int i = 0; i < PIECES; i++) {
+        // a wave's pieces are of one chunk; one beyond the last: its scales are 0
+        const int w = (64 * wave + i * THREADS) / (256 * CT);
+        dma16_s(x0 + (size_t)min(steps * w + step, c.chunks - 1) * 128, offset[i],
                 lds_addr(&lds[(step & 1) * XS + i * THREADS + 64 * wave]));
+      }
     } else {
-      const bool whole = (step + 1) * (WK * 128) <= c.d_in;
+      const bool whole = (steps * (WK - 1) + step + 1) * 128 <= c.d_in;
 #pragma unroll
       for (int i = 0; i < PIECES; i++) {
         const int p = threadIdx.x + i * THREADS;
-        const int k = (step * WK + p / (256 * CT)) * 128 + p / 64 % 4 * 32 + p % 64 / 16 * 8;
+        const int k = (steps * (p / (256 * CT)) + step) * 128 + p / 64 % 4 * 32 + p % 64 / 16 * 8;
         if (whole) ex[i].load(from[i], k);
         else ex[i].load_within(from[i], k, c.d_in);
       }
     }
   };
-  struct Weights {
-    u4v q[RT];
-    uint32_t s[RT][(GP + 1) / 2], z[RT];
-    __device__ __forceinline__ void load(const Linear4Call &c, int rt0, int chunk, int lane) {
-      const int ch = min(chunk, c.chunks - 1);
+  u4v q[RT];
+  auto load_q = [&](int step) {
+    const int ch = min(steps * wk + step, c.chunks - 1);
 #pragma unroll
-      for (int r = 0; r < RT; r++) {
-        const int rt = min(rt0 + r, c.tiles - 1);
-        q[r] = c.q[((size_t)rt * c.chunks + ch) * 64 + lane];
-        const uint32_t at = (lane & 15) * (4 * GP);
-        const uint16_t *sp = c.s + ((size_t)rt * c.quads + (ch >> 2)) * (64 * GP) + (ch & 3) * GP;
-        const uint8_t *zp = c.z + (size_t)rt * c.z_tile + (size_t)(ch >> 2) * c.z_quad + (ch & 3) * GP;
-        if constexpr (GP == 1) {
-          s[r][0] = sp[at];
-          z[r] = zp[at];
-        } else if constexpr (GP == 2) {
-          s[r][0] = *(const uint32_t *)(sp + at);
-          z[r] = *(const uint16_t *)(zp + at);
-        } else {
-          const uint2 v = *(const uint2 *)(sp + at);
-          s[r][0] = v.x;
-          s[r][1] = v.y;
-          z[r] = *(const uint32_t *)(zp + at);
-        }
-      }
+    for (int r = 0; r < RT; r++)
+      q[r] = c.q[((size_t)min(rt0 + r, c.tiles - 1) * c.chunks + ch) * 64 + lane];
+  };
+  uint64_t sr[RT];  // scales and zero points of 4 groups: SQ chunks
+  uint32_t zr[RT];
+  auto load_s = [&](int step) {
+    const int ch = min(steps * wk + step, c.chunks - 1), qd = ch >> 2;
+    const uint32_t at = (lane & 15) * (4 * GP) + ((ch & 3) / SQ) * 4;
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+      const int rt = min(rt0 + r, c.tiles - 1);
+      sr[r] = *(const uint64_t *)(c.s + ((size_t)rt * c.quads + qd) * (64 * GP) + at);
+      zr[r] = *(const uint32_t *)(c.z + ((size_t)rt * c.z_tile + (size_t)qd * c.z_quad + at));
     }
   };
-  Weights next;
   float acc[RT][CT][4], off[GP][RT];  // off: -s z of the chunk before
 #pragma unroll
   for (int r = 0; r < RT; r++) {
@@ -433,9 +428,11 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c)
   if (wn == 0)
     for (int i = lane; i < CT * GP * 4; i += 64) (&sums[1][wk][0][0][0])[i] = (f4v){0, 0, 0, 0};
 
-  const int steps = (c.chunks + WK - 1) / WK;
+  // the token tiles in each wave's own order: place t is tile (wn + t) % CT
+  const uint32_t one = Op<X>::both(1.0f);
   fetch(0);
-  next.load(c, rt0, wk, lane);
+  load_s(0);
+  load_q(0);
   for (int step = 0; step < steps; step++) {
     if constexpr (DMA) {
       wait_copies_and_barrier<0>();
@@ -445,63 +442,52 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c)
       for (int i = 0; i < PIECES; i++) {
         const int p = threadIdx.x + i * THREADS;
 #pragma unroll
-        for (int q = 0; q < PARTS; q++)
-          lds[(p / (256 * CT) * PARTS + q) * (256 * CT) + p % (256 * CT)] = ex[i].operand(q);
+        for (int part = 0; part < PARTS; part++)
+          lds[(p / (256 * CT) * PARTS + part) * (256 * CT) + p % (256 * CT)] =
+              ex[i].operand(part);
       }
       __syncthreads();
     }
     u4v b[4][RT];
     float s[GP][RT], z[GP][RT];
+    const int ch = steps * wk + step, at = GP * (ch % SQ);  // the chunk's first of 4 groups
 #pragma unroll
     for (int r = 0; r < RT; r++) {
 #pragma unroll
       for (int g = 0; g < GP; g++) {
-        s[g][r] = scale_of(next.s[r][g / 2] >> (16 * (g & 1)) & 0xffffu, c.s16);
-        z[g][r] = (float)(next.z[r] >> (8 * g) & 255);
+        const int k = at + g;
+        const float v = scale_of((uint32_t)(sr[r] >> (16 * k)) & 0xffffu, c.s16);
+        s[g][r] = ch < c.chunks ? v : 0.0f;
+        z[g][r] = (float)(zr[r] >> (8 * k) & 255);
       }
 #pragma unroll
-      for (int j = 0; j < 4; j++) b[j][r] = weights<X>(next.q[r][j]);
+      for (int j = 0; j < 4; j++) b[j][r] = weights<X>(q[r][j]);
     }
     if (step + 1 < steps) {
       fetch(step + 1);
-      next.load(c, rt0, (step + 1) * WK + wk, lane);
+      load_q(step + 1);
+      if ((ch + 1) % SQ == 0) load_s(step + 1);
     }
-    // a chunk beyond d_in meets zeros of x
     const u4v *xs = &lds[(DMA ? (step & 1) * XS : 0) + wk * (PARTS * CT * 256) + lane];
-    {  // the sums of this wave's share of the token tiles
-      const uint32_t one = Op<X>::both(1.0f);
-#pragma unroll
-      for (int o = 0; o < (CT + WN - 1) / WN; o++) {
-        const int t = wn + o * WN;
-        if (CT % WN && t >= CT) break;
-#pragma unroll
-        for (int g = 0; g < GP; g++) {
-          f4v d = {0, 0, 0, 0};
-#pragma unroll
-          for (int j = g * 4 / GP; j < (g + 1) * 4 / GP; j++)
-#pragma unroll
-            for (int q = 0; q < PARTS; q++)
-              d = Op<X>::mma(xs[(q * CT + t) * 256 + j * 64], (u4v){one, one, one, one}, d);
-          if (col == 0) sums[step & 1][wk][t][g][h] = d;
-        }
-      }
-    }
 #pragma unroll
     for (int t = 0; t < CT; t++) {
+      const int tile = (wn + t) % CT;
 #pragma unroll
       for (int g = 0; g < GP; g++) {
-        f4v d[RT];
+        const f4v before = sums[~step & 1][wk][tile][g][h];
+        f4v d[RT], sum = {0, 0, 0, 0};
 #pragma unroll
         for (int r = 0; r < RT; r++) d[r] = (f4v){0, 0, 0, 0};
 #pragma unroll
         for (int j = g * 4 / GP; j < (g + 1) * 4 / GP; j++)
 #pragma unroll
-          for (int q = 0; q < PARTS; q++) {
-            const u4v a = xs[(q * CT + t) * 256 + j * 64];
+          for (int part = 0; part < PARTS; part++) {
+            const u4v a = xs[(part * CT + tile) * 256 + j * 64];
 #pragma unroll
             for (int r = 0; r < RT; r++) d[r] = Op<X>::mma(a, b[j][r], d[r]);
+            if (t % WN == 0) sum = Op<X>::mma(a, (u4v){one, one, one, one}, sum);
           }
-        const f4v before = sums[~step & 1][wk][t][g][h];
+        if (t % WN == 0 && col == 0) sums[step & 1][wk][tile][g][h] = sum;
 #pragma unroll
         for (int r = 0; r < RT; r++)
 #pragma unroll
@@ -515,13 +501,13 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c)
     for (int g = 0; g < GP; g++)
 #pragma unroll
       for (int r = 0; r < RT; r++) off[g][r] = -s[g][r] * z[g][r];
-  }
+    }
   __syncthreads();
 #pragma unroll
   for (int t = 0; t < CT; t++)
 #pragma unroll
     for (int g = 0; g < GP; g++) {
-      const f4v before = sums[~steps & 1][wk][t][g][h];
+      const f4v before = sums[~steps & 1][wk][(wn + t) % CT][g][h];
 #pragma unroll
       for (int r = 0; r < RT; r++)
 #pragma unroll
@@ -553,7 +539,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c)
   for (int t = 0; t < CT; t++)
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const int64_t token = t0 + 16 * t + 4 * h + i;
+      const int64_t token = t0 + 16 * ((wn + t) % CT) + 4 * h + i;
       if (token >= c.T) continue;
       float v[RT];
 #pragma unroll
@@ -595,6 +581,35 @@ bool few(const Linear4Call &c, hipStream_t st) {
   return true;
 }
 
+template <class X, int GP, bool DMA>
+void by_size(const Linear4Call &c, hipStream_t st) {
+  constexpr bool SPLIT = Op<X>::PARTS == 3;
+  const int64_t size = (int64_t)((c.T + 15) / 16) * c.tiles;  // in tiles of 16 x 16 outputs
+  if (c.T <= 16) {
+    if (size <= 384) return many<X, GP, 1, 1, 1, 8, DMA>(c, st);
+    if (size <= 2048) return many<X, GP, 2, 1, 2, 4, DMA>(c, st);
+    return many<X, GP, 4, 1, 4, 1, DMA>(c, st);
+  }
+  if (size <= 1536) {
+    if (c.chunks >= 24) return many<X, GP, 4, 1, 1, 8, DMA>(c, st);
+    return many<X, GP, 2, 1, 2, 4, DMA>(c, st);
+  }
+  if (size <= 2560) return many<X, GP, 4, 1, 2, 4, DMA>(c, st);
+  if (size <= 4096) {
+    if constexpr (SPLIT) return many<X, GP, 4, 1, 4, 2, DMA>(c, st);
+    else return many<X, GP, 4, 2, 2, 2, DMA>(c, st);
+  }
+  if (size <= 12288) return many<X, GP, 2, 2, 4, 1, DMA>(c, st);
+  if constexpr (GP == 4) {  // four rows' groups of 32 do not fit the registers
+    if (SPLIT || c.T <= 32) return many<X, GP, 2, 2, 4, 1, DMA>(c, st);
+    return many<X, GP, 2, 4, 4, 1, DMA>(c, st);
+  } else {
+    if (SPLIT || c.T <= 32) return many<X, GP, 4, 2, 4, 1, DMA>(c, st);
+    if (size <= 24576 && c.T > 64) return many<X, GP, 2, 4, 4, 1, DMA>(c, st);
+    return many<X, GP, 4, 4, 4, 1, DMA>(c, st);
+  }
+}
+
 template <class X, int GP>
 void launch_group(const Linear4Call &c, hipStream_t st) {
   constexpr bool SPLIT = Op<X>::PARTS == 3;
@@ -603,17 +618,11 @@ void launch_group(const Linear4Call &c, hipStream_t st) {
   } else if (!SPLIT && c.T <= 16) {
     if (few<X, GP, SPLIT ? 1 : 4>(c, st)) return;
   }
-  if (c.T <= 16) return many<X, GP, 1, 1, 1, 8, false>(c, st);
-  if (c.T <= 32) return many<X, GP, 2, 2, 2, 2, false>(c, st);
-  const int64_t big = (int64_t)((c.T + 63) / 64) * ((c.tiles + 15) / 16);
-  if (big >= 256) {
-    if constexpr (!SPLIT)  // 32-bit offsets of 64 rows
-      if (c.d_in % 128 == 0 && (uintptr_t)c.x % 16 == 0 && c.x_stride % 8 == 0 &&
-          c.x_stride <= 1 << 24)
-        return many<X, GP, 4, 4, 4, 1, true>(c, st);
-    return many<X, GP, 4, 4, 4, 1, false>(c, st);
-  }
-  return many<X, GP, 2, 2, 2, 2, false>(c, st);
+  if constexpr (!SPLIT)  // 32-bit offsets of 64 rows
+    if (c.d_in % 128 == 0 && (uintptr_t)c.x % 16 == 0 && c.x_stride % 8 == 0 &&
+        c.x_stride <= 1 << 24)
+      return by_size<X, GP, true>(c, st);
+  by_size<X, GP, false>(c, st);
 }
 
 }  // namespace linear4
