@@ -357,12 +357,11 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c)
   const int lane = threadIdx.x & 63, col = lane & 15, h = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave / WK, wk = wave % WK;
-  // XCDs take blocks in turn: each gets a run of neighbouring tiles, token tiles first
+  // token tiles first (2048 tokens, 8192 rows of 4096: 160 us, with a run of neighbouring
+  // tiles for each XCD 165, its rows first 162)
   const uint32_t token_tiles = (c.T + 16 * CT - 1) / (16 * CT);
-  const uint32_t per = gridDim.x / 8, left = gridDim.x % 8;
-  const uint32_t xcd = blockIdx.x % 8, item = xcd * per + min(xcd, left) + blockIdx.x / 8;
-  const int rt0 = (int)(item / token_tiles) * (RT * WN) + wn * RT;
-  const int64_t t0 = (int64_t)(item % token_tiles) * (16 * CT);
+  const int rt0 = (int)(blockIdx.x / token_tiles) * (RT * WN) + wn * RT;
+  const int64_t t0 = (int64_t)(blockIdx.x % token_tiles) * (16 * CT);
   const int steps = (c.chunks + WK - 1) / WK;  // wave wk's chunks: from steps wk on
   // piece p of a step: [wk][ct][j][lane], run j of 32 k and (lane / 16) of 8 of a token
   const X *const x0 = (const X *)c.x + t0 * c.x_stride;
@@ -566,19 +565,30 @@ template <class X, int GP, int HQ, int NR, int RING>
 void few(const Linear4Call &c, int waves, int blocks, hipStream_t st) {
   k_linear4_few<X, GP, HQ, NR, RING><<<blocks, 64 * waves, 0, st>>>(c);
 }
-// Where all row tiles fit the card at once each has a block, and no ring.
+// Whether x in registers serves this call, and if so its launch. Where all row tiles fit the
+// card at once each has a block of 16 waves and no ring. Longer ones have a ring where the
+// waves are enough for the card (from 5 quads), and two quads a wave only where the registers
+// are (groups of 128).
 template <class X, int GP, int NR>
 bool few(const Linear4Call &c, hipStream_t st) {
-  constexpr int ONCE = few_waves<X, 1>(), RING = few_waves<X, 2>();
-  if (c.quads <= ONCE && (int64_t)c.tiles * c.quads <= 256 * ONCE)
-    few<X, GP, 1, NR, 1>(c, c.quads, c.tiles, st);
-  else if (c.quads <= RING)
+  constexpr int RING = few_waves<X, 2>();
+  if constexpr (Op<X>::PARTS == 1) {
+    constexpr int ONCE = few_waves<X, 1>();
+    if (c.quads <= ONCE && (int64_t)c.tiles * c.quads <= 256 * ONCE) {
+      few<X, GP, 1, NR, 1>(c, c.quads, c.tiles, st);
+      return true;
+    }
+    if constexpr (GP == 1 && NR == 1)
+      if (c.quads > RING && c.quads <= 2 * RING) {
+        few<X, GP, 2, NR, 2>(c, (c.quads + 1) / 2, std::min(c.tiles, 256), st);
+        return true;
+      }
+  }
+  if (c.quads > 4 && c.quads <= RING) {
     few<X, GP, 1, NR, 3>(c, c.quads, std::min(c.tiles, 256), st);
-  else if (c.quads <= 2 * RING)
-    few<X, GP, 2, NR, 2>(c, (c.quads + 1) / 2, std::min(c.tiles, 256), st);
-  else
-    return false;
-  return true;
+    return true;
+  }
+  return false;
 }
 
 template <class X, int GP, bool DMA>
@@ -586,9 +596,10 @@ void by_size(const Linear4Call &c, hipStream_t st) {
   constexpr bool SPLIT = Op<X>::PARTS == 3;
   const int64_t size = (int64_t)((c.T + 15) / 16) * c.tiles;  // in tiles of 16 x 16 outputs
   if (c.T <= 16) {
-    if (size <= 384) return many<X, GP, 1, 1, 1, 8, DMA>(c, st);
-    if (size <= 2048) return many<X, GP, 2, 1, 2, 4, DMA>(c, st);
-    return many<X, GP, 4, 1, 4, 1, DMA>(c, st);
+    if (size > 2048) return many<X, GP, 4, 1, 4, 1, DMA>(c, st);
+    if (c.chunks < 24) return many<X, GP, 1, 1, 2, 4, DMA>(c, st);
+    if (size > 384) return many<X, GP, 2, 1, 1, 8, DMA>(c, st);
+    return many<X, GP, 1, 1, 1, 8, DMA>(c, st);
   }
   if (size <= 1536) {
     if (c.chunks >= 24) return many<X, GP, 4, 1, 1, 8, DMA>(c, st);
@@ -613,10 +624,12 @@ void by_size(const Linear4Call &c, hipStream_t st) {
 template <class X, int GP>
 void launch_group(const Linear4Call &c, hipStream_t st) {
   constexpr bool SPLIT = Op<X>::PARTS == 3;
-  if (c.T <= 4) {
-    if (few<X, GP, 1>(c, st)) return;
-  } else if (!SPLIT && c.T <= 16) {
-    if (few<X, GP, SPLIT ? 1 : 4>(c, st)) return;
+  if (c.T <= 4 && (!SPLIT || c.tiles > 1024)) {
+    if constexpr (!SPLIT || GP < 4)  // fp32 x and groups of 32: not enough registers
+      if (few<X, GP, 1>(c, st)) return;
+  } else if (!SPLIT && c.T <= (c.tiles > 256 && c.tiles <= 1024 ? 8 : 16)) {
+    if constexpr (GP < 4)
+      if (few<X, GP, SPLIT ? 1 : 4>(c, st)) return;
   }
   if constexpr (!SPLIT)  // 32-bit offsets of 64 rows
     if (c.d_in % 128 == 0 && (uintptr_t)c.x % 16 == 0 && c.x_stride % 8 == 0 &&
