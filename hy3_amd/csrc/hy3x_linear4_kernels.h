@@ -3,7 +3,13 @@
 //
 // Products: v_mfma_f32_16x16x32_{bf16,f16}, rows = tokens, columns = 16 rows of W.
 // The integers are exact in both types, so a group's sum is the fp32 accumulator of
-// its MFMAs, and its scale is one FMA. fp32 x meets them as three bf16 parts.
+// its MFMAs, and its scale is one FMA. fp32 x meets them as three bf16 parts, which hold
+// all of its 24 bits (two would leave 2^-16 of it).
+//
+// A lane's 8 integers become an operand by 2 ANDs, a shift and 4 conversions, 12 ns a wave
+// and SIMD, about the time of one MFMA (9 ns): weights that only one tile of tokens meets
+// cost as much to unpack as to multiply, and bytes bound them (few tokens); unpacked once
+// for 4 tiles of tokens they are a quarter of that, and the MFMAs bound them (many).
 #pragma once
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -16,11 +22,8 @@
 namespace hy3x {
 namespace linear4 {
 
-typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
-typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
-typedef short s2v __attribute__((ext_vector_type(2)));
 
 // The MFMAs' operand type for x: its own two-byte type, bf16 parts of fp32.
 template <class X>
@@ -195,6 +198,10 @@ struct Groups {
 // Tokens: one tile of 16 (fp32: of 4, whose three parts are rows 4 t + p). Token t is row
 // 4 (t % 4) + t / 4, so that up to 4 tokens end in one register of the accumulator: NR of
 // its 4 are used.
+//
+// Bytes bound it where W is large: one token of bf16, 120832 rows of 4096, groups of 128: 46
+// us, 5.5 TB/s of weights; fp32 51 us. Small ones are a chain of waits (x, operands, their
+// sums, the tile, the join): 4096 rows of 4096 4.5 us.
 
 // Waves of a block, at most: the registers of a SIMD are enough for 4, or for 2 with a
 // ring or with fp32 on its way to parts.
@@ -225,7 +232,7 @@ template <class X, int GP, int HQ, int NR, int RING>
 __global__ __launch_bounds__((64 * few_waves<X, RING>()), (few_waves<X, RING>() / 4)) void k_linear4_few(
     Linear4Call c) {
   constexpr bool SPLIT = Op<X>::PARTS == 3;
-  constexpr int TT = SPLIT ? 4 : 16, OUT = SPLIT ? 1 : NR;  // sums of a lane
+  constexpr int OUT = SPLIT ? 1 : NR;  // sums of a lane
   constexpr int REGS = SPLIT ? 3 : NR, WAVES = few_waves<X, RING>();
   __shared__ float red[RING == 1 ? 1 : 2][WAVES][OUT][64];
   __shared__ f4v sums[WAVES][HQ * 4 * GP][4];  // of x over the groups: registers of 4 rows
@@ -277,7 +284,7 @@ __global__ __launch_bounds__((64 * few_waves<X, RING>()), (few_waves<X, RING>() 
       __builtin_amdgcn_sched_barrier(0);
     }
 
-  auto tile = [&](const FewWeights<HQ, GP> &w, int rt, int turn) {
+  auto tile = [&](const FewWeights<HQ, GP> &w, int turn) {
     float acc[REGS];
 #pragma unroll
     for (int r = 0; r < REGS; r++) acc[r] = 0.0f;
@@ -314,7 +321,7 @@ __global__ __launch_bounds__((64 * few_waves<X, RING>()), (few_waves<X, RING>() 
     }
   };
   if constexpr (RING == 1) {
-    tile(ring[0], blockIdx.x, 0);
+    tile(ring[0], 0);
     join(blockIdx.x, 0);
   } else {
     int turn = 0;
@@ -323,7 +330,7 @@ __global__ __launch_bounds__((64 * few_waves<X, RING>()), (few_waves<X, RING>() 
       for (int p = 0; p < RING; p++, turn++) {
         const int rt = rt0 + p * gridDim.x;
         if (p && rt >= c.tiles) return;
-        tile(ring[p], rt, turn);
+        tile(ring[p], turn);
         if (rt + RING * (int)gridDim.x < c.tiles)
           ring[p].load(c, rt + RING * gridDim.x, wave, waves, lane);
         join(rt, turn);
@@ -343,6 +350,13 @@ __global__ __launch_bounds__((64 * few_waves<X, RING>()), (few_waves<X, RING>() 
 // Operands are the integers q. What the zero points take off, s z sum x, follows a step
 // behind: the waves that share a chunk find the sums of its token tiles on the MFMAs (x
 // times ones), each those of the tiles that it comes to first, and leave them in LDS.
+//
+// 2048 tokens, 8192 rows of 4096, bf16, groups of 128: 153 us, 895 TFLOP/s (a bf16 product
+// of 8192^3 reaches 1266 on the same card). No one part bounds it: without the MFMAs 122 us,
+// without the reads of LDS 126, without the copies 131, without both of these 105 of 157 then:
+// the two waves of a SIMD do not hide all of each other's. All operands by way of LDS, as 16-bit
+// numbers that one wave unpacks for all, in three buffers: 156; products of a chunk ordered by
+// k first: 167. fp32 x is three products: 16-bit 300 tokens, 4096 rows of 1536 15 us, fp32 30.
 template <class X, int GP, int RT, int CT, int WN, int WK, bool DMA>
 __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c) {
   constexpr int PARTS = Op<X>::PARTS, THREADS = 64 * WN * WK;
@@ -500,7 +514,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c)
     for (int g = 0; g < GP; g++)
 #pragma unroll
       for (int r = 0; r < RT; r++) off[g][r] = -s[g][r] * z[g][r];
-    }
+  }
   __syncthreads();
 #pragma unroll
   for (int t = 0; t < CT; t++)
@@ -566,9 +580,12 @@ void few(const Linear4Call &c, int waves, int blocks, hipStream_t st) {
   k_linear4_few<X, GP, HQ, NR, RING><<<blocks, 64 * waves, 0, st>>>(c);
 }
 // Whether x in registers serves this call, and if so its launch. Where all row tiles fit the
-// card at once each has a block of 16 waves and no ring. Longer ones have a ring where the
-// waves are enough for the card (from 5 quads), and two quads a wave only where the registers
-// are (groups of 128).
+// card at once (16 waves on each of 256 CUs) each has a block and no ring; longer ones have
+// a ring where the waves are enough for the card (from 5 quads), and two quads a wave only
+// where the registers are (groups of 128, up to 4 tokens). us for one bf16 token, then of the
+// next kernel's best shape: 4096 rows of 4096 4.5 and 5.3 (once), 8192 of 4096 7.0 and 7.3
+// (once), 4096 of 8192 7.0 and 8.7 (once), 120832 of 4096 46.1 and 55.3 (ring); 8192 of 8192
+// 11.8 and 11.0 (two quads a wave, what it costs at its worst).
 template <class X, int GP, int NR>
 bool few(const Linear4Call &c, hipStream_t st) {
   constexpr int RING = few_waves<X, 2>();
@@ -591,18 +608,32 @@ bool few(const Linear4Call &c, hipStream_t st) {
   return false;
 }
 
+// The tile's shape by the size of the result: small tiles and a split of k where blocks are
+// few, large ones, which read and unpack less, where they are many. us, groups of 128, shapes
+// as RT CT WN WK, the chosen one and the next best (16-bit x, tokens x rows of d_in):
+//   16 x 4096 of 1536   1124  5.3, 1118  5.6    24 x 4096 of 1536   2124  6.1, 4118  7.1
+//   16 x 4096 of 4096   1118  7.8, 2118  8.8    24 x 4096 of 4096   2124 11.3, 4118 11.5
+//   16 x 8192 of 4096   2118  9.9, 1124 10.3    24 x 4096 of 8192   4118 17.4, 2124 19.5
+//   16 x 16384 of 4096  1124 12.5, 2118 14.6    100 x 4096 of 4096  4124 16.6, 2124 16.6
+//   16 x 120832 of 4096 4141 57.5, 1124 81.6    200 x 4096 of 4096  4222 23.3, 4142 24.6
+//   300 x 4096 of 4096  2241 32.2, 4222 32.1    512 x 8192 of 4096  2441 52.9, 4241 55.4
+// fp32 x:
+//   64 x 4096 of 8192   2124 31.8, 4118 32.8    100 x 4096 of 4096  4124 25.3, 2124 33.5
+//   200 x 4096 of 4096  4142 39.9, 4124 45.9    300 x 4096 of 4096  2241 64.3, 4124 67.9
+//   512 x 8192 of 4096  4241 107, 2241 127
 template <class X, int GP, bool DMA>
 void by_size(const Linear4Call &c, hipStream_t st) {
   constexpr bool SPLIT = Op<X>::PARTS == 3;
   const int64_t size = (int64_t)((c.T + 15) / 16) * c.tiles;  // in tiles of 16 x 16 outputs
   if (c.T <= 16) {
     if (size > 2048) return many<X, GP, 4, 1, 4, 1, DMA>(c, st);
-    if (c.chunks < 24) return many<X, GP, 1, 1, 2, 4, DMA>(c, st);
+    if (size > 768 || c.chunks < 24) return many<X, GP, 1, 1, 2, 4, DMA>(c, st);
     if (size > 384) return many<X, GP, 2, 1, 1, 8, DMA>(c, st);
     return many<X, GP, 1, 1, 1, 8, DMA>(c, st);
   }
   if (size <= 1536) {
-    if (c.chunks >= 24) return many<X, GP, 4, 1, 1, 8, DMA>(c, st);
+    if constexpr (!SPLIT)
+      if (c.chunks >= 48) return many<X, GP, 4, 1, 1, 8, DMA>(c, st);
     return many<X, GP, 2, 1, 2, 4, DMA>(c, st);
   }
   if (size <= 2560) return many<X, GP, 4, 1, 2, 4, DMA>(c, st);
@@ -621,16 +652,26 @@ void by_size(const Linear4Call &c, hipStream_t st) {
   }
 }
 
+// x in registers up to 4 tokens, for 16-bit x up to 16: there one wave's 4 sums a lane cost it
+// 4 times the FMAs, and it is the faster one only for few row tiles, which are all there at
+// once, and for many: 16 tokens, 4096 rows of 4096 7.0 us and 7.8, 8192 of 4096 11.2 and 9.9,
+// 16384 13.5 and 12.5, 120832 55.6 and 57.5. With groups of 32 the FMAs of 16 tokens outweigh the
+// bytes, and the registers spill (4096 of 4096 17.7 and 9.2). fp32 x has the ring alone: one
+// token, 8192 rows of 4096 12.5 and 11.5, 16384 15.9 and 19.4, 120832 51.7 and 68.3; its
+// groups of 32 do not fit the registers.
 template <class X, int GP>
 void launch_group(const Linear4Call &c, hipStream_t st) {
   constexpr bool SPLIT = Op<X>::PARTS == 3;
-  if (c.T <= 4 && (!SPLIT || c.tiles > 1024)) {
-    if constexpr (!SPLIT || GP < 4)  // fp32 x and groups of 32: not enough registers
-      if (few<X, GP, 1>(c, st)) return;
-  } else if (!SPLIT && c.T <= (c.tiles > 256 && c.tiles <= 1024 ? 8 : 16)) {
-    if constexpr (GP < 4)
-      if (few<X, GP, SPLIT ? 1 : 4>(c, st)) return;
+  if (c.T <= 4) {
+    if constexpr (!SPLIT || GP < 4)
+      if (!SPLIT || c.tiles > 768)
+        if (few<X, GP, 1>(c, st)) return;
+  } else if (c.T <= 16 && (c.tiles <= 256 || c.tiles > 1024)) {
+    if constexpr (!SPLIT && GP < 4)
+      if (few<X, GP, 4>(c, st)) return;
   }
+  // copies to LDS (2048 tokens, 8192 rows of 4096: 153 us; rows that begin at odd
+  // elements, by way of registers, 252)
   if constexpr (!SPLIT)  // 32-bit offsets of 64 rows
     if (c.d_in % 128 == 0 && (uintptr_t)c.x % 16 == 0 && c.x_stride % 8 == 0 &&
         c.x_stride <= 1 << 24)
