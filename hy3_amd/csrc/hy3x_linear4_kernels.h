@@ -39,7 +39,8 @@ struct Op<__half> {
   // 2^-9 of themselves
   template <bool HI>
   static __device__ __forceinline__ uint32_t ints(uint32_t bytes) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes, 512.0f, HI));
+    return __builtin_bit_cast(uint32_t,
+                              __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes, 512.0f, HI));
   }
   static __device__ __forceinline__ uint32_t both(float v) {  // v in both halves
     return 0x10001u * __builtin_bit_cast(uint16_t, (_Float16)v);
@@ -183,7 +184,9 @@ struct Groups {
   __device__ __forceinline__ float scale(int g, bool s16) const {
     return scale_of(s[g / 2] >> (16 * (g & 1)) & 0xffffu, s16);
   }
-  __device__ __forceinline__ float zero(int g) const { return (float)(z[g / 4] >> (8 * (g & 3)) & 255); }
+  __device__ __forceinline__ float zero(int g) const {
+    return (float)(z[g / 4] >> (8 * (g & 3)) & 255);
+  }
 };
 
 // ---- few tokens ---------------------------------------------------------------
@@ -229,8 +232,8 @@ struct FewWeights {
 };
 
 template <class X, int GP, int HQ, int NR, int RING>
-__global__ __launch_bounds__((64 * few_waves<X, RING>()), (few_waves<X, RING>() / 4)) void k_linear4_few(
-    Linear4Call c) {
+__global__ __launch_bounds__((64 * few_waves<X, RING>()),
+                             (few_waves<X, RING>() / 4)) void k_linear4_few(Linear4Call c) {
   constexpr bool SPLIT = Op<X>::PARTS == 3;
   constexpr int OUT = SPLIT ? 1 : NR;  // sums of a lane
   constexpr int REGS = SPLIT ? 3 : NR, WAVES = few_waves<X, RING>();
@@ -621,6 +624,9 @@ bool few(const Linear4Call &c, hipStream_t st) {
 //   64 x 4096 of 8192   2124 31.8, 4118 32.8    100 x 4096 of 4096  4124 25.3, 2124 33.5
 //   200 x 4096 of 4096  4142 39.9, 4124 45.9    300 x 4096 of 4096  2241 64.3, 4124 67.9
 //   512 x 8192 of 4096  4241 107, 2241 127
+// Groups of 32 and 64 hold more sums of x and scales, and shapes of 4 rows and several token
+// tiles spill: 200 x 4096 of 4096 by 32 4142 41.7, 4222 58.2; 2048 x 8192 of 4096 by 64
+// 2441 202, 4441 209.
 template <class X, int GP, bool DMA>
 void by_size(const Linear4Call &c, hipStream_t st) {
   constexpr bool SPLIT = Op<X>::PARTS == 3;
@@ -638,17 +644,17 @@ void by_size(const Linear4Call &c, hipStream_t st) {
   }
   if (size <= 2560) return many<X, GP, 4, 1, 2, 4, DMA>(c, st);
   if (size <= 4096) {
-    if constexpr (SPLIT) return many<X, GP, 4, 1, 4, 2, DMA>(c, st);
+    if constexpr (SPLIT || GP == 4) return many<X, GP, 4, 1, 4, 2, DMA>(c, st);
     else return many<X, GP, 4, 2, 2, 2, DMA>(c, st);
   }
   if (size <= 12288) return many<X, GP, 2, 2, 4, 1, DMA>(c, st);
-  if constexpr (GP == 4) {  // four rows' groups of 32 do not fit the registers
-    if (SPLIT || c.T <= 32) return many<X, GP, 2, 2, 4, 1, DMA>(c, st);
-    return many<X, GP, 2, 4, 4, 1, DMA>(c, st);
+  constexpr int RT = GP == 4 ? 2 : 4;
+  if constexpr (SPLIT) {
+    return many<X, GP, RT, 2, 4, 1, DMA>(c, st);
   } else {
-    if (SPLIT || c.T <= 32) return many<X, GP, 4, 2, 4, 1, DMA>(c, st);
+    if (c.T <= 32) return many<X, GP, RT, 2, 4, 1, DMA>(c, st);
     if (size <= 24576 && c.T > 64) return many<X, GP, 2, 4, 4, 1, DMA>(c, st);
-    return many<X, GP, 4, 4, 4, 1, DMA>(c, st);
+    return many<X, GP, GP == 1 ? 4 : 2, 4, 4, 1, DMA>(c, st);
   }
 }
 
