@@ -26,34 +26,36 @@ namespace {
 // zeros [d_out x groups] to the kernels' layout.
 __global__ __launch_bounds__(256) void k_pack_q(const uint8_t *q, int d_out, int d_in, int chunks,
                                                 int64_t n, uint32_t *out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // a dword
-  if (i >= n) return;
-  const int j = (int)(i & 3), lane = (int)(i >> 2 & 63);
-  const int64_t tile = i >> 8;
-  const int64_t row = linear4_row(tile / chunks, lane & 15);
-  const int k0 = (int)(tile % chunks) * 128 + 32 * j + 8 * (lane >> 4);
-  uint32_t w = 0;
-  if (row < d_out)
-    for (int e = 0; e < 8; e++) {
-      const int k = k0 + e;
-      if (k >= d_in) break;
-      const uint32_t v = q[row * ((d_in + 1) / 2) + k / 2] >> (4 * (k & 1)) & 15;
-      w |= v << (8 * (e & 3) + 4 * (e >> 2));
-    }
-  out[i] = w;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n;  // a dword
+       i += (int64_t)gridDim.x * 256) {
+    const int j = (int)(i & 3), lane = (int)(i >> 2 & 63);
+    const int64_t tile = i >> 8;
+    const int64_t row = linear4_row(tile / chunks, lane & 15);
+    const int k0 = (int)(tile % chunks) * 128 + 32 * j + 8 * (lane >> 4);
+    uint32_t w = 0;
+    if (row < d_out)
+      for (int e = 0; e < 8; e++) {
+        const int k = k0 + e;
+        if (k >= d_in) break;
+        const uint32_t v = q[row * ((d_in + 1) / 2) + k / 2] >> (4 * (k & 1)) & 15;
+        w |= v << (8 * (e & 3) + 4 * (e >> 2));
+      }
+    out[i] = w;
+  }
 }
 __global__ __launch_bounds__(256) void k_pack_s(const uint16_t *s, const uint8_t *z, int d_out,
                                                 int groups, int quads, int gp, int64_t n,
                                                 uint16_t *so, uint8_t *zo) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // a group
-  if (i >= n) return;
-  const int64_t tile = i / (64 * gp);
-  const int64_t row = linear4_row(tile / quads, (int)(i / (4 * gp) % 16));
-  const int64_t g = tile % quads * (4 * gp) + i % (4 * gp);
-  const bool in = row < d_out && g < groups;
-  so[i] = in ? s[row * groups + g] : 0;
-  if (z) zo[i] = in ? z[row * groups + g] : 0;
-  else if (i < 64 * gp) zo[i] = 8;  // one quad for all
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n;  // a group
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t tile = i / (64 * gp);
+    const int64_t row = linear4_row(tile / quads, (int)(i / (4 * gp) % 16));
+    const int64_t g = tile % quads * (4 * gp) + i % (4 * gp);
+    const bool in = row < d_out && g < groups;
+    so[i] = in ? s[row * groups + g] : 0;
+    if (z) zo[i] = in ? z[row * groups + g] : 0;
+    else if (i < 64 * gp) zo[i] = 8;  // one quad for all
+  }
 }
 __global__ __launch_bounds__(256) void k_check_zeros(const uint8_t *z, int64_t n, int *bad) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
@@ -166,12 +168,14 @@ int hy3x_linear4_set(hy3x_linear4 *h, const void *q, const void *scales, const v
   const int gp = 128 / h->group;
   const int64_t dwords = (int64_t)h->tiles * h->chunks * 256;
   const int64_t spots = (int64_t)h->tiles * h->quads * 64 * gp;
-  k_pack_q<<<(uint32_t)((dwords + 255) / 256), 256>>>((const uint8_t *)q, h->d_out, h->d_in,
-                                                       h->chunks, dwords, h->q);
+  const auto blocks = [](int64_t n) {
+    return (uint32_t)std::min<int64_t>((n + 255) / 256, 1 << 20);
+  };
+  k_pack_q<<<blocks(dwords), 256>>>((const uint8_t *)q, h->d_out, h->d_in, h->chunks, dwords,
+                                    h->q);
   OP_HIP_TRY(hipGetLastError());
-  k_pack_s<<<(uint32_t)((spots + 255) / 256), 256>>>((const uint16_t *)scales,
-                                                      (const uint8_t *)zeros, h->d_out, groups,
-                                                      h->quads, gp, spots, h->s, h->z);
+  k_pack_s<<<blocks(spots), 256>>>((const uint16_t *)scales, (const uint8_t *)zeros, h->d_out,
+                                   groups, h->quads, gp, spots, h->s, h->z);
   OP_HIP_TRY(hipGetLastError());
   OP_HIP_TRY(hipDeviceSynchronize());
   h->zeros = zeros != nullptr;
@@ -219,19 +223,24 @@ int hy3x_linear4_apply(const hy3x_linear4 *h, const void *x, int x_type, int64_t
   c.quads = h->quads;
   c.group = h->group;
   c.s16 = h->type == HY3X_F16;
-  c.x = x;
-  c.base = base;
-  c.y = y;
   c.x_stride = x_stride;
   c.base_stride = base_stride;
   c.y_stride = y_stride;
-  c.T = T;
   c.y_type = y_type;
   const hipStream_t st = (hipStream_t)stream;
-  if (x_type == HY3X_F32) launch_linear4<float>(c, st);
-  else if (x_type == HY3X_F16) launch_linear4<__half>(c, st);
-  else launch_linear4<__hip_bfloat16>(c, st);
-  OP_HIP_TRY(hipGetLastError());
+  // A launch has less than 2^32 threads; the smallest tiles of that many outputs, 32 tokens
+  // and 8 row tiles, have 256.
+  const int most_tokens = 32 * (((1 << 24) - 1) / ((h->tiles + 7) / 8));
+  for (int t = 0; t < T; t += c.T) {
+    c.x = (const uint8_t *)x + t * x_stride * xs;
+    c.base = base ? (const uint8_t *)base + t * base_stride * ys : nullptr;
+    c.y = (uint8_t *)y + t * y_stride * ys;
+    c.T = std::min(T - t, most_tokens);
+    if (x_type == HY3X_F32) launch_linear4<float>(c, st);
+    else if (x_type == HY3X_F16) launch_linear4<__half>(c, st);
+    else launch_linear4<__hip_bfloat16>(c, st);
+    OP_HIP_TRY(hipGetLastError());
+  }
   return HY3X_OK;
 }
 

@@ -497,6 +497,7 @@ int parts_of(int T, int V) {
 // 9.0 and 9.0, of 64000 13.3 and 12.1; bf16 256 of 120832 30.7 and 20.6, 333 of 32003 14.5
 // and 14.4, 511 of 50021 20.4 and 21.5, 2048 of 120832 108 and 113.
 constexpr int EIGHT_T = 384, EIGHT_V = 24576;
+constexpr int ROWS = 1 << 23;  // of a launch, which has less than 2^32 threads
 
 template <class X, int WAVES>
 void launch_waves(const Call &c, hipStream_t st) {
@@ -575,23 +576,30 @@ int hy3x_logprobs(const void *logits, int type, int64_t row_stride, int V, const
   c.logits = logits;
   c.stride = row_stride;
   c.V = V;
-  c.T = T;
   c.top = n_top;
   c.tokens = tokens;
   c.logp = logp;
   c.entropy = entropy;
-  c.top_logp = top_logp;
   c.top_ids = top_ids;
+  c.top_logp = top_logp;
   c.parts = parts_of(T, V);
   c.part = ((V + c.parts - 1) / c.parts + 7) & ~7;  // whole 16 bytes
   c.parts = (V + c.part - 1) / c.part;
   c.stats = (Stats *)workspace;
   c.lists = (Entry *)(c.stats + (int64_t)T * c.parts);
   const hipStream_t st = (hipStream_t)stream;
-  if (type == HY3X_F32) launch<float>(c, st);
-  else if (type == HY3X_F16) launch<__half>(c, st);
-  else launch<__hip_bfloat16>(c, st);
-  OP_HIP_TRY(hipGetLastError());
+  for (int t = 0; t < T; t += ROWS) {
+    c.T = std::min(T - t, ROWS);
+    if (type == HY3X_F32) launch<float>(c, st);
+    else if (type == HY3X_F16) launch<__half>(c, st);
+    else launch<__hip_bfloat16>(c, st);
+    OP_HIP_TRY(hipGetLastError());
+    c.logits = (const uint8_t *)c.logits + c.T * row_stride * es;
+    c.tokens += c.T;
+    c.logp += c.T;
+    if (entropy) c.entropy += c.T;
+    if (n_top) c.top_ids += (int64_t)c.T * n_top, c.top_logp += (int64_t)c.T * n_top;
+  }
   return HY3X_OK;
 }
 

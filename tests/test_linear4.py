@@ -384,3 +384,48 @@ def test_many_weights(torch):
         exact, a = definition(q, s[tail].cpu(), None, 128, x, None, torch)
         check(y[:, tail], exact, a, d_in, 128, None, torch)
     h.close()
+
+
+@pytest.mark.gpu
+def test_most_weights(torch):
+    """More weights than a launch has threads to lay them out: its first and last rows."""
+    d_out, d_in = 1 << 20, 32776
+    torch.cuda.empty_cache()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    packed = torch.randint(0, 256, (d_out, d_in // 2), generator=g, dtype=torch.uint8,
+                           device="cuda")
+    s = (0.01 * torch.rand(d_out, 257, generator=g, device="cuda")).bfloat16()
+    h = H.Linear4(d_out, d_in, group=128, dtype="bf16")
+    h.set(packed, s, on_device=True)
+    rows = torch.cat((torch.arange(50), torch.arange(d_out - 50, d_out)))
+    p = packed[rows.cuda()].cpu()
+    q = torch.stack((p & 15, p >> 4), 2).view(100, -1)
+    for T in (1, 20):
+        x = torch.randn(T, d_in, generator=g, device="cuda").bfloat16()
+        y = torch.empty(T, d_out, device="cuda")
+        h.apply(x, y, T)
+        exact, a = definition(q, s[rows.cuda()].cpu(), None, 128, x, None, torch)
+        check(y[:, rows.cuda()], exact, a, d_in, 128, None, torch)
+    h.close()
+
+
+@pytest.mark.gpu
+def test_most_outputs(torch):
+    """More outputs than a launch has threads for: a second one has the last tokens."""
+    T, d_out = 4194300, 1 << 14
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 145 << 30:
+        pytest.skip("needs 145 GB of free device memory")
+    q, s, z, packed = make(d_out, 8, 32, torch.bfloat16, True, 5, torch)
+    h = held(d_out, 8, 32, "bf16", q, s, z, packed)
+    x = torch.randn(T, 8, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    y = torch.empty(T, d_out, dtype=torch.bfloat16, device="cuda")
+    h.apply(x, y, T)
+    torch.cuda.synchronize()
+    for at in (0, T // 2, T - 40, T - 8):
+        n = slice(at, at + 8)
+        exact, a = definition(q, s, z, 32, x[n], None, torch)
+        check(y[n], exact, a, 8, 32, None, torch)
+    del y
+    torch.cuda.empty_cache()
+    h.close()

@@ -353,3 +353,23 @@ def test_projection_with_adapters(torch):
     assert (y.double().cpu() - want).abs().max() < 1e-5 * want.abs().max()
     proj.close()
     ad.close()
+
+
+@pytest.mark.gpu
+def test_most_rows(torch):
+    """More rows than a launch has threads for."""
+    T, V = 1 << 24, 3
+    g = torch.Generator(device="cuda").manual_seed(4)
+    l = torch.randn(T, V, generator=g, device="cuda")
+    tokens = torch.randint(0, V, (T,), generator=g, dtype=torch.int32, device="cuda")
+    call = Call(torch, l, tokens, 2)()
+    lp = torch.log_softmax(l.double(), 1)
+    d = (lp.exp() * (l.double().amax(1, keepdim=True) - l)).sum(1)
+    tol = (V / 256 + 8 + 2 * d) * HALF  # as in check
+    mine = lp.gather(1, tokens.long()[:, None])[:, 0]
+    assert ((call.logp - mine).abs() <= tol + 2 * HALF * mine.abs()).all()
+    order = torch.sort(-l, dim=1, stable=True).indices[:, :2]
+    assert torch.equal(call.ids.long(), order)
+    best = lp.gather(1, order)
+    assert ((call.best - best).abs() <= tol[:, None] + 2 * HALF * best.abs()).all()
+    assert (call.entropy + (lp.exp() * lp).sum(1)).abs().max() < 1e-5
