@@ -10,8 +10,8 @@
 //      128 c + 32 j + 8 (l / 16) + i of the tile's row l % 16, element i < 4 in the
 //      low half of byte i, i >= 4 in the high half of byte i - 4;
 //   s  [row tile][quad of chunks][row][4 GP] (GP groups in a chunk), 0 beyond d_in
-//      and d_out; z the same, in bytes. Without zero points one quad of 8s stands
-//      for all of them (z_tile and z_quad 0).
+//      and d_out; z the same, in bytes. Without zero points all are 8, and one quad
+//      is read for all (z_tile and z_quad 0).
 // Row i of tile 4 b + r is row 64 b + 4 i + r of W: the lane that has column i of four
 // tiles has four outputs that follow each other.
 #pragma once

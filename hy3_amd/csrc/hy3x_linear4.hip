@@ -4,6 +4,7 @@
 #include <hip/hip_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <new>
 
 #include "hy3x_error.h"
@@ -14,6 +15,7 @@ struct hy3x_linear4 {
   int device = 0, d_out = 0, d_in = 0, group = 0, type = 0;
   int tiles = 0, chunks = 0, quads = 0;  // row tiles of 16, chunks of 128 k, quads of chunks
   bool set = false, zeros = false;
+  mutable std::atomic<bool> kept{false};  // a captured call knows of no zero points
   uint32_t *q = nullptr;
   uint16_t *s = nullptr;
   uint8_t *z = nullptr;
@@ -53,8 +55,7 @@ __global__ __launch_bounds__(256) void k_pack_s(const uint16_t *s, const uint8_t
     const int64_t g = tile % quads * (4 * gp) + i % (4 * gp);
     const bool in = row < d_out && g < groups;
     so[i] = in ? s[row * groups + g] : 0;
-    if (z) zo[i] = in ? z[row * groups + g] : 0;
-    else if (i < 64 * gp) zo[i] = 8;  // one quad for all
+    zo[i] = !z ? 8 : in ? z[row * groups + g] : 0;
   }
 }
 __global__ __launch_bounds__(256) void k_check_zeros(const uint8_t *z, int64_t n, int *bad) {
@@ -130,6 +131,8 @@ int hy3x_linear4_set(hy3x_linear4 *h, const void *q, const void *scales, const v
                      int src_on_device) {
   if (!h || !q || !scales) return op_fail(HY3X_E_ARG, "NULL argument");
   if ((uintptr_t)scales % 2) return op_fail(HY3X_E_ARG, "scales is not aligned to its elements");
+  if (zeros && h->kept)
+    return op_fail(HY3X_E_STATE, "zero points for weights that a captured call has without them");
   const int rc = check_device(h);
   if (rc) return rc;
   OP_HIP_TRY(hipDeviceSynchronize());
@@ -228,6 +231,11 @@ int hy3x_linear4_apply(const hy3x_linear4 *h, const void *x, int x_type, int64_t
   c.y_stride = y_stride;
   c.y_type = y_type;
   const hipStream_t st = (hipStream_t)stream;
+  if (!h->zeros && st && !h->kept) {  // its replays will read one quad's zero points for all
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    OP_HIP_TRY(hipStreamIsCapturing(st, &status));
+    if (status == hipStreamCaptureStatusActive) h->kept = true;
+  }
   // A launch has less than 2^32 threads; the smallest tiles of that many outputs, 32 tokens
   // and 8 row tiles, have 256.
   const int most_tokens = 32 * (((1 << 24) - 1) / ((h->tiles + 7) / 8));

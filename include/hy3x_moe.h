@@ -387,7 +387,9 @@ int hy3x_linear4_destroy(hy3x_linear4 *weights);
  * handle's type; zeros, bytes of the same shape, 0 to 16 (HY3X_E_ARG above, and the
  * handle keeps what it had), or NULL: 8 everywhere. Dense, row-major (host pointers, or
  * device pointers with src_on_device != 0; copied and laid out for the kernels). Waits
- * for the device before and after the copy. */
+ * for the device before and after the copy. A captured call reads the weights that are
+ * set when it is replayed; weights that one was captured with without zero points take
+ * none later (HY3X_E_STATE). */
 int hy3x_linear4_set(hy3x_linear4 *weights, const void *q, const void *scales, const void *zeros,
                      int src_on_device);
 /* y[t] = base[t] + W x[t] for T tokens. base NULL: 0 in its place. base may be y itself

@@ -429,3 +429,86 @@ def test_most_outputs(torch):
     del y
     torch.cuda.empty_cache()
     h.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 40])
+def test_weights_set_again_after_a_capture(torch, T):
+    """A replay reads the weights set last; where that cannot be, they are refused."""
+    first = make(100, 1300, 64, torch.bfloat16, True, 5, torch)
+    other = make(100, 1300, 64, torch.bfloat16, True, 6, torch)
+    x = torch.randn(T, 1300, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    for zeros in (True, False):
+        q, s, z, packed = first
+        h = held(100, 1300, 64, "bf16", q, s, z if zeros else None, packed)
+        y = torch.empty(T, 100, device="cuda")
+        h.apply(x, y, T)
+        st, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            h.apply(x, y, T, stream=torch.cuda.current_stream().cuda_stream)
+        q, s, z, packed = other
+        for zz in ((z, None, z) if zeros else (None,)):
+            h.set(packed.cuda(), s.cuda(), None if zz is None else zz.cuda(), on_device=True)
+            for _ in range(2):
+                y.fill_(-1.0)
+                graph.replay()
+                torch.cuda.synchronize()
+                exact, a = definition(q, s, zz, 64, x, None, torch)
+                check(y, exact, a, 1300, 64, None, torch)
+        if not zeros:
+            kept = y.clone()
+            with pytest.raises(H.HY3XError, match="captured"):
+                h.set(packed.cuda(), s.cuda(), z.cuda(), on_device=True)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, kept)
+        h.close()
+
+
+# one of each path: x in registers (all tiles at once; streams of weights, with one and two
+# quads a wave), then the shapes of tiles through LDS, by tokens, inputs and outputs
+SHAPES = [(1, 7000, 4000), (4, 512, 5000), (16, 4000, 4000), (11, 8192, 900),
+          (1, 2500, 20000), (3, 4096, 20000), (16, 3900, 20000), (9, 2560, 17000),
+          (4, 8192, 9000), (2, 5000, 9000), (1, 6400, 12600),
+          (9, 1152, 33000), (16, 1152, 13000), (9, 3200, 7000), (13, 8320, 1000), (3, 8448, 70),
+          (20, 256, 5000), (20, 6272, 500), (33, 384, 12000), (50, 256, 13000),
+          (130, 256, 12000), (30, 256, 110000), (200, 256, 20000), (60, 128, 60000),
+          (500, 256, 20000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("x", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("T,d_in,d_out", SHAPES)
+def test_every_shape_is_exact(torch, T, d_in, d_out, group, x):
+    """Small integers x, scales 1/2, 1 and 2: every sum is below 2^24 halves, so that fp32
+    sums in any order are exact. Rows of whole chunks, aligned to 16 bytes, and others."""
+    kind = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[x]
+    g = torch.Generator(device="cuda").manual_seed(T + d_in)
+
+    def whole(low, high, *shape):
+        return torch.randint(low, high, shape, generator=g, device="cuda")
+    for n in {d_in // 128 * 128, d_in - 21}:
+        packed = whole(0, 256, d_out, (n + 1) // 2).to(torch.uint8)
+        groups = -(-n // group)
+        z = whole(0, 17, d_out, groups).to(torch.uint8)
+        s = (2.0 ** (whole(0, 3, d_out, groups) - 1)).bfloat16()
+        xs = whole(-8, 9, T, n + 8).to(kind)[:, :n]
+        of = torch.arange(n, device="cuda") // group
+        q = torch.stack((packed & 15, packed >> 4), 2).view(d_out, -1)[:, :n]
+        w = (q.float() - z.float()[:, of]) * s.float()[:, of]
+        want = xs.float() @ w.t()
+        h = H.Linear4(d_out, n, group=group, dtype="bf16")
+        h.set(packed, s, z, on_device=True)
+        y = torch.full((T, d_out), 5.0, device="cuda")
+        h.apply(xs, y, T)
+        assert torch.equal(y, want), (n, (y != want).nonzero()[:5].tolist())
+        if n % 128 == 0 and T > 1:  # rows at odd elements
+            h.apply(xs[1:], y, T - 1, x_stride=n + 8)
+            assert torch.equal(y[:T - 1], want[1:])
+            odd = torch.empty(T * (n + 1) + 1, dtype=kind, device="cuda")[1:].view(T, n + 1)[:, :n]
+            odd.copy_(xs)
+            y.fill_(5.0)
+            h.apply(odd, y, T)
+            assert torch.equal(y, want)
+        h.close()
