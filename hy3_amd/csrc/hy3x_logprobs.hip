@@ -18,6 +18,12 @@
 // little more than is wanted, is ranked: a candidate's place is the number of better
 // ones. Rows where too many logits reach it (equal ones) are gone through again, the
 // wave's best in its lanes.
+//
+// Bytes bound many long rows: 2048 of 120832 bf16 logits 97 us, 5.1 TB/s, as fast as a copy.
+// 11 vector instructions a logit, one of them an exponential, 14 with alternatives, bound what
+// the last caches hold: 511 rows of 50021 fp16 with 20 of them 21 us, 2.4 TB/s. Few rows are a
+// chain of waits (a lane's loads, the bound, the candidates, the join): one row of 120832 with
+// 20, 59 parts, 6.9 and 4.3 us.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
@@ -52,8 +58,11 @@ struct Type<__hip_bfloat16> {
   static constexpr uint32_t MASKED = 0xff80ff80u;
 };
 
-// e^(-FAR) is 0 in fp32: what lies further below a maximum counts as this far, so that a
-// masked logit, -inf or NaN (which max passes over), adds 0 to both sums.
+// e^(-FAR) is 0 in fp32 (its least number is e^-103): what lies further below a maximum
+// counts as this far, so that a masked logit, -inf or NaN (which max passes over), adds 0 to both sums. (Where a lane has
+// met nothing but the type's lowest value, these count as 1 each until a larger maximum takes
+// their sums to 0 with it, in fp16 at most to e^-32 of them, its least step being 32; if none
+// comes the row has nothing left, and its sums are not used.)
 constexpr float FAR = 200.0f;
 constexpr int MAX_PARTS = 64;  // of a row: a lane for each in k_join
 
@@ -156,10 +165,10 @@ __device__ __forceinline__ int reached_by(float v, int n) {
 }
 
 constexpr int MAX_TOP = HY3X_LOGPROBS_MAX_TOP;
-constexpr int CANDIDATES = 384;
-constexpr int AGAIN = 512;  // batches of a lane that are read again
-constexpr int ROUND = 4;  // logits of a lane that are ranked at once
-struct Ranking {          // a wave's, in LDS
+constexpr int CANDIDATES = 384;  // normally 1 to 3 times the tokens that are wanted
+constexpr int AGAIN = 512;       // batches of a lane that are read again
+constexpr int ROUND = 4;         // logits of a lane that are ranked at once
+struct Ranking {                 // a wave's, in LDS
   Entry all[MAX_TOP + 64 * ROUND], sorted[MAX_TOP];
 };
 
