@@ -359,7 +359,7 @@ __global__ __launch_bounds__((64 * few_waves<X, RING>()),
 // without the reads of LDS 126, without the copies 131, without both of these 105 of 157 then:
 // the two waves of a SIMD do not hide all of each other's. All operands by way of LDS, as 16-bit
 // numbers that one wave unpacks for all, in three buffers: 156; products of a chunk ordered by
-// k first: 167. fp32 x is three products: 16-bit 300 tokens, 4096 rows of 1536 15 us, fp32 30.
+// k first: 167. fp32 x is three products: 300 tokens, 4096 rows of 1536 15 us in bf16, in fp32 24.
 template <class X, int GP, int RT, int CT, int WN, int WK, bool DMA>
 __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c) {
   constexpr int PARTS = Op<X>::PARTS, THREADS = 64 * WN * WK;
@@ -622,8 +622,10 @@ bool few(const Linear4Call &c, hipStream_t st) {
 //   300 x 4096 of 4096  2241 32.2, 4222 32.1    512 x 8192 of 4096  2441 52.9, 4241 55.4
 // fp32 x:
 //   64 x 4096 of 8192   2124 31.8, 4118 32.8    100 x 4096 of 4096  4124 25.3, 2124 33.5
-//   200 x 4096 of 4096  4142 39.9, 4124 45.9    300 x 4096 of 4096  2241 64.3, 4124 67.9
+//   200 x 4096 of 4096  4142 38.2, 4124 45.9    300 x 4096 of 4096  2141 54.7, 2241 63.6
+//   512 x 4096 of 4096  2281 61.0, 2241 67.1    300 x 8192 of 4096  2241 86.3, 2141 92.6
 //   512 x 8192 of 4096  4241 107, 2241 127
+// (2281 has a block for each CU up to there)
 // Groups of 32 and 64 hold more sums of x and scales, and shapes of 4 rows and several token
 // tiles spill: 200 x 4096 of 4096 by 32 4142 41.7, 4222 58.2; 2048 x 8192 of 4096 by 64
 // 2441 202, 4441 209.
@@ -646,6 +648,10 @@ void by_size(const Linear4Call &c, hipStream_t st) {
   if (size <= 4096) {
     if constexpr (SPLIT || GP == 4) return many<X, GP, 4, 1, 4, 2, DMA>(c, st);
     else return many<X, GP, 4, 2, 2, 2, DMA>(c, st);
+  }
+  if constexpr (SPLIT) {
+    if (size <= 5120) return many<X, GP, 2, 1, 4, 1, DMA>(c, st);
+    if (size <= 8192) return many<X, GP, 2, 2, 8, 1, DMA>(c, st);
   }
   if (size <= 12288) return many<X, GP, 2, 2, 4, 1, DMA>(c, st);
   constexpr int RT = GP == 4 ? 2 : 4;
