@@ -612,26 +612,30 @@ bool few(const Linear4Call &c, hipStream_t st) {
 }
 
 // The tile's shape by the size of the result: small tiles and a split of k where blocks are
-// few, large ones, which read and unpack less, where they are many. us, groups of 128, shapes
-// as RT CT WN WK, the chosen one and the next best (16-bit x, tokens x rows of d_in):
-//   16 x 4096 of 1536   1124  5.3, 1118  5.6    24 x 4096 of 1536   2124  6.1, 4118  7.1
-//   16 x 4096 of 4096   1118  7.8, 2118  8.8    24 x 4096 of 4096   2124 11.3, 4118 11.5
+// few, large ones, which read and unpack less, where they are many; the limits of those with 8
+// waves are where each CU has a block (2124: two). us, groups of 128 (those
+// of 32 in brackets: more sums and scales a chunk, so that larger shapes spill), shapes as
+// RT CT WN WK, the chosen one and the next best; tokens x rows of d_in, 16-bit x:
+//   16 x 4096 of 1536   1124  5.3, 1118  5.6    24 x 4096 of 1536   2124  5.9, 2142  7.5
+//   16 x 4096 of 4096   1118  7.8, 2118  8.8    24 x 4096 of 4096   2124 10.5, 4118 11.5
 //   16 x 8192 of 4096   2118  9.9, 1124 10.3    24 x 4096 of 8192   4118 17.4, 2124 19.5
-//   16 x 16384 of 4096  1124 12.5, 2118 14.6    100 x 4096 of 4096  4124 16.6, 2124 16.6
-//   16 x 120832 of 4096 4141 57.5, 1124 81.6    200 x 4096 of 4096  4222 23.3, 4142 24.6
-//   300 x 4096 of 4096  2241 32.2, 4222 32.1    512 x 8192 of 4096  2441 52.9, 4241 55.4
+//   16 x 16384 of 4096  1124 12.5, 2118 14.6    64 x 8192 of 4096   2124 15.4, 2224 16.2
+//   16 x 120832 of 4096 4141 57.5, 1124 81.6    200 x 4096 of 4096  2242 20.6, 2142 22.6
+//   300 x 4096 of 1536  2241 15.1, 2442 15.9        (1242 29.5, 2242 31.9)
+//   300 x 8192 of 4096  2241 41.0, 2242 43.3    512 x 4096 of 4096  2442 29.6, 2241 31.7
+//   512 x 8192 of 4096  2441 49.5, 2281 53.5        (2442 44.3, 2241 51.0)
+//   2048 x 8192 of 4096 4441  152; by 64 2441 196, 4441 209
+// 16-bit x that goes by way of registers (larger tiles share that work):
+//   64 x 8192 of 4096   4124 25.9, 2124 32.6    400 x 4096 of 4096  2241 58.4, 2442 66.3
 // fp32 x:
 //   64 x 4096 of 8192   2124 31.8, 4118 32.8    100 x 4096 of 4096  4124 25.3, 2124 33.5
-//   200 x 4096 of 4096  4142 38.2, 4124 45.9    300 x 4096 of 4096  2141 54.7, 2241 63.6
+//   150 x 4096 of 4096  4142 38.0, 4124 46.0    300 x 4096 of 4096  2141 54.7, 2241 63.6
 //   512 x 4096 of 4096  2281 61.0, 2241 67.1    300 x 8192 of 4096  2241 86.3, 2141 92.6
-//   512 x 8192 of 4096  4241 107, 2241 127
-// (2281 has a block for each CU up to there)
-// Groups of 32 and 64 hold more sums of x and scales, and shapes of 4 rows and several token
-// tiles spill: 200 x 4096 of 4096 by 32 4142 41.7, 4222 58.2; 2048 x 8192 of 4096 by 64
-// 2441 202, 4441 209.
+//   512 x 8192 of 4096  4241  107, 2241  127   
 template <class X, int GP, bool DMA>
 void by_size(const Linear4Call &c, hipStream_t st) {
   constexpr bool SPLIT = Op<X>::PARTS == 3;
+  constexpr int RT = GP == 4 ? 2 : 4;
   const int64_t size = (int64_t)((c.T + 15) / 16) * c.tiles;  // in tiles of 16 x 16 outputs
   if (c.T <= 16) {
     if (size > 2048) return many<X, GP, 4, 1, 4, 1, DMA>(c, st);
@@ -639,25 +643,25 @@ void by_size(const Linear4Call &c, hipStream_t st) {
     if (size > 384) return many<X, GP, 2, 1, 1, 8, DMA>(c, st);
     return many<X, GP, 1, 1, 1, 8, DMA>(c, st);
   }
-  if (size <= 1536) {
-    if constexpr (!SPLIT)
-      if (c.chunks >= 48) return many<X, GP, 4, 1, 1, 8, DMA>(c, st);
-    return many<X, GP, 2, 1, 2, 4, DMA>(c, st);
-  }
-  if (size <= 2560) return many<X, GP, 4, 1, 2, 4, DMA>(c, st);
-  if (size <= 4096) {
-    if constexpr (SPLIT || GP == 4) return many<X, GP, 4, 1, 4, 2, DMA>(c, st);
-    else return many<X, GP, 4, 2, 2, 2, DMA>(c, st);
-  }
   if constexpr (SPLIT) {
+    if (size <= 1536) return many<X, GP, 2, 1, 2, 4, DMA>(c, st);
+    if (size <= 2048) return many<X, GP, 4, 1, 2, 4, DMA>(c, st);
+    if (size <= 4096) return many<X, GP, 4, 1, 4, 2, DMA>(c, st);
     if (size <= 5120) return many<X, GP, 2, 1, 4, 1, DMA>(c, st);
     if (size <= 8192) return many<X, GP, 2, 2, 8, 1, DMA>(c, st);
-  }
-  if (size <= 12288) return many<X, GP, 2, 2, 4, 1, DMA>(c, st);
-  constexpr int RT = GP == 4 ? 2 : 4;
-  if constexpr (SPLIT) {
+    if (size <= 12288) return many<X, GP, 2, 2, 4, 1, DMA>(c, st);
     return many<X, GP, RT, 2, 4, 1, DMA>(c, st);
   } else {
+    if (size <= 1536 && c.chunks >= 48) return many<X, GP, 4, 1, 1, 8, DMA>(c, st);
+    if (size <= (DMA ? 2048 : 1536)) return many<X, GP, 2, 1, 2, 4, DMA>(c, st);
+    if constexpr (DMA) {
+      if (size <= 4096) return many<X, GP, GP == 4 ? 1 : 2, 2, 4, 2, DMA>(c, st);
+      if (size <= 8192 && (GP == 4 || c.chunks >= 24)) return many<X, GP, 2, 4, 4, 2, DMA>(c, st);
+    } else {
+      if (size <= 2048) return many<X, GP, 4, 1, 2, 4, DMA>(c, st);
+      if (size <= 4096) return many<X, GP, 2, 2, 4, 2, DMA>(c, st);
+    }
+    if (size <= 12288) return many<X, GP, 2, 2, 4, 1, DMA>(c, st);
     if (c.T <= 32) return many<X, GP, RT, 2, 4, 1, DMA>(c, st);
     if (size <= 24576 && c.T > 64) return many<X, GP, 2, 4, 4, 1, DMA>(c, st);
     return many<X, GP, GP == 1 ? 4 : 2, 4, 4, 1, DMA>(c, st);

@@ -472,7 +472,8 @@ SHAPES = [(1, 7000, 4000), (4, 512, 5000), (16, 4000, 4000), (11, 8192, 900),
           (4, 8192, 9000), (2, 5000, 9000), (1, 6400, 12600),
           (9, 1152, 33000), (16, 1152, 13000), (9, 3200, 7000), (13, 8320, 1000), (3, 8448, 70),
           (20, 256, 5000), (20, 6272, 500), (33, 384, 12000), (50, 256, 13000),
-          (130, 256, 8000), (130, 256, 12000), (170, 256, 14000), (30, 256, 110000), (200, 256, 20000), (60, 128, 60000),
+          (130, 256, 8000), (130, 256, 12000), (170, 256, 14000), (40, 256, 10000),
+          (100, 3200, 7500), (300, 3200, 4000), (30, 256, 110000), (200, 256, 20000), (60, 128, 60000),
           (500, 256, 20000)]
 
 
