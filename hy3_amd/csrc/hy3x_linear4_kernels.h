@@ -613,9 +613,9 @@ bool few(const Linear4Call &c, hipStream_t st) {
 
 // The tile's shape by the size of the result: small tiles and a split of k where blocks are
 // few, large ones, which read and unpack less, where they are many; the limits of those with 8
-// waves are where each CU has a block (2124: two). us, groups of 128 (those
-// of 32 in brackets: more sums and scales a chunk, so that larger shapes spill), shapes as
-// RT CT WN WK, the chosen one and the next best; tokens x rows of d_in, 16-bit x:
+// waves are where each CU has a block (2124: two). us, groups of 128 (those of 32 in brackets:
+// more sums and scales a chunk, so that larger shapes spill), shapes as RT CT WN WK, the
+// chosen one and the next best; tokens x rows of d_in, 16-bit x:
 //   16 x 4096 of 1536   1124  5.3, 1118  5.6    24 x 4096 of 1536   2124  5.9, 2142  7.5
 //   16 x 4096 of 4096   1118  7.8, 2118  8.8    24 x 4096 of 4096   2124 10.5, 4118 11.5
 //   16 x 8192 of 4096   2118  9.9, 1124 10.3    24 x 4096 of 8192   4118 17.4, 2124 19.5
@@ -631,7 +631,7 @@ bool few(const Linear4Call &c, hipStream_t st) {
 //   64 x 4096 of 8192   2124 31.8, 4118 32.8    100 x 4096 of 4096  4124 25.3, 2124 33.5
 //   150 x 4096 of 4096  4142 38.0, 4124 46.0    300 x 4096 of 4096  2141 54.7, 2241 63.6
 //   512 x 4096 of 4096  2281 61.0, 2241 67.1    300 x 8192 of 4096  2241 86.3, 2141 92.6
-//   512 x 8192 of 4096  4241  107, 2241  127   
+//   512 x 8192 of 4096  4241  107, 2241  127
 template <class X, int GP, bool DMA>
 void by_size(const Linear4Call &c, hipStream_t st) {
   constexpr bool SPLIT = Op<X>::PARTS == 3;
