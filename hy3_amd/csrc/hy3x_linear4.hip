@@ -1,5 +1,5 @@
 // hy3x_linear4.hip -- products of 4-bit weights with group scales (hy3x_linear4_*):
-// the handle, its weights' layout and the entry points. The kernels are hy3x_linear4.h's.
+// the handle, its weights' layout and the entry points. The kernels are in hy3x_linear4_kernels.h.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
