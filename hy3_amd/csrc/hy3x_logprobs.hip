@@ -378,12 +378,15 @@ __global__ __launch_bounds__(64 * WAVES) void k_logprobs(Call c) {
     const float to = fmaxf(m, top);
     rescale(m, to, S, E);
     m = to;
+    float Sb = 0.0f, Eb = 0.0f;  // of the batch: a row's sums round once a batch
 #pragma unroll
     for (int j = 0; j < B::COUNT; j++) {
       const float x = fmaxf(v[j] - m, -FAR), e = __expf(x);
-      S += e;
-      E = fmaf(e, x, E);
+      Sb += e;
+      Eb = fmaf(e, x, Eb);
     }
+    S += Sb;
+    E += Eb;
   }
   // the block's maximum, then the sums
   const float wave_high = wave_max(m);  // every lane takes part
