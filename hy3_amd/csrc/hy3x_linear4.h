@@ -7,11 +7,13 @@
 //
 // Weights as the MFMAs read them:
 //   q  [row tile][chunk of 128 k][lane][4 dwords]: dword j of lane l holds k =
-//      128 c + 32 j + 8 (l / 16) + i of the tile's row l % 16, element i < 4 in the
-//      low half of byte i, i >= 4 in the high half of byte i - 4;
+//      128 c + 32 j + 8 (l / 16) + i of the tile's row l % 16, elements i and i + 4 in
+//      byte i, each as sign and magnitude of the odd number 2 q - 15 = +-(2 m + 1): element
+//      i < 4 has its sign in bit 7 and m in bits 3 .. 1, i >= 4 its sign in bit 0 and m in
+//      bits 6 .. 4;
 //   s  [row tile][quad of chunks][row][4 GP] (GP groups in a chunk), 0 beyond d_in
-//      and d_out; z the same, in bytes. Without zero points all are 8, and one quad
-//      is read for all (z_tile and z_quad 0).
+//      and d_out; 2 z - 15 the same, in bytes. Without zero points z is 8 everywhere, and
+//      one quad is read for all (z_tile and z_quad 0).
 // Row i of tile 4 b + r is row 64 b + 4 i + r of W: the lane that has column i of four
 // tiles has four outputs that follow each other.
 #pragma once
@@ -24,6 +26,12 @@ namespace hy3x {
 
 __host__ __device__ inline int64_t linear4_row(int64_t tile, int i) {
   return (tile >> 2) * 64 + 4 * i + (tile & 3);
+}
+
+// q as element i of its lane's dword.
+__host__ __device__ inline uint32_t linear4_code(uint32_t q, int i) {
+  const uint32_t below = q < 8, m = (below ? ~q : q) & 7;
+  return (i < 4 ? below << 7 | m << 1 : below | m << 4) << (8 * (i & 3));
 }
 
 typedef float f4v __attribute__((ext_vector_type(4)));

@@ -39,8 +39,7 @@ __global__ __launch_bounds__(256) void k_pack_q(const uint8_t *q, int d_out, int
       for (int e = 0; e < 8; e++) {
         const int k = k0 + e;
         if (k >= d_in) break;
-        const uint32_t v = q[row * ((d_in + 1) / 2) + k / 2] >> (4 * (k & 1)) & 15;
-        w |= v << (8 * (e & 3) + 4 * (e >> 2));
+        w |= linear4_code(q[row * ((d_in + 1) / 2) + k / 2] >> (4 * (k & 1)) & 15, e);
       }
     out[i] = w;
   }
@@ -55,7 +54,7 @@ __global__ __launch_bounds__(256) void k_pack_s(const uint16_t *s, const uint8_t
     const int64_t g = tile % quads * (4 * gp) + i % (4 * gp);
     const bool in = row < d_out && g < groups;
     so[i] = in ? s[row * groups + g] : 0;
-    zo[i] = !z ? 8 : in ? z[row * groups + g] : 0;
+    zo[i] = 2 * (!z ? 8 : in ? z[row * groups + g] : 0) - 15;
   }
 }
 __global__ __launch_bounds__(256) void k_check_zeros(const uint8_t *z, int64_t n, int *bad) {

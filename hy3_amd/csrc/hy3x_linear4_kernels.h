@@ -2,13 +2,18 @@
 // mathematics and the weights' layout: hy3x_linear4.h).
 //
 // Products: v_mfma_f32_16x16x32_{bf16,f16}, rows = tokens, columns = 16 rows of W.
-// The integers are exact in both types, so a group's sum is the fp32 accumulator of
+// Operands are q - 7.5, exact in both types, so a group's sum is the fp32 accumulator of
 // its MFMAs, and its scale is one FMA. fp32 x meets them as three bf16 parts, which hold
-// all of its 24 bits (two would leave 2^-16 of it).
+// all of its 24 bits (two would leave 2^-16 of it). q itself would take 7 instructions a lane's
+// 8 weights in place of 9, and 2048 tokens, 8192 rows of 4096 154 us in place of 159, but
+// sums over x of one sign then come to many times the output before the zero points take
+// that off again: relative errors of fp32 outputs, 64 tokens of |N(0, 1)|, 4096 rows of 4096,
+// 9e-7 (bf16 x) and 4.1e-6 (fp32 x), centred 1.0e-7 and 3.0e-7 (a plain fp32 product 2.1e-7
+// and 5.2e-7).
 //
-// A lane's 8 integers become an operand by 2 ANDs, a shift and 4 conversions, 12 ns a wave
-// and SIMD, about the time of one MFMA (9 ns): weights that only one tile of tokens meets
-// cost as much to unpack as to multiply, and bytes bound them (few tokens); unpacked once
+// A lane's 8 weights become an operand by 2 shifts, 3 bit selections and 4 conversions, 15 ns a
+// wave and SIMD, more than the time of one MFMA (9 ns): weights that only one tile of tokens meets
+// cost more to unpack than to multiply, and bytes bound them (few tokens); unpacked once
 // for 4 tiles of tokens they are a quarter of that, and the MFMAs bound them (many).
 #pragma once
 #include <hip/hip_bf16.h>
@@ -35,12 +40,12 @@ struct Op<__half> {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a),
                                                   __builtin_bit_cast(h8v, b), c, 0, 0, 0);
   }
-  // two bytes below 16 (the low or the high ones) as numbers: as e4m3 they stand for
-  // 2^-9 of themselves
+  // two bytes (the low or the high ones), sign and magnitude below 16, as half of these
+  // numbers: as e4m3 they stand for 2^-9 of them
   template <bool HI>
   static __device__ __forceinline__ uint32_t ints(uint32_t bytes) {
     return __builtin_bit_cast(uint32_t,
-                              __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes, 512.0f, HI));
+                              __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes, 256.0f, HI));
   }
   static __device__ __forceinline__ uint32_t both(float v) {  // v in both halves
     return 0x10001u * __builtin_bit_cast(uint16_t, (_Float16)v);
@@ -56,7 +61,7 @@ struct Op<__hip_bfloat16> {
   template <bool HI>
   static __device__ __forceinline__ uint32_t ints(uint32_t bytes) {
     return __builtin_bit_cast(uint32_t,
-                              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(bytes, 512.0f, HI));
+                              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(bytes, 256.0f, HI));
   }
   static __device__ __forceinline__ uint32_t both(float v) {  // exact: at most 8 bits
     return (__float_as_uint(v) >> 16) * 0x10001u;
@@ -67,10 +72,13 @@ struct Op<float> : Op<__hip_bfloat16> {
   static constexpr int PARTS = 3;
 };
 
-// 8 weights q of a lane as an operand, in the order of k.
+// 8 weights of a lane as an operand, q - 7.5 in the order of k.
 template <class X>
 __device__ __forceinline__ u4v weights(uint32_t w) {
-  const uint32_t lo = w & 0x0f0f0f0fu, hi = w >> 4 & 0x0f0f0f0fu;
+  // a & b | c, then twice a & b | c & ~b: one instruction each
+  const uint32_t lo = __builtin_amdgcn_bitop3_b32(w, 0x8e8e8e8eu, 0x01010101u, 0xea);
+  const uint32_t m = __builtin_amdgcn_bitop3_b32(w >> 3, 0x0e0e0e0eu, lo, 0xe2);
+  const uint32_t hi = __builtin_amdgcn_bitop3_b32(w << 7, 0x80808080u, m, 0xe2);
   return (u4v){Op<X>::template ints<false>(lo), Op<X>::template ints<true>(lo),
                Op<X>::template ints<false>(hi), Op<X>::template ints<true>(hi)};
 }
@@ -171,7 +179,7 @@ __device__ __forceinline__ void put_run(const Linear4Call &c, int64_t token, int
   __builtin_memcpy((Y *)c.y + token * c.y_stride + n, e, sizeof(e));
 }
 
-// A quad's scales and zero points of one row: 4 GP of each.
+// A quad's scales and zero points (as 2 z - 15) of one row: 4 GP of each.
 template <int GP>
 struct Groups {
   uint32_t s[2 * GP], z[GP];
@@ -184,8 +192,8 @@ struct Groups {
   __device__ __forceinline__ float scale(int g, bool s16) const {
     return scale_of(s[g / 2] >> (16 * (g & 1)) & 0xffffu, s16);
   }
-  __device__ __forceinline__ float zero(int g) const {
-    return (float)(z[g / 4] >> (8 * (g & 3)) & 255);
+  __device__ __forceinline__ float zero(int g) const {  // 2 z - 15
+    return (float)(int8_t)(z[g / 4] >> (8 * (g & 3)));
   }
 };
 
@@ -194,9 +202,8 @@ struct Groups {
 // operands for as long as the block lasts, and the weights stream past, a row tile at
 // a time, RING of them in flight. The waves' sums meet in LDS.
 //
-// Operands are the integers q; what the zero points take off, z sum x, is formed from
-// sums of x over the groups, which the MFMAs find (times a matrix of ones) while the
-// first weights are on their way.
+// What the zero points take off, (z - 7.5) sum x, is formed from sums of x / 2 over the groups,
+// which the MFMAs find (times a matrix of halves) while the first weights are on their way.
 //
 // Tokens: one tile of 16 (fp32: of 4, whose three parts are rows 4 t + p). Token t is row
 // 4 (t % 4) + t / 4, so that up to 4 tokens end in one register of the accumulator: NR of
@@ -235,10 +242,9 @@ template <class X, int GP, int HQ, int NR, int RING>
 __global__ __launch_bounds__((64 * few_waves<X, RING>()),
                              (few_waves<X, RING>() / 4)) void k_linear4_few(Linear4Call c) {
   constexpr bool SPLIT = Op<X>::PARTS == 3;
-  constexpr int OUT = SPLIT ? 1 : NR;  // sums of a lane
-  constexpr int REGS = SPLIT ? 3 : NR, WAVES = few_waves<X, RING>();
+  constexpr int OUT = SPLIT ? 1 : NR, WAVES = few_waves<X, RING>();  // OUT: sums of a lane
   __shared__ float red[RING == 1 ? 1 : 2][WAVES][OUT][64];
-  __shared__ f4v sums[WAVES][HQ * 4 * GP][4];  // of x over the groups: registers of 4 rows
+  __shared__ alignas(16) float sums[WAVES][HQ * 4 * GP][4][SPLIT ? 1 : 4];  // of x / 2
   const int lane = threadIdx.x & 63, col = lane & 15, h = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
 
@@ -274,7 +280,7 @@ __global__ __launch_bounds__((64 * few_waves<X, RING>()),
   for (int p = 1; p < RING; p++)
     if (blockIdx.x + p * gridDim.x < (uint32_t)c.tiles)
       ring[p].load(c, blockIdx.x + p * gridDim.x, wave, waves, lane);
-  const uint32_t one = Op<X>::both(1.0f);
+  const uint32_t half = Op<X>::both(0.5f);
 #pragma unroll
   for (int i = 0; i < HQ; i++)
 #pragma unroll
@@ -282,15 +288,18 @@ __global__ __launch_bounds__((64 * few_waves<X, RING>()),
       f4v d = {0, 0, 0, 0};
 #pragma unroll
       for (int j = g * 4 / GP; j < (g + 1) * 4 / GP; j++)
-        d = Op<X>::mma(a[i][j / 4][j % 4], (u4v){one, one, one, one}, d);
-      if (col == 0) sums[wave][i * 4 * GP + g][h] = d;
+        d = Op<X>::mma(a[i][j / 4][j % 4], (u4v){half, half, half, half}, d);
+      if (col == 0) {
+        if constexpr (SPLIT) sums[wave][i * 4 * GP + g][h][0] = d[0] + (d[1] + d[2]);
+        else *(f4v *)sums[wave][i * 4 * GP + g][h] = d;
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
 
   auto tile = [&](const FewWeights<HQ, GP> &w, int turn) {
-    float acc[REGS];
+    float acc[OUT];
 #pragma unroll
-    for (int r = 0; r < REGS; r++) acc[r] = 0.0f;
+    for (int r = 0; r < OUT; r++) acc[r] = 0.0f;
     asm volatile("" ::: "memory");  // the sums stay in LDS from tile to tile
 #pragma unroll
     for (int i = 0; i < HQ; i++)
@@ -301,14 +310,15 @@ __global__ __launch_bounds__((64 * few_waves<X, RING>()),
         for (int j = g * 4 / GP; j < (g + 1) * 4 / GP; j++)  // 32 k of the quad's 512
           d = Op<X>::mma(a[i][j / 4][j % 4], weights<X>(w.q[i][j / 4][j % 4]), d);
         const float s = w.g[i].scale(g, c.s16), z = w.g[i].zero(g);
-        const float *x = (const float *)&sums[wave][i * 4 * GP + g][h];
+        if (SPLIT) d[0] += d[1] + d[2];
 #pragma unroll
-        for (int r = 0; r < REGS; r++) acc[r] = fmaf(s, fmaf(-z, x[r], d[r]), acc[r]);
+        for (int r = 0; r < OUT; r++)
+          acc[r] = fmaf(s, fmaf(-z, sums[wave][i * 4 * GP + g][h][r], d[r]), acc[r]);
         if (g % GP == GP - 1) __builtin_amdgcn_sched_barrier(0);  // registers of one chunk
       }
 #pragma unroll
     for (int r = 0; r < OUT; r++)
-      red[turn & 1][wave][r][lane] = SPLIT ? acc[0] + (acc[REGS / 2] + acc[REGS - 1]) : acc[r];
+      red[turn & 1][wave][r][lane] = acc[r];
   };
   auto join = [&](int rt, int turn) {
     __syncthreads();
@@ -350,9 +360,9 @@ __global__ __launch_bounds__((64 * few_waves<X, RING>()),
 // them, and a chunk's operands stay in registers while its token tiles pass; scales and
 // zero points come for several chunks at once, as every load costs the same address cycles.
 //
-// Operands are the integers q. What the zero points take off, s z sum x, follows a step
-// behind: the waves that share a chunk find the sums of its token tiles on the MFMAs (x
-// times ones), each those of the tiles that it comes to first, and leave them in LDS.
+// What the zero points take off, s (z - 7.5) sum x, follows a step behind: the waves that share
+// a chunk find the sums of its token tiles on the MFMAs (x times halves), each those of the
+// tiles that it comes to first, and leave them in LDS.
 //
 // 2048 tokens, 8192 rows of 4096, bf16, groups of 128: 153 us, 895 TFLOP/s (a bf16 product
 // of 8192^3 reaches 1266 on the same card). No one part bounds it: without the MFMAs 122 us,
@@ -370,7 +380,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c)
   constexpr int RED = WK > 1 ? (WK - 1) * WN * RT * CT * 64 : 1;
   constexpr int SQ = 4 / GP;  // chunks of a quad whose scales come in one load: 4 groups
   __shared__ u4v lds[BUFS * XS > RED ? BUFS * XS : RED];
-  __shared__ f4v sums[2][WK][CT][GP][4];  // of x over a chunk's groups
+  __shared__ f4v sums[2][WK][CT][GP][4];  // of x / 2 over a chunk's groups
   const int lane = threadIdx.x & 63, col = lane & 15, h = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave / WK, wk = wave % WK;
@@ -431,7 +441,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c)
       zr[r] = *(const uint32_t *)(c.z + ((size_t)rt * c.z_tile + (size_t)qd * c.z_quad + at));
     }
   };
-  float acc[RT][CT][4], off[GP][RT];  // off: -s z of the chunk before
+  float acc[RT][CT][4], off[GP][RT];  // off: -s (2 z - 15) of the chunk before
 #pragma unroll
   for (int r = 0; r < RT; r++) {
 #pragma unroll
@@ -445,7 +455,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c)
     for (int i = lane; i < CT * GP * 4; i += 64) (&sums[1][wk][0][0][0])[i] = (f4v){0, 0, 0, 0};
 
   // the token tiles in each wave's own order: place t is tile (wn + t) % CT
-  const uint32_t one = Op<X>::both(1.0f);
+  const uint32_t half = Op<X>::both(0.5f);
   fetch(0);
   load_s(0);
   load_q(0);
@@ -474,7 +484,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c)
         const int k = at + g;
         const float v = scale_of((uint32_t)(sr[r] >> (16 * k)) & 0xffffu, c.s16);
         s[g][r] = ch < c.chunks ? v : 0.0f;
-        z[g][r] = (float)(zr[r] >> (8 * k) & 255);
+        z[g][r] = (float)(int8_t)(zr[r] >> (8 * k));
       }
 #pragma unroll
       for (int j = 0; j < 4; j++) b[j][r] = weights<X>(q[r][j]);
@@ -501,7 +511,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c)
             const u4v a = xs[(part * CT + tile) * 256 + j * 64];
 #pragma unroll
             for (int r = 0; r < RT; r++) d[r] = Op<X>::mma(a, b[j][r], d[r]);
-            if (t % WN == 0) sum = Op<X>::mma(a, (u4v){one, one, one, one}, sum);
+            if (t % WN == 0) sum = Op<X>::mma(a, (u4v){half, half, half, half}, sum);
           }
         if (t % WN == 0 && col == 0) sums[step & 1][wk][tile][g][h] = sum;
 #pragma unroll

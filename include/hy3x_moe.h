@@ -396,15 +396,15 @@ int hy3x_linear4_set(hy3x_linear4 *weights, const void *q, const void *scales, c
  * (same pointer and stride: added in place); otherwise y may overlap neither x nor base
  * (rows of one wider buffer may lie between each other). x: device [T x d_in], base, y:
  * device [T x d_out], x_type and y_type each HY3X_F32, HY3X_F16 or HY3X_BF16; strides in
- * elements, from the row length to 2^32. x and the integers q and zero meet exactly, in
- * fp32 sums, which the scales multiply group by group; y is rounded once. Tokens do not
+ * elements, from the row length to 2^32. x meets q - 7.5 and zero - 7.5 exactly, in fp32
+ * sums, which the scales multiply group by group; y is rounded once. Tokens do not
  * affect each other's results. An x that is infinite or NaN makes its token's outputs
- * infinite or NaN (as the formula does), but which of the two is not specified: q x and
- * zero x may meet as sums, and inf - inf is NaN where the formula has inf. The same
- * holds for sums of 16 |x| beyond fp32's range. T = 0 does nothing. The handle's device
- * must be current. No allocation, no scratch: calls on one handle may overlap, and a
- * call may be captured into a graph. HY3X_E_STATE before hy3x_linear4_set. stream: a
- * hipStream_t of the handle's device (NULL = default stream). Asynchronous. */
+ * infinite or NaN (as the formula does), but which of the two is not specified: the two
+ * products meet as sums, and inf - inf is NaN where the formula has inf. The same holds
+ * for sums of 16 |x|, and for scales times 17, beyond fp32's range. T = 0 does nothing.
+ * The handle's device must be current. No allocation, no scratch: calls on one handle may
+ * overlap, and a call may be captured into a graph. HY3X_E_STATE before hy3x_linear4_set.
+ * stream: a hipStream_t of the handle's device (NULL = default stream). Asynchronous. */
 int hy3x_linear4_apply(const hy3x_linear4 *weights, const void *x, int x_type, int64_t x_stride,
                        const void *base, int64_t base_stride, void *y, int y_type,
                        int64_t y_stride, int T, void *stream);
