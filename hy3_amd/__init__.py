@@ -496,7 +496,7 @@ class Linear4:
 
 
 def logprobs_workspace(T, vocab, top=0):
-    """Bytes of workspace that logprobs needs for T rows of `vocab` logits and `top`
+    """Bytes of workspace that logprobs needs for up to T rows of `vocab` logits and `top`
     alternatives; 0: none (hy3x_logprobs_workspace)."""
     n = lib().hy3x_logprobs_workspace(T, vocab, top)
     if n < 0:
@@ -511,7 +511,8 @@ def logprobs(logits, tokens, T, logp, entropy=None, top_ids=None, top_logp=None,
     device memory (hy3x_logprobs): tensors, whose types, places and sizes are checked, or
     pointers. Without them: vocab and top are those of the tensors' last axes, dtype and
     row_stride the logits' own (of a pointer, "f32" and dense rows; vocab is named then).
-    workspace: a byte tensor of logprobs_workspace(T, vocab, top), or a pointer to as many."""
+    workspace: a byte tensor of logprobs_workspace(T, vocab, top), of this T or a larger one,
+    or a pointer to as many."""
     here = _here()
     try:
         if vocab is None:

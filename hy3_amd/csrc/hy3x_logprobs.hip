@@ -504,6 +504,11 @@ int parts_of(int T, int V) {
   if (T < 1 || (int64_t)(90 - T) * V < 3000000) return 1;
   return std::min({MAX_PARTS, (V + PART - 1) / PART, BLOCKS / T});
 }
+// Bytes of workspace of a call.
+int64_t room_of(int T, int V, int n_top) {
+  const int64_t parts = parts_of(T, V);
+  return parts == 1 ? 0 : T * parts * (int64_t)(sizeof(Stats) + n_top * sizeof(Entry));
+}
 // Whole rows: 8 waves each where the rows are too few for all of the card's, and long.
 // us with 4 waves and with 8, 5 alternatives: fp32 16 rows of 16000 7.6 and 7.8, of 32003
 // 9.0 and 9.0, of 64000 13.3 and 12.1; bf16 256 of 120832 30.7 and 20.6, 333 of 32003 14.5
@@ -535,8 +540,9 @@ int64_t hy3x_logprobs_workspace(int T, int V, int n_top) {
   if (T < 0 || T > HY3X_LOGPROBS_MAX_TOKENS || V < 1 || V > HY3X_LOGPROBS_MAX_VOCAB ||
       n_top < 0 || n_top > HY3X_LOGPROBS_MAX_TOP || n_top > V)
     return op_fail(HY3X_E_ARG, "T=%d, V=%d or n_top=%d out of range", T, V, n_top);
-  const int64_t parts = parts_of(T, V);
-  return parts == 1 ? 0 : T * parts * (int64_t)(sizeof(Stats) + n_top * sizeof(Entry));
+  int64_t room = 0;  // fewer rows may have more parts
+  for (int t = 1; t <= std::min(T, BLOCKS); t++) room = std::max(room, room_of(t, V, n_top));
+  return room;
 }
 
 int hy3x_logprobs(const void *logits, int type, int64_t row_stride, int V, const int32_t *tokens,
@@ -558,7 +564,7 @@ int hy3x_logprobs(const void *logits, int type, int64_t row_stride, int V, const
   if (!logits || !tokens || !logp) return op_fail(HY3X_E_ARG, "NULL logits, tokens or logp");
   if (n_top && (!top_ids || !top_logp))
     return op_fail(HY3X_E_ARG, "n_top=%d without top_ids and top_logp", n_top);
-  const int64_t room = hy3x_logprobs_workspace(T, V, n_top);
+  const int64_t room = room_of(T, V, n_top);
   if (room && (!workspace || workspace_bytes < room))
     return op_fail(HY3X_E_ARG, "a workspace of %lld bytes is needed", (long long)room);
   const int64_t es = type == HY3X_F32 ? 4 : 2;

@@ -416,8 +416,9 @@ int hy3x_linear4_apply(const hy3x_linear4 *weights, const void *x, int x_type, i
 #define HY3X_LOGPROBS_MAX_TOP 32
 #define HY3X_LOGPROBS_MAX_TOKENS (1 << 24)
 
-/* Bytes of workspace that hy3x_logprobs needs for T rows of V logits and n_top
- * alternatives (0 where it needs none), or a negative HY3X_E* code. */
+/* Bytes of workspace that hy3x_logprobs may need for up to T rows of V logits and n_top
+ * alternatives (0 where it needs none), or a negative HY3X_E* code. Of two row counts the
+ * larger has no smaller value: a workspace for the largest batch serves every batch. */
 int64_t hy3x_logprobs_workspace(int T, int V, int n_top);
 /* With p = softmax of a row of V logits:
  *   logp[t]     = log p[tokens[t]]; 0 where tokens[t] is outside [0, V) (a row of padding);
@@ -432,7 +433,8 @@ int64_t hy3x_logprobs_workspace(int T, int V, int n_top);
  * logits: device [T rows of V elements], `type` HY3X_F32 / F16 / BF16, rows row_stride
  * elements apart (V .. 2^32); tokens: device int32[T]; outputs: device, dense, overlapping
  * nothing else (logits are a range from their first to their last element). workspace:
- * device memory of at least hy3x_logprobs_workspace bytes, aligned to 16, for this call
+ * device memory of hy3x_logprobs_workspace bytes (of T, or of any larger number of rows; less
+ * than this call needs is refused, and a call may need less), aligned to 16, for this call
  * alone until it has run (calls in order on one stream may share one, and so may the
  * replays of a captured one; calls that may overlap need one each); its contents are of
  * no account before and after. NULL where 0 bytes are needed. T = 0 does nothing. No
