@@ -1,11 +1,15 @@
 // hy3x_logprobs.hip -- log-probabilities of given tokens, entropy and the most
 // probable tokens of rows of logits (hy3x_logprobs):
 //
-//   m = max l,  S = sum_v e^(l_v - m),  E = sum_v (l_v - m) e^(l_v - m)
+//   m = max l,  S = 1 + R = sum_v e^(l_v - m),  E = sum_v (l_v - m) e^(l_v - m)
 //   log p_v = (l_v - m) - log S,   H = log S - E / S
 //
-// Both terms of H are at least 0, so it keeps its precision where one token has
-// nearly all of the mass.
+// Both terms of H are at least 0, so where one token has nearly all of the mass it keeps the
+// precision of R, of what the others have. fp32 sums that hold the 1 would lose R below 2^-24
+// (and keep three digits of it at 2^-14): where R is below PEAK, the logits of the lane that
+// has the largest one are summed again without it, by all threads (2048 rows of 120832 bf16
+// logits, a few in a hundred of them such rows, 102 us with it and without; 511 of 50021 22.6
+// and 22.5; by one wave alone 104 and 23.4).
 //
 // One pass: a lane keeps the maximum of the logits it has met and the two sums relative
 // to it (a larger maximum scales them down), in fp32; lanes, waves and the parts of a row
@@ -64,10 +68,11 @@ struct Type<__hip_bfloat16> {
 // their sums to 0 with it, in fp16 at most to e^-32 of them, its least step being 32; if none
 // comes the row has nothing left, and its sums are not used.)
 constexpr float FAR = 200.0f;
-constexpr int MAX_PARTS = 64;  // of a row: a lane for each in k_join
+constexpr double PEAK = 0.0625;  // from there on R has lost at most 4 bits of a lane's sum
+constexpr int MAX_PARTS = 64;    // of a row: a lane for each in k_join
 
 struct Stats {  // of a part of a row; m: the type's lowest value where all is masked
-  double S, E;
+  double R, E;
   float m, unused;
 };
 // A logit and its index as one number: the better one is the larger one. 0: none.
@@ -204,17 +209,17 @@ __device__ __forceinline__ void rescale(float m, float top, float &S, float &E) 
 // The row's results from its statistics and its candidates, which stand in LDS (some may
 // be none). Every thread of the block calls it.
 template <class X>
-__device__ void finish(const Call &c, int t, int token, float given, float m, double S, double E,
+__device__ void finish(const Call &c, int t, int token, float given, float m, double R, double E,
                        const Entry *cand, int n_cand, int live) {
   const X *row = (const X *)c.logits + t * c.stride;
   const bool some = m > -Type<X>::HIGH;
-  const double lse = some ? log(S) : 0.0;
+  const double lse = !some ? 0.0 : R < PEAK ? log1p(R) : log(1.0 + R);
   auto logp = [&](float l) {
     return l > -Type<X>::HIGH ? (float)(((double)fminf(l, Type<X>::HIGH) - m) - lse) : -INFINITY;
   };
   if (threadIdx.x == 0) {
     c.logp[t] = token >= 0 && token < c.V ? logp(given) : 0.0f;
-    if (c.entropy) c.entropy[t] = some ? (float)(lse - E / S) : 0.0f;
+    if (c.entropy) c.entropy[t] = some ? (float)(lse - E / (1.0 + R)) : 0.0f;
   }
   if (!c.top) return;
   for (int i = threadIdx.x; i < n_cand; i += blockDim.x) {
@@ -333,6 +338,22 @@ __device__ void best_of_all(const X *row, int first, int end, int n, Ranking &ro
   if (lane < n) cand[tid / 64 * n + lane] = best.e;
 }
 
+// This thread's share of the sum over thread `of`'s logits of a part, relative to the largest
+// one, `top`, and without it.
+template <class X, int WAVES>
+__device__ __forceinline__ float others(const X *row, int first, int end, float top, int of) {
+  using B = Batch<X, WAVES>;
+  const int items = (end - first + B::SIZE - 1) / B::SIZE * B::COUNT;
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < items; i += B::THREADS) {
+    const int id = first + i / B::COUNT * B::SIZE + B::place(i % B::COUNT, of);
+    const float v = id < end ? elem(row[id]) : -INFINITY;
+    sum += v < top && v > -Type<X>::HIGH ? __expf(fmaxf(v - top, -FAR)) : 0.0f;
+  }
+  return sum;
+}
+
 // A part of a row.
 template <class X, bool TOP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_logprobs(Call c) {
@@ -344,7 +365,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_logprobs(Call c) {
   __shared__ Entry cand[TOP ? CANDIDATES : 1];
   __shared__ Ranking room[TOP ? WAVES : 1];
   __shared__ int again[TOP ? AGAIN : 1];  // batch of the part and thread
-  __shared__ int n_cand, n_again;
+  __shared__ int n_cand, n_again, peak;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int t = blockIdx.x / c.parts, p = blockIdx.x % c.parts;
   const int first = p * c.part, end = min(c.V, first + c.part);
@@ -428,9 +449,21 @@ __global__ __launch_bounds__(64 * WAVES) void k_logprobs(Call c) {
     }
   }
   __syncthreads();
-  double Sd = 0.0, Ed = 0.0;
+  double Rd = -1.0, Ed = 0.0;
 #pragma unroll
-  for (int w = 0; w < WAVES; w++) Sd += sums[w][0], Ed += sums[w][1];
+  for (int w = 0; w < WAVES; w++) Rd += sums[w][0], Ed += sums[w][1];
+  if (Rd < PEAK && top > -HIGH) {  // only one logit is the largest
+    if (m == top) peak = tid;
+    __syncthreads();
+    const double rest = (double)others<X, WAVES>(row, first, end, top, peak) +
+                        (tid == peak ? 0.0 : (double)S);
+    const double Rw = sum_of_wave(rest);
+    if (lane == 0) sums[wave][0] = Rw;
+    __syncthreads();
+    Rd = 0.0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) Rd += sums[w][0];
+  }
   int count = TOP ? n_cand : 0, live = count;
   if (TOP && (count > CANDIDATES || n_again > AGAIN)) {
     __syncthreads();
@@ -440,10 +473,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_logprobs(Call c) {
     live = better_than(0, cand, count);
   }
   if (c.parts == 1) {
-    finish<X>(c, t, token, given, top, Sd, Ed, cand, count, live);
+    finish<X>(c, t, token, given, top, Rd, Ed, cand, count, live);
     return;
   }
-  if (tid == 0) c.stats[blockIdx.x] = {Sd, Ed, top, 0.0f};
+  if (tid == 0) c.stats[blockIdx.x] = {Rd, Ed, top, 0.0f};
   if (TOP) {
     Entry *list = c.lists + (int64_t)blockIdx.x * c.top;
     for (int i = tid; i < count; i += THREADS) {
@@ -482,7 +515,10 @@ __global__ __launch_bounds__(JOIN) void k_join(Call c) {
   const float given = given_logit<X>(c, t, token);
   const float m = wave_max(part.m);
   const float d = fmaxf(part.m - m, -FAR), f = in ? __expf(d) : 0.0f;
-  const double S = sum_of_wave(part.S * f), E = sum_of_wave((part.E + part.S * d) * f);
+  // one of the largest logits is the row's 1
+  const int lead = __builtin_ctzll(__ballot(in && part.m == m));
+  const double S = 1.0 + part.R, E = sum_of_wave((part.E + S * d) * f);
+  const double R = sum_of_wave(lane == lead ? part.R : S * f);
   if (threadIdx.x == 0) n_cand = 0;
   __syncthreads();
   if (c.top) {
@@ -492,7 +528,7 @@ __global__ __launch_bounds__(JOIN) void k_join(Call c) {
       if (mine[i] && order_of(value_of(mine[i])) >= bound) cand[atomicAdd(&n_cand, 1)] = mine[i];
     __syncthreads();
   }
-  finish<X>(c, t, token, given, m, S, E, cand, n_cand, n_cand);
+  finish<X>(c, t, token, given, m, R, E, cand, n_cand, n_cand);
 }
 
 // Rows in parts: few rows over a long vocabulary, whose parts then have no less than PART
