@@ -531,18 +531,29 @@ __global__ __launch_bounds__(JOIN) void k_join(Call c) {
   finish<X>(c, t, token, given, m, R, E, cand, n_cand, n_cand);
 }
 
-// Rows in parts: few rows over a long vocabulary, whose parts then have no less than PART
-// logits. us of whole rows (8 waves each) and of parts and their join, fp32 with 5
-// alternatives: one row of 32003 8.3 and 9.8, of 64000 11.0 and 9.9, of 120832 15.7 and
-// 9.9; 64 rows of 64000 13.1 and 14.0, of 120832 18.0 and 17.4; 100 of 120832 19.0, 19.7.
+// Rows in parts: rows that are fewer than the CUs, over a long vocabulary; parts have no less
+// than PART logits. A row as a whole takes 75 us for a million logits more, whatever their type,
+// and the card's rate for all parts is twice as high (in logits) for 16-bit ones. us of whole
+// rows (8 waves each) and of parts and their join, 5 alternatives:
+//   fp32     1 row of 32003   8.3   9.8    16-bit   8 rows of 32003  10.2  11.6
+//            8 of 64000      12.7  11.4             8 of 64000      13.1  11.5
+//           64 of 64000      13.7  13.3            64 of 64000      14.1  13.2
+//          100 of 64000      13.7  15.1           128 of 64000      14.2  14.7
+//           64 of 120832     18.1  15.8           128 of 120832     19.6  18.5
+//          100 of 120832     19.8  20.0           160 of 120832     21.0  21.2
+//          128 of 120832     20.0  22.3           200 of 120832     21.2  22.9
+//           90 of 260000     32.6  27.3           200 of 260000     35.0  33.2
+//          160 of 260000     33.7  38.1           255 of 260000     35.6  36.9
 constexpr int PART = 2048, BLOCKS = 1024;
-int parts_of(int T, int V) {
-  if (T < 1 || (int64_t)(90 - T) * V < 3000000) return 1;
+int parts_of(int T, int V, int type) {
+  if (T < 1 || (type == HY3X_F32 ? (int64_t)(160 - T) * V < 6000000
+                                 : (int64_t)(260 - T) * V < 12000000))
+    return 1;
   return std::min({MAX_PARTS, (V + PART - 1) / PART, BLOCKS / T});
 }
 // Bytes of workspace of a call.
-int64_t room_of(int T, int V, int n_top) {
-  const int64_t parts = parts_of(T, V);
+int64_t room_of(int T, int V, int type, int n_top) {
+  const int64_t parts = parts_of(T, V, type);
   return parts == 1 ? 0 : T * parts * (int64_t)(sizeof(Stats) + n_top * sizeof(Entry));
 }
 // Whole rows: 8 waves each where the rows are too few for all of the card's, and long.
@@ -576,8 +587,9 @@ int64_t hy3x_logprobs_workspace(int T, int V, int n_top) {
   if (T < 0 || T > HY3X_LOGPROBS_MAX_TOKENS || V < 1 || V > HY3X_LOGPROBS_MAX_VOCAB ||
       n_top < 0 || n_top > HY3X_LOGPROBS_MAX_TOP || n_top > V)
     return op_fail(HY3X_E_ARG, "T=%d, V=%d or n_top=%d out of range", T, V, n_top);
-  int64_t room = 0;  // fewer rows may have more parts
-  for (int t = 1; t <= std::min(T, BLOCKS); t++) room = std::max(room, room_of(t, V, n_top));
+  int64_t room = 0;  // of either type; fewer rows may have more parts
+  for (int t = 1; t <= std::min(T, BLOCKS); t++)
+    room = std::max({room, room_of(t, V, HY3X_F32, n_top), room_of(t, V, HY3X_F16, n_top)});
   return room;
 }
 
@@ -600,7 +612,7 @@ int hy3x_logprobs(const void *logits, int type, int64_t row_stride, int V, const
   if (!logits || !tokens || !logp) return op_fail(HY3X_E_ARG, "NULL logits, tokens or logp");
   if (n_top && (!top_ids || !top_logp))
     return op_fail(HY3X_E_ARG, "n_top=%d without top_ids and top_logp", n_top);
-  const int64_t room = room_of(T, V, n_top);
+  const int64_t room = room_of(T, V, type, n_top);
   if (room && (!workspace || workspace_bytes < room))
     return op_fail(HY3X_E_ARG, "a workspace of %lld bytes is needed", (long long)room);
   const int64_t es = type == HY3X_F32 ? 4 : 2;
@@ -636,7 +648,7 @@ int hy3x_logprobs(const void *logits, int type, int64_t row_stride, int V, const
   c.entropy = entropy;
   c.top_ids = top_ids;
   c.top_logp = top_logp;
-  c.parts = parts_of(T, V);
+  c.parts = parts_of(T, V, type);
   c.part = ((V + c.parts - 1) / c.parts + 7) & ~7;  // whole 16 bytes
   c.parts = (V + c.part - 1) / c.part;
   c.stats = (Stats *)workspace;

@@ -35,3 +35,17 @@ def test_one_workspace_for_every_batch(torch):  # noqa: F811
         call = Call(torch, l[:T], tokens[:T], top)
         call.ws = ws
         check(torch, call())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V,kind", [(100, 120832, "f32"), (140, 120832, "bf16"),
+                                      (20, 500000, "f16"), (258, 32003, "bf16")])
+def test_rows_in_parts(torch, T, V, kind):  # noqa: F811
+    """As many rows as are split, a few more, and longer ones; masked parts among them."""
+    l = logits(torch, T, V, kind, 2).clone()
+    l[3, V // 3:] = float("-inf")
+    l[4, :V // 2] = float("nan")
+    l[5] = float("-inf")
+    l[6] = float("-inf")
+    l[6, V - 2:] = 1.0
+    check(torch, Call(torch, l, given(torch, T, V, 3), 20)())
