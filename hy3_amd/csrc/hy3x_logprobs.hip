@@ -556,11 +556,20 @@ int64_t room_of(int T, int V, int type, int n_top) {
   const int64_t parts = parts_of(T, V, type);
   return parts == 1 ? 0 : T * parts * (int64_t)(sizeof(Stats) + n_top * sizeof(Entry));
 }
-// Whole rows: 8 waves each where the rows are too few for all of the card's, and long.
-// us with 4 waves and with 8, 5 alternatives: fp32 16 rows of 16000 7.6 and 7.8, of 32003
-// 9.0 and 9.0, of 64000 13.3 and 12.1; bf16 256 of 120832 30.7 and 20.6, 333 of 32003 14.5
-// and 14.4, 511 of 50021 20.4 and 21.5, 2048 of 120832 108 and 113.
-constexpr int EIGHT_T = 384, EIGHT_V = 24576;
+// Whole rows: 8 waves each where the rows are long and each has a CU (up to 256), longer 16-bit
+// rows also where two have one (up to 512). us with 4 waves and with 8, 5 alternatives:
+//   fp32   256 rows of 20003 10.2 10.0    16-bit  256 rows of 20003 10.2 10.3
+//          256 of 32003      13.3 11.9            256 of 24576      10.4 10.2
+//          256 of 120832     29.6 27.8            256 of 50021      15.7 14.0
+//          270 of 32003      13.4 14.5            256 of 120832     31.2 22.6
+//          270 of 120832     30.3 33.8            333 of 50021      19.2 19.2
+//          511 of 50021      23.8 25.8            333 of 64000      21.9 21.1
+//          511 of 120832     47.1 45.0            511 of 120832     37.0 32.4
+//          800 of 120832     81.5 80.2            560 of 64000      27.3 28.2
+constexpr int CUS = 256, EIGHT = 24576, EIGHT_FOR_TWO = 65536;
+bool eight_waves(int T, int V, int type) {
+  return (T <= CUS && V >= EIGHT) || (T <= 2 * CUS && V >= EIGHT_FOR_TWO && type != HY3X_F32);
+}
 constexpr int ROWS = 1 << 23;  // of a launch, which has less than 2^32 threads
 
 template <class X, int WAVES>
@@ -571,7 +580,8 @@ void launch_waves(const Call &c, hipStream_t st) {
 }
 template <class X>
 void launch(const Call &c, hipStream_t st) {
-  if (c.parts == 1 && c.T < EIGHT_T && c.V >= EIGHT_V) launch_waves<X, 8>(c, st);
+  constexpr int TYPE = sizeof(X) == 4 ? HY3X_F32 : HY3X_F16;
+  if (c.parts == 1 && eight_waves(c.T, c.V, TYPE)) launch_waves<X, 8>(c, st);
   else launch_waves<X, 4>(c, st);
   if (c.parts > 1) k_join<X><<<c.T, JOIN, 0, st>>>(c);
 }
