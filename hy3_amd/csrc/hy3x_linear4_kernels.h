@@ -639,9 +639,13 @@ bool few(const Linear4Call &c, hipStream_t st) {
 //   64 x 8192 of 4096   4124 25.9, 2124 32.6    400 x 4096 of 4096  2241 58.4, 2442 66.3
 // fp32 x:
 //   64 x 4096 of 8192   2124 31.8, 4118 32.8    100 x 4096 of 4096  4124 25.3, 2124 33.5
-//   150 x 4096 of 4096  4142 38.0, 4124 46.0    300 x 4096 of 4096  2141 54.7, 2241 63.6
-//   512 x 4096 of 4096  2281 61.0, 2241 67.1    300 x 8192 of 4096  2241 86.3, 2141 92.6
+//   150 x 4096 of 4096  4142 38.0, 4124 46.0    256 x 4096 of 4096  4142 41.9, 2141 48.3
+//   264 x 4096 of 4096  2141 56.9, 2281 60.9    320 x 4096 of 4096  2141 56.1, 2281 61.0
+//   352 x 4096 of 4096  2281 61.1, 2141 59.1    400 x 4096 of 4096  2281 61.2, 2241 65.5
+//   512 x 4096 of 4096  2281 62.9, 2241 68.5    300 x 8192 of 4096  2241 86.3, 2141 92.6
 //   512 x 8192 of 4096  4241  107, 2241  127
+// and where 2141 has three blocks on each CU (groups of 32; of 64 352 x 4096 2281 64.9, 2141 67.7):
+//   384 x 4096 of 4096  (2141 75.5, 2281 82.6)  400 x 4096 of 4096  (2281 82.8, 2141 104)
 template <class X, int GP, bool DMA>
 void by_size(const Linear4Call &c, hipStream_t st) {
   constexpr bool SPLIT = Op<X>::PARTS == 3;
@@ -657,7 +661,7 @@ void by_size(const Linear4Call &c, hipStream_t st) {
     if (size <= 1536) return many<X, GP, 2, 1, 2, 4, DMA>(c, st);
     if (size <= 2048) return many<X, GP, 4, 1, 2, 4, DMA>(c, st);
     if (size <= 4096) return many<X, GP, 4, 1, 4, 2, DMA>(c, st);
-    if (size <= 5120) return many<X, GP, 2, 1, 4, 1, DMA>(c, st);
+    if (size <= (GP == 4 ? 6144 : 5120)) return many<X, GP, 2, 1, 4, 1, DMA>(c, st);
     if (size <= 8192) return many<X, GP, 2, 2, 8, 1, DMA>(c, st);
     if (size <= 12288) return many<X, GP, 2, 2, 4, 1, DMA>(c, st);
     return many<X, GP, RT, 2, 4, 1, DMA>(c, st);
