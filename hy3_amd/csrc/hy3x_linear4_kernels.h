@@ -623,9 +623,9 @@ bool few(const Linear4Call &c, hipStream_t st) {
 
 // The tile's shape by the size of the result: small tiles and a split of k where blocks are
 // few, large ones, which read and unpack less, where they are many; the limits of those with 8
-// waves are where each CU has a block (2124: two). us, groups of 128 (those of 32 in brackets:
-// more sums and scales a chunk, so that larger shapes spill), shapes as RT CT WN WK, the
-// chosen one and the next best; tokens x rows of d_in, 16-bit x:
+// waves are where each CU has a block (2124: two). us, shapes as RT CT WN WK, the chosen one and
+// the next best, groups of 128 (in brackets: of 32, whose sums and scales leave no registers for
+// 4 x 4 tiles); tokens x rows of d_in, 16-bit x:
 //   16 x 4096 of 1536   1124  5.3, 1118  5.6    24 x 4096 of 1536   2124  5.9, 2142  7.5
 //   16 x 4096 of 4096   1118  7.8, 2118  8.8    24 x 4096 of 4096   2124 10.5, 4118 11.5
 //   16 x 8192 of 4096   2118  9.9, 1124 10.3    24 x 4096 of 8192   4118 17.4, 2124 19.5
@@ -634,7 +634,16 @@ bool few(const Linear4Call &c, hipStream_t st) {
 //   300 x 4096 of 1536  2241 15.1, 2442 15.9        (1242 29.5, 2242 31.9)
 //   300 x 8192 of 4096  2241 41.0, 2242 43.3    512 x 4096 of 4096  2442 29.6, 2241 31.7
 //   512 x 8192 of 4096  2441 49.5, 2281 53.5        (2442 44.3, 2241 51.0)
+//   32 x 65536 of 4096  2241 41.5, 2442 57.2    528 x 4096 of 4096  2241 41.8, 2242 43.1
+//   768 x 4096 of 4096  2241 44.2, 2441 47.8    832 x 4096 of 4096  2441 47.9, 4241 52.0
+//       (2241 66.3, 2441 74.4)                      (2441 74.8, 2241 90.6)
+//   768 x 8192 of 4096  2441 76.0, 4441 78.1    784 x 8192 of 4096  4441 79.3, 2441 89.8
+//   32 x 120832 of 4096 4241 67.4, 2241 72.0    40 x 120832 of 4096 4441 89.7, 2441 96.5
+//       (2241  100, 2441  141)                      (2441  143, 2241  165)
 //   2048 x 8192 of 4096 4441  152; by 64 2441 196, 4441 209
+// and groups of 64:
+//   256 x 4096 of 4096  2242 24.6, 2241 30.2    512 x 4096 of 4096  2442 35.9, 2242 37.4
+//   768 x 4096 of 4096  2241 51.8, 2242 54.3    448 x 8192 of 4096  2441 57.4, 2242 66.7
 // 16-bit x that goes by way of registers (larger tiles share that work):
 //   64 x 8192 of 4096   4124 25.9, 2124 32.6    400 x 4096 of 4096  2241 58.4, 2442 66.3
 // fp32 x:
@@ -670,7 +679,8 @@ void by_size(const Linear4Call &c, hipStream_t st) {
     if (size <= (DMA ? 2048 : 1536)) return many<X, GP, 2, 1, 2, 4, DMA>(c, st);
     if constexpr (DMA) {
       if (size <= 4096) return many<X, GP, GP == 4 ? 1 : 2, 2, 4, 2, DMA>(c, st);
-      if (size <= 8192 && (GP == 4 || c.chunks >= 24)) return many<X, GP, 2, 4, 4, 2, DMA>(c, st);
+      if (size <= 8192 && c.T > 32 && (GP == 4 || c.chunks >= 24))
+        return many<X, GP, 2, 4, 4, 2, DMA>(c, st);
     } else {
       if (size <= 2048) return many<X, GP, 4, 1, 2, 4, DMA>(c, st);
       if (size <= 4096) return many<X, GP, 2, 2, 4, 2, DMA>(c, st);
@@ -685,8 +695,8 @@ void by_size(const Linear4Call &c, hipStream_t st) {
 // x in registers up to 4 tokens, for 16-bit x up to 16: there one wave's 4 sums a lane cost it
 // 4 times the FMAs, and it is the faster one only for few row tiles, which are all there at
 // once, and for many: 16 tokens, 4096 rows of 4096 7.0 us and 7.8, 8192 of 4096 11.2 and 9.9,
-// 16384 13.5 and 12.5, 120832 55.6 and 57.5. With groups of 32 the FMAs of 16 tokens outweigh the
-// bytes, and the registers spill (4096 of 4096 17.7 and 9.2). fp32 x has the ring alone: one
+// 16384 13.5 and 12.5, 120832 55.6 and 57.5. With groups of 32 the FMAs of 16 tokens outweigh
+// the bytes (4096 of 4096, when it was built, 17.7 and 9.2). fp32 x has the ring alone: one
 // token, 8192 rows of 4096 12.5 and 11.5, 16384 15.9 and 19.4, 120832 51.7 and 68.3; its
 // groups of 32 do not fit the registers.
 template <class X, int GP>
