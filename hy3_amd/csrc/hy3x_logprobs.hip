@@ -23,11 +23,13 @@
 // ones. Rows where too many logits reach it (equal ones) are gone through again, the
 // wave's best in its lanes.
 //
-// Bytes bound many long rows: 2048 of 120832 bf16 logits 97 us, 5.1 TB/s, as fast as a copy.
-// 11 vector instructions a logit, one of them an exponential, 14 with alternatives, bound what
-// the last caches hold: 511 rows of 50021 fp16 with 20 of them 21 us, 2.4 TB/s. Few rows are a
-// chain of waits (a lane's loads, the bound, the candidates, the join): one row of 120832 with
-// 20, 59 parts, 6.9 and 4.3 us.
+// Bytes bound many long rows: 2048 of 120832 bf16 logits 97 us, 5.1 TB/s, a copy's rate (plain
+// reads reach 6.2). Where each CU has a row or two, waits bound it, 55 % of the waves' cycles: 511
+// rows of 50021 fp16 16.6 us, with 20 alternatives 22.4, 2.3 TB/s, of which the 11 vector
+// instructions a logit (14 with alternatives) are 9; what comes after the pass (the bound, the
+// candidates' reads, their ranks, the logarithm) is a chain that nothing overlaps. Few rows are
+// chains alone (a lane's loads, that end, the join): one row of 120832 with 20, 59 parts, 7.0 and
+// 4.3 us.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
@@ -63,10 +65,10 @@ struct Type<__hip_bfloat16> {
 };
 
 // e^(-FAR) is 0 in fp32 (its least number is e^-103): what lies further below a maximum
-// counts as this far, so that a masked logit, -inf or NaN (which max passes over), adds 0 to both sums. (Where a lane has
-// met nothing but the type's lowest value, these count as 1 each until a larger maximum takes
-// their sums to 0 with it, in fp16 at most to e^-32 of them, its least step being 32; if none
-// comes the row has nothing left, and its sums are not used.)
+// counts as this far, so that a masked logit, -inf or NaN (which max passes over), adds 0 to
+// both sums. (Where a lane has met nothing but the type's lowest value, these count as 1 each
+// until a larger maximum takes their sums to 0 with it, in fp16 at most to e^-32 of them, its
+// least step being 32; if none comes the row has nothing left, and its sums are not used.)
 constexpr float FAR = 200.0f;
 constexpr double PEAK = 0.0625;  // from there on R has lost at most 4 bits of a lane's sum
 constexpr int MAX_PARTS = 64;    // of a row: a lane for each in k_join
@@ -545,10 +547,11 @@ __global__ __launch_bounds__(JOIN) void k_join(Call c) {
 //           90 of 260000     32.6  27.3           200 of 260000     35.0  33.2
 //          160 of 260000     33.7  38.1           255 of 260000     35.6  36.9
 constexpr int PART = 2048, BLOCKS = 1024;
+int most_split(int V, int type) {  // rows
+  return type == HY3X_F32 ? 160 - (6000000 + V - 1) / V : 260 - (12000000 + V - 1) / V;
+}
 int parts_of(int T, int V, int type) {
-  if (T < 1 || (type == HY3X_F32 ? (int64_t)(160 - T) * V < 6000000
-                                 : (int64_t)(260 - T) * V < 12000000))
-    return 1;
+  if (T < 1 || T > most_split(V, type)) return 1;
   return std::min({MAX_PARTS, (V + PART - 1) / PART, BLOCKS / T});
 }
 // Bytes of workspace of a call.
@@ -597,10 +600,10 @@ int64_t hy3x_logprobs_workspace(int T, int V, int n_top) {
   if (T < 0 || T > HY3X_LOGPROBS_MAX_TOKENS || V < 1 || V > HY3X_LOGPROBS_MAX_VOCAB ||
       n_top < 0 || n_top > HY3X_LOGPROBS_MAX_TOP || n_top > V)
     return op_fail(HY3X_E_ARG, "T=%d, V=%d or n_top=%d out of range", T, V, n_top);
-  int64_t room = 0;  // of either type; fewer rows may have more parts
-  for (int t = 1; t <= std::min(T, BLOCKS); t++)
-    room = std::max({room, room_of(t, V, HY3X_F32, n_top), room_of(t, V, HY3X_F16, n_top)});
-  return room;
+  // the most parts that up to T rows of either type have together
+  const int rows = std::min(T, std::max({most_split(V, HY3X_F32), most_split(V, HY3X_F16), 0}));
+  const int parts = std::min(rows * std::min(MAX_PARTS, (V + PART - 1) / PART), BLOCKS);
+  return parts * (int64_t)(sizeof(Stats) + n_top * sizeof(Entry));
 }
 
 int hy3x_logprobs(const void *logits, int type, int64_t row_stride, int V, const int32_t *tokens,

@@ -16,13 +16,14 @@ def test_no_batch_needs_more_than_a_larger_one(V):
 def test_a_call_accepts_what_a_larger_batch_was_told():
     """Too little is refused before the launch; what a batch of 256 was told is not."""
     lib = H.lib()
-    for V in (64000, 120832, 1 << 20):
+    for V in (64000, 120832, 1 << 20, 1 << 24):
         room = H.logprobs_workspace(256, V, 20)
-        for T in (1, 2, 16, 17, 40, 60, 64, 65, 66, 89, 128, 256):
-            # the outputs overlap: refused for that, after the workspace was looked at
-            rc = lib.hy3x_logprobs(1 << 40, 0, V, V, 1 << 20, T, 20, 1 << 20, 1 << 21, 1 << 22,
-                                   1 << 23, 1 << 24, room, None)
-            assert rc == -1 and b"overlaps" in lib.hy3x_last_error(), (V, T)
+        for T in (*range(1, 140), 159, 160, 200, 255, 256):
+            for kind in (0, 1, 2):
+                # the outputs overlap: refused for that, after the workspace was looked at
+                rc = lib.hy3x_logprobs(1 << 40, kind, V, V, 1 << 20, T, 20, 1 << 20, 1 << 21,
+                                       1 << 22, 1 << 23, 1 << 24, room, None)
+                assert rc == -1 and b"overlaps" in lib.hy3x_last_error(), (V, T, kind)
 
 
 @pytest.mark.gpu
