@@ -211,7 +211,7 @@ struct Groups {
 //
 // Bytes bound it where W is large: one token of bf16, 120832 rows of 4096, groups of 128: 46
 // us, 5.5 TB/s of weights; fp32 51 us. Small ones are a chain of waits (x, operands, their
-// sums, the tile, the join): 4096 rows of 4096 4.5 us.
+// sums, the tile, the join): 4096 rows of 4096 4.7 us.
 
 // Waves of a block, at most: the registers of a SIMD are enough for 4, or for 2 with a
 // ring or with fp32 on its way to parts.
@@ -364,12 +364,14 @@ __global__ __launch_bounds__((64 * few_waves<X, RING>()),
 // a chunk find the sums of its token tiles on the MFMAs (x times halves), each those of the
 // tiles that it comes to first, and leave them in LDS.
 //
-// 2048 tokens, 8192 rows of 4096, bf16, groups of 128: 153 us, 895 TFLOP/s (a bf16 product
-// of 8192^3 reaches 1266 on the same card). No one part bounds it: without the MFMAs 122 us,
-// without the reads of LDS 126, without the copies 131, without both of these 105 of 157 then:
-// the two waves of a SIMD do not hide all of each other's. All operands by way of LDS, as 16-bit
-// numbers that one wave unpacks for all, in three buffers: 156; products of a chunk ordered by
-// k first: 167. fp32 x is three products: 300 tokens, 4096 rows of 1536 15 us in bf16, in fp32 24.
+// 2048 tokens, 8192 rows of 4096, bf16, groups of 128: 158 us, 870 TFLOP/s (a bf16 product
+// of 8192^3 reaches 1266 on the same card). No one part bounds it: its vector
+// instructions are 91 us of a SIMD, its MFMAs 58, and the two waves of a SIMD do not hide all of
+// each other's. (With 7 instructions to unpack and 154 us: without the MFMAs 122 us, without the
+// reads of LDS 126, without the copies 131, without both of these 105 of 157 then; all operands by
+// way of LDS, as 16-bit numbers that one wave unpacks for all, in three buffers 156; products of
+// a chunk ordered by k first 167.) fp32 x is three products: 300 tokens, 4096 rows of 1536 16 us
+// in bf16, in fp32 24.
 template <class X, int GP, int RT, int CT, int WN, int WK, bool DMA>
 __global__ __launch_bounds__(64 * WN * WK, 2) void k_linear4_many(Linear4Call c) {
   constexpr int PARTS = Op<X>::PARTS, THREADS = 64 * WN * WK;
@@ -596,9 +598,9 @@ void few(const Linear4Call &c, int waves, int blocks, hipStream_t st) {
 // card at once (16 waves on each of 256 CUs) each has a block and no ring; longer ones have
 // a ring where the waves are enough for the card (from 5 quads), and two quads a wave only
 // where the registers are (groups of 128, up to 4 tokens). us for one bf16 token, then of the
-// next kernel's best shape: 4096 rows of 4096 4.5 and 5.3 (once), 8192 of 4096 7.0 and 7.3
-// (once), 4096 of 8192 7.0 and 8.7 (once), 120832 of 4096 46.1 and 55.3 (ring); 8192 of 8192
-// 11.8 and 11.0 (two quads a wave, what it costs at its worst).
+// next kernel's best shape: 4096 rows of 4096 4.7 and 5.5 (once), 8192 of 4096 6.8 and 7.7
+// (once), 4096 of 8192 6.8 and 8.7 (once), 120832 of 4096 46.0 and 53.3 (ring); 8192 of 8192
+// 12.3 and 11.3 (two quads a wave, what it costs at its worst).
 template <class X, int GP, int NR>
 bool few(const Linear4Call &c, hipStream_t st) {
   constexpr int RING = few_waves<X, 2>();
@@ -626,35 +628,36 @@ bool few(const Linear4Call &c, hipStream_t st) {
 // waves are where each CU has a block (2124: two). us, shapes as RT CT WN WK, the chosen one and
 // the next best, groups of 128 (in brackets: of 32, whose sums and scales leave no registers for
 // 4 x 4 tiles); tokens x rows of d_in, 16-bit x:
-//   16 x 4096 of 1536   1124  5.3, 1118  5.6    24 x 4096 of 1536   2124  5.9, 2142  7.5
-//   16 x 4096 of 4096   1118  7.8, 2118  8.8    24 x 4096 of 4096   2124 10.5, 4118 11.5
-//   16 x 8192 of 4096   2118  9.9, 1124 10.3    24 x 4096 of 8192   4118 17.4, 2124 19.5
-//   16 x 16384 of 4096  1124 12.5, 2118 14.6    64 x 8192 of 4096   2124 15.4, 2224 16.2
-//   16 x 120832 of 4096 4141 57.5, 1124 81.6    200 x 4096 of 4096  2242 20.6, 2142 22.6
-//   300 x 4096 of 1536  2241 15.1, 2442 15.9        (1242 29.5, 2242 31.9)
-//   300 x 8192 of 4096  2241 41.0, 2242 43.3    512 x 4096 of 4096  2442 29.6, 2241 31.7
-//   512 x 8192 of 4096  2441 49.5, 2281 53.5        (2442 44.3, 2241 51.0)
-//   32 x 65536 of 4096  2241 41.5, 2442 57.2    528 x 4096 of 4096  2241 41.8, 2242 43.1
-//   768 x 4096 of 4096  2241 44.2, 2441 47.8    832 x 4096 of 4096  2441 47.9, 4241 52.0
-//       (2241 66.3, 2441 74.4)                      (2441 74.8, 2241 90.6)
-//   768 x 8192 of 4096  2441 76.0, 4441 78.1    784 x 8192 of 4096  4441 79.3, 2441 89.8
-//   32 x 120832 of 4096 4241 67.4, 2241 72.0    40 x 120832 of 4096 4441 89.7, 2441 96.5
-//       (2241  100, 2441  141)                      (2441  143, 2241  165)
-//   2048 x 8192 of 4096 4441  152; by 64 2441 196, 4441 209
-// and groups of 64:
-//   256 x 4096 of 4096  2242 24.6, 2241 30.2    512 x 4096 of 4096  2442 35.9, 2242 37.4
-//   768 x 4096 of 4096  2241 51.8, 2242 54.3    448 x 8192 of 4096  2441 57.4, 2242 66.7
+//   16 x 4096 of 1536   1124  5.4, 1118  5.7    24 x 4096 of 1536   2124  6.3, 2142  8.0
+//   16 x 4096 of 4096   1118  7.7, 2118  8.9    24 x 4096 of 4096   2124 11.0, 4118 11.4
+//   16 x 8192 of 4096   2118 10.1, 1124 10.6    24 x 4096 of 8192   4118 17.1, 2124 18.3
+//   16 x 16384 of 4096  1124 13.0, 2118 14.7    64 x 8192 of 4096   2124 16.5, 2224 17.0
+//   16 x 120832 of 4096 4141 57.4, 1124 80.8    200 x 4096 of 4096  2242 22.0, 2142 25.3
+//   300 x 4096 of 1536  2241 16.6, 2442 16.4        (1242 33.1, 2242 33.3)
+//   300 x 8192 of 4096  2241 45.0, 2242 45.4    512 x 4096 of 4096  2442 31.8, 2241 33.9
+//   512 x 8192 of 4096  2441 55.9, 2281 61.4        (2442 45.4, 2241 52.1)
+//   32 x 65536 of 4096  2241 40.9, 2442 54.6    528 x 4096 of 4096  2241 45.0, 2242 43.9
+//   768 x 4096 of 4096  2241 46.2, 2441 48.8    832 x 4096 of 4096  2441 48.5, 4241 56.8
+//       (2241 66.0, 2441 73.9)                      (2441 74.4, 2241 90.9)
+//   768 x 8192 of 4096  2441 71.9, 4441 83.1    784 x 8192 of 4096  4441 78.9, 2441 90.8
+//   32 x 120832 of 4096 4241 65.6, 2241 70.5    40 x 120832 of 4096 4441 87.3, 2441 93.0
+//       (2241  100, 2441  139)                      (2441  141, 2241  164)
+//   2048 x 8192 of 4096 4441  157, 2441  175; by 64 2441 199, 2241 243
+// groups of 64:
+//   256 x 4096 of 4096  2242 24.6, 2241 30.6    512 x 4096 of 4096  2442 35.9, 2242 37.6
+//   768 x 4096 of 4096  2241 53.2, 2242 54.2    448 x 8192 of 4096  2441 56.8, 2242 66.5
 // 16-bit x that goes by way of registers (larger tiles share that work):
-//   64 x 8192 of 4096   4124 25.9, 2124 32.6    400 x 4096 of 4096  2241 58.4, 2442 66.3
+//   64 x 8192 of 4096   4124 24.4, 2124 25.6    400 x 4096 of 4096  2241 48.3, 2442 53.2
 // fp32 x:
-//   64 x 4096 of 8192   2124 31.8, 4118 32.8    100 x 4096 of 4096  4124 25.3, 2124 33.5
-//   150 x 4096 of 4096  4142 38.0, 4124 46.0    256 x 4096 of 4096  4142 41.9, 2141 48.3
-//   264 x 4096 of 4096  2141 56.9, 2281 60.9    320 x 4096 of 4096  2141 56.1, 2281 61.0
-//   352 x 4096 of 4096  2281 61.1, 2141 59.1    400 x 4096 of 4096  2281 61.2, 2241 65.5
-//   512 x 4096 of 4096  2281 62.9, 2241 68.5    300 x 8192 of 4096  2241 86.3, 2141 92.6
-//   512 x 8192 of 4096  4241  107, 2241  127
-// and where 2141 has three blocks on each CU (groups of 32; of 64 352 x 4096 2281 64.9, 2141 67.7):
-//   384 x 4096 of 4096  (2141 75.5, 2281 82.6)  400 x 4096 of 4096  (2281 82.8, 2141 104)
+//   64 x 4096 of 8192   2124 33.5, 4118 33.1    100 x 4096 of 4096  4124 26.5, 2124 33.5
+//   150 x 4096 of 4096  4142 40.7, 4124 47.0    256 x 4096 of 4096  4142 40.4, 2141 49.0
+//   264 x 4096 of 4096  2141 57.3, 2281 60.7    320 x 4096 of 4096  2141 57.0, 2281 60.8
+//   352 x 4096 of 4096  2281 60.9, 2141 59.2    400 x 4096 of 4096  2281 61.1, 2241 66.5
+//   512 x 4096 of 4096  2281 63.5, 2241 68.7    300 x 8192 of 4096  2241 89.1, 2141 95.9
+//   512 x 8192 of 4096  4241  110, 2241  128
+// and, up to where 2141 has three blocks on each CU, groups of 32 (of 64 already 352 x 4096
+// 2281 64.7, 2141 66.3):
+//   384 x 4096 of 4096  (2141 74.8, 2281 82.4)  400 x 4096 of 4096  (2281 82.7, 2141  105)
 template <class X, int GP, bool DMA>
 void by_size(const Linear4Call &c, hipStream_t st) {
   constexpr bool SPLIT = Op<X>::PARTS == 3;
@@ -694,10 +697,10 @@ void by_size(const Linear4Call &c, hipStream_t st) {
 
 // x in registers up to 4 tokens, for 16-bit x up to 16: there one wave's 4 sums a lane cost it
 // 4 times the FMAs, and it is the faster one only for few row tiles, which are all there at
-// once, and for many: 16 tokens, 4096 rows of 4096 7.0 us and 7.8, 8192 of 4096 11.2 and 9.9,
-// 16384 13.5 and 12.5, 120832 55.6 and 57.5. With groups of 32 the FMAs of 16 tokens outweigh
+// once, and for many: 16 tokens, 4096 rows of 4096 7.1 us and 7.7, 8192 of 4096 11.2 and 10.0,
+// 16384 13.5 and 12.6, 120832 55.0 and 57.4. With groups of 32 the FMAs of 16 tokens outweigh
 // the bytes (4096 of 4096, when it was built, 17.7 and 9.2). fp32 x has the ring alone: one
-// token, 8192 rows of 4096 12.5 and 11.5, 16384 15.9 and 19.4, 120832 51.7 and 68.3; its
+// token, 8192 rows of 4096 12.5 and 11.8, 16384 15.9 and 19.9, 120832 51.0 and 70.9; its
 // groups of 32 do not fit the registers.
 template <class X, int GP>
 void launch_group(const Linear4Call &c, hipStream_t st) {
@@ -710,8 +713,8 @@ void launch_group(const Linear4Call &c, hipStream_t st) {
     if constexpr (!SPLIT && GP < 4)
       if (few<X, GP, 4>(c, st)) return;
   }
-  // copies to LDS (2048 tokens, 8192 rows of 4096: 153 us; rows that begin at odd
-  // elements, by way of registers, 252)
+  // copies to LDS (2048 tokens, 8192 rows of 4096: 158 us; rows that begin at odd
+  // elements, by way of registers, 237)
   if constexpr (!SPLIT)  // 32-bit offsets of 64 rows
     if (c.d_in % 128 == 0 && (uintptr_t)c.x % 16 == 0 && c.x_stride % 8 == 0 &&
         c.x_stride <= 1 << 24)

@@ -429,7 +429,8 @@ int64_t hy3x_logprobs_workspace(int T, int V, int n_top);
  *    They have p = 0 and log p = -inf and come after every other token, in index order.
  *    A row with nothing left has logp -inf, entropy 0 and tokens 0 .. n_top - 1.
  *  - A logit of +inf counts as the largest finite value of its type.
- *  - fp32 exponentials, whose sums over a row are joined in 64 bits.
+ *  - fp32 exponentials, whose sums over a row are joined in 64 bits. Where one token has nearly
+ *    all of the mass, its logp and the entropy keep the relative precision of the others' share.
  * logits: device [T rows of V elements], `type` HY3X_F32 / F16 / BF16, rows row_stride
  * elements apart (V .. 2^32); tokens: device int32[T]; outputs: device, dense, overlapping
  * nothing else (logits are a range from their first to their last element). workspace:
